@@ -277,6 +277,73 @@ int ress_block_sparse_fwd(const void* q_i8, const void* k_i8, const void* v, int
                           long long soH, long long soT, float sm_scale, void* workspace,
                           long long workspace_bytes, hipStream_t stream);
 
+/* ---- paged 8-bit key/value cache (kvcache.hip, cache_attn.hip) ------------ */
+/* The cache that a streamed sequence's global attention reads: the reference attends over all frames
+ * at once and has no counterpart. A page holds 64 tokens of one key/value head in 8 bits with one scale
+ * for its keys and one for its values; the tokens of a sequence's last, unfinished page are held in
+ * 16 bits, by slot. All buffers are device memory owned by the caller:
+ *   k_codes [n_pages][kv_heads][64][head_dim], v_codes [n_pages][kv_heads][head_dim][64] (the tokens of a
+ *     row in the order csrc/kvcache.h gives), k_scale, v_scale [n_pages][kv_heads] f32
+ *   tail_k [max_seqs][kv_heads][64][head_dim], tail_v [max_seqs][kv_heads][head_dim][64] 16-bit elements,
+ *     tail_top [max_seqs][kv_heads] f32
+ *   table [max_seqs][max_pages] int32: the page that holds tokens 64 j .. 64 j + 63 of a slot
+ *   held [max_seqs] int32: pages reserved for the slot (its first `held` table entries)
+ *   lens [max_seqs] int32: tokens in the slot
+ *   arrived [max_seqs] int32: zero between calls
+ *   status int32, OR-ed: 1 tokens that found no reserved page were dropped, 2 a position outside the
+ *     rotation table (clamped into it), 4 a page number outside the pool (not read or written),
+ *     8 a page with a key or value that is not finite (its scale is NaN)
+ * dtype: 1 bf16, 2 fp16 (keys, values and queries). codes: 0 int8, 1 e4m3. head_dim: 64 or 128. */
+typedef struct ress_kv_cache {
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  void* tail_k;
+  void* tail_v;
+  float* tail_top;
+  int* table;
+  int* held;
+  int* lens;
+  int* arrived;
+  int* status;
+  int n_pages;
+  int max_pages;
+  int max_seqs;
+  int kv_heads;
+  int head_dim;
+  int dtype;
+  int codes;
+} ress_kv_cache;
+
+/* Appends n tokens a sequence: k, v (B,kv_heads,n,head_dim), element strides (sB,sH,sT), unit-stride
+ * dims, to slots[b] (int32[B] in device memory, each at most once; null: slot b), the first new_lens[b] of
+ * them (int32[B] in device memory, clamped to 0..n; null: all), and moves lens on. pos (B,n,axes) int64 or
+ * null: keys, and queries q (B,Hq,n,head_dim) if given, are rotated with the rows pos of
+ * rope (positions, 2, head_dim / 2 / axes) f32, cosines before sines; q_out (B,Hq,n,head_dim) receives
+ * the rotated queries, zeros in the rows past new_lens. Calls on one cache run one after the other. */
+int ress_kv_append(const ress_kv_cache* cache, const void* k, long long skB, long long skH, long long skT,
+                   const void* v, long long svB, long long svH, long long svT, const void* q, long long sqB,
+                   long long sqH, long long sqT, int B, int Hq, int n, const long long* pos, const float* rope,
+                   int positions, int axes, const int* slots, const int* new_lens, void* q_out, hipStream_t stream);
+
+/* Tokens start[b] .. start[b]+n-1 (int32[B] in device memory; null: the last n) of each sequence as the
+ * cache holds them: k, v (B,kv_heads,n,head_dim) in its 16-bit type, zeros where there is no token. */
+int ress_kv_read(const ress_kv_cache* cache, int B, int n, const int* slots, const int* start, void* k, void* v,
+                 hipStream_t stream);
+
+/* softmax(sm_scale q K^T) V over the cache: q (B,Hq,n,head_dim), element strides (sB,sH,sT); query head h
+ * reads key/value head h / (Hq / kv_heads). Row i of sequence b sees every token, or with causal = 1 the
+ * tokens up to its own, the rows being the sequence's last new_lens[b] tokens (null: n). Rows past
+ * new_lens[b] are not written; rows that see nothing are zero. most_tokens: no sequence is longer (it sizes
+ * the split of the keys; a longer one is still right). workspace: ress_kv_attend_workspace_size bytes,
+ * 16-byte aligned, for the same arguments (may be 0 bytes). sm_scale > 0. */
+long long ress_kv_attend_workspace_size(const ress_kv_cache* cache, int B, int Hq, int n, int most_tokens);
+int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long sqB, long long sqH, long long sqT, int B,
+                   int Hq, int n, const int* slots, const int* new_lens, int causal, float sm_scale,
+                   int most_tokens, void* out, long long soB, long long soH, long long soT, void* workspace,
+                   long long workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,9 @@ _SIGS = {
     "ress_meansim_block_map": "ppp" + "iiii" + "llllll" + "ppi" + "ppppppppp" + "pl" + "s",
     "ress_qk_norm_rope": "piii" + "pppp" + "f" + "pf" + "ppp" + "s",
     "ress_bf16_selfcheck": "Il" + "p" + "s",
+    "ress_kv_append": "p" + "plll" * 3 + "iii" + "ppii" + "ppp" + "s",
+    "ress_kv_read": "pii" + "pp" + "pp" + "s",
+    "ress_kv_attend": "p" + "plll" + "iii" + "pp" + "ifi" + "plll" + "pl" + "s",
 }
 _CT = {
     "p": ctypes.c_void_p,
@@ -67,6 +70,8 @@ def lib():
         L.ress_restore_swap_workspace_size.argtypes = [ctypes.c_int] * 4
         L.ress_meansim_workspace_size.restype = ctypes.c_longlong
         L.ress_meansim_workspace_size.argtypes = [ctypes.c_int] * 4
+        L.ress_kv_attend_workspace_size.restype = ctypes.c_longlong
+        L.ress_kv_attend_workspace_size.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
         L.ress_noalloc_scratch_bytes.restype = ctypes.c_longlong
         L.ress_noalloc_scratch_bytes.argtypes = []
         L.ress_noalloc_status_address.restype = ctypes.c_int
@@ -113,5 +118,5 @@ def last_error():
 def exported_symbols():
     return list(_SIGS) + ["ress_last_error", "ress_abi_version", "ress_qattn_workspace_size",
                           "ress_attn_sched_bytes", "ress_restore_swap_workspace_size", "ress_meansim_workspace_size",
-                          "ress_noalloc_scratch_bytes",
+                          "ress_noalloc_scratch_bytes", "ress_kv_attend_workspace_size",
                           "ress_noalloc_status_address"]

@@ -1,0 +1,725 @@
+// Attention over the paged 8-bit key/value cache (layout: kvcache.h).
+//
+// o = softmax(s q K^T) V with K = code * k_scale, V = code * v_scale per (page, head). With 16x16x32
+// MFMAs and the operands transposed, S^T = K Q^T (A = codes of 16 keys, B = 16 queries) and
+// O^T += V^T P^T (A = values of 16 dims), a lane holds for ITS query four keys of each 16, which is what
+// the second product takes as its B operand once the keys of a value row are stored in that order (v_token): P
+// never leaves the registers. The codes are widened to 16 bits exactly; the scales of a page multiply
+// the scores (folded into the exponent's multiply-add) and P (before it is rounded to 16 bits), so that
+// nothing but Q, P and the output is rounded to 16 bits. Max, sum and output accumulate in fp32.
+//
+// Running max. m starts at the lowest finite value and moves only when a score of the wave lies more than
+// LAZY = 8 (in log2) above its row's m: P is then at most 2^8, sums are unaffected, and most pages need
+// neither the exchange between a row's four lanes nor a pass over the accumulators.
+//
+// fp16. P * v_scale is formed relative to the largest v_scale met so far (R, uniform in the wave; the
+// accumulator is rescaled when it grows), times 2^7, to keep it inside fp16's range for any v_scale.
+//
+// Masked places (past the sequence's end, after the row's own token) are selected away after every
+// multiplication, so a NaN scale or tail element there reaches no row that does not see its page.
+#include "kvcache.h"
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+constexpr float LOWEST = -0x1.fffffep127f;
+constexpr float LAZY = 8.0f;
+constexpr float F16_LIFT = 128.0f;  // 2^7; P <= 2^8 keeps P * lift below fp16's 65504
+
+struct AttendArgs {
+  ress_kv_cache c;
+  const uint16_t* q;
+  uint16_t* out;
+  long long sqb, sqh, sqt, sob, soh, sot;
+  int B, Hq, n, G;   // G = Hq / kv_heads
+  const int *slots, *new_lens;
+  int causal;
+  float scale;       // sm_scale * log2(e)
+  int splits, tiles; // splits of the keys; row tiles of a (sequence, kv head)
+  float *part_o, *part_ml;  // [splits][B * kv_heads * n * G][D], [..][2]
+  bool qvec, ovec;
+};
+
+template <int DT>
+__device__ __forceinline__ v4f mfma(const uint4& a, const uint4& b, const v4f& c) {
+  if constexpr (DT == KV_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == KV_BF16) {
+    const v2bf r = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(uint32_t, r);
+  } else {
+    const v2h r = {(_Float16)lo, (_Float16)hi};
+    return __builtin_bit_cast(uint32_t, r);
+  }
+}
+
+// One sequence and key/value head: what it holds.
+template <int D>
+struct Head {
+  int len, nv, slot, h;
+  const uint8_t *kc, *vc;      // codes of page 0 of this head
+  const uint16_t *tk, *tv;     // the unfinished page
+  long long stride;            // bytes from page to page
+  __device__ __forceinline__ Head(const AttendArgs& a, int b, int h_) : h(h_) {
+    slot = a.slots ? a.slots[b] : b;
+    len = a.c.lens[slot];
+    nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
+    const long long one = (long long)KV_PAGE * D;
+    kc = reinterpret_cast<const uint8_t*>(a.c.k_codes) + h * one;
+    vc = reinterpret_cast<const uint8_t*>(a.c.v_codes) + h * one;
+    tk = reinterpret_cast<const uint16_t*>(a.c.tail_k) + ((long long)slot * a.c.kv_heads + h) * one;
+    tv = reinterpret_cast<const uint16_t*>(a.c.tail_v) + ((long long)slot * a.c.kv_heads + h) * one;
+    stride = one * a.c.kv_heads;
+  }
+};
+
+// The tail's values are scaled by a power of two to at most 128 (like codes), undone by its v_scale; NaN
+// where a value is not finite.
+struct TailScale {
+  float down, vs;  // multiply the values by down, P by vs
+  bool bad;
+  __device__ __forceinline__ explicit TailScale(float top) {
+    bad = top != top;
+    int e = 0;
+    if (!bad && top > 0.0f) frexpf(top, &e);  // top < 2^e
+    e = min(max(e - 7, -100), 100);
+    down = bad ? 0.0f : ldexpf(1.0f, -e);
+    vs = bad ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, e);
+  }
+};
+
+// A lane's state for CT tiles of 16 queries: query 16 ct + (lane & 15), shared by the four lanes of a column.
+template <int DT, int D, int CT>
+struct Rows {
+  v4f o[CT][D / 16];  // dims 16 dt + 4 (lane >> 4) + r
+  float m[CT], l[CT]; // l: this lane's keys alone
+  float R;            // fp16: the v_scale that o is relative to
+  __device__ __forceinline__ void clear() {
+    R = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      m[c] = LOWEST;
+      l[c] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[c][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // Scores s of 64 keys -> P as the second product's B operand p. cs = k_scale * scale, vs = v_scale;
+  // MASK: query c sees the tile's keys below lim[c].
+  template <bool MASK>
+  __device__ __forceinline__ void softmax(const v4f (&s)[CT][4], float cs, float vs, const int (&lim)[CT], int h4,
+                                          uint4 (&p)[CT][2]) {
+    float top[CT];
+    bool up = false;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      float t = LOWEST;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = s[c][k][r];
+          if constexpr (MASK) x = 16 * k + 4 * h4 + r < lim[c] ? x : -__builtin_huge_valf();
+          t = fmaxf(t, x);
+        }
+      if constexpr (MASK) top[c] = t == LOWEST ? LOWEST : t * cs;
+      else top[c] = t * cs;
+      up = up || top[c] > m[c] + LAZY;
+    }
+    if (__any(up)) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        float t = fmaxf(top[c], m[c]);
+        t = fmaxf(t, xor_lane_f<16>(t));
+        t = fmaxf(t, xor_lane_f<32>(t));
+        t = t > m[c] + LAZY ? t : m[c];  // a row moves by its own scores, so its bits do not hang on its neighbours
+        const float a = exp2f(m[c] - t);
+        m[c] = t;
+        l[c] *= a;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) o[c][d] *= a;
+      }
+    }
+    float f = vs;
+    if constexpr (DT == KV_F16) {
+      if (vs > R) {
+        const float a = R / vs;
+        R = vs;
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) o[c][d] *= a;
+      }
+      f = R > 0.0f ? vs / R * F16_LIFT : vs;  // vs is 0 or NaN where R is 0
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool sees = !MASK || 16 * k + 4 * h4 + r < lim[c];
+          float x = __builtin_amdgcn_exp2f(fmaf(s[c][k][r], cs, -m[c]));
+          if constexpr (MASK) x = sees ? x : 0.0f;
+          l[c] += x;
+          e[r] = x * f;
+          if constexpr (MASK) e[r] = sees ? e[r] : 0.0f;
+        }
+        w[2 * k] = pack2<DT>(e[0], e[1]);
+        w[2 * k + 1] = pack2<DT>(e[2], e[3]);
+      }
+      p[c][0] = make_uint4(w[0], w[1], w[2], w[3]);
+      p[c][1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+
+  // The factor that takes o to its own units, and the row's whole sum
+  __device__ __forceinline__ float unit() const { return DT == KV_F16 ? R * (1.0f / F16_LIFT) : 1.0f; }
+  __device__ __forceinline__ float sum(int c) const {
+    float t = l[c] + xor_lane_f<16>(l[c]);
+    return t + xor_lane_f<32>(t);
+  }
+};
+
+// Row r of a (sequence, kv head): token r / G, query head h G + r % G.
+template <int D, int CT>
+__device__ __forceinline__ void load_q(const AttendArgs& a, int b, int h, int row0, int rows, int lane,
+                                       uint4 (&qv)[CT][D / 32]) {
+  const int h4 = lane >> 4;
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int r = row0 + 16 * c + (lane & 15);
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      qv[c][s] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {  // dims of step s: 64 (s / 2) + 16 h4 + 8 (s % 2) + 0..7, as the codes are read
+        const int tok = r / a.G, hq = h * a.G + r % a.G;
+        qv[c][s] = ld8(a.q + b * a.sqb + hq * a.sqh + tok * a.sqt + 64 * (s >> 1) + 16 * h4 + 8 * (s & 1), a.qvec);
+      }
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(uint16_t* p, const v4f& v, bool vec) {
+  const uint32_t lo = pack2<DT>(v[0], v[1]), hi = pack2<DT>(v[2], v[3]);
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+  } else {
+    p[0] = (uint16_t)lo; p[1] = (uint16_t)(lo >> 16); p[2] = (uint16_t)hi; p[3] = (uint16_t)(hi >> 16);
+  }
+}
+
+// 16 codes (two steps' operands) widened
+template <int DT, int CODES>
+__device__ __forceinline__ void widen16(const uint4& w, uint4& a, uint4& b) {
+  const uint2 x = widen4<DT, CODES>(w.x), y = widen4<DT, CODES>(w.y), z = widen4<DT, CODES>(w.z), u = widen4<DT, CODES>(w.w);
+  a = make_uint4(x.x, x.y, y.x, y.y);
+  b = make_uint4(z.x, z.y, u.x, u.y);
+}
+// 16-bit tail values times a power of two; places of tokens from cnt on are zero
+template <int DT>
+__device__ __forceinline__ uint4 tail_v8(const uint4& w, float down, int place, int cnt) {
+  uint16_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = Elem<DT>::get(elem8(w, i));
+    e[i] = down != 0.0f && v_token(place + i) < cnt ? Elem<DT>::put(x * down) : 0;
+  }
+  return pack8(e);
+}
+
+// ---- few rows: one wave a page --------------------------------------------------------------------
+// A workgroup of four waves takes 16 CT rows of a (sequence, kv head) and a share of its pages, a wave every
+// fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
+// joined in LDS.
+template <int DT, int CODES, int D, int CT>
+__global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
+  constexpr int NW = 4;
+  __shared__ __align__(16) float so[NW][64][4 * CT];  // one dim tile at a time
+  __shared__ float sm[NW][CT][16], sl[NW][CT][16];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h4 = lane >> 4;
+  const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / a.splits / a.tiles;
+  const int H = a.c.kv_heads, b = bh / H, h = bh % H;
+  const Head<D> hd(a, b, h);
+  const int rows = hd.nv * a.G, row0 = tile * 16 * CT;
+  const long long all_rows = (long long)a.B * H * a.n * a.G;
+  if (row0 >= rows) return;
+  uint4 qv[CT][D / 32];
+  load_q<D, CT>(a, b, h, row0, rows, lane, qv);
+
+  const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
+  const int per = cdiv(pages, a.splits);
+  const int lo = min(pages, split * per), hi = min(pages, lo + per);
+  int limit[CT];  // tokens that the lane's query sees
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int tok = (row0 + 16 * c + (lane & 15)) / a.G;
+    limit[c] = a.causal ? max(0, hd.len - hd.nv + tok + 1) : hd.len;
+  }
+  const int seen_by_all = a.causal ? max(0, hd.len - hd.nv + row0 / a.G + 1) : hd.len;
+  const int seen_by_any =
+      a.causal ? max(0, hd.len - hd.nv + (min(row0 + 16 * CT, rows) - 1) / a.G + 1) : hd.len;
+
+  Rows<DT, D, CT> st;
+  st.clear();
+  const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
+  constexpr int KU = D / 16, VU = D / 16;  // 1 KB units of a page: keys (4 tiles x D / 64 halves), values (D / 16)
+  uint4 kw[KU], vw[VU];
+  float ks = 0.0f, vs = 0.0f;
+  auto load = [&](int pg) {  // a whole page's codes and scales; a bad page number reads as empty
+    int pid = pg < a.c.max_pages ? table[pg] : -1;
+    const bool ok = pid >= 0 && pid < a.c.n_pages;
+    if (!ok && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
+    pid = ok ? pid : 0;
+    const uint8_t* kp = hd.kc + pid * hd.stride + (lane & 15) * D + h4 * 16;
+    const uint8_t* vp = hd.vc + pid * hd.stride + lane % 16 * KV_PAGE + h4 * 16;
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+      kw[u] = *reinterpret_cast<const uint4*>(kp + u / (D / 64) * 16 * D + u % (D / 64) * 64);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) vw[u] = *reinterpret_cast<const uint4*>(vp + u * 16 * KV_PAGE);
+    const long long at = (long long)pid * H + h;
+    ks = ok ? a.c.k_scale[at] : 0.0f;
+    vs = ok ? a.c.v_scale[at] : 0.0f;
+  };
+  auto finish = [&](const v4f (&s)[CT][4], const uint4 (&va)[VU][2], float cs, float v, int pg) {
+    uint4 p[CT][2];
+    int lim[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
+    if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p);
+    else st.template softmax<true>(s, cs, v, lim, h4, p);
+#pragma unroll
+    for (int d = 0; d < VU; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) st.o[c][d] = mfma<DT>(va[d][u], p[c][u], st.o[c][d]);
+  };
+
+  const int last = min(min(hi, full), cdiv(seen_by_any, KV_PAGE));
+  int pg = lo + w;
+  if (pg < last) load(pg);
+  for (; pg < last; pg += NW) {
+    v4f s[CT][4];
+    uint4 va[VU][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) {
+        uint4 x, y;
+        widen16<DT, CODES>(kw[k * (D / 64) + e], x, y);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          s[c][k] = mfma<DT>(x, qv[c][2 * e], s[c][k]);
+          s[c][k] = mfma<DT>(y, qv[c][2 * e + 1], s[c][k]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < VU; ++u) widen16<DT, CODES>(vw[u], va[u][0], va[u][1]);
+    const float cs = ks * a.scale, v = vs;
+    if (pg + NW < last) load(pg + NW);
+    finish(s, va, cs, v, pg);
+  }
+  // the unfinished page, by the wave whose turn it would be
+  if (left && full >= lo && full < hi && (full - lo) % NW == w && full * KV_PAGE < seen_by_any) {
+    const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
+    v4f s[CT][4];
+    uint4 va[VU][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        const uint4 x = *reinterpret_cast<const uint4*>(hd.tk + (16 * k + (lane & 15)) * D + 64 * (e >> 1) + 16 * h4 + 8 * (e & 1));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < VU; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        va[d][u] = tail_v8<DT>(*reinterpret_cast<const uint4*>(hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4 + 8 * u),
+                               ts.down, 16 * h4 + 8 * u, left);
+    finish(s, va, a.scale, ts.vs, full);
+  }
+
+  // join the four waves
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const float t = st.sum(c);
+    if (lane < 16) {
+      sm[w][c][lane] = st.m[c];
+      sl[w][c][lane] = t;
+    }
+  }
+  __syncthreads();
+  float f[CT], M[CT], L[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int i = lane & 15;
+    M[c] = fmaxf(fmaxf(sm[0][c][i], sm[1][c][i]), fmaxf(sm[2][c][i], sm[3][c][i]));
+    L[c] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) L[c] += sl[k][c][i] * exp2f(sm[k][c][i] - M[c]);
+    f[c] = exp2f(st.m[c] - M[c]) * st.unit();
+  }
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d) {
+    if (d) __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CT; ++c) *reinterpret_cast<v4f*>(&so[w][lane][4 * c]) = st.o[c][d] * f[c];
+    __syncthreads();
+    if (w < CT) {  // wave c adds column tile c
+      v4f t = *reinterpret_cast<const v4f*>(&so[0][lane][4 * w]);
+#pragma unroll
+      for (int k = 1; k < NW; ++k) t += *reinterpret_cast<const v4f*>(&so[k][lane][4 * w]);
+      float Lw = L[0], Mw = M[0];
+#pragma unroll
+      for (int c = 1; c < CT; ++c) {
+        Lw = w == c ? L[c] : Lw;
+        Mw = w == c ? M[c] : Mw;
+      }
+      const int r = row0 + 16 * w + (lane & 15);
+      if (r < rows) {
+        const int dim = 16 * d + 4 * h4;
+        if (a.splits == 1) {
+          const int tok = r / a.G, hq = h * a.G + r % a.G;
+          const float inv = Lw == 0.0f ? 0.0f : 1.0f / Lw;
+          const v4f y = t * inv;
+          store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, y, a.ovec);
+        } else {
+          const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
+          *reinterpret_cast<v4f*>(a.part_o + at * D + dim) = t;
+          if (d == 0 && lane < 16) {
+            a.part_ml[2 * at] = Mw;
+            a.part_ml[2 * at + 1] = Lw;
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---- many rows: pages widened once for a workgroup ---------------------------------------------------
+// NW waves of 16 CT rows each share a page, widened into LDS in the order in which the operands are read (1 KB
+// a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page.
+template <int DT, int CODES, int D, int CT, int NW>
+__global__ __launch_bounds__(64 * NW) void k_cache_attn_rows(AttendArgs a) {
+  constexpr int THREADS = 64 * NW;
+  constexpr int PIECES = KV_PAGE * D / 16;       // 16-code pieces of a page's keys (and of its values)
+  constexpr int PT = PIECES / THREADS;           // a thread's pieces of each
+  static_assert(PT >= 1 && PT * THREADS == PIECES, "every thread has whole pieces");
+  constexpr int OPS = KV_PAGE * D / 8 / 64;      // 1 KB operand blocks of the keys (and of the values)
+  __shared__ uint4 lk[2][OPS * 64], lv[2][OPS * 64];
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, h4 = lane >> 4;
+  const int H = a.c.kv_heads, groups = a.B * H * a.splits;
+  // workgroups that read the same pages go to one XCD (workgroup i runs on XCD i % 8)
+  const int x = blockIdx.x >> 3, group = x / a.tiles * 8 + (blockIdx.x & 7), tile = a.tiles - 1 - x % a.tiles;
+  if (group >= groups) return;
+  const int split = group % a.splits, bh = group / a.splits, b = bh / H, h = bh % H;
+  const Head<D> hd(a, b, h);
+  const int rows = hd.nv * a.G, row0 = tile * 16 * CT * NW;
+  const long long all_rows = (long long)a.B * H * a.n * a.G;
+  if (row0 >= rows) return;
+  const int wrow = row0 + 16 * CT * w;
+  uint4 qv[CT][D / 32];
+  load_q<D, CT>(a, b, h, wrow, rows, lane, qv);
+
+  const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
+  const int per = cdiv(pages, a.splits);
+  const int before = hd.len - hd.nv;  // causal: row of token i sees before + i + 1 tokens
+  auto sees = [&](int r) { return a.causal ? max(0, before + r / a.G + 1) : hd.len; };
+  const int lo = min(pages, split * per);
+  const int hi = min(min(pages, lo + per), cdiv(sees(min(row0 + 16 * CT * NW, rows) - 1), KV_PAGE));
+  int limit[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) limit[c] = sees(wrow + 16 * c + (lane & 15));
+  const int seen_by_all = sees(wrow), seen_by_any = wrow < rows ? sees(min(wrow + 16 * CT, rows) - 1) : 0;
+
+  Rows<DT, D, CT> st;
+  st.clear();
+  const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
+  uint4 kw[PT], vw[PT];
+  float ks = 0.0f, vs = 0.0f, ks1, vs1;
+  auto load = [&](int pg) {
+    int pid = pg < a.c.max_pages ? table[pg] : -1;
+    const bool ok = pid >= 0 && pid < a.c.n_pages;
+    if (!ok && t == 0) atomicOr(a.c.status, KV_ST_PAGE);
+    pid = ok ? pid : 0;
+    const uint8_t* kp = hd.kc + pid * hd.stride + t * 16;
+    const uint8_t* vp = hd.vc + pid * hd.stride + t * 16;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      kw[i] = *reinterpret_cast<const uint4*>(kp + i * THREADS * 16);
+      vw[i] = *reinterpret_cast<const uint4*>(vp + i * THREADS * 16);
+    }
+    const long long at = (long long)pid * H + h;
+    ks1 = ok ? a.c.k_scale[at] : 0.0f;
+    vs1 = ok ? a.c.v_scale[at] : 0.0f;
+  };
+  // where piece i's two operands go: keys, row i / (D / 16) and chunk i % (D / 16); values, row i / 4, chunk i % 4
+  auto k_slot = [&](int i) {
+    const int row = i / (D / 16), ch = i % (D / 16);
+    return (((row >> 4) * (D / 64) + (ch >> 2)) * 2) * 64 + (ch & 3) * 16 + (row & 15);
+  };
+  auto v_slot = [&](int i) {
+    const int row = i >> 2, ch = i & 3;
+    return ((row >> 4) * 2) * 64 + ch * 16 + (row & 15);
+  };
+  auto stage = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int p = t + i * THREADS, sk = k_slot(p), sv = v_slot(p);
+      uint4 x, y;
+      widen16<DT, CODES>(kw[i], x, y);
+      lk[buf][sk] = x;
+      lk[buf][sk + 64] = y;
+      widen16<DT, CODES>(vw[i], x, y);
+      lv[buf][sv] = x;
+      lv[buf][sv + 64] = y;
+    }
+  };
+  auto stage_tail = [&](int buf, const TailScale& ts) {
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int p = t + i * THREADS, sk = k_slot(p), sv = v_slot(p);
+      lk[buf][sk] = reinterpret_cast<const uint4*>(hd.tk)[2 * p];
+      lk[buf][sk + 64] = reinterpret_cast<const uint4*>(hd.tk)[2 * p + 1];
+      const int place = (p & 3) * 16;
+      lv[buf][sv] = tail_v8<DT>(reinterpret_cast<const uint4*>(hd.tv)[2 * p], ts.down, place, left);
+      lv[buf][sv + 64] = tail_v8<DT>(reinterpret_cast<const uint4*>(hd.tv)[2 * p + 1], ts.down, place + 8, left);
+    }
+  };
+  auto fetch = [&](int pg) {  // start page pg's way into a stage
+    if (pg < full) load(pg);
+  };
+  auto put = [&](int pg, int buf) {
+    if (pg < full) {
+      stage(buf);
+    } else {
+      const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
+      stage_tail(buf, ts);
+      ks1 = 1.0f;
+      vs1 = ts.vs;
+    }
+  };
+  if (lo < hi) {
+    fetch(lo);
+    put(lo, 0);
+    ks = ks1;
+    vs = vs1;
+    if (lo + 1 < hi) fetch(lo + 1);
+    __syncthreads();
+  }
+  for (int pg = lo; pg < hi; ++pg) {
+    const int buf = (pg - lo) & 1;
+    if (pg + 1 < hi) put(pg + 1, buf ^ 1);  // read last before the barrier that ended the step before
+    const float nks = ks1, nvs = vs1;
+    if (pg + 2 < hi) fetch(pg + 2);
+    if (pg * KV_PAGE < seen_by_any) {
+      v4f s[CT][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+          const uint4 x = lk[buf][(k * (D / 32) + e) * 64 + lane];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
+        }
+      }
+      uint4 p[CT][2];
+      int lim[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
+      if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, ks * a.scale, vs, lim, h4, p);
+      else st.template softmax<true>(s, ks * a.scale, vs, lim, h4, p);
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 x = lv[buf][(d * 2 + u) * 64 + lane];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) st.o[c][d] = mfma<DT>(x, p[c][u], st.o[c][d]);
+        }
+    }
+    ks = nks;
+    vs = nvs;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const float L = st.sum(c);
+    const int r = wrow + 16 * c + (lane & 15);
+    if (r >= rows) continue;
+    const float unit = st.unit();
+    if (a.splits == 1) {
+      const int tok = r / a.G, hq = h * a.G + r % a.G;
+      const float inv = L == 0.0f ? 0.0f : unit / L;
+      uint16_t* o = a.out + b * a.sob + hq * a.soh + tok * a.sot + 4 * h4;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) store4<DT>(o + 16 * d, st.o[c][d] * inv, a.ovec);
+    } else {
+      const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f*>(a.part_o + at * D + 16 * d + 4 * h4) = st.o[c][d] * unit;
+      if (h4 == 0) {
+        a.part_ml[2 * at] = st.m[c];
+        a.part_ml[2 * at + 1] = L;
+      }
+    }
+  }
+}
+
+// ---- joining the splits ---------------------------------------------------------------------------------
+// D / 4 lanes a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A split without a page for the row
+// has m = LOWEST and l = 0.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
+  constexpr int LPR = D / 4;
+  const long long all_rows = (long long)a.B * a.c.kv_heads * a.n * a.G;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (row >= all_rows) return;
+  const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(row / per), r = (int)(row % per), b = bh / H, h = bh % H;
+  const int nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
+  const int tok = r / a.G;
+  if (tok >= nv) return;
+  float M = LOWEST;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * all_rows + row)]);
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float L = 0.0f;
+  const int d = threadIdx.x % LPR * 4;
+  for (int s = 0; s < a.splits; ++s) {
+    const long long at = s * all_rows + row;
+    const float f = exp2f(a.part_ml[2 * at] - M);
+    L += a.part_ml[2 * at + 1] * f;
+    o += *reinterpret_cast<const v4f*>(a.part_o + at * D + d) * f;
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  store4<DT>(a.out + b * a.sob + (h * a.G + r % a.G) * a.soh + tok * a.sot + d, o * inv, a.ovec);
+}
+
+// How a call is cut: which kernel, row tiles of a (sequence, kv head), and splits of the keys.
+struct Cut {
+  int ct, nw;   // nw = 0: the few-rows kernel
+  int tiles, splits;
+};
+constexpr int CUS = 256;
+
+Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
+  Cut k{};
+  const long long rows = (long long)n * (Hq / c.kv_heads), heads = (long long)B * c.kv_heads;
+  const int pages = cdiv(most_tokens > 0 ? most_tokens : 1, KV_PAGE);
+  long long target;  // workgroups wanted
+  int least;         // pages a split has at least
+  if (rows <= 32) {
+    k.ct = rows <= 16 ? 1 : 2;
+    k.nw = 0;
+    target = 4 * CUS;
+    least = 4;
+  } else {
+    k.ct = 2;
+    k.nw = 4;
+    target = 2 * CUS;
+    least = 8;
+  }
+  const int per = 16 * k.ct * (k.nw ? k.nw : 1);
+  k.tiles = (int)((rows + per - 1) / per);
+  const long long wgs = heads * k.tiles;
+  long long s = wgs ? target / wgs : 1;
+  s = s < 1 ? 1 : s;
+  const int most = pages / least < 1 ? 1 : pages / least;
+  k.splits = (int)(s > most ? most : s);
+  return k;
+}
+
+long long part_floats(const ress_kv_cache& c, int B, int Hq, int n, const Cut& k) {
+  return k.splits == 1 ? 0 : (long long)k.splits * B * Hq * n * (c.head_dim + 2);
+}
+
+template <int DT, int CODES, int D>
+int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
+  const long long heads = (long long)a.B * a.c.kv_heads;
+  if (k.nw == 0) {
+    const long long g = heads * k.tiles * k.splits;
+    RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
+    if (k.ct == 1)
+      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 1>), dim3((unsigned)g), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 2>), dim3((unsigned)g), dim3(256), 0, stream, a);
+    RESS_LAUNCHED("k_cache_attn_few");
+  } else {
+    const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
+    RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
+    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, 2, 4>), dim3((unsigned)g), dim3(256), 0, stream, a);
+    RESS_LAUNCHED("k_cache_attn_rows");
+  }
+  if (k.splits > 1) {
+    const long long rows = heads * a.n * a.G, per = 256 / (D / 4);
+    hipLaunchKernelGGL((k_cache_attn_join<DT, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+    RESS_LAUNCHED("k_cache_attn_join");
+  }
+  return 0;
+}
+
+}  // namespace
+
+RESS_API long long ress_kv_attend_workspace_size(const ress_kv_cache* cache, int B, int Hq, int n, int most_tokens) {
+  if (!cache || cache->kv_heads <= 0 || B < 0 || n < 0 || Hq <= 0 || Hq % cache->kv_heads) return -1;
+  return 4 * part_floats(*cache, B, Hq, n, cut(*cache, B, Hq, n, most_tokens));
+}
+
+RESS_API int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long sqB, long long sqH, long long sqT,
+                            int B, int Hq, int n, const int* slots, const int* new_lens, int causal, float sm_scale,
+                            int most_tokens, void* out, long long soB, long long soH, long long soT, void* workspace,
+                            long long workspace_bytes, hipStream_t stream) {
+  if (int rc = ress_kv_check(cache, B, "ress_kv_attend")) return rc;
+  RESS_REQUIRE(Hq > 0 && Hq % cache->kv_heads == 0, "ress_kv_attend: %d query heads are no multiple of the cache's %d",
+               Hq, cache->kv_heads);
+  RESS_REQUIRE(n >= 0 && (long long)B * Hq * n < (1ll << 31), "ress_kv_attend: bad row count");
+  RESS_REQUIRE(sm_scale > 0.0f && sm_scale < __builtin_huge_valf(), "ress_kv_attend: the scale must be positive and finite");
+  if (B == 0 || n == 0) return 0;
+  RESS_REQUIRE(q && out, "ress_kv_attend: null queries or output");
+  const Cut k = cut(*cache, B, Hq, n, most_tokens);
+  const long long need = part_floats(*cache, B, Hq, n, k);
+  RESS_REQUIRE(workspace_bytes >= 4 * need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
+               "ress_kv_attend: the workspace needs %lld bytes, 16-byte aligned", 4 * need);
+  AttendArgs a{};
+  a.c = *cache;
+  a.q = (const uint16_t*)q; a.out = (uint16_t*)out;
+  a.sqb = sqB; a.sqh = sqH; a.sqt = sqT; a.sob = soB; a.soh = soH; a.sot = soT;
+  a.B = B; a.Hq = Hq; a.n = n; a.G = Hq / cache->kv_heads;
+  a.slots = slots; a.new_lens = new_lens; a.causal = causal ? 1 : 0;
+  a.scale = sm_scale * 1.4426950408889634f;
+  a.splits = k.splits; a.tiles = k.tiles;
+  a.part_o = (float*)workspace;
+  a.part_ml = need ? a.part_o + (long long)k.splits * B * Hq * n * cache->head_dim : nullptr;
+  a.qvec = (uintptr_t)q % 16 == 0 && sqB % 8 == 0 && sqH % 8 == 0 && sqT % 8 == 0;
+  a.ovec = (uintptr_t)out % 8 == 0 && soB % 4 == 0 && soH % 4 == 0 && soT % 4 == 0;
+  const bool f16 = a.c.dtype == KV_F16, fp8 = a.c.codes == KV_FP8;
+  if (a.c.head_dim == 64) {
+    if (f16) return fp8 ? launch<KV_F16, KV_FP8, 64>(a, k, stream) : launch<KV_F16, KV_I8, 64>(a, k, stream);
+    return fp8 ? launch<KV_BF16, KV_FP8, 64>(a, k, stream) : launch<KV_BF16, KV_I8, 64>(a, k, stream);
+  }
+  if (f16) return fp8 ? launch<KV_F16, KV_FP8, 128>(a, k, stream) : launch<KV_F16, KV_I8, 128>(a, k, stream);
+  return fp8 ? launch<KV_BF16, KV_FP8, 128>(a, k, stream) : launch<KV_BF16, KV_I8, 128>(a, k, stream);
+}
