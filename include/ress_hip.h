@@ -344,6 +344,22 @@ int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long sqB, lon
                    int most_tokens, void* out, long long soB, long long soH, long long soT, void* workspace,
                    long long workspace_bytes, hipStream_t stream);
 
+/* ---- linear layer in 8-bit integers (int8_linear.hip) ---------------------- */
+/* Codes and scales of M rows of K 16-bit elements (dtype 1 bf16, 2 fp16; K a multiple of 16, row stride in
+ * elements, unit-stride elements): scale = a * fl(1/127), code = rne(x * min(127/a, FLT_MAX)) with a the row's
+ * largest magnitude; scale NaN and codes 0 where an element is not finite. Code rows (code_stride bytes, a multiple
+ * of 8) are filled with zeros from K to code_stride. No counterpart in the reference. */
+int ress_quantize_rows(const void* x, long long stride, int dtype, int M, int K, void* codes, long long code_stride,
+                       float* scale, hipStream_t stream);
+/* out (M,N) = act((s_m sum_k c_mk w_nk) * w_scale_n + bias_n) in x's type, c and s being the codes and scales of x's
+ * rows as above, w int8 (N,K) contiguous, 16-byte aligned. bias: f32 (N) or null. act: 0 none, 1 gelu (erf). workspace:
+ * ress_int8_linear_workspace_size bytes, 16-byte aligned (may be 0 bytes). No counterpart in the reference, whose
+ * linear layers are torch's. */
+long long ress_int8_linear_workspace_size(int M, int K, int N);
+int ress_int8_linear(const void* x, long long stride, int dtype, int M, int K, int N, const void* w,
+                     const float* w_scale, const float* bias, int act, void* out, long long out_stride,
+                     void* workspace, long long workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

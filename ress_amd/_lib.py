@@ -34,6 +34,8 @@ _SIGS = {
     "ress_meansim_block_map": "ppp" + "iiii" + "llllll" + "ppi" + "ppppppppp" + "pl" + "s",
     "ress_qk_norm_rope": "piii" + "pppp" + "f" + "pf" + "ppp" + "s",
     "ress_bf16_selfcheck": "Il" + "p" + "s",
+    "ress_quantize_rows": "pliiiplp" + "s",
+    "ress_int8_linear": "pliiii" + "pppi" + "plpl" + "s",
     "ress_kv_append": "p" + "plll" * 3 + "iii" + "ppii" + "ppp" + "s",
     "ress_kv_read": "pii" + "pp" + "pp" + "s",
     "ress_kv_attend": "p" + "plll" + "iii" + "pp" + "ifi" + "plll" + "pl" + "s",
@@ -70,6 +72,8 @@ def lib():
         L.ress_restore_swap_workspace_size.argtypes = [ctypes.c_int] * 4
         L.ress_meansim_workspace_size.restype = ctypes.c_longlong
         L.ress_meansim_workspace_size.argtypes = [ctypes.c_int] * 4
+        L.ress_int8_linear_workspace_size.restype = ctypes.c_longlong
+        L.ress_int8_linear_workspace_size.argtypes = [ctypes.c_int] * 3
         L.ress_kv_attend_workspace_size.restype = ctypes.c_longlong
         L.ress_kv_attend_workspace_size.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
         L.ress_noalloc_scratch_bytes.restype = ctypes.c_longlong
@@ -111,6 +115,16 @@ def call(name, *args):
         raise RuntimeError(f"{name} failed ({rc}): {msg}")
 
 
+def call_on(device, name, *args):
+    """`call` on the current stream of `device` (an indexed torch.device), which is made current for the
+    call where it is not."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            call(name, *args, stream_handle(device))
+    else:
+        call(name, *args, stream_handle(device))
+
+
 def last_error():
     return lib().ress_last_error().decode(errors="replace")
 
@@ -119,4 +133,5 @@ def exported_symbols():
     return list(_SIGS) + ["ress_last_error", "ress_abi_version", "ress_qattn_workspace_size",
                           "ress_attn_sched_bytes", "ress_restore_swap_workspace_size", "ress_meansim_workspace_size",
                           "ress_noalloc_scratch_bytes", "ress_kv_attend_workspace_size",
+                          "ress_int8_linear_workspace_size",
                           "ress_noalloc_status_address"]

@@ -1,0 +1,129 @@
+"""Linear layers in 8-bit integers: weights held as int8 codes with a scale for each output channel,
+activations quantised per token on the way in, products summed exactly in int32.
+
+    quantize_linears(model)          # every suitable nn.Linear becomes an Int8Linear
+    y = int8_linear(x, codes, scale, bias, act="gelu")
+
+Half the bytes of 16-bit weights, which is what a call of a few tokens costs, and the matrix cores' 8-bit
+rate for many. The reference's layers are torch's 16-bit ones; nothing here is used unless asked for.
+"""
+
+import torch
+import torch.nn as nn
+
+from ress_amd import _lib
+
+DTYPES = {torch.bfloat16: 1, torch.float16: 2}
+ACTS = {None: 0, "gelu": 1}
+MOST_FEATURES = 131072  # |sum| <= 127^2 * 131072 < 2^31
+
+
+def _rows(x, name):
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise RuntimeError(f"{name} must be a device tensor (the 8-bit product runs only on the GPU)")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{name} must be bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] % 16 or not 0 < x.shape[-1] <= MOST_FEATURES:
+        raise ValueError(f"{name} must have a last dim that is a multiple of 16 up to {MOST_FEATURES}, got {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires grad: the 8-bit product has no backward pass (use torch.no_grad())")
+    rows = x.reshape(-1, x.shape[-1])
+    if rows.stride(1) != 1 or (len(rows) > 1 and rows.stride(0) < rows.shape[1]):
+        rows = rows.contiguous()
+    return rows
+
+
+def quantize_tokens(x):
+    """(codes int8, scale float32) of x (..., K), bfloat16 or float16, a scale for each row: code =
+    round(x * 127 / max|x|) (ties to even), scale = max|x| / 127. A row with an element that is not finite has
+    scale NaN and codes 0."""
+    rows = _rows(x, "x")
+    codes = torch.empty(rows.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(len(rows), device=x.device)
+    _lib.call_on(x.device, "ress_quantize_rows", _lib.ptr(rows), rows.stride(0), DTYPES[x.dtype], len(rows),
+                 rows.shape[1], _lib.ptr(codes), rows.shape[1], _lib.ptr(scale))
+    return codes.reshape(x.shape), scale.reshape(x.shape[:-1])
+
+
+def quantize_weight(weight):
+    """(codes int8 (N, K), scale float32 (N,)) of a weight matrix of any floating type, once per model."""
+    if weight.dim() != 2 or weight.shape[1] % 16 or not 0 < weight.shape[1] <= MOST_FEATURES:
+        raise ValueError(f"weight must be (N, K) with K a multiple of 16 up to {MOST_FEATURES}, got {tuple(weight.shape)}")
+    w = weight.detach().float()
+    if not torch.isfinite(w).all():
+        raise ValueError("weight has values that are not finite")
+    scale = w.abs().amax(1) / 127.0
+    safe = torch.where(scale > 0, scale, torch.ones_like(scale))
+    return torch.round(w / safe[:, None]).clamp(-127, 127).to(torch.int8).contiguous(), scale
+
+
+def int8_linear(x, w_codes, w_scale, bias=None, act=None):
+    """act(x W^T + bias) in x's type, (..., N): x (..., K) bfloat16 or float16, quantised per token as by
+    quantize_tokens; W = w_codes (N, K) int8 * w_scale (N,) float32; bias (N,) float32; act None or "gelu" (erf)."""
+    rows = _rows(x, "x")
+    M, K = rows.shape
+    if w_codes.dim() != 2 or w_codes.shape[1] != K or w_codes.dtype != torch.int8 or not w_codes.is_contiguous():
+        raise ValueError(f"w_codes must be contiguous int8 (N, {K}), got {tuple(w_codes.shape)} {w_codes.dtype}")
+    N = w_codes.shape[0]
+    for name, t in (("w_scale", w_scale), ("bias", bias)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (N,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 ({N},), got {tuple(t.shape)} {t.dtype}")
+    if any(t is not None and t.device != x.device for t in (w_codes, w_scale, bias)):
+        raise ValueError(f"the weights are not on {x.device}")
+    if act not in ACTS:
+        raise ValueError(f"act must be one of {tuple(ACTS)}, got {act!r}")
+    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    size = _lib.lib().ress_int8_linear_workspace_size(M, K, N)
+    work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    P = _lib.ptr
+    _lib.call_on(x.device, "ress_int8_linear", P(rows), rows.stride(0), DTYPES[x.dtype], M, K, N, P(w_codes), P(w_scale),
+                 P(bias), ACTS[act], P(out), N, P(work), size)
+    return out
+
+
+class Int8Linear(nn.Module):
+    """An nn.Linear's place-holder with 8-bit weights (buffers, not parameters)."""
+
+    def __init__(self, linear):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        self.dtype = linear.weight.dtype
+        codes, scale = quantize_weight(linear.weight)
+        self.register_buffer("codes", codes)
+        self.register_buffer("scale", scale)
+        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float().contiguous())
+
+    def _apply(self, fn, recurse=True):
+        # a cast of the model to 16 bits must not round the scales and the bias, which are fp32
+        kept = {n: getattr(self, n) for n in ("scale", "bias") if getattr(self, n) is not None}
+        super()._apply(fn, recurse)
+        for n, t in kept.items():
+            setattr(self, n, t.to(self.codes.device))
+        return self
+
+    @property
+    def weight(self):
+        """The weights that the codes stand for, in the original layer's type."""
+        return (self.codes.float() * self.scale[:, None]).to(self.dtype)
+
+    def forward(self, x, act=None):
+        return int8_linear(x, self.codes, self.scale, self.bias, act)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def quantize_linears(model, keep=lambda name, linear: False):
+    """Replaces every nn.Linear of the model by an Int8Linear, in place, but for those whose in_features are
+    not a multiple of 16 and those that keep(name, linear) names. Returns the names replaced."""
+    done = []
+    for name, module in list(model.named_modules()):
+        for child, linear in list(module.named_children()):
+            full = f"{name}.{child}" if name else child
+            if (type(linear) is nn.Linear and linear.in_features % 16 == 0 and linear.in_features <= MOST_FEATURES
+                    and not keep(full, linear)):
+                setattr(module, child, Int8Linear(linear))
+                done.append(full)
+    return done

@@ -322,11 +322,7 @@ class PagedKVCache:
         return torch.tensor(got, dtype=torch.int32, device=self.device), got
 
     def _call(self, name, *args):
-        if torch.cuda.current_device() != self.device.index:
-            with torch.cuda.device(self.device):
-                _lib.call(name, *args, _lib.stream_handle(self.device))
-        else:
-            _lib.call(name, *args, _lib.stream_handle(self.device))
+        _lib.call_on(self.device, name, *args)
 
     # ---- the operators ------------------------------------------------------
     def append(self, k, v, pos=None, rope=None, q=None, slots=None, new_lens=None):
