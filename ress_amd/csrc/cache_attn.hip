@@ -5,15 +5,18 @@
 // O^T += V^T P^T (A = values of 16 dims), a lane holds for ITS query four keys of each 16, which is what
 // the second product takes as its B operand once the keys of a value row are stored in that order (v_token): P
 // never leaves the registers. The codes are widened to 16 bits exactly; the scales of a page multiply
-// the scores (folded into the exponent's multiply-add) and P (before it is rounded to 16 bits), so that
-// nothing but Q, P and the output is rounded to 16 bits. Max, sum and output accumulate in fp32.
+// the scores (folded into the exponent's multiply-add) and P or P V (below), so that nothing but P and the
+// output is rounded to 16 bits. Max, sum and output accumulate in fp32.
 //
 // Running max. m starts at the lowest finite value and moves only when a score of the wave lies more than
 // LAZY = 8 (in log2) above its row's m: P is then at most 2^8, sums are unaffected, and most pages need
 // neither the exchange between a row's four lanes nor a pass over the accumulators.
 //
-// fp16. P * v_scale is formed relative to the largest v_scale met so far (R, uniform in the wave; the
-// accumulator is rescaled when it grows), times 2^7, to keep it inside fp16's range for any v_scale.
+// v_scale. In bf16 it enters as an addend of the exponent (PageScale), relative to a power of two, so it costs no
+// multiplication per element. fp16 has no exponents to spare for that: there a page's P V is formed by itself and
+// added times v_scale in fp32, one multiply-add per output element and page.
+// The sum of P is a product with ones on the matrix cores, of the rounded P, so numerator and denominator carry the
+// same roundings.
 //
 // Masked places (past the sequence's end, after the row's own token) are selected away after every
 // multiplication, so a NaN scale or tail element there reaches no row that does not see its page.
@@ -27,7 +30,6 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr float LOWEST = -0x1.fffffep127f;
 constexpr float LAZY = 8.0f;
-constexpr float F16_LIFT = 128.0f;  // 2^7; P <= 2^8 keeps P * lift below fp16's 65504
 
 struct AttendArgs {
   ress_kv_cache c;
@@ -38,7 +40,8 @@ struct AttendArgs {
   const int *slots, *new_lens;
   int causal;
   float scale;       // sm_scale * log2(e)
-  int splits, tiles; // splits of the keys; row tiles of a (sequence, kv head)
+  int splits, per;   // the keys are cut every `per` pages, into at most `splits` parts (the last takes the rest)
+  int tiles;         // row tiles of a (sequence, kv head)
   float *part_o, *part_ml;  // [splits][B * kv_heads * n * G][D], [..][2]
   bool qvec, ovec;
 };
@@ -96,14 +99,35 @@ struct TailScale {
   }
 };
 
+// bf16: a page's v_scale relative to R = 2^eR, a power of two at least as large as any v_scale met so far (exact to
+// rescale by, so a row's bits do not hang on the pages that only its neighbours see): P comes out of the
+// exponential already multiplied by v_scale / R, and its sum is divided by that again. At most 2^-60 of R is lost to
+// the clamp (a page of zeros has v_scale 0). fp16: P is lifted by 2^7 (it is at most 2^LAZY, so below 2^15), which
+// the quotient of sums takes out again.
+template <int DT>
+struct PageScale {
+  float lift;  // bf16: log2(v_scale / R); fp16: 7
+  float down;  // bf16: 2^-lift; fp16: 1
+  __device__ __forceinline__ PageScale(float vs, int eR) {
+    if constexpr (DT == KV_F16) {
+      lift = 7.0f;
+      down = 1.0f;
+    } else {
+      const float q = __builtin_amdgcn_logf(ldexpf(vs, -eR));  // log2
+      lift = q < -60.0f ? -60.0f : q;                          // NaN stays
+      down = __builtin_amdgcn_exp2f(-lift);
+    }
+  }
+};
+
 // A lane's state for CT tiles of 16 queries: query 16 ct + (lane & 15), shared by the four lanes of a column.
 template <int DT, int D, int CT>
 struct Rows {
-  v4f o[CT][D / 16];  // dims 16 dt + 4 (lane >> 4) + r
-  float m[CT], l[CT]; // l: this lane's keys alone
-  float R;            // fp16: the v_scale that o is relative to
+  v4f o[CT][D / 16];   // dims 16 dt + 4 (lane >> 4) + r; bf16: relative to 2^eR
+  float m[CT], l[CT];
+  int eR;
   __device__ __forceinline__ void clear() {
-    R = 0.0f;
+    eR = -120;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       m[c] = LOWEST;
@@ -113,22 +137,24 @@ struct Rows {
     }
   }
 
-  // Scores s of 64 keys -> P as the second product's B operand p. cs = k_scale * scale, vs = v_scale;
-  // MASK: query c sees the tile's keys below lim[c].
+  // Scores s of 64 keys -> P as the second product's B operand p, and in fp16 what its product with the codes is
+  // to be multiplied by. cs = k_scale * sm_scale * log2(e). MASK: query c sees the tile's keys below lim[c].
   template <bool MASK>
   __device__ __forceinline__ void softmax(const v4f (&s)[CT][4], float cs, float vs, const int (&lim)[CT], int h4,
-                                          uint4 (&p)[CT][2]) {
+                                          uint4 (&p)[CT][2], float (&pv)[CT]) {
     float top[CT];
+    int below[CT];  // the lane's keys 16 k + 4 h4 + r that are seen: 16 k + r < below
     bool up = false;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
+      below[c] = lim[c] - 4 * h4;
       float t = LOWEST;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float x = s[c][k][r];
-          if constexpr (MASK) x = 16 * k + 4 * h4 + r < lim[c] ? x : -__builtin_huge_valf();
+          if constexpr (MASK) x = 16 * k + r < below[c] ? x : -__builtin_huge_valf();
           t = fmaxf(t, x);
         }
       if constexpr (MASK) top[c] = t == LOWEST ? LOWEST : t * cs;
@@ -149,47 +175,61 @@ struct Rows {
         for (int d = 0; d < D / 16; ++d) o[c][d] *= a;
       }
     }
-    float f = vs;
-    if constexpr (DT == KV_F16) {
-      if (vs > R) {
-        const float a = R / vs;
-        R = vs;
+    if (DT == KV_BF16 && vs > ldexpf(1.0f, eR)) {
+      const int e = (int)((__float_as_uint(vs) + 0x7fffffu) >> 23) - 127;  // vs <= 2^e
+      const float a = ldexpf(1.0f, eR - e);
+      eR = e;
 #pragma unroll
-        for (int c = 0; c < CT; ++c)
+      for (int c = 0; c < CT; ++c)
 #pragma unroll
-          for (int d = 0; d < D / 16; ++d) o[c][d] *= a;
-      }
-      f = R > 0.0f ? vs / R * F16_LIFT : vs;  // vs is 0 or NaN where R is 0
+        for (int d = 0; d < D / 16; ++d) o[c][d] *= a;
     }
+    const PageScale<DT> ps(vs, eR);
+    const uint4 ones = DT == KV_F16 ? make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u)
+                                    : make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       uint32_t w[8];
+      const float off = ps.lift - m[c];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float e[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const bool sees = !MASK || 16 * k + 4 * h4 + r < lim[c];
-          float x = __builtin_amdgcn_exp2f(fmaf(s[c][k][r], cs, -m[c]));
-          if constexpr (MASK) x = sees ? x : 0.0f;
-          l[c] += x;
-          e[r] = x * f;
-          if constexpr (MASK) e[r] = sees ? e[r] : 0.0f;
+          e[r] = __builtin_amdgcn_exp2f(fmaf(s[c][k][r], cs, off));
+          if constexpr (MASK) e[r] = 16 * k + r < below[c] ? e[r] : 0.0f;
         }
         w[2 * k] = pack2<DT>(e[0], e[1]);
         w[2 * k + 1] = pack2<DT>(e[2], e[3]);
       }
       p[c][0] = make_uint4(w[0], w[1], w[2], w[3]);
       p[c][1] = make_uint4(w[4], w[5], w[6], w[7]);
+      // the row's sum over the page, in every lane of its column: a product with ones
+      v4f t = {0.0f, 0.0f, 0.0f, 0.0f};
+      t = mfma<DT>(ones, p[c][0], t);
+      t = mfma<DT>(ones, p[c][1], t);
+      const bool none = MASK && lim[c] <= 0;  // 0 * NaN would not be 0
+      l[c] = none ? l[c] : fmaf(t[0], ps.down, l[c]);
+      pv[c] = none ? 0.0f : vs;
     }
   }
 
-  // The factor that takes o to its own units, and the row's whole sum
-  __device__ __forceinline__ float unit() const { return DT == KV_F16 ? R * (1.0f / F16_LIFT) : 1.0f; }
-  __device__ __forceinline__ float sum(int c) const {
-    float t = l[c] + xor_lane_f<16>(l[c]);
-    return t + xor_lane_f<32>(t);
+  // o of dims 16 d.. += P V, the page's values as the A operands a (32 keys each)
+  __device__ __forceinline__ void add(int d, const uint4& a0, const uint4& a1, const uint4 (&p)[CT][2], const float (&pv)[CT]) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      if constexpr (DT == KV_BF16) {
+        o[c][d] = mfma<DT>(a1, p[c][1], mfma<DT>(a0, p[c][0], o[c][d]));
+      } else {
+        const v4f t = mfma<DT>(a1, p[c][1], mfma<DT>(a0, p[c][0], v4f{0.0f, 0.0f, 0.0f, 0.0f}));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[c][d][r] = fmaf(t[r], pv[c], o[c][d][r]);
+      }
+    }
   }
+
+  // The factor that takes o to its own units
+  __device__ __forceinline__ float unit() const { return DT == KV_F16 ? 1.0f : ldexpf(1.0f, eR); }
 };
 
 // Row r of a (sequence, kv head): token r / G, query head h G + r % G.
@@ -260,8 +300,8 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
   load_q<D, CT>(a, b, h, row0, rows, lane, qv);
 
   const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
-  const int per = cdiv(pages, a.splits);
-  const int lo = min(pages, split * per), hi = min(pages, lo + per);
+  const int lo = min(pages, split * a.per), hi = split == a.splits - 1 ? pages : min(pages, lo + a.per);
+  if (split && lo >= pages) return;  // the join goes by the same count
   int limit[CT];  // tokens that the lane's query sees
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
@@ -299,14 +339,11 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
     int lim[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
-    if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p);
-    else st.template softmax<true>(s, cs, v, lim, h4, p);
+    float pv[CT];
+    if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p, pv);
+    else st.template softmax<true>(s, cs, v, lim, h4, p, pv);
 #pragma unroll
-    for (int d = 0; d < VU; ++d)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) st.o[c][d] = mfma<DT>(va[d][u], p[c][u], st.o[c][d]);
+    for (int d = 0; d < VU; ++d) st.add(d, va[d][0], va[d][1], p, pv);
   };
 
   const int last = min(min(hi, full), cdiv(seen_by_any, KV_PAGE));
@@ -364,10 +401,9 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
   // join the four waves
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const float t = st.sum(c);
     if (lane < 16) {
       sm[w][c][lane] = st.m[c];
-      sl[w][c][lane] = t;
+      sl[w][c][lane] = st.l[c];
     }
   }
   __syncthreads();
@@ -422,7 +458,7 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
 // NW waves of 16 CT rows each share a page, widened into LDS in the order in which the operands are read (1 KB
 // a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page.
 template <int DT, int CODES, int D, int CT, int NW>
-__global__ __launch_bounds__(64 * NW) void k_cache_attn_rows(AttendArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(AttendArgs a) {
   constexpr int THREADS = 64 * NW;
   constexpr int PIECES = KV_PAGE * D / 16;       // 16-code pieces of a page's keys (and of its values)
   constexpr int PT = PIECES / THREADS;           // a thread's pieces of each
@@ -444,32 +480,32 @@ __global__ __launch_bounds__(64 * NW) void k_cache_attn_rows(AttendArgs a) {
   load_q<D, CT>(a, b, h, wrow, rows, lane, qv);
 
   const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
-  const int per = cdiv(pages, a.splits);
   const int before = hd.len - hd.nv;  // causal: row of token i sees before + i + 1 tokens
   auto sees = [&](int r) { return a.causal ? max(0, before + r / a.G + 1) : hd.len; };
-  const int lo = min(pages, split * per);
-  const int hi = min(min(pages, lo + per), cdiv(sees(min(row0 + 16 * CT * NW, rows) - 1), KV_PAGE));
+  const int lo = min(pages, split * a.per);
+  if (split && lo >= pages) return;  // the join goes by the same count
+  const int hi = min(split == a.splits - 1 ? pages : min(pages, lo + a.per), cdiv(sees(min(row0 + 16 * CT * NW, rows) - 1), KV_PAGE));
   int limit[CT];
 #pragma unroll
   for (int c = 0; c < CT; ++c) limit[c] = sees(wrow + 16 * c + (lane & 15));
-  const int seen_by_all = sees(wrow), seen_by_any = wrow < rows ? sees(min(wrow + 16 * CT, rows) - 1) : 0;
+  const int seen_by_any = wrow < rows ? sees(min(wrow + 16 * CT, rows) - 1) : 0;
 
   Rows<DT, D, CT> st;
   st.clear();
   const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
   uint4 kw[PT], vw[PT];
   float ks = 0.0f, vs = 0.0f, ks1, vs1;
+  int bad = 0;
   auto load = [&](int pg) {
     int pid = pg < a.c.max_pages ? table[pg] : -1;
     const bool ok = pid >= 0 && pid < a.c.n_pages;
-    if (!ok && t == 0) atomicOr(a.c.status, KV_ST_PAGE);
+    bad |= !ok;
     pid = ok ? pid : 0;
-    const uint8_t* kp = hd.kc + pid * hd.stride + t * 16;
-    const uint8_t* vp = hd.vc + pid * hd.stride + t * 16;
+    const uint8_t *kp = hd.kc + pid * hd.stride, *vp = hd.vc + pid * hd.stride;
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
-      kw[i] = *reinterpret_cast<const uint4*>(kp + i * THREADS * 16);
-      vw[i] = *reinterpret_cast<const uint4*>(vp + i * THREADS * 16);
+      kw[i] = at_u32(reinterpret_cast<const uint4*>(kp), (unsigned)(t + i * THREADS));
+      vw[i] = at_u32(reinterpret_cast<const uint4*>(vp), (unsigned)(t + i * THREADS));
     }
     const long long at = (long long)pid * H + h;
     ks1 = ok ? a.c.k_scale[at] : 0.0f;
@@ -508,67 +544,69 @@ __global__ __launch_bounds__(64 * NW) void k_cache_attn_rows(AttendArgs a) {
       lv[buf][sv + 64] = tail_v8<DT>(reinterpret_cast<const uint4*>(hd.tv)[2 * p + 1], ts.down, place + 8, left);
     }
   };
-  auto fetch = [&](int pg) {  // start page pg's way into a stage
-    if (pg < full) load(pg);
+  // LDS writes done, then the barrier; unlike __syncthreads() it leaves the loads of later pages in flight
+  auto barrier = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   };
-  auto put = [&](int pg, int buf) {
-    if (pg < full) {
-      stage(buf);
-    } else {
-      const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
-      stage_tail(buf, ts);
-      ks1 = 1.0f;
-      vs1 = ts.vs;
+  auto compute = [&](auto mask_tag, int buf, int pg, float cs, float v) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    v4f s[CT][4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        const uint4 x = lk[buf][(k * (D / 32) + e) * 64 + lane];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
+      }
     }
+    uint4 p[CT][2];
+    int lim[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
+    float pv[CT];
+    st.template softmax<MASK>(s, cs, v, lim, h4, p, pv);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) st.add(d, lv[buf][d * 128 + lane], lv[buf][d * 128 + 64 + lane], p, pv);
   };
-  if (lo < hi) {
-    fetch(lo);
-    put(lo, 0);
+  // pages lo..open-1 are seen whole by every row of the workgroup, open..last-1 by some in part (causal)
+  const int last = min(hi, full), open = max(lo, min(last, sees(row0) / KV_PAGE));
+  if (lo < last) {
+    load(lo);
+    stage(0);
     ks = ks1;
     vs = vs1;
-    if (lo + 1 < hi) fetch(lo + 1);
-    __syncthreads();
+    if (lo + 1 < last) load(lo + 1);
+    barrier();
   }
-  for (int pg = lo; pg < hi; ++pg) {
+  auto step = [&](auto mask_tag, int pg) {
     const int buf = (pg - lo) & 1;
-    if (pg + 1 < hi) put(pg + 1, buf ^ 1);  // read last before the barrier that ended the step before
-    const float nks = ks1, nvs = vs1;
-    if (pg + 2 < hi) fetch(pg + 2);
-    if (pg * KV_PAGE < seen_by_any) {
-      v4f s[CT][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-#pragma unroll
-        for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) {
-          const uint4 x = lk[buf][(k * (D / 32) + e) * 64 + lane];
-#pragma unroll
-          for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
-        }
-      }
-      uint4 p[CT][2];
-      int lim[CT];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
-      if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, ks * a.scale, vs, lim, h4, p);
-      else st.template softmax<true>(s, ks * a.scale, vs, lim, h4, p);
-#pragma unroll
-      for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4 x = lv[buf][(d * 2 + u) * 64 + lane];
-#pragma unroll
-          for (int c = 0; c < CT; ++c) st.o[c][d] = mfma<DT>(x, p[c][u], st.o[c][d]);
-        }
+    const float cs = ks * a.scale, v = vs;
+    if (pg + 1 < last) {
+      stage(buf ^ 1);  // read last before the barrier that ended the step before
+      ks = ks1;
+      vs = vs1;
+      if (pg + 2 < last) load(pg + 2);
     }
-    ks = nks;
-    vs = nvs;
-    __syncthreads();
+    if (!decltype(mask_tag)::value || pg * KV_PAGE < seen_by_any) compute(mask_tag, buf, pg, cs, v);
+    barrier();
+  };
+  for (int pg = lo; pg < open; ++pg) step(std::false_type{}, pg);
+  for (int pg = open; pg < last; ++pg) step(std::true_type{}, pg);
+  if (full < hi) {  // the unfinished page
+    const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
+    stage_tail(0, ts);
+    barrier();
+    if (full * KV_PAGE < seen_by_any) compute(std::true_type{}, 0, full, a.scale, ts.vs);
   }
+  if (bad && t == 0) atomicOr(a.c.status, KV_ST_PAGE);
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
-    const float L = st.sum(c);
+    const float L = st.l[c];
     const int r = wrow + 16 * c + (lane & 15);
     if (r >= rows) continue;
     const float unit = st.unit();
@@ -591,39 +629,88 @@ __global__ __launch_bounds__(64 * NW) void k_cache_attn_rows(AttendArgs a) {
 }
 
 // ---- joining the splits ---------------------------------------------------------------------------------
-// D / 4 lanes a row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A split without a page for the row
-// has m = LOWEST and l = 0.
-template <int DT, int D>
+// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. D / 4 lanes hold a row; SG such groups share its parts
+// (SG = 1 where there are rows enough to fill the chip, so that a wave reads whole rows; else all 256 threads one row).
+template <int DT, int D, int SG>
 __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
-  constexpr int LPR = D / 4;
+  constexpr int LPR = D / 4, RPW = 256 / (LPR * SG);
+  __shared__ float sm[SG][RPW], sl[SG][RPW];
+  __shared__ __align__(16) v4f so[SG][RPW * LPR];
   const long long all_rows = (long long)a.B * a.c.kv_heads * a.n * a.G;
-  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (row >= all_rows) return;
-  const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(row / per), r = (int)(row % per), b = bh / H, h = bh % H;
+  const int lane = threadIdx.x % LPR, g = threadIdx.x / LPR % SG, rw = threadIdx.x / (LPR * SG);
+  const long long row = (long long)blockIdx.x * RPW + rw;
+  const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(min(row, all_rows - 1) / per), r = (int)(row - (long long)bh * per);
+  const int b = bh / H, h = bh % H, tok = r / a.G;
   const int nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
-  const int tok = r / a.G;
-  if (tok >= nv) return;
-  float M = LOWEST;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.part_ml[2 * (s * all_rows + row)]);
+  const bool live = row < all_rows && tok < nv;
+  const int len = a.c.lens[a.slots ? a.slots[b] : b];
+  const int ns = min(a.splits, max(1, cdiv(cdiv(len, KV_PAGE), a.per)));
+  float M = LOWEST, L = 0.0f;
   v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-  float L = 0.0f;
-  const int d = threadIdx.x % LPR * 4;
-  for (int s = 0; s < a.splits; ++s) {
-    const long long at = s * all_rows + row;
-    const float f = exp2f(a.part_ml[2 * at] - M);
-    L += a.part_ml[2 * at + 1] * f;
-    o += *reinterpret_cast<const v4f*>(a.part_o + at * D + d) * f;
+  if (live) {
+    const float* ml = a.part_ml + 2 * row;
+    const float* po = a.part_o + row * D + lane * 4;
+    for (int s0 = g; s0 < ns; s0 += 4 * SG) {  // four parts at a time, their loads together
+      float m[4], l[4];
+      v4f v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * SG;
+        const bool in = s < ns;
+        m[i] = in ? ml[2 * s * all_rows] : LOWEST;
+        l[i] = in ? ml[2 * s * all_rows + 1] : 0.0f;
+        v[i] = in ? *reinterpret_cast<const v4f*>(po + s * all_rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+      const float t = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), M), f0 = exp2f(M - t);
+      L *= f0;
+      o *= f0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = exp2f(m[i] - t);
+        L += l[i] * f;
+        o += v[i] * f;
+      }
+      M = t;
+    }
   }
+  if constexpr (SG > 1) {
+    if (lane == 0) {
+      sm[g][rw] = M;
+      sl[g][rw] = L;
+    }
+    so[g][rw * LPR + lane] = o;
+    __syncthreads();
+    if (g) return;
+    float t = M;
+#pragma unroll
+    for (int i = 1; i < SG; ++i) t = fmaxf(t, sm[i][rw]);
+    const float f0 = exp2f(M - t);
+    L *= f0;
+    o *= f0;
+#pragma unroll
+    for (int i = 1; i < SG; ++i) {
+      const float f = exp2f(sm[i][rw] - t);
+      L += sl[i][rw] * f;
+      o += so[i][rw * LPR + lane] * f;
+    }
+  }
+  if (!live) return;
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  store4<DT>(a.out + b * a.sob + (h * a.G + r % a.G) * a.soh + tok * a.sot + d, o * inv, a.ovec);
+  store4<DT>(a.out + b * a.sob + (h * a.G + r % a.G) * a.soh + tok * a.sot + lane * 4, o * inv, a.ovec);
 }
 
 // How a call is cut: which kernel, row tiles of a (sequence, kv head), and splits of the keys.
 struct Cut {
   int ct, nw;   // nw = 0: the few-rows kernel
-  int tiles, splits;
+  int tiles, splits, per;
 };
 constexpr int CUS = 256;
+#ifndef RESS_FEW_TARGET
+#define RESS_FEW_TARGET 4
+#define RESS_FEW_LEAST 8
+#define RESS_ROWS_TARGET 4
+#define RESS_ROWS_LEAST 8
+#endif
 
 Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   Cut k{};
@@ -634,21 +721,22 @@ Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   if (rows <= 32) {
     k.ct = rows <= 16 ? 1 : 2;
     k.nw = 0;
-    target = 4 * CUS;
-    least = 4;
+    target = RESS_FEW_TARGET * CUS;
+    least = RESS_FEW_LEAST;
   } else {
     k.ct = 2;
     k.nw = 4;
-    target = 2 * CUS;
-    least = 8;
+    target = RESS_ROWS_TARGET * CUS;
+    least = RESS_ROWS_LEAST;
   }
-  const int per = 16 * k.ct * (k.nw ? k.nw : 1);
-  k.tiles = (int)((rows + per - 1) / per);
+  const int tile = 16 * k.ct * (k.nw ? k.nw : 1);
+  k.tiles = (int)((rows + tile - 1) / tile);
   const long long wgs = heads * k.tiles;
   long long s = wgs ? target / wgs : 1;
   s = s < 1 ? 1 : s;
-  const int most = pages / least < 1 ? 1 : pages / least;
-  k.splits = (int)(s > most ? most : s);
+  k.per = (int)((pages + s - 1) / s);
+  if (k.per < least) k.per = least;
+  k.splits = (pages + k.per - 1) / k.per;
   return k;
 }
 
@@ -675,7 +763,10 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
   }
   if (k.splits > 1) {
     const long long rows = heads * a.n * a.G, per = 256 / (D / 4);
-    hipLaunchKernelGGL((k_cache_attn_join<DT, D>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+    if (rows >= 4 * CUS * per)
+      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 1>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 256 / (D / 4)>), dim3((unsigned)rows), dim3(256), 0, stream, a);
     RESS_LAUNCHED("k_cache_attn_join");
   }
   return 0;
@@ -710,7 +801,7 @@ RESS_API int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long
   a.B = B; a.Hq = Hq; a.n = n; a.G = Hq / cache->kv_heads;
   a.slots = slots; a.new_lens = new_lens; a.causal = causal ? 1 : 0;
   a.scale = sm_scale * 1.4426950408889634f;
-  a.splits = k.splits; a.tiles = k.tiles;
+  a.splits = k.splits; a.per = k.per; a.tiles = k.tiles;
   a.part_o = (float*)workspace;
   a.part_ml = need ? a.part_o + (long long)k.splits * B * Hq * n * cache->head_dim : nullptr;
   a.qvec = (uintptr_t)q % 16 == 0 && sqB % 8 == 0 && sqH % 8 == 0 && sqT % 8 == 0;
