@@ -22,6 +22,28 @@
 // multiplication, so a NaN scale or tail element there reaches no row that does not see its page.
 #include "kvcache.h"
 
+#ifndef RESS_FEW_TARGET
+#define RESS_FEW_TARGET 4
+#endif
+#ifndef RESS_FEW_LEAST
+#define RESS_FEW_LEAST 8
+#endif
+#ifndef RESS_ROWS_NW
+#define RESS_ROWS_NW 4
+#endif
+#ifndef RESS_ROWS_LEAST
+#define RESS_ROWS_LEAST 8
+#endif
+#ifndef RESS_ROWS_OCC
+#define RESS_ROWS_OCC 4
+#endif
+#ifndef RESS_ROWS_OCC2
+#define RESS_ROWS_OCC2 2
+#endif
+#ifndef RESS_ROWS_CT
+#define RESS_ROWS_CT 2
+#endif
+
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -142,12 +164,10 @@ struct Rows {
   template <bool MASK>
   __device__ __forceinline__ void softmax(const v4f (&s)[CT][4], float cs, float vs, const int (&lim)[CT], int h4,
                                           uint4 (&p)[CT][2], float (&pv)[CT]) {
-    float top[CT];
     int below[CT];  // the lane's keys 16 k + 4 h4 + r that are seen: 16 k + r < below
-    bool up = false;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      below[c] = lim[c] - 4 * h4;
+    for (int c = 0; c < CT; ++c) below[c] = lim[c] - 4 * h4;
+    auto highest = [&](int c) {  // of the lane's scores of row c, times cs
       float t = LOWEST;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -157,14 +177,29 @@ struct Rows {
           if constexpr (MASK) x = 16 * k + r < below[c] ? x : -__builtin_huge_valf();
           t = fmaxf(t, x);
         }
-      if constexpr (MASK) top[c] = t == LOWEST ? LOWEST : t * cs;
-      else top[c] = t * cs;
-      up = up || top[c] > m[c] + LAZY;
+      return MASK && t == LOWEST ? LOWEST : t * cs;
+    };
+    // Whether a score lies more than LAZY above its row's m. Where m + LAZY is not negative only positive scores can,
+    // and they order as their bits do: integer maxima, which need no pass that quiets NaNs.
+    bool up = false, below0 = false;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      int t = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          int x = __float_as_int(s[c][k][r]);
+          if constexpr (MASK) x = 16 * k + r < below[c] ? x : 0;
+          t = max(t, x);
+        }
+      up = up || __int_as_float(t) * cs > m[c] + LAZY;
+      below0 = below0 || m[c] + LAZY < 0.0f;
     }
-    if (__any(up)) {
+    if (__any(up || below0)) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        float t = fmaxf(top[c], m[c]);
+        float t = fmaxf(highest(c), m[c]);
         t = fmaxf(t, xor_lane_f<16>(t));
         t = fmaxf(t, xor_lane_f<32>(t));
         t = t > m[c] + LAZY ? t : m[c];  // a row moves by its own scores, so its bits do not hang on its neighbours
@@ -458,13 +493,11 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
 // NW waves of 16 CT rows each share a page, widened into LDS in the order in which the operands are read (1 KB
 // a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page.
 template <int DT, int CODES, int D, int CT, int NW>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(AttendArgs a) {
-  constexpr int THREADS = 64 * NW;
-  constexpr int PIECES = KV_PAGE * D / 16;       // 16-code pieces of a page's keys (and of its values)
-  constexpr int PT = PIECES / THREADS;           // a thread's pieces of each
-  static_assert(PT >= 1 && PT * THREADS == PIECES, "every thread has whole pieces");
-  constexpr int OPS = KV_PAGE * D / 8 / 64;      // 1 KB operand blocks of the keys (and of the values)
-  __shared__ uint4 lk[2][OPS * 64], lv[2][OPS * 64];
+__global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) void k_cache_attn_rows(AttendArgs a) {
+  constexpr int KU = D / 16, UNITS = 2 * KU;  // 1 KB units of a page's codes: keys, then values
+  constexpr int UPW = UNITS / NW;             // of each wave
+  static_assert(UPW >= 1 && UPW * NW == UNITS, "every wave has whole units");
+  __shared__ uint4 lds[2][UNITS * 128];       // a unit widened: two operand blocks of 1 KB
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, h4 = lane >> 4;
   const int H = a.c.kv_heads, groups = a.B * H * a.splits;
   // workgroups that read the same pages go to one XCD (workgroup i runs on XCD i % 8)
@@ -493,7 +526,16 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(At
   Rows<DT, D, CT> st;
   st.clear();
   const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
-  uint4 kw[PT], vw[PT];
+  // Unit u: 16 rows with four 16-code pieces each, lane l taking the piece whose two operands lie at place l of the
+  // unit's blocks. Rows of the keys are tokens (D / 16 pieces), of the values dims (4 pieces).
+  unsigned piece[UPW];
+#pragma unroll
+  for (int i = 0; i < UPW; ++i) {
+    const int u = w * UPW + i;
+    piece[i] = u < KU ? (unsigned)((u / (D / 64) * 16 + (lane & 15)) * (D / 16) + u % (D / 64) * 4 + h4)
+                      : (unsigned)(((u - KU) * 16 + (lane & 15)) * 4 + h4);
+  }
+  uint4 cw[UPW];
   float ks = 0.0f, vs = 0.0f, ks1, vs1;
   int bad = 0;
   auto load = [&](int pg) {
@@ -503,45 +545,33 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(At
     pid = ok ? pid : 0;
     const uint8_t *kp = hd.kc + pid * hd.stride, *vp = hd.vc + pid * hd.stride;
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      kw[i] = at_u32(reinterpret_cast<const uint4*>(kp), (unsigned)(t + i * THREADS));
-      vw[i] = at_u32(reinterpret_cast<const uint4*>(vp), (unsigned)(t + i * THREADS));
-    }
+    for (int i = 0; i < UPW; ++i)
+      cw[i] = at_u32(reinterpret_cast<const uint4*>(w * UPW + i < KU ? kp : vp), piece[i]);
     const long long at = (long long)pid * H + h;
     ks1 = ok ? a.c.k_scale[at] : 0.0f;
     vs1 = ok ? a.c.v_scale[at] : 0.0f;
   };
-  // where piece i's two operands go: keys, row i / (D / 16) and chunk i % (D / 16); values, row i / 4, chunk i % 4
-  auto k_slot = [&](int i) {
-    const int row = i / (D / 16), ch = i % (D / 16);
-    return (((row >> 4) * (D / 64) + (ch >> 2)) * 2) * 64 + (ch & 3) * 16 + (row & 15);
-  };
-  auto v_slot = [&](int i) {
-    const int row = i >> 2, ch = i & 3;
-    return ((row >> 4) * 2) * 64 + ch * 16 + (row & 15);
-  };
   auto stage = [&](int buf) {
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int p = t + i * THREADS, sk = k_slot(p), sv = v_slot(p);
+    for (int i = 0; i < UPW; ++i) {
       uint4 x, y;
-      widen16<DT, CODES>(kw[i], x, y);
-      lk[buf][sk] = x;
-      lk[buf][sk + 64] = y;
-      widen16<DT, CODES>(vw[i], x, y);
-      lv[buf][sv] = x;
-      lv[buf][sv + 64] = y;
+      widen16<DT, CODES>(cw[i], x, y);
+      lds[buf][(w * UPW + i) * 128 + lane] = x;
+      lds[buf][(w * UPW + i) * 128 + 64 + lane] = y;
     }
   };
   auto stage_tail = [&](int buf, const TailScale& ts) {
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int p = t + i * THREADS, sk = k_slot(p), sv = v_slot(p);
-      lk[buf][sk] = reinterpret_cast<const uint4*>(hd.tk)[2 * p];
-      lk[buf][sk + 64] = reinterpret_cast<const uint4*>(hd.tk)[2 * p + 1];
-      const int place = (p & 3) * 16;
-      lv[buf][sv] = tail_v8<DT>(reinterpret_cast<const uint4*>(hd.tv)[2 * p], ts.down, place, left);
-      lv[buf][sv + 64] = tail_v8<DT>(reinterpret_cast<const uint4*>(hd.tv)[2 * p + 1], ts.down, place + 8, left);
+    for (int i = 0; i < UPW; ++i) {
+      const bool key = w * UPW + i < KU;
+      const uint4* src = reinterpret_cast<const uint4*>(key ? hd.tk : hd.tv) + 2 * piece[i];
+      uint4 x = src[0], y = src[1];
+      if (!key) {
+        x = tail_v8<DT>(x, ts.down, 16 * h4, left);
+        y = tail_v8<DT>(y, ts.down, 16 * h4 + 8, left);
+      }
+      lds[buf][(w * UPW + i) * 128 + lane] = x;
+      lds[buf][(w * UPW + i) * 128 + 64 + lane] = y;
     }
   };
   // LDS writes done, then the barrier; unlike __syncthreads() it leaves the loads of later pages in flight
@@ -559,7 +589,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(At
       for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) {
-        const uint4 x = lk[buf][(k * (D / 32) + e) * 64 + lane];
+        const uint4 x = lds[buf][(k * (D / 32) + e) * 64 + lane];
 #pragma unroll
         for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
       }
@@ -571,7 +601,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(At
     float pv[CT];
     st.template softmax<MASK>(s, cs, v, lim, h4, p, pv);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) st.add(d, lv[buf][d * 128 + lane], lv[buf][d * 128 + 64 + lane], p, pv);
+    for (int d = 0; d < D / 16; ++d) st.add(d, lds[buf][(KU + d) * 128 + lane], lds[buf][(KU + d) * 128 + 64 + lane], p, pv);
   };
   // pages lo..open-1 are seen whole by every row of the workgroup, open..last-1 by some in part (causal)
   const int last = min(hi, full), open = max(lo, min(last, sees(row0) / KV_PAGE));
@@ -592,7 +622,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void k_cache_attn_rows(At
       vs = vs1;
       if (pg + 2 < last) load(pg + 2);
     }
-    if (!decltype(mask_tag)::value || pg * KV_PAGE < seen_by_any) compute(mask_tag, buf, pg, cs, v);
+    if (pg * KV_PAGE < seen_by_any) compute(mask_tag, buf, pg, cs, v);  // 0 for a wave past the rows
     barrier();
   };
   for (int pg = lo; pg < open; ++pg) step(std::false_type{}, pg);
@@ -705,37 +735,42 @@ struct Cut {
   int tiles, splits, per;
 };
 constexpr int CUS = 256;
-#ifndef RESS_FEW_TARGET
-#define RESS_FEW_TARGET 4
-#define RESS_FEW_LEAST 8
-#define RESS_ROWS_TARGET 4
-#define RESS_ROWS_LEAST 8
-#endif
-
 Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   Cut k{};
   const long long rows = (long long)n * (Hq / c.kv_heads), heads = (long long)B * c.kv_heads;
   const int pages = cdiv(most_tokens > 0 ? most_tokens : 1, KV_PAGE);
-  long long target;  // workgroups wanted
-  int least;         // pages a split has at least
+  long long slots;  // workgroups that run at once
+  int least;        // pages a split has at least
   if (rows <= 32) {
     k.ct = rows <= 16 ? 1 : 2;
     k.nw = 0;
-    target = RESS_FEW_TARGET * CUS;
+    slots = RESS_FEW_TARGET * CUS;
     least = RESS_FEW_LEAST;
   } else {
-    k.ct = 2;
-    k.nw = 4;
-    target = RESS_ROWS_TARGET * CUS;
+    k.ct = RESS_ROWS_CT;
+    k.nw = RESS_ROWS_NW;
+    slots = (c.head_dim == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) * CUS / (RESS_ROWS_NW / 4);
     least = RESS_ROWS_LEAST;
   }
   const int tile = 16 * k.ct * (k.nw ? k.nw : 1);
   k.tiles = (int)((rows + tile - 1) / tile);
+  // The smallest number of splits that keeps the resident slots over 90% busy, else the best of those up to
+  // four rounds; a split has at least `least` pages.
   const long long wgs = heads * k.tiles;
-  long long s = wgs ? target / wgs : 1;
-  s = s < 1 ? 1 : s;
-  k.per = (int)((pages + s - 1) / s);
-  if (k.per < least) k.per = least;
+  const int most = pages / least < 1 ? 1 : pages / least;
+  double best = 0.0;
+  int s = 1;
+  for (int i = 1; i <= most && wgs > 0; ++i) {
+    const long long all = wgs * i, rounds = (all + slots - 1) / slots;
+    if (i > 1 && rounds > 4) break;
+    const double fill = (double)all / (double)(rounds * slots);
+    if (fill > best + 0.01) {
+      best = fill;
+      s = i;
+    }
+    if (fill > 0.9) break;
+  }
+  k.per = (pages + s - 1) / s;
   k.splits = (pages + k.per - 1) / k.per;
   return k;
 }
@@ -758,7 +793,7 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
   } else {
     const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
     RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
-    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, 2, 4>), dim3((unsigned)g), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, RESS_ROWS_CT, RESS_ROWS_NW>), dim3((unsigned)g), dim3(64 * RESS_ROWS_NW), 0, stream, a);
     RESS_LAUNCHED("k_cache_attn_rows");
   }
   if (k.splits > 1) {
