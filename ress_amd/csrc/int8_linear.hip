@@ -8,6 +8,10 @@
 // four consecutive channels of one token, one 8-byte store.
 #include "kvcache.h"
 
+#ifndef RESS_GEMM
+#define RESS_GEMM 128, 128, 2, 2, 2
+#endif
+
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
@@ -23,17 +27,29 @@ struct Out {
   bool vec;  // rows are 8-byte aligned and N a multiple of 4
 };
 
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
+// x Phi(x). Phi(-z) = erfc(z / sqrt 2) / 2 for z >= 0 by the rational approximation 7.1.26 of Abramowitz and Stegun,
+// erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + p u), within 1.5e-7: an absolute error of |x| 2^-23 beside
+// outputs of 8 or 11 bits, in a quarter of erff's instructions (they take 8 us of a product of 1374 x 1024 x 4096).
+__device__ __forceinline__ float gelu(float x) {
+  const float u = fabsf(x) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.0f));
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float half_erfc = 0.5f * (p * t) * __builtin_amdgcn_exp2f(u * u * -1.4426950408889634f);
+  return x * (x < 0.0f ? half_erfc : 1.0f - half_erfc);  // NaN: t is NaN
+}
 
 // four channels n.. of token m from their sums
 template <int DT>
-__device__ __forceinline__ void finish4(const Out& o, int m, int n, const v4i& acc, float sx) {
+__device__ __forceinline__ void finish4(const Out& o, int m, int n, const v4i& acc, float sx, const float (&ws)[4],
+                                        const float (&bias)[4]) {
   uint16_t e[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const int c = min(n + r, o.N - 1);
-    float y = (float)acc[r] * sx * o.ws[c];
-    if (o.bias) y = y + o.bias[c];
+    float y = (float)acc[r] * sx * ws[r];
+    if (o.bias) y = y + bias[r];
     if (o.act == ACT_GELU) y = gelu(y);
     e[r] = Elem<DT>::put(y);
   }
@@ -110,17 +126,28 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned voff
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, (int)voffset, soffset,
                                            0, 0);
 }
+// Waits until at most N of the wave's DMAs are in flight, then for the workgroup. __syncthreads() would wait for
+// all of them.
+template <int N>
+__device__ __forceinline__ void dma_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-// BM tokens x BN channels a workgroup of 2 x 2 waves, 128 bytes of K a step, two LDS stages filled by DMA one
-// step ahead. A row's eight 16-byte chunks lie at place chunk ^ (row & 7), so the operand reads (16 rows, one
-// chunk) meet no bank twice.
-template <int DT, int BM, int BN>
-__global__ __launch_bounds__(256) void k_int8_gemm(const uint8_t* __restrict__ x, long long kp,
-                                                   const float* __restrict__ sx, const uint8_t* __restrict__ w, int K,
-                                                   Out o) {
-  constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
+// BM tokens x BN channels a workgroup of GM x GN waves, 128 bytes of K a step, LDS stages filled by DMA ahead of
+// their use (STAGES - 1 steps). A row's eight 16-byte chunks lie at place chunk ^ (row & 7), so the operand reads
+// (16 rows, one chunk) meet no bank twice.
+template <int DT, int BM, int BN, int GM, int GN, int STAGES>
+__global__ __launch_bounds__(64 * GM * GN) void k_int8_gemm(const uint8_t* __restrict__ x, long long kp,
+                                                            const float* __restrict__ sx, const uint8_t* __restrict__ w,
+                                                            int K, Out o) {
+  constexpr int NW = GM * GN, WM = BM / GM, WN = BN / GN, TM = WM / 16, TN = WN / 16;
   constexpr int ROWS = BM + BN;             // tokens, then channels
-  __shared__ __align__(16) uint8_t s0[ROWS * 128], s1[ROWS * 128];
+  constexpr int XD = BM / 8 / NW, WD = BN / 8 / NW;  // 1 KB DMAs of a wave: eight rows each
+  static_assert(XD * 8 * NW == BM && WD * 8 * NW == BN, "every wave has whole DMAs");
+  // distinct objects: the compiler sees that a DMA writes no stage that is being read
+  __shared__ __align__(16) uint8_t s0[ROWS * 128], s1[ROWS * 128], s2[STAGES > 2 ? ROWS * 128 : 16];
   const int t = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, h4 = lane >> 4, r16 = lane & 15;
   // an XCD takes consecutive tiles, channels fastest: its L2 keeps the weights, and a row of tiles its tokens
   const int tn = cdiv(o.N, BN), total = cdiv(o.M, BM) * tn, per = cdiv(total, 8);
@@ -132,9 +159,8 @@ __global__ __launch_bounds__(256) void k_int8_gemm(const uint8_t* __restrict__ x
       const_cast<uint8_t*>(x + (long long)m0 * kp), (short)0, (int)(mrows * kp), RESS_I8_DWORD3);
   const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(w + (long long)n0 * K), (short)0, nrows * K, RESS_I8_DWORD3);
-  // A wave's DMA fills 1 KB: eight rows. Rows past the end repeat the last (never stored); chunks past a channel's
-  // row repeat its last, where the token codes are zero.
-  constexpr int XD = BM / 8 / 4, WD = BN / 8 / 4;  // of each wave
+  // Rows past the end repeat the last (never stored); chunks past a channel's row repeat its last, where the token
+  // codes are zero.
   unsigned xo[XD], wo[WD];
 #pragma unroll
   for (int i = 0; i < XD; ++i) {
@@ -159,7 +185,7 @@ __global__ __launch_bounds__(256) void k_int8_gemm(const uint8_t* __restrict__ x
       dma16(wr, off, k, s + BM * 128 + (wv * WD + i) * 1024);
     }
   };
-  const int wm = (wv >> 1) * WM, wn = (wv & 1) * WN;
+  const int wm = wv / GN * WM, wn = wv % GN * WN;
   v4i acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -180,28 +206,65 @@ __global__ __launch_bounds__(256) void k_int8_gemm(const uint8_t* __restrict__ x
         for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], b[i], acc[i][j], 0, 0, 0);
     }
   };
-  auto step = [&](const uint8_t* cur, uint8_t* nxt, int k) {
-    if (k + 128 < kp) fetch(nxt, k + 128);
-    compute(cur);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  };
-  fetch(s0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  for (int k = 0; k < (int)kp; k += 256) {
-    step(s0, s1, k);
-    if (k + 128 < kp) step(s1, s0, k + 128);
+  const int steps = (int)(kp / 128);
+  constexpr int DMAS = XD + WD;
+  if constexpr (STAGES == 3) {
+    // a step's DMA was started two steps before: the newest may stay in flight
+    auto step = [&](const uint8_t* cur, uint8_t* ahead, int i) {
+      if (i + 2 < steps) fetch(ahead, (i + 2) * 128);
+      compute(cur);
+      if (i + 2 < steps) dma_barrier<DMAS>();
+      else dma_barrier<0>();
+    };
+    fetch(s0, 0);
+    if (steps > 1) {
+      fetch(s1, 128);
+      dma_barrier<DMAS>();
+    } else {
+      dma_barrier<0>();
+    }
+    int i = 0;
+    for (; i + 3 <= steps; i += 3) {
+      step(s0, s2, i);
+      step(s1, s0, i + 1);
+      step(s2, s1, i + 2);
+    }
+    if (i < steps) step(s0, s2, i++);
+    if (i < steps) step(s1, s0, i++);
+  } else {
+    auto step = [&](const uint8_t* cur, uint8_t* nxt, int i) {
+      if (i + 1 < steps) fetch(nxt, (i + 1) * 128);
+      compute(cur);
+      dma_barrier<0>();
+    };
+    fetch(s0, 0);
+    dma_barrier<0>();
+    int i = 0;
+    for (; i + 2 <= steps; i += 2) {
+      step(s0, s1, i);
+      step(s1, s0, i + 1);
+    }
+    if (i < steps) step(s0, s1, i);
   }
+  // the epilogue's scales once per lane
+  float sm[TM];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm + 16 * i + r16;
-    if (m >= o.M) continue;
-    const float s = sx[m];
+  for (int i = 0; i < TM; ++i) sm[i] = sx[min(m0 + wm + 16 * i + r16, o.M - 1)];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n0 + wn + 16 * j + 4 * h4;
-      if (n < o.N) finish4<DT>(o, m, n, acc[i][j], s);
+  for (int j = 0; j < TN; ++j) {
+    const int n = n0 + wn + 16 * j + 4 * h4;
+    if (n >= o.N) continue;
+    float ws[4], bias[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = min(n + r, o.N - 1);
+      ws[r] = o.ws[c];
+      bias[r] = o.bias ? o.bias[c] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      const int m = m0 + wm + 16 * i + r16;
+      if (m < o.M) finish4<DT>(o, m, n, acc[i][j], sm[i], ws, bias);
     }
   }
 }
@@ -229,6 +292,15 @@ __global__ __launch_bounds__(64 * NW) void k_int8_few(const uint16_t* __restrict
     }
   };
   fetch(wv);
+  float ws[4], bias[4];  // of the epilogue, loaded ahead like the weights
+  if (wv == 0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = min(n0 + 4 * h4 + r, o.N - 1);
+      ws[r] = o.ws[c];
+      bias[r] = o.bias ? o.bias[c] : 0.0f;
+    }
+  }
   for (int m = wv; m < o.M; m += NW) {
     const uint16_t* row = x + m * stride;
     uint32_t top = 0;
@@ -258,7 +330,7 @@ __global__ __launch_bounds__(64 * NW) void k_int8_few(const uint16_t* __restrict
   if (wv == 0 && r16 < o.M && n0 + 4 * h4 < o.N) {
 #pragma unroll
     for (int i = 1; i < NW; ++i) acc += part[i][lane];
-    finish4<DT>(o, r16, n0 + 4 * h4, acc, sxs[r16]);
+    finish4<DT>(o, r16, n0 + 4 * h4, acc, sxs[r16], ws, bias);
   }
 }
 
@@ -275,12 +347,13 @@ int quantize(const void* x, long long stride, int M, int K, void* codes, long lo
   return 0;
 }
 
-template <int DT, int BM, int BN>
+template <int DT, int BM, int BN, int GM, int GN, int STAGES>
 int gemm(const uint8_t* codes, long long kp, const float* sx, const void* w, int K, const Out& o, hipStream_t stream) {
   const long long tiles = (long long)cdiv(o.M, BM) * cdiv(o.N, BN);
   RESS_REQUIRE(tiles < (1ll << 30), "ress_int8_linear: the call needs too many workgroups");
   const int grid = (int)((tiles + 7) / 8 * 8);
-  hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN>), dim3(grid), dim3(256), 0, stream, codes, kp, sx, (const uint8_t*)w, K, o);
+  hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN, GM, GN, STAGES>), dim3(grid), dim3(64 * GM * GN), 0, stream, codes, kp, sx,
+                     (const uint8_t*)w, K, o);
   RESS_LAUNCHED("k_int8_gemm");
   return 0;
 }
@@ -303,7 +376,7 @@ int linear(const void* x, long long stride, int K, const void* w, const Out& o, 
   uint8_t* codes = (uint8_t*)workspace;
   float* sx = (float*)(codes + (long long)o.M * kp);
   if (int rc = quantize<DT>(x, stride, o.M, K, codes, kp, sx, stream)) return rc;
-  return gemm<DT, 128, 128>(codes, kp, sx, w, K, o, stream);
+  return gemm<DT, RESS_GEMM>(codes, kp, sx, w, K, o, stream);
 }
 
 int check_rows(const char* who, int dtype, int M, int K) {
