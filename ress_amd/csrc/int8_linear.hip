@@ -4,20 +4,16 @@
 // with w int8 [N][K] and t its channels' scales. The sum is exact (int32); the rest is fp32, rounded once to
 // the activations' 16-bit type. A token with an element that is not finite has scale NaN, so its row of y is NaN.
 //
-// v_mfma_i32_16x16x64_i8 with the weights as the A operand (16 channels) and the tokens as B: a lane ends with
-// four consecutive channels of one token, one 8-byte store.
+// v_mfma_i32_16x16x64_i8 with the weights as the A operand (16 channels) and the tokens as B: a lane ends with four
+// channels of one token.
 #include "kvcache.h"
-
-#ifndef RESS_GEMM
-#define RESS_GEMM 128, 128, 2, 2, 2
-#endif
 
 namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int ACT_NONE = 0, ACT_GELU = 1;
-constexpr int KALIGN = 128;  // token codes are padded to this with zeros, so a product's last step needs no mask
+constexpr int KALIGN = 256;  // token codes are padded to this with zeros, so a product's last steps need no mask
 
 struct Out {
   uint16_t* p;
@@ -121,68 +117,77 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint16_t* __restric
 }
 
 // ---- many tokens: LDS-tiled product ---------------------------------------------------------------------
-#define RESS_I8_DWORD3 0x00020000
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned voffset, int soffset, void* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, (int)voffset, soffset,
-                                           0, 0);
+// A buffer of `bytes` bytes at `base` (wave-uniform) as the four words of its descriptor: reads past the end give zero.
+__device__ __forceinline__ v4i descriptor(const void* base, unsigned bytes) {
+  const unsigned long long p = (unsigned long long)base;
+  return v4i{(int)(unsigned)p, (int)(unsigned)(p >> 32), (int)bytes, 0x00020000};
 }
-// Waits until at most N of the wave's DMAs are in flight, then for the workgroup. __syncthreads() would wait for
-// all of them.
-template <int N>
+// 16 bytes a lane from the buffer at off + soff into LDS at lds + 16 lane. Written as assembly because the compiler,
+// which does not know what the explicit waits below cover, waits for every DMA in flight before an LDS read of a
+// stage that one has filled; nothing here has an output register, and m0 is set in the same block.
+__device__ __forceinline__ unsigned lds_address(void* p) {
+  return (unsigned)(unsigned long long)(__attribute__((address_space(3))) void*)p;
+}
+__device__ __forceinline__ void dma16(const v4i& rsrc, unsigned off, int soff, unsigned lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(lds), "v"(off), "s"(rsrc), "s"(soff)
+      : "memory", "m0");
+}
+// Every DMA of the wave has landed and its LDS reads are done, then the workgroup's.
 __device__ __forceinline__ void dma_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// BM tokens x BN channels a workgroup of GM x GN waves, 128 bytes of K a step, LDS stages filled by DMA ahead of
-// their use (STAGES - 1 steps). A row's eight 16-byte chunks lie at place chunk ^ (row & 7), so the operand reads
-// (16 rows, one chunk) meet no bank twice.
-template <int DT, int BM, int BN, int GM, int GN, int STAGES>
-__global__ __launch_bounds__(64 * GM * GN) void k_int8_gemm(const uint8_t* __restrict__ x, long long kp,
+// BM tokens x BN channels a workgroup of GM x GN waves, 128 bytes of K a step in two halves, two LDS stages filled by
+// DMA. A row's eight 16-byte chunks lie at place chunk ^ (row & 7), so the operand reads (16 rows, one chunk) meet no
+// bank twice. A step is
+//   multiply half 0, reading half 1 | its reads done and the next stage landed, barrier
+//   multiply half 1, reading half 0 of the next stage, the stage just read being filled for the step after
+// so there is one barrier a step, and a DMA has a whole step to land. The reads and DMAs go between the products of a
+// row of tiles, a few at a time: in one run they would hold up the products behind them. A token operand is read into
+// the registers of the one just used.
+template <int DT, int BM, int BN, int GM, int GN, bool EVEN>
+__global__ __launch_bounds__(64 * GM * GN, BM * BN / (GM * GN) > 8192 ? 1 : 2) void k_int8_gemm(const uint8_t* __restrict__ x, int kp,
                                                             const float* __restrict__ sx, const uint8_t* __restrict__ w,
                                                             int K, Out o) {
   constexpr int NW = GM * GN, WM = BM / GM, WN = BN / GN, TM = WM / 16, TN = WN / 16;
-  constexpr int ROWS = BM + BN;             // tokens, then channels
-  constexpr int XD = BM / 8 / NW, WD = BN / 8 / NW;  // 1 KB DMAs of a wave: eight rows each
+  constexpr int XD = BM / 8 / NW, WD = BN / 8 / NW;  // 1 KB DMAs of a wave and step, eight rows each
   static_assert(XD * 8 * NW == BM && WD * 8 * NW == BN, "every wave has whole DMAs");
-  // distinct objects: the compiler sees that a DMA writes no stage that is being read
-  __shared__ __align__(16) uint8_t s0[ROWS * 128], s1[ROWS * 128], s2[STAGES > 2 ? ROWS * 128 : 16];
+  __shared__ __align__(16) uint8_t s0[(BM + BN) * 128], s1[(BM + BN) * 128];
   const int t = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, h4 = lane >> 4, r16 = lane & 15;
-  // an XCD takes consecutive tiles, channels fastest: its L2 keeps the weights, and a row of tiles its tokens
+  // an XCD takes consecutive tiles, and these run down eight rows of tiles before they go on to the next channels:
+  // what its workgroups read at one time is about square
   const int tn = cdiv(o.N, BN), total = cdiv(o.M, BM) * tn, per = cdiv(total, 8);
   const int lin = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || lin >= total) return;
-  const int m0 = lin / tn * BM, n0 = lin % tn * BN;
-  const int mrows = min(BM, o.M - m0), nrows = min(BN, o.N - n0);
-  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(x + (long long)m0 * kp), (short)0, (int)(mrows * kp), RESS_I8_DWORD3);
-  const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(w + (long long)n0 * K), (short)0, nrows * K, RESS_I8_DWORD3);
-  // Rows past the end repeat the last (never stored); chunks past a channel's row repeat its last, where the token
-  // codes are zero.
-  unsigned xo[XD], wo[WD];
+  const int tm = cdiv(o.M, BM), group = lin / (8 * tn), gm = min(8, tm - 8 * group), in = lin - group * 8 * tn;
+  const int m0 = (8 * group + in % gm) * BM, n0 = in / gm * BN;
+  const int nrows = min(BN, o.N - n0);
+  const v4i xr = descriptor(x + (long long)m0 * kp, (unsigned)(BM * kp));
+  const v4i wr = descriptor(w + (long long)n0 * K, (unsigned)(nrows * K));
+  // The workspace holds whole tiles of tokens (what lies past the last is multiplied, never stored). Channels past the
+  // end repeat the last; chunks past a channel's row are the next one's or, past the buffer, zero: the token codes there
+  // are zero.
+  const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  const unsigned xo = (unsigned)((wv * XD * 8 + (lane >> 3)) * kp + chunk);
+  unsigned wo[WD];
 #pragma unroll
-  for (int i = 0; i < XD; ++i) {
-    const int row = (wv * XD + i) * 8 + (lane >> 3);
-    xo[i] = (unsigned)(min(row, mrows - 1) * (int)kp + ((lane & 7) ^ (row & 7)) * 16);
-  }
-#pragma unroll
-  for (int i = 0; i < WD; ++i) {
-    const int row = (wv * WD + i) * 8 + (lane >> 3);
-    wo[i] = (unsigned)(min(row, nrows - 1) * K + ((lane & 7) ^ (row & 7)) * 16);
-  }
-  auto fetch = [&](uint8_t* s, int k) {
-#pragma unroll
-    for (int i = 0; i < XD; ++i) dma16(xr, xo[i], k, s + (wv * XD + i) * 1024);
-#pragma unroll
-    for (int i = 0; i < WD; ++i) {
-      unsigned off = wo[i];
-      if (k + 128 > K) {  // the last step of a K that is no multiple of 128
-        const int row = (wv * WD + i) * 8 + (lane >> 3);
-        off = (unsigned)(min(row, nrows - 1) * K + min(((lane & 7) ^ (row & 7)) * 16, K - 16 - k));
-      }
-      dma16(wr, off, k, s + BM * 128 + (wv * WD + i) * 1024);
+  for (int i = 0; i < WD; ++i) wo[i] = (unsigned)(min((wv * WD + i) * 8 + (lane >> 3), nrows - 1) * K + chunk);
+  // DMA i of the wave's XD + WD
+  auto fetch = [&](unsigned s, int k, int i) {
+    if (i < XD) {
+      dma16(xr, xo, k + i * 8 * kp, s + (wv * XD + i) * 1024);
+    } else {
+      // EVEN: K is a multiple of 256. Else k goes into the offset that is checked: the last channel's chunks past K lie
+      // outside the buffer (an addition more a DMA, for which the largest tile has no registers left)
+      const unsigned off = wo[i < XD ? 0 : i - XD];
+      dma16(wr, EVEN ? off : off + k, EVEN ? k : 0, s + BM * 128 + (wv * WD + i - XD) * 1024);
     }
   };
   const int wm = wv / GN * WM, wn = wv % GN * WN;
@@ -191,68 +196,71 @@ __global__ __launch_bounds__(64 * GM * GN) void k_int8_gemm(const uint8_t* __res
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-  auto compute = [&](const uint8_t* s) {
+  v4i fa[2][TN], fb[TM];  // channels' operands of this half and the next, tokens' operands
+  const int rd0 = r16 * 128 + (h4 ^ (r16 & 7)) * 16, rd1 = r16 * 128 + ((4 + h4) ^ (r16 & 7)) * 16;
+  auto read_a = [&](const uint8_t* s, int c, int j) {
+    return *reinterpret_cast<const v4i*>(s + (BM + wn + 16 * j) * 128 + (c ? rd1 : rd0));
+  };
+  auto read_b = [&](const uint8_t* s, int c, int i) {
+    return *reinterpret_cast<const v4i*>(s + (wm + 16 * i) * 128 + (c ? rd1 : rd0));
+  };
+  // multiply half h; READ: the operands of half rd of stage s; FETCH: the DMAs of a stage at `at`, step k
+  auto half = [&](auto h_tag, auto read_tag, auto fetch_tag, const uint8_t* s, int rd, unsigned at, int k) {
+    constexpr int h = decltype(h_tag)::value;
+    constexpr bool READ = decltype(read_tag)::value, FETCH = decltype(fetch_tag)::value;
+    constexpr int AR = (TN + TM - 1) / TM, DR = (XD + WD + TM - 1) / TM;  // channel reads and DMAs a row of tiles
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      v4i a[TN], b[TM];
-      const int place = ((4 * k + h4) ^ (r16 & 7)) * 16;
+    for (int i = 0; i < TM; ++i) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i) b[i] = *reinterpret_cast<const v4i*>(s + (wm + 16 * i + r16) * 128 + place);
+      for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[h][j], fb[i], acc[i][j], 0, 0, 0);
+      if constexpr (READ) {
+        fb[i] = read_b(s, rd, i);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) a[j] = *reinterpret_cast<const v4i*>(s + (BM + wn + 16 * j + r16) * 128 + place);
+        for (int j = i * AR; j < i * AR + AR; ++j)
+          if (j < TN) fa[h ^ 1][j] = read_a(s, rd, j);
+      }
+      if constexpr (FETCH) {
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], b[i], acc[i][j], 0, 0, 0);
+        for (int d = i * DR; d < i * DR + DR; ++d)
+          if (d < XD + WD) fetch(at, k, d);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const int steps = (int)(kp / 128);
-  constexpr int DMAS = XD + WD;
-  if constexpr (STAGES == 3) {
-    // a step's DMA was started two steps before: the newest may stay in flight
-    auto step = [&](const uint8_t* cur, uint8_t* ahead, int i) {
-      if (i + 2 < steps) fetch(ahead, (i + 2) * 128);
-      compute(cur);
-      if (i + 2 < steps) dma_barrier<DMAS>();
-      else dma_barrier<0>();
-    };
-    fetch(s0, 0);
-    if (steps > 1) {
-      fetch(s1, 128);
-      dma_barrier<DMAS>();
-    } else {
-      dma_barrier<0>();
-    }
-    int i = 0;
-    for (; i + 3 <= steps; i += 3) {
-      step(s0, s2, i);
-      step(s1, s0, i + 1);
-      step(s2, s1, i + 2);
-    }
-    if (i < steps) step(s0, s2, i++);
-    if (i < steps) step(s1, s0, i++);
-  } else {
-    auto step = [&](const uint8_t* cur, uint8_t* nxt, int i) {
-      if (i + 1 < steps) fetch(nxt, (i + 1) * 128);
-      compute(cur);
-      dma_barrier<0>();
-    };
-    fetch(s0, 0);
-    dma_barrier<0>();
-    int i = 0;
-    for (; i + 2 <= steps; i += 2) {
-      step(s0, s1, i);
-      step(s1, s0, i + 1);
-    }
-    if (i < steps) step(s0, s1, i);
+  const unsigned at0 = __builtin_amdgcn_readfirstlane(lds_address(s0)), at1 = __builtin_amdgcn_readfirstlane(lds_address(s1));
+  const int steps = (int)(kp / 128);  // even
+  constexpr std::integral_constant<int, 0> first{};
+  constexpr std::integral_constant<int, 1> second{};
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+#pragma unroll
+  for (int d = 0; d < XD + WD; ++d) fetch(at0, 0, d);
+  dma_barrier();
+#pragma unroll
+  for (int d = 0; d < XD + WD; ++d) fetch(at1, 128, d);
+#pragma unroll
+  for (int j = 0; j < TN; ++j) fa[0][j] = read_a(s0, 0, j);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) fb[i] = read_b(s0, 0, i);
+  for (int i = 0; i + 2 < steps; i += 2) {
+    half(first, yes, no, s0, 1, 0, 0);
+    dma_barrier();
+    half(second, yes, yes, s1, 0, at0, (i + 2) * 128);
+    half(first, yes, no, s1, 1, 0, 0);
+    dma_barrier();
+    half(second, yes, yes, s0, 0, at1, (i + 3) * 128);
   }
-  // the epilogue's scales once per lane
-  float sm[TM];
+  half(first, yes, no, s0, 1, 0, 0);
+  dma_barrier();
+  half(second, yes, no, s1, 0, 0, 0);
+  half(first, yes, no, s1, 1, 0, 0);
+  half(second, no, no, s1, 0, 0, 0);
+  float sm[TM];  // loaded together: one at a time each store would wait for its own
 #pragma unroll
   for (int i = 0; i < TM; ++i) sm[i] = sx[min(m0 + wm + 16 * i + r16, o.M - 1)];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int n = n0 + wn + 16 * j + 4 * h4;
+    const int n = n0 + wn + 16 * j + 4 * h4;  // the lane's four channels
     if (n >= o.N) continue;
     float ws[4], bias[4];
 #pragma unroll
@@ -336,6 +344,8 @@ __global__ __launch_bounds__(64 * NW) void k_int8_few(const uint16_t* __restrict
 
 constexpr int FEW = 16, FEW_BYTES = 40 * 1024;
 long long padded(int K) { return (K + KALIGN - 1) / KALIGN * (long long)KALIGN; }
+// Bytes of the token codes in the workspace: whole rows of the largest tiles (192 and 256 tokens).
+long long code_bytes(int M, int K) { return ((M + 255ll) / 256 * 256 + 192) * padded(K); }
 bool few(int M, int K) { return M <= FEW && M * padded(K) <= FEW_BYTES; }
 
 template <int DT>
@@ -347,15 +357,46 @@ int quantize(const void* x, long long stride, int M, int K, void* codes, long lo
   return 0;
 }
 
-template <int DT, int BM, int BN, int GM, int GN, int STAGES>
-int gemm(const uint8_t* codes, long long kp, const float* sx, const void* w, int K, const Out& o, hipStream_t stream) {
+template <int DT, int BM, int BN, int GM, int GN>
+int gemm(const uint8_t* codes, int kp, const float* sx, const void* w, int K, const Out& o, hipStream_t stream) {
   const long long tiles = (long long)cdiv(o.M, BM) * cdiv(o.N, BN);
   RESS_REQUIRE(tiles < (1ll << 30), "ress_int8_linear: the call needs too many workgroups");
   const int grid = (int)((tiles + 7) / 8 * 8);
-  hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN, GM, GN, STAGES>), dim3(grid), dim3(64 * GM * GN), 0, stream, codes, kp, sx,
-                     (const uint8_t*)w, K, o);
+  if (K == kp)
+    hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN, GM, GN, true>), dim3(grid), dim3(64 * GM * GN), 0, stream, codes, kp, sx,
+                       (const uint8_t*)w, K, o);
+  else
+    hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN, GM, GN, false>), dim3(grid), dim3(64 * GM * GN), 0, stream, codes, kp, sx,
+                       (const uint8_t*)w, K, o);
   RESS_LAUNCHED("k_int8_gemm");
   return 0;
+}
+
+// The tile of a product: the one whose rounds of workgroups add up to the least time. A step (128 of K) takes `alone` us
+// where each CU has one tile and `full` where every CU holds the `held` that fit; a round's start and end (the output
+// is written then) take `ends`. Measured, us of the product (256 x 256, 192 x 256, 128 x 128 | taken):
+//   4096 x 4096 x 4096 58, 80, 66 | 58        21984 x 1024 (N) x 4096 (K) 105, 91, 102 | 91
+//   8192 x 8192 x 8192 495, 479, 544 | 495    21984 x 4096 (N) x 1024 (K) 143, 151, 135 | 135
+// and 1374 x 1024 (N) x 4096 (K): 128 x 128 17, 64 x 128 15, 64 x 64 12 | 12.
+int pick(int M, int N, int steps) {
+  static const struct {
+    int bm, bn, held;
+    double alone, full, ends;
+  } tiles[] = {{256, 256, 1, 1.20, 1.75, 10.0}, {192, 256, 1, 0.97, 1.30, 8.5}, {128, 128, 2, 0.52, 1.06, 3.7},
+               {64, 128, 3, 0.47, 0.92, 2.5}, {64, 64, 5, 0.37, 0.95, 2.0}};
+  int best = 0;
+  double least = 0.0;
+  for (int i = 0; i < 5; ++i) {
+    const double slots = 256.0 * tiles[i].held, n = (double)cdiv(M, tiles[i].bm) * cdiv(N, tiles[i].bn);
+    const double rounds = floor(n / slots), rest = n / slots - rounds;
+    double t = rounds * (steps * tiles[i].full + tiles[i].ends);
+    if (rest > 0.0) t += steps * fmax(tiles[i].alone, rest * tiles[i].full) + 0.6 * tiles[i].ends;
+    if (i == 0 || t < least) {
+      least = t;
+      best = i;
+    }
+  }
+  return best;
 }
 
 template <int DT>
@@ -374,9 +415,15 @@ int linear(const void* x, long long stride, int K, const void* w, const Out& o, 
     return 0;
   }
   uint8_t* codes = (uint8_t*)workspace;
-  float* sx = (float*)(codes + (long long)o.M * kp);
+  float* sx = (float*)(codes + code_bytes(o.M, K));
   if (int rc = quantize<DT>(x, stride, o.M, K, codes, kp, sx, stream)) return rc;
-  return gemm<DT, RESS_GEMM>(codes, kp, sx, w, K, o, stream);
+  switch (pick(o.M, o.N, (int)(kp / 128))) {
+    case 0: return gemm<DT, 256, 256, 2, 4>(codes, (int)kp, sx, w, K, o, stream);
+    case 1: return gemm<DT, 192, 256, 2, 4>(codes, (int)kp, sx, w, K, o, stream);
+    case 2: return gemm<DT, 128, 128, 2, 4>(codes, (int)kp, sx, w, K, o, stream);
+    case 3: return gemm<DT, 64, 128, 2, 2>(codes, (int)kp, sx, w, K, o, stream);
+    default: return gemm<DT, 64, 64, 2, 2>(codes, (int)kp, sx, w, K, o, stream);
+  }
 }
 
 int check_rows(const char* who, int dtype, int M, int K) {
@@ -402,7 +449,7 @@ RESS_API int ress_quantize_rows(const void* x, long long stride, int dtype, int 
 
 RESS_API long long ress_int8_linear_workspace_size(int M, int K, int N) {
   if (M < 0 || K < 0 || N < 0) return -1;
-  return few(M, K) ? 0 : (long long)M * padded(K) + 4ll * M;
+  return few(M, K) ? 0 : code_bytes(M, K) + 4ll * M;
 }
 
 RESS_API int ress_int8_linear(const void* x, long long stride, int dtype, int M, int K, int N, const void* w,

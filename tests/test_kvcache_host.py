@@ -96,11 +96,11 @@ def test_the_library_refuses_a_bad_linear():
     for kw, msg in ((dict(dtype=0), b"dtype code 0"), (dict(K=40), b"multiple of 16"), (dict(M=-1), b"multiple of 16"),
                     (dict(K=1 << 18), b"at most 131072"), (dict(N=-1), b"channel count"), (dict(act=2), b"act 2"),
                     (dict(x=None), b"null"), (dict(K=0), b"without elements"), (dict(w=ctypes.c_void_p(4104)), b"aligned"),
-                    (dict(size=20 * 128), b"workspace needs"), (dict(work=None), b"workspace needs")):
+                    (dict(size=448 * 256), b"workspace needs"), (dict(work=None), b"workspace needs")):
         a = {**ok, **kw}
         assert L.ress_int8_linear(a["x"], 64, a["dtype"], a["M"], a["K"], a["N"], a["w"], a["ws"], None, a["act"], a["out"], 8,
                                   a["work"], a["size"], None) == -1
         assert msg in L.ress_last_error(), (kw, L.ress_last_error())
     assert L.ress_int8_linear_workspace_size(1, 64, 8) == 0
-    assert L.ress_int8_linear_workspace_size(20, 64, 8) == 20 * 128 + 80
+    assert L.ress_int8_linear_workspace_size(20, 64, 8) == (256 + 192) * 256 + 80
     assert L.ress_quantize_rows(p, 64, 1, 2, 64, p, 60, p, None) == -1 and b"8-byte aligned" in L.ress_last_error()
