@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ress_amd.int8 import Int8Linear
 from ress_amd.synth import hilbert_permutation
 from ress_amd.wiring import wire_ress_attention
 
@@ -91,6 +92,8 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden, dim)
 
     def forward(self, x):
+        if isinstance(self.fc1, Int8Linear) and isinstance(self.act, nn.GELU) and self.act.approximate == "none":
+            return self.fc2(self.fc1(x, act="gelu"))
         return self.fc2(self.act(self.fc1(x)))
 
 
@@ -136,10 +139,11 @@ class Aggregator(nn.Module):
         self.register_buffer("std", torch.tensor(_IMAGENET_STD).view(1, 1, 3, 1, 1), persistent=False)
         self._hilbert = {}  # (w, h) -> the patch grid's Hilbert gather table
 
-    def _special(self, B, S):
+    def _special(self, B, S, first_frame=0):
         def pick(tok):  # frame 0 takes index 0, the other frames index 1
-            first = tok[:, :1].expand(B, 1, *tok.shape[2:])
-            rest = tok[:, 1:].expand(B, S - 1, *tok.shape[2:])
+            n = 1 if first_frame == 0 else 0
+            first = tok[:, :1].expand(B, n, *tok.shape[2:])
+            rest = tok[:, 1:].expand(B, S - n, *tok.shape[2:])
             return torch.cat([first, rest], dim=1).reshape(B * S, *tok.shape[2:])
         return torch.cat([pick(self.camera_token), pick(self.register_token)], dim=1)
 
@@ -155,15 +159,25 @@ class Aggregator(nn.Module):
         weight = self.patch_embed.weight.reshape(self.patch_embed.out_channels, cin * p * p)
         return F.linear(x, weight, self.patch_embed.bias), h, w
 
+    def tokens(self, images, first_frame=0):
+        """(x (B, S, P, dim), pos (P, 2), (h, w)): the tokens of frames first_frame.. before the first block,
+        special tokens in front, and their positions on the h x w patch grid."""
+        B, S, _, Hi, Wi = images.shape
+        x = ((images - self.mean) / self.std).to(self.patch_embed.weight.dtype)
+        x, h, w = self._embed_patches(x.reshape(B * S, 3, Hi, Wi))  # (B*S, h*w, dim)
+        x = torch.cat([self._special(B, S, first_frame).to(x.dtype), x], dim=1)
+        yy, xx = torch.meshgrid(torch.arange(h, device=x.device), torch.arange(w, device=x.device), indexing="ij")
+        grid = torch.stack([yy.flatten(), xx.flatten()], dim=-1) + 1
+        pos = torch.cat([torch.zeros(self.n_special, 2, dtype=grid.dtype, device=x.device), grid], dim=0)
+        return x.reshape(B, S, *x.shape[1:]), pos, (h, w)
+
     def forward(self, images, use_hilbert=False):
         """use_hilbert: the reference aggregator's flag (src/ress/models/vggt.py:32, 62-64):
         the global layers form their blocks along the per-frame Hilbert curve of the patch
         grid. The tokens stay in raster order: each global attention reads them through the
         curve's gather table (its patch_order) instead of the reference's permuted copy, and
         frame attention, being per-frame dense, is unaffected by the order."""
-        B, S, _, Hi, Wi = images.shape
-        x = ((images - self.mean) / self.std).to(self.patch_embed.weight.dtype)
-        x, h, w = self._embed_patches(x.reshape(B * S, 3, Hi, Wi))  # (B*S, h*w, dim)
+        x, pos, (h, w) = self.tokens(images)
         order = None
         if use_hilbert:
             order = self._hilbert.get((w, h))
@@ -171,11 +185,7 @@ class Aggregator(nn.Module):
                 order = self._hilbert[(w, h)] = torch.from_numpy(hilbert_permutation(w, h))
         for gb in self.global_blocks:
             gb.attn.patch_order = order
-        x = torch.cat([self._special(B, S).to(x.dtype), x], dim=1)
-        P, C = x.shape[1], x.shape[2]
-        yy, xx = torch.meshgrid(torch.arange(h, device=x.device), torch.arange(w, device=x.device), indexing="ij")
-        grid = torch.stack([yy.flatten(), xx.flatten()], dim=-1) + 1
-        pos = torch.cat([torch.zeros(self.n_special, 2, dtype=grid.dtype, device=x.device), grid], dim=0)
+        B, S, P, C = x.shape
         pos_f = pos[None].expand(B * S, P, 2)
         pos_g = pos[None].expand(B, S, P, 2).reshape(B, S * P, 2)
         pos_g.ress_patch_grid = (h, w)  # so that the global layers need not read it back from the device

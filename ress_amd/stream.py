@@ -1,0 +1,131 @@
+"""Reconstruction from frames that arrive one after the other: each new frame's tokens attend, in every
+global layer, to all frames seen so far and to their own, over 8-bit key/value caches (kvcache.py).
+
+    stream = FrameStream(model, max_frames=200)
+    with torch.no_grad():
+        for frame in frames:                      # (B, 3, H, W) or several: (B, s, 3, H, W)
+            tokens = stream.step(frame)           # (B, s * P, dim)
+
+One step over all frames of a scene is the aggregator's forward with dense global attention (frames of
+one step see each other). A global layer costs a step of s frames s * P queries over the frames held,
+instead of all queries over all keys again, and holds 2 * dim bytes a token.
+
+The reference runs over all frames at once and has no counterpart.
+"""
+
+import torch
+
+from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable
+from ress_amd.qkv import _fusable, fused_qk_norm_rope, rope_base
+from ress_amd.wiring import global_blocks
+
+
+def cached_attention(attn, x, pos, cache, tables):
+    """The output of the attention module `attn` for new tokens x (B, T, dim) at positions pos (B, T, 2), which
+    are appended to `cache` first. The module's q/k norms and rotation are its own: fused where the fused kernel
+    implements them, else the norms as modules and a rotation of known base (rope_base) while appending.
+    tables: a dict that keeps the rotation tables."""
+    B, T, C = x.shape
+    nh = attn.num_heads
+    hd = C // nh
+    if _fusable(attn, x, hd) and attn.q_norm.eps == attn.k_norm.eps:
+        q, k, v = fused_qk_norm_rope(attn, attn.qkv(x), pos, nh)
+        cache.append(k, v)
+    else:
+        q, k, v = attn.qkv(x).reshape(B, T, 3, nh, hd).permute(2, 0, 3, 1, 4).unbind(0)
+        q, k = attn.q_norm(q), attn.k_norm(k)
+        rope = getattr(attn, "rope", None)
+        base = None if rope is None else rope_base(rope)
+        if rope is None:
+            cache.append(k, v)
+        elif base is None:
+            q, k = rope(q, pos), rope(k, pos)
+            cache.append(k, v)
+        else:
+            table = tables.get((hd, base))
+            if table is None:
+                table = tables[(hd, base)] = RotaryTable(hd, 1024, base=base, axes=2, device=x.device)
+            q = cache.append(k, v, pos=pos, rope=table, q=q)
+    # written as the projection reads it
+    o = torch.empty(B, T, nh, hd, dtype=x.dtype, device=x.device)
+    cache.attend(q, out=o.transpose(1, 2))
+    return attn.proj_drop(attn.proj(o.reshape(B, T, C)))
+
+
+class FrameStream:
+    """Streams frames through a VGGT-style model (an `aggregator` with frame and global blocks, in bf16 or fp16
+    on the GPU). Up to max_frames frames of one size for each of `batch` scenes; codes: "int8" or "fp8" (e4m3)."""
+
+    def __init__(self, model, max_frames, batch=1, codes="int8"):
+        if int(max_frames) < 1 or int(batch) < 1:
+            raise ValueError(f"max_frames and batch must be at least 1, got {max_frames} and {batch}")
+        self.aggregator = model.aggregator
+        self.blocks = global_blocks(model)
+        self.max_frames, self.batch, self.codes = int(max_frames), int(batch), codes
+        self.frames = 0       # held now
+        self.grid = None      # patch grid of the frames
+        self.caches = None    # one a global layer, made with the first step
+        self._whole = True    # every cache holds the same frames
+        self._tables = {}
+
+    def _make(self, x, P):
+        pages = self.batch * (-(-self.max_frames * P // PAGE) + 1)
+        self.caches = [PagedKVCache(pages, b.attn.num_heads, x.shape[-1] // b.attn.num_heads, max_seqs=self.batch,
+                                    max_len=self.max_frames * P, dtype=x.dtype, codes=self.codes, device=x.device)
+                       for b in self.blocks]
+
+    @torch.no_grad()
+    def step(self, images):
+        """Tokens (B, s * P, dim) of s new frames, images (B, s, 3, H, W) or (B, 3, H, W) in [0, 1]."""
+        if images.dim() == 4:
+            images = images[:, None]
+        if images.dim() != 5 or images.shape[0] != self.batch or images.shape[1] < 1:
+            raise ValueError(f"images must be ({self.batch}, s, 3, H, W), got {tuple(images.shape)}")
+        if not self._whole:
+            raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
+        if self.frames + images.shape[1] > self.max_frames:
+            raise ValueError(f"{self.frames} frames are held and {images.shape[1]} more do not fit max_frames={self.max_frames}")
+        agg = self.aggregator
+        x, pos, grid = agg.tokens(images, first_frame=self.frames)
+        if self.grid not in (None, grid):
+            raise ValueError(f"the stream's frames have a {self.grid} patch grid, got {grid}")
+        B, s, P, C = x.shape
+        if self.caches is None:
+            self._make(x, P)
+        self.grid = grid
+        self._whole = False
+        pos_f = pos[None].expand(B * s, P, 2)
+        pos_g = pos[None, None].expand(B, s, P, 2).reshape(B, s * P, 2)
+        for fb, gb, cache in zip(agg.frame_blocks, self.blocks, self.caches):
+            x = fb(x.reshape(B * s, P, C), pos=pos_f).reshape(B, s * P, C)
+            x = x + gb.ls1(cached_attention(gb.attn, gb.norm1(x), pos_g, cache, self._tables))
+            x = x + gb.ls2(gb.mlp(gb.norm2(x)))
+        self._whole = True
+        self.frames += s
+        return x.reshape(B, s * P, C)
+
+    def snapshot(self):
+        """For restore: takes back the frames of later steps (a frame that is not kept as a key frame)."""
+        if self.caches is None:
+            raise RuntimeError("no frame has been streamed yet")
+        return self.frames, [c.snapshot() for c in self.caches]
+
+    def restore(self, snapshot):
+        frames, snaps = snapshot
+        if self.caches is None or len(snaps) != len(self.caches):
+            raise ValueError("the snapshot belongs to another stream")
+        for c, s in zip(self.caches, snaps):
+            c.restore(s)
+        self.frames, self._whole = frames, True
+
+    def reset(self):
+        """Forgets every frame; the caches stay allocated."""
+        for c in self.caches or ():
+            for slot in range(self.batch):
+                c.release(slot)
+        self.frames, self.grid, self._whole = 0, None, True
+
+    def check(self):
+        """Raises what a cache has met since the last check (PagedKVCache.check; waits for the device)."""
+        for c in self.caches or ():
+            c.check()

@@ -104,3 +104,37 @@ def test_the_library_refuses_a_bad_linear():
     assert L.ress_int8_linear_workspace_size(1, 64, 8) == 0
     assert L.ress_int8_linear_workspace_size(20, 64, 8) == (256 + 192) * 256 + 80
     assert L.ress_quantize_rows(p, 64, 1, 2, 64, p, 60, p, None) == -1 and b"8-byte aligned" in L.ress_last_error()
+
+
+def test_stream_refusals():
+    from ress_amd import FrameStream
+    from ress_amd.aggregator import build_vggt_aggregator
+    model = build_vggt_aggregator(depth=1, dim=64, num_heads=1, device="cpu", dtype=torch.float32)
+    for bad in (dict(max_frames=0), dict(max_frames=2, batch=0)):
+        with pytest.raises(ValueError, match="at least 1"):
+            FrameStream(model, **bad)
+    s = FrameStream(model, 2)
+    for shape in ((2, 3, 28, 28), (1, 0, 3, 28, 28), (3, 28, 28)):
+        with pytest.raises(ValueError, match="images must"):
+            s.step(torch.zeros(shape))
+    with pytest.raises(ValueError, match="do not fit"):
+        s.step(torch.zeros(1, 3, 3, 28, 28))
+    with pytest.raises(RuntimeError, match="no frame"):
+        s.snapshot()
+    with pytest.raises(ValueError, match="another stream"):
+        s.restore((0, []))
+    with pytest.raises(TypeError, match="dtype"):  # a cache of 32-bit keys
+        s.step(torch.zeros(1, 3, 28, 28))
+
+
+def test_special_tokens_of_later_frames():
+    """Frame 0 has its own special tokens, every later one the shared ones, however the frames come."""
+    from ress_amd.aggregator import build_vggt_aggregator
+    agg = build_vggt_aggregator(depth=1, dim=64, num_heads=1, device="cpu", dtype=torch.float32).aggregator
+    images = torch.rand(2, 3, 3, 28, 42)
+    with torch.no_grad():
+        whole, pos, grid = agg.tokens(images)
+        assert grid == (2, 3) and tuple(whole.shape) == (2, 3, 11, 64) and tuple(pos.shape) == (11, 2)
+        for i in range(3):
+            x, p, _ = agg.tokens(images[:, i:i + 1], first_frame=i)
+            assert torch.equal(x[:, 0], whole[:, i]) and torch.equal(p, pos)
