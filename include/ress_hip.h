@@ -289,7 +289,7 @@ int ress_block_sparse_fwd(const void* q_i8, const void* k_i8, const void* v, int
  *   table [max_seqs][max_pages] int32: the page that holds tokens 64 j .. 64 j + 63 of a slot
  *   held [max_seqs] int32: pages reserved for the slot (its first `held` table entries)
  *   lens [max_seqs] int32: tokens in the slot
- *   arrived [max_seqs] int32: zero between calls
+ *   arrived [max_seqs][32] int32: zero between calls (a cache line for each slot)
  *   status int32, OR-ed: 1 tokens that found no reserved page were dropped, 2 a position outside the
  *     rotation table (clamped into it), 4 a page number outside the pool (not read or written),
  *     8 a page with a key or value that is not finite (its scale is NaN)

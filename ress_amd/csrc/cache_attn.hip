@@ -23,10 +23,16 @@
 #include "kvcache.h"
 
 #ifndef RESS_FEW_TARGET
-#define RESS_FEW_TARGET 4
+#define RESS_FEW_TARGET 2
+#endif
+#ifndef RESS_FEW_OCC64
+#define RESS_FEW_OCC64 3
+#endif
+#ifndef RESS_FEW_OCC128
+#define RESS_FEW_OCC128 2
 #endif
 #ifndef RESS_FEW_LEAST
-#define RESS_FEW_LEAST 8
+#define RESS_FEW_LEAST 16
 #endif
 #ifndef RESS_ROWS_NW
 #define RESS_ROWS_NW 4
@@ -315,14 +321,18 @@ __device__ __forceinline__ uint4 tail_v8(const uint4& w, float down, int place, 
   return pack8(e);
 }
 
+// Waves a SIMD has room for (its registers are shared out so).
+constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D == 64 ? RESS_FEW_OCC64 : RESS_FEW_OCC128; }
+
 // ---- few rows: one wave a page --------------------------------------------------------------------
 // A workgroup of four waves takes 16 CT rows of a (sequence, kv head) and a share of its pages, a wave every
 // fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
 // joined in LDS.
 template <int DT, int CODES, int D, int CT>
-__global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
+__global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a) {
   constexpr int NW = 4;
-  __shared__ __align__(16) float so[NW][64][4 * CT];  // one dim tile at a time
+  constexpr int TILES = CT * D / 16;  // of the output: 16 queries, 16 dims
+  __shared__ v4f so[NW][TILES][64];
   __shared__ float sm[NW][CT][16], sl[NW][CT][16];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h4 = lane >> 4;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / a.splits / a.tiles;
@@ -351,42 +361,50 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
   st.clear();
   const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
   constexpr int KU = D / 16, VU = D / 16;  // 1 KB units of a page: keys (4 tiles x D / 64 halves), values (D / 16)
+  // A page's codes are loaded as soon as the registers are free: the next one's keys behind the scores, its values
+  // behind P V. A bad page number reads as a page of zeros.
   uint4 kw[KU], vw[VU];
   float ks = 0.0f, vs = 0.0f;
-  auto load = [&](int pg) {  // a whole page's codes and scales; a bad page number reads as empty
-    int pid = pg < a.c.max_pages ? table[pg] : -1;
-    const bool ok = pid >= 0 && pid < a.c.n_pages;
-    if (!ok && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
-    pid = ok ? pid : 0;
-    const uint8_t* kp = hd.kc + pid * hd.stride + (lane & 15) * D + h4 * 16;
-    const uint8_t* vp = hd.vc + pid * hd.stride + lane % 16 * KV_PAGE + h4 * 16;
-#pragma unroll
-    for (int u = 0; u < KU; ++u)
-      kw[u] = *reinterpret_cast<const uint4*>(kp + u / (D / 64) * 16 * D + u % (D / 64) * 64);
-#pragma unroll
-    for (int u = 0; u < VU; ++u) vw[u] = *reinterpret_cast<const uint4*>(vp + u * 16 * KV_PAGE);
-    const long long at = (long long)pid * H + h;
-    ks = ok ? a.c.k_scale[at] : 0.0f;
-    vs = ok ? a.c.v_scale[at] : 0.0f;
+  int bad = 0;
+  auto page_id = [&](int pg, bool& ok) {
+    const int pid = pg < a.c.max_pages ? table[pg] : -1;
+    ok = pid >= 0 && pid < a.c.n_pages;
+    bad |= !ok;
+    return ok ? pid : 0;
   };
-  auto finish = [&](const v4f (&s)[CT][4], const uint4 (&va)[VU][2], float cs, float v, int pg) {
-    uint4 p[CT][2];
+  const unsigned k0 = (lane & 15) * (D / 16) + h4, v0 = (lane & 15) * 4 + h4;  // in 16-byte pieces
+  auto load_k = [&](int pg) {
+    bool ok;
+    const int pid = page_id(pg, ok);
+    const uint4* p = reinterpret_cast<const uint4*>(hd.kc + pid * hd.stride);
+#pragma unroll
+    for (int u = 0; u < KU; ++u) kw[u] = at_u32(p, k0 + u / (D / 64) * D + u % (D / 64) * 4);
+    ks = ok ? a.c.k_scale[(long long)pid * H + h] : 0.0f;
+  };
+  auto load_v = [&](int pg) {
+    bool ok;
+    const int pid = page_id(pg, ok);
+    const uint4* p = reinterpret_cast<const uint4*>(hd.vc + pid * hd.stride);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) vw[u] = at_u32(p, v0 + u * 64);
+    vs = ok ? a.c.v_scale[(long long)pid * H + h] : 0.0f;
+  };
+  auto weights = [&](const v4f (&s)[CT][4], float cs, float v, int pg, uint4 (&p)[CT][2], float (&pv)[CT]) {
     int lim[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
-    float pv[CT];
     if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p, pv);
     else st.template softmax<true>(s, cs, v, lim, h4, p, pv);
-#pragma unroll
-    for (int d = 0; d < VU; ++d) st.add(d, va[d][0], va[d][1], p, pv);
   };
 
   const int last = min(min(hi, full), cdiv(seen_by_any, KV_PAGE));
   int pg = lo + w;
-  if (pg < last) load(pg);
+  if (pg < last) {
+    load_k(pg);
+    load_v(pg);
+  }
   for (; pg < last; pg += NW) {
     v4f s[CT][4];
-    uint4 va[VU][2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
@@ -402,17 +420,24 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
         }
       }
     }
-#pragma unroll
-    for (int u = 0; u < VU; ++u) widen16<DT, CODES>(vw[u], va[u][0], va[u][1]);
     const float cs = ks * a.scale, v = vs;
-    if (pg + NW < last) load(pg + NW);
-    finish(s, va, cs, v, pg);
+    if (pg + NW < last) load_k(pg + NW);
+    uint4 p[CT][2];
+    float pv[CT];
+    weights(s, cs, v, pg, p, pv);
+#pragma unroll
+    for (int d = 0; d < VU; ++d) {
+      uint4 x, y;
+      widen16<DT, CODES>(vw[d], x, y);
+      st.add(d, x, y, p, pv);
+    }
+    if (pg + NW < last) load_v(pg + NW);
   }
+  if (bad && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
   // the unfinished page, by the wave whose turn it would be
   if (left && full >= lo && full < hi && (full - lo) % NW == w && full * KV_PAGE < seen_by_any) {
     const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
     v4f s[CT][4];
-    uint4 va[VU][2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
@@ -424,13 +449,15 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
         for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
       }
     }
+    uint4 p[CT][2];
+    float pv[CT];
+    weights(s, a.scale, ts.vs, full, p, pv);
 #pragma unroll
-    for (int d = 0; d < VU; ++d)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        va[d][u] = tail_v8<DT>(*reinterpret_cast<const uint4*>(hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4 + 8 * u),
-                               ts.down, 16 * h4 + 8 * u, left);
-    finish(s, va, a.scale, ts.vs, full);
+    for (int d = 0; d < VU; ++d) {
+      const uint16_t* row = hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4;
+      st.add(d, tail_v8<DT>(*reinterpret_cast<const uint4*>(row), ts.down, 16 * h4, left),
+             tail_v8<DT>(*reinterpret_cast<const uint4*>(row + 8), ts.down, 16 * h4 + 8, left), p, pv);
+    }
   }
 
   // join the four waves
@@ -453,37 +480,29 @@ __global__ __launch_bounds__(256) void k_cache_attn_few(AttendArgs a) {
     f[c] = exp2f(st.m[c] - M[c]) * st.unit();
   }
 #pragma unroll
-  for (int d = 0; d < D / 16; ++d) {
-    if (d) __syncthreads();
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
-    for (int c = 0; c < CT; ++c) *reinterpret_cast<v4f*>(&so[w][lane][4 * c]) = st.o[c][d] * f[c];
-    __syncthreads();
-    if (w < CT) {  // wave c adds column tile c
-      v4f t = *reinterpret_cast<const v4f*>(&so[0][lane][4 * w]);
+    for (int d = 0; d < D / 16; ++d) so[w][c * (D / 16) + d][lane] = st.o[c][d] * f[c];
+  __syncthreads();
 #pragma unroll
-      for (int k = 1; k < NW; ++k) t += *reinterpret_cast<const v4f*>(&so[k][lane][4 * w]);
-      float Lw = L[0], Mw = M[0];
+  for (int i = 0; i < TILES / NW; ++i) {  // wave w's tiles
+    const int tile = i * NW + w, c = i * NW / (D / 16), d = tile % (D / 16);
+    v4f t = so[0][tile][lane];
 #pragma unroll
-      for (int c = 1; c < CT; ++c) {
-        Lw = w == c ? L[c] : Lw;
-        Mw = w == c ? M[c] : Mw;
-      }
-      const int r = row0 + 16 * w + (lane & 15);
-      if (r < rows) {
-        const int dim = 16 * d + 4 * h4;
-        if (a.splits == 1) {
-          const int tok = r / a.G, hq = h * a.G + r % a.G;
-          const float inv = Lw == 0.0f ? 0.0f : 1.0f / Lw;
-          const v4f y = t * inv;
-          store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, y, a.ovec);
-        } else {
-          const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
-          *reinterpret_cast<v4f*>(a.part_o + at * D + dim) = t;
-          if (d == 0 && lane < 16) {
-            a.part_ml[2 * at] = Mw;
-            a.part_ml[2 * at + 1] = Lw;
-          }
-        }
+    for (int k = 1; k < NW; ++k) t += so[k][tile][lane];
+    const int r = row0 + 16 * c + (lane & 15);
+    if (r >= rows) continue;
+    const int dim = 16 * d + 4 * h4;
+    if (a.splits == 1) {
+      const int tok = r / a.G, hq = h * a.G + r % a.G;
+      const float inv = L[c] == 0.0f ? 0.0f : 1.0f / L[c];
+      store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, t * inv, a.ovec);
+    } else {
+      const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
+      *reinterpret_cast<v4f*>(a.part_o + at * D + dim) = t;
+      if (d == 0 && lane < 16) {
+        a.part_ml[2 * at] = M[c];
+        a.part_ml[2 * at + 1] = L[c];
       }
     }
   }

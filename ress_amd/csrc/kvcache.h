@@ -15,6 +15,7 @@
 #include "common.h"
 
 constexpr int KV_PAGE = 64;
+constexpr int KV_LINE = 32;                // ints from one slot's `arrived` to the next: a cache line
 constexpr int KV_I8 = 0, KV_FP8 = 1;       // ress_kv_cache.codes
 constexpr int KV_BF16 = 1, KV_F16 = 2;     // ress_kv_cache.dtype
 // ress_kv_cache.status bits

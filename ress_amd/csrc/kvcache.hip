@@ -16,6 +16,7 @@
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int QH = 4;  // query heads a workgroup rotates together
 
 struct AppendArgs {
   ress_kv_cache c;
@@ -63,10 +64,11 @@ __device__ __forceinline__ void rotate(uint4& a, uint4& b, const float* __restri
   b = pack8(rb);
 }
 
-// The table row of a token, its positions clamped into the table (and the fault noted).
-__device__ __forceinline__ const float* rope_row(const AppendArgs& a, int b, int i, int axis, int half) {
+// The table row of a token, its positions clamped into the table (`out` set, for the status word: an atomic here would
+// keep the loads behind it from being issued early).
+__device__ __forceinline__ const float* rope_row(const AppendArgs& a, int b, int i, int axis, int half, bool& out) {
   const long long p = a.pos[((long long)b * a.n + i) * a.axes + axis];
-  if (p < 0 || p >= a.positions) atomicOr(a.c.status, KV_ST_POS);
+  out = out || p < 0 || p >= a.positions;
   const long long pc = p < 0 ? 0 : p >= a.positions ? a.positions - 1 : p;
   return a.rope + pc * 2 * half;
 }
@@ -95,35 +97,76 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
   const int half = D / 2 / a.axes;
   const Pair<D> pr(t % LPR, a.axes);
 
-  if ((int)blockIdx.x >= kv_groups) {  // the queries: ROWS rows of (B, Hq, n) a workgroup
-    const long long row = (long long)(blockIdx.x - kv_groups) * ROWS + t / LPR;
-    if (row >= (long long)a.B * a.Hq * a.n) return;
-    const int i = (int)(row % a.n), h = (int)(row / a.n % a.Hq), b = (int)(row / a.n / a.Hq);
-    uint4 x = make_uint4(0, 0, 0, 0), y = x;
-    if (i < new_tokens(a.new_lens, b, a.n)) {
-      const uint16_t* src = a.q + b * a.sqb + h * a.sqh + i * a.sqt;
-      x = ld8(src + pr.x1, a.vec);
-      y = ld8(src + pr.x2, a.vec);
-      const float* tb = rope_row(a, b, i, pr.axis, half) + pr.f;
-      rotate<DT>(x, y, tb, tb + half);
+  bool outside = false;
+  if ((int)blockIdx.x >= kv_groups) {  // the queries: ROWS tokens of QH heads a workgroup, the table read once for them
+    const int hgs = cdiv(a.Hq, QH), tgs = cdiv(a.n, ROWS);
+    int g = blockIdx.x - kv_groups;
+    const int tg = g % tgs, hg = g / tgs % hgs, b = g / tgs / hgs, i = tg * ROWS + t / LPR, h0 = hg * QH;
+    if (i >= a.n) return;
+    const bool there = i < new_tokens(a.new_lens, b, a.n);
+    uint4 x[QH], y[QH];
+#pragma unroll
+    for (int j = 0; j < QH; ++j) {
+      x[j] = y[j] = make_uint4(0, 0, 0, 0);
+      if (there && h0 + j < a.Hq) {
+        const uint16_t* src = a.q + b * a.sqb + (h0 + j) * a.sqh + i * a.sqt;
+        x[j] = ld8(src + pr.x1, a.vec);
+        y[j] = ld8(src + pr.x2, a.vec);
+      }
     }
-    uint16_t* dst = a.q_out + row * D;
-    *reinterpret_cast<uint4*>(dst + pr.x1) = x;
-    *reinterpret_cast<uint4*>(dst + pr.x2) = y;
+    float cs[8], sn[8];
+    if (there) {
+      const float* tb = rope_row(a, b, i, pr.axis, half, outside) + pr.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = tb[j];
+        sn[j] = tb[half + j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < QH; ++j) {
+      if (h0 + j >= a.Hq) break;
+      if (there) rotate<DT>(x[j], y[j], cs, sn);
+      uint16_t* dst = a.q_out + (((long long)b * a.Hq + h0 + j) * a.n + i) * D;
+      *reinterpret_cast<uint4*>(dst + pr.x1) = x[j];
+      *reinterpret_cast<uint4*>(dst + pr.x2) = y[j];
+    }
+    if (outside) atomicOr(a.c.status, KV_ST_POS);
     return;
   }
 
   const int part = blockIdx.x % a.pages, h = blockIdx.x / a.pages % H, b = blockIdx.x / a.pages / H;
   const int slot = a.slots ? a.slots[b] : b;
-  const int len = a.c.lens[slot], cap = a.c.held[slot] * KV_PAGE;
-  const int want = len + new_tokens(a.new_lens, b, a.n), end = min(want, cap);
-  const int p0 = len / KV_PAGE, p1 = end / KV_PAGE;  // pages p0..p1-1 get full, p1 stays open
-  if (t == 0 && part == 0 && h == 0 && want > cap) atomicOr(a.c.status, KV_ST_FULL);
 
+  const int len = a.c.lens[slot], cap = a.c.held[slot] * KV_PAGE, fresh = new_tokens(a.new_lens, b, a.n);
   const long long tail = ((long long)slot * H + h) * KV_PAGE * D;
   uint16_t* tail_k = reinterpret_cast<uint16_t*>(a.c.tail_k) + tail;
   uint16_t* tail_v = reinterpret_cast<uint16_t*>(a.c.tail_v) + tail;
   float* tail_top = a.c.tail_top + (long long)slot * H + h;
+  const float top0 = part == 0 ? *tail_top : 0.0f;
+
+  // new token i of the sequence, this lane's dims, rotated
+  auto token = [&](int i, uint4& kx, uint4& ky, uint4& vx, uint4& vy) {
+    const uint16_t* ks = a.k + b * a.skb + h * a.skh + i * a.skt;
+    const uint16_t* vs = a.v + b * a.svb + h * a.svh + i * a.svt;
+    kx = ld8(ks + pr.x1, a.vec);
+    ky = ld8(ks + pr.x2, a.vec);
+    vx = ld8(vs + pr.x1, a.vec);
+    vy = ld8(vs + pr.x2, a.vec);
+    if (a.pos) {
+      const float* tb = rope_row(a, b, i, pr.axis, half, outside) + pr.f;
+      rotate<DT>(kx, ky, tb, tb + half);
+    }
+  };
+  // The first tokens (all of them in a decoding step) on their way before the sequence's length is known, for the
+  // case that they fill no page.
+  const int mine = t / LPR;
+  uint4 kx0, ky0, vx0, vy0;
+  kx0 = ky0 = vx0 = vy0 = make_uint4(0, 0, 0, 0);
+  if (a.n < KV_PAGE && part == 0 && mine < fresh) token(mine, kx0, ky0, vx0, vy0);
+  const int want = len + fresh, end = min(want, cap);
+  const int p0 = len / KV_PAGE, p1 = end / KV_PAGE;  // pages p0..p1-1 get full, p1 stays open
+  if (t == 0 && part == 0 && h == 0 && want > cap) atomicOr(a.c.status, KV_ST_FULL);
 
   auto page = [&](int pg, bool full) {
     uint4 kx[IT], ky[IT], vx[IT], vy[IT];
@@ -147,17 +190,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
           vy[it] = pack8(f);
         }
       } else if (tok < end) {
-        const int i = tok - len;
-        const uint16_t* ks = a.k + b * a.skb + h * a.skh + i * a.skt;
-        const uint16_t* vs = a.v + b * a.svb + h * a.svh + i * a.svt;
-        kx[it] = ld8(ks + pr.x1, a.vec);
-        ky[it] = ld8(ks + pr.x2, a.vec);
-        vx[it] = ld8(vs + pr.x1, a.vec);
-        vy[it] = ld8(vs + pr.x2, a.vec);
-        if (a.pos) {
-          const float* tb = rope_row(a, b, i, pr.axis, half) + pr.f;
-          rotate<DT>(kx[it], ky[it], tb, tb + half);
-        }
+        token(tok - len, kx[it], ky[it], vx[it], vy[it]);
       }
       ktop = top_bits(ky[it], top_bits(kx[it], ktop));
       vtop = top_bits(vy[it], top_bits(vx[it], vtop));
@@ -195,7 +228,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
       }
       if (t == 0) {
         // the tokens of an earlier call in this page count too; a NaN stays
-        const float old = pg * KV_PAGE < len ? *tail_top : 0.0f;
+        const float old = pg * KV_PAGE < len ? top0 : 0.0f;
         *tail_top = vbad || old != old ? nan : fmaxf(old, vt_);
       }
       return;
@@ -244,19 +277,45 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
     }
   };
 
-  if (part == 0) {
+  if (part == 0 && p1 == p0 && a.n < KV_PAGE) {
+    uint32_t top = 0;
+    for (int i = mine; i < end - len; i += ROWS) {
+      if (i != mine) token(i, kx0, ky0, vx0, vy0);
+      const int r = len - p0 * KV_PAGE + i, pl = v_place(r);
+      *reinterpret_cast<uint4*>(tail_k + r * D + pr.x1) = kx0;
+      *reinterpret_cast<uint4*>(tail_k + r * D + pr.x2) = ky0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        tail_v[(pr.x1 + j) * KV_PAGE + pl] = elem8(vx0, j);
+        tail_v[(pr.x2 + j) * KV_PAGE + pl] = elem8(vy0, j);
+      }
+      top = top_bits(vy0, top_bits(vx0, top));
+    }
+    top = wave_max_u32(top);
+    if ((t & 63) == 0) red[0][t >> 6] = top;
+    __syncthreads();
+    if (t == 0 && end > len) {
+#pragma unroll
+      for (int w = 1; w < THREADS / 64; ++w) top = max(top, red[0][w]);
+      const float old = p0 * KV_PAGE < len ? top0 : 0.0f;
+      *tail_top = top >= Elem<DT>::INF || old != old ? __uint_as_float(0x7fc00000u)
+                                                     : fmaxf(old, Elem<DT>::get((uint16_t)top));
+    }
+  } else if (part == 0) {
     if (p1 > p0) page(p0, true);
     if (end > max(len, p1 * KV_PAGE)) page(p1, false);
   } else if (p0 + part < p1) {
     page(p0 + part, true);
   }
 
+  if (outside) atomicOr(a.c.status, KV_ST_POS);
   // The last workgroup of the sequence to finish moves its length on: each has read it by then.
   __syncthreads();
   if (t == 0) {
     const int all = a.pages * H;
-    if (atomicAdd(a.c.arrived + slot, 1) == all - 1) {
-      a.c.arrived[slot] = 0;
+    int* arrived = a.c.arrived + (long long)slot * KV_LINE;  // a line of its own: sharing one cost 6 ns an arrival
+    if (atomicAdd(arrived, 1) == all - 1) {
+      *arrived = 0;
       a.c.lens[slot] = max(end, len);
     }
   }
@@ -291,7 +350,13 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
   const long long at = (long long)pid * H + h;
   const long long tail = ((long long)slot * H + h) * KV_PAGE * D;
   const float ks = pid >= 0 ? c.k_scale[at] : 0.0f, vs = pid >= 0 ? c.v_scale[at] : 0.0f;
-  // values: the page's rows of 64 places, in the order of the places, into LDS
+  // the keys on their way, then the page's values, rows of 64 places in their order, into LDS
+  constexpr int KI = KV_PAGE * D / 8 / THREADS;
+  uint2 kc[KI];
+#pragma unroll
+  for (int j = 0; j < KI; ++j)
+    if (pid >= 0)
+      kc[j] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(c.k_codes) + at * KV_PAGE * D + (t + j * THREADS) * 8);
   for (int i = t; i < D * KV_PAGE / 8; i += THREADS) {
     const int d = i >> 3, p = (i & 7) * 8;
     uint4 w = make_uint4(0, 0, 0, 0);
@@ -308,8 +373,9 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
     dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
   }
   __syncthreads();
-  for (int i = t; i < KV_PAGE * D / 8; i += THREADS) {
-    const int r = i / (D / 8), d = (i % (D / 8)) * 8;
+#pragma unroll
+  for (int it = 0; it < KI; ++it) {
+    const int i = t + it * THREADS, r = i / (D / 8), d = (i % (D / 8)) * 8;
     const long long tok = lo + r;
     if (tok < s0 || tok >= s0 + n) continue;
     uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
@@ -317,7 +383,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
       if (open) {
         kw = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(c.tail_k) + tail + r * D + d);
       } else if (pid >= 0) {
-        const uint2 cv = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(c.k_codes) + at * KV_PAGE * D + r * D + d);
+        const uint2 cv = kc[it];
         uint16_t e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = Elem<DT>::put(code_value<CODES>((uint8_t)((j < 4 ? cv.x : cv.y) >> (8 * (j & 3)))) * ks);
@@ -350,8 +416,7 @@ template <int DT, int CODES, int D>
 struct Append {
   static int go(const AppendArgs& a, hipStream_t stream) {
     const long long kv = (long long)a.B * a.c.kv_heads * a.pages;
-    const long long rows = THREADS / (D / 16);
-    const long long qg = a.q_out ? ((long long)a.B * a.Hq * a.n + rows - 1) / rows : 0;
+    const long long qg = a.q_out ? (long long)a.B * cdiv(a.Hq, QH) * cdiv(a.n, THREADS / (D / 16)) : 0;
     RESS_REQUIRE(kv + qg < (1ll << 31), "ress_kv_append: the call needs more than 2^31 workgroups");
     hipLaunchKernelGGL((k_kv_append<DT, CODES, D>), dim3((unsigned)(kv + qg)), dim3(THREADS), 0, stream, a, (int)kv);
     RESS_LAUNCHED("k_kv_append");

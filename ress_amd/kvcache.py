@@ -144,11 +144,15 @@ class PagedKVCache:
         self.lens = self._state[2 * tail + 4 * S * H:].view(torch.int32)
         self.table = torch.full((S, self.max_pages), -1, dtype=torch.int32, device=dev)
         self.held = torch.zeros(S, dtype=torch.int32, device=dev)
-        self._arrived = torch.zeros(S, dtype=torch.int32, device=dev)
+        self._arrived = torch.zeros(S, 32, dtype=torch.int32, device=dev)
         self._status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._free = list(range(P - 1, -1, -1))
         self._pages = [[] for _ in range(S)]
         self._bound = [0] * S     # no slot holds more tokens than this
+        self._cap = [0] * S       # tokens that a slot's pages have room for
+        # Appends of one batch that needed no pages, not yet in _bound: `_lag` tokens for each slot of `_key` (a
+        # SlotBatch, or B for slots 0..B-1), which has room for `_slack` more and holds at most `_most`.
+        self._key, self._lag, self._slack, self._most = None, 0, 0, 0
         self._captured = False    # a captured append moves lengths that the host does not see
         self._snapshots = weakref.WeakSet()
         self._serial = 0
@@ -181,13 +185,21 @@ class PagedKVCache:
             raise ValueError(f"the batch has {B} rows and {len(slots)} slots, or they belong to another cache")
         return slots.ids, slots.tensor
 
+    def _settle(self):
+        """Brings _bound up to date."""
+        if self._lag:
+            for i in range(self._key) if isinstance(self._key, int) else self._key.ids:
+                self._bound[i] = min(self._bound[i] + self._lag, self._cap[i])
+        self._key, self._lag = None, 0
+
     def free_pages(self):
         return len(self._free)
 
     def lengths(self):
         """Tokens in each slot (waits for the device)."""
         got = self.lens.tolist()
-        self._bound = list(got)
+        self._key, self._lag = None, 0
+        self._bound[:] = got
         return got
 
     def _room(self, ids, more, exact):
@@ -204,7 +216,7 @@ class PagedKVCache:
         if self._captured and not capturing:
             self.lengths()
         need = wanted()
-        if all(n <= PAGE * len(self._pages[i]) for i, n in need.items()):
+        if all(n <= self._cap[i] for i, n in need.items()):
             return
         if capturing:
             raise RuntimeError("an append inside a graph capture needs its pages reserved before (reserve)")
@@ -235,6 +247,7 @@ class PagedKVCache:
             return
         new = [self._free.pop() for _ in range(need - have)]
         self._pages[slot] += new
+        self._cap[slot] = PAGE * need
         with torch.cuda.device(self.device):
             self.table[slot, have:need] = torch.tensor(new, dtype=torch.int32, device=self.device)
             self.held[slot:slot + 1].fill_(need)
@@ -244,6 +257,7 @@ class PagedKVCache:
         itself what it needs, except inside a graph capture."""
         if not 0 <= slot < self.max_seqs:
             raise IndexError(f"slot must lie in 0..{self.max_seqs - 1}, got {slot}")
+        self._settle()
         self._fits({slot: int(n_tokens)}, refuse=True)
         self._take(slot, int(n_tokens))
 
@@ -251,21 +265,22 @@ class PagedKVCache:
         """Empties a slot and gives its pages back. Work that reads them has to be ordered before."""
         if not 0 <= slot < self.max_seqs:
             raise IndexError(f"slot must lie in 0..{self.max_seqs - 1}, got {slot}")
+        self._settle()
         with torch.cuda.device(self.device):
             self.held[slot:slot + 1].fill_(0)
             self.lens[slot:slot + 1].fill_(0)
             self.table[slot].fill_(-1)
         self._free += reversed(self._pages[slot])
         self._pages[slot] = []
-        self._bound[slot] = 0
+        self._bound[slot] = self._cap[slot] = 0
         for snap in self._snapshots:
             snap.alive = False
 
     def snapshot(self):
         """The state that restore goes back to (a copy of the unfinished pages and the lengths)."""
+        self._settle()
         self._serial += 1
-        with torch.cuda.device(self.device):
-            snap = Snapshot(self._state.clone(), list(self._bound), self._serial)
+        snap = Snapshot(self._state.clone(), list(self._bound), self._serial)
         self._snapshots.add(snap)
         return snap
 
@@ -276,12 +291,13 @@ class PagedKVCache:
             raise ValueError("the snapshot belongs to another cache")
         if not snapshot.alive:
             raise RuntimeError("the snapshot no longer holds: a slot was released, or an older snapshot restored, since")
-        with torch.cuda.device(self.device):
-            self._state.copy_(snapshot.state)
-        self._bound = list(snapshot.bounds)
-        for snap in self._snapshots:
-            if snap.serial > snapshot.serial:
-                snap.alive = False
+        self._state.copy_(snapshot.state)
+        self._key, self._lag = None, 0
+        self._bound[:] = snapshot.bounds
+        if snapshot.serial < self._serial:
+            for snap in self._snapshots:
+                if snap.serial > snapshot.serial:
+                    snap.alive = False
 
     def check(self):
         """Raises if a call since the last check met something it could not do (waits for the device)."""
@@ -292,6 +308,14 @@ class PagedKVCache:
 
     # ---- operands -----------------------------------------------------------
     def _operand(self, t, name, heads=None, like=None):
+        """Strides of a (B, heads, n, head_dim) operand; raises what is wrong with one."""
+        if torch.is_tensor(t) and t.dtype is self.dtype and t.device == self.device and t.dim() == 4:
+            B, H, n, D = t.shape
+            st = t.stride()
+            if (D == self.head_dim and st[3] == 1 and (heads is None or H == heads)
+                    and (like is None or (B == like.shape[0] and n == like.shape[2]))
+                    and not (t.requires_grad and torch.is_grad_enabled())):
+                return st[:3]
         if not torch.is_tensor(t) or not t.is_cuda:
             raise RuntimeError(f"{name} must be a device tensor (the cache lives on the GPU)")
         if t.device != self.device:
@@ -304,18 +328,17 @@ class PagedKVCache:
             raise ValueError(f"{name} must have the batch and tokens of k, ({like.shape[0]}, {like.shape[2]}), got {tuple(t.shape)}")
         if t.stride(3) != 1:
             raise ValueError(f"{name} must have a unit-stride head dim")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires grad: the cache has no backward pass (use torch.no_grad())")
+        raise RuntimeError(f"{name} requires grad: the cache has no backward pass (use torch.no_grad())")
 
     def _new_lens(self, new_lens, B, n):
-        """(device int32 (B,) or None, upper bounds on the host)."""
+        """(device int32 (B,) or None, counts on the host: empty where they are n or not known but for that)."""
         if new_lens is None:
-            return None, [n] * B
+            return None, ()
         if torch.is_tensor(new_lens):
             if new_lens.device != self.device or new_lens.dtype != torch.int32 or tuple(new_lens.shape) != (B,):
                 raise ValueError(f"new_lens must be ({B},) int32 on {self.device}, got {tuple(new_lens.shape)} "
                                  f"{new_lens.dtype} on {new_lens.device}")
-            return new_lens.contiguous(), [n] * B
+            return new_lens.contiguous(), ()
         got = [int(x) for x in new_lens]
         if len(got) != B or any(not 0 <= x <= n for x in got):
             raise ValueError(f"new_lens must be {B} counts of 0..{n}, got {got}")
@@ -335,39 +358,59 @@ class PagedKVCache:
         pos (B, n) or (B, n, axes) with a RotaryTable `rope`: k, and the queries q (B, heads, n, head_dim) if
         given, are rotated by it on the way. Returns the rotated queries (zeros in padding), or None.
         Positions outside the table are clamped and reported by check()."""
-        self._operand(k, "k", self.kv_heads)
-        self._operand(v, "v", self.kv_heads, like=k)
+        ks = self._operand(k, "k", self.kv_heads)
+        vs = self._operand(v, "v", self.kv_heads, like=k)
         B, n = k.shape[0], k.shape[2]
         ids, slot_t = self._batch(slots, B)
         if (pos is None) != (rope is None):
             raise ValueError("pos and rope go together")
+        qs, q_out, q_heads = (0, 0, 0), None, 0
         if q is not None:
             if pos is None:
                 raise ValueError("queries are rotated beside the keys: q needs pos and rope")
-            self._operand(q, "q", like=k)
+            qs = self._operand(q, "q", like=k)
+            q_heads = q.shape[1]
         axes, positions, table = 1, 0, None
         if pos is not None:
-            axes, table, positions = rope.axes, rope.table, rope.table.shape[0]
+            axes, table = rope.axes, rope.table
+            positions = table.shape[0]
             if rope.head_dim != self.head_dim or table.device != self.device:
                 raise ValueError(f"rope is for head_dim {rope.head_dim} on {table.device}, the cache has {self.head_dim} on {self.device}")
             want = ((B, n), (B, n, 1)) if axes == 1 else ((B, n, 2),)
             if tuple(pos.shape) not in want or pos.is_floating_point():
                 raise ValueError(f"pos must be {want[0]} whole numbers, got {tuple(pos.shape)} {pos.dtype}")
-            pos = pos.to(device=self.device, dtype=torch.int64).contiguous()
+            if pos.dtype is not torch.int64 or pos.device != self.device:
+                pos = pos.to(device=self.device, dtype=torch.int64)
+            pos = pos.contiguous()
         lens_t, counts = self._new_lens(new_lens, B, n)
-        q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        if q is not None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         if B == 0 or n == 0:
             return q_out
-        self._room(ids, counts, exact=not torch.is_tensor(new_lens))
-        qs = (0, 0, 0) if q is None else q.stride()[:3]
-        P = _lib.ptr
-        self._call("ress_kv_append", self._handle, P(k), *k.stride()[:3], P(v), *v.stride()[:3], P(q), *qs, B,
-                   0 if q is None else q.shape[1], n, P(pos), P(table), positions, axes, P(slot_t), P(lens_t), P(q_out))
-        if torch.cuda.is_current_stream_capturing():
-            self._captured = True
+        capturing = torch.cuda.is_current_stream_capturing()
+        key = B if slot_t is None else slots
+        same = not counts and key == self._key and n <= self._slack and not self._captured and not capturing
+        if same:
+            self._lag += n
+            self._slack -= n
+            self._most += n
         else:
-            for i, c in zip(ids, counts):
-                self._bound[i] = min(self._bound[i] + c, PAGE * len(self._pages[i]))
+            self._settle()
+            counts = counts or [n] * B
+            bound, cap = self._bound, self._cap
+            if self._captured or capturing or any(bound[i] + c > cap[i] for i, c in zip(ids, counts)):
+                self._room(ids, counts, exact=not torch.is_tensor(new_lens))
+            if capturing:
+                self._captured = True
+            else:
+                for i, c in zip(ids, counts):
+                    bound[i] = min(bound[i] + c, cap[i])
+                if isinstance(key, (int, SlotBatch)):
+                    self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
+                    self._most = max(bound[i] for i in ids)
+        P = _lib.ptr
+        self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),
+                   positions, axes, P(slot_t), P(lens_t), P(q_out))
         return q_out
 
     def read(self, n, slots=None, start=None, batch=None):
@@ -399,7 +442,7 @@ class PagedKVCache:
 
         Returns (B, heads, n, head_dim), zeros in padding and in rows that see nothing; a given `out` is
         written in place, its padding left as it was."""
-        self._operand(q, "q")
+        qs = self._operand(q, "q")
         B, Hq, n, D = q.shape
         if Hq == 0 or Hq % self.kv_heads:
             raise ValueError(f"q must have a multiple of {self.kv_heads} heads, got {Hq}")
@@ -410,8 +453,9 @@ class PagedKVCache:
             raise ValueError(f"scale must be positive and finite, got {scale}")
         if out is None:
             out = (torch.empty if lens_t is None else torch.zeros)(q.shape, dtype=q.dtype, device=self.device)
+            os = out.stride()[:3]
         else:
-            self._operand(out, "out")
+            os = self._operand(out, "out")
             if out.shape != q.shape:
                 raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
             if any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape)):
@@ -419,12 +463,15 @@ class PagedKVCache:
         if q.numel() == 0:
             return out
         if self._captured or torch.cuda.is_current_stream_capturing():
-            most = max(len(self._pages[i]) for i in ids) * PAGE
+            most = max(self._cap[i] for i in ids)
+        elif self._key is not None and self._key == (B if slot_t is None else slots):
+            most = self._most
         else:
+            self._settle()
             most = max(self._bound[i] for i in ids)
-        size = _lib.lib().ress_kv_attend_workspace_size(self._handle, B, Hq, n, most)
+        size = (_lib._lib or _lib.lib()).ress_kv_attend_workspace_size(self._handle, B, Hq, n, most)
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        self._call("ress_kv_attend", self._handle, _lib.ptr(q), *q.stride()[:3], B, Hq, n, _lib.ptr(slot_t),
-                   _lib.ptr(lens_t), 1 if causal else 0, scale, most, _lib.ptr(out), *out.stride()[:3],
-                   _lib.ptr(work), size)
+        P = _lib.ptr
+        self._call("ress_kv_attend", self._handle, P(q), *qs, B, Hq, n, P(slot_t), P(lens_t), 1 if causal else 0, scale,
+                   most, P(out), *os, P(work), size)
         return out
