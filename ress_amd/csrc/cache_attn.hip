@@ -12,9 +12,10 @@
 // LAZY = 8 (in log2) above its row's m: P is then at most 2^8, sums are unaffected, and most pages need
 // neither the exchange between a row's four lanes nor a pass over the accumulators.
 //
-// v_scale. In bf16 it enters as an addend of the exponent (PageScale), relative to a power of two, so it costs no
-// multiplication per element. fp16 has no exponents to spare for that: there a page's P V is formed by itself and
-// added times v_scale in fp32, one multiply-add per output element and page.
+// v_scale. In bf16 it enters as an addend of the exponent (PageScale), relative to a power of two: the codes stay whole
+// and it costs no multiplication per element. fp16 has no exponents to spare for that: there the codes are multiplied,
+// as they are widened, by v_scale rounded to fp16 (the values are in fp16's range, as the values they came from were),
+// and what that rounding took enters the exponent.
 // The sum of P is a product with ones on the matrix cores, of the rounded P, so numerator and denominator carry the
 // same roundings.
 //
@@ -112,34 +113,43 @@ struct Head {
   }
 };
 
-// The tail's values are scaled by a power of two to at most 128 (like codes), undone by its v_scale; NaN
-// where a value is not finite.
+// The unfinished page's values as the second product takes them. bf16: scaled by a power of two to at most 128 (like
+// codes), undone by its v_scale, so that it does not set R off. fp16: as they are. NaN v_scale (and values 0) where one
+// is not finite.
+template <int DT>
 struct TailScale {
   float down, vs;  // multiply the values by down, P by vs
-  bool bad;
   __device__ __forceinline__ explicit TailScale(float top) {
-    bad = top != top;
+    const bool bad = top != top;
     int e = 0;
-    if (!bad && top > 0.0f) frexpf(top, &e);  // top < 2^e
-    e = min(max(e - 7, -100), 100);
+    if (DT == KV_BF16 && !bad && top > 0.0f) {
+      frexpf(top, &e);  // top < 2^e
+      e = min(max(e - 7, -100), 100);
+    }
     down = bad ? 0.0f : ldexpf(1.0f, -e);
     vs = bad ? __uint_as_float(0x7fc00000u) : ldexpf(1.0f, e);
   }
 };
 
-// bf16: a page's v_scale relative to R = 2^eR, a power of two at least as large as any v_scale met so far (exact to
-// rescale by, so a row's bits do not hang on the pages that only its neighbours see): P comes out of the
-// exponential already multiplied by v_scale / R, and its sum is divided by that again. At most 2^-60 of R is lost to
-// the clamp (a page of zeros has v_scale 0). fp16: P is lifted by 2^7 (it is at most 2^LAZY, so below 2^15), which
-// the quotient of sums takes out again.
+// How a page's v_scale enters P: P comes out of the exponential times 2^lift, and its sum is multiplied by `down` again.
+// bf16: relative to R = 2^eR, a power of two at least as large as any v_scale met so far (exact to rescale by, so a row's
+// bits do not hang on the pages that only its neighbours see); at most 2^-60 of R is lost to the clamp (a page of
+// zeros has v_scale 0). fp16: P is lifted by 2^7 (it is at most 2^LAZY, so below 2^15), which the quotient of the sums
+// takes out again, and carries v_scale / value_scale(v_scale).
+template <int DT>
+__device__ __forceinline__ float value_scale(float vs) {
+  if constexpr (DT == KV_BF16) return 1.0f;
+  // never 0 (the smallest subnormal serves the smallest scales) and finite, so that 0 * V is 0
+  return vs > 0.0f ? fmaxf((float)(_Float16)vs, 0x1p-24f) : 1.0f;
+}
 template <int DT>
 struct PageScale {
-  float lift;  // bf16: log2(v_scale / R); fp16: 7
-  float down;  // bf16: 2^-lift; fp16: 1
+  float lift, down;
   __device__ __forceinline__ PageScale(float vs, int eR) {
     if constexpr (DT == KV_F16) {
-      lift = 7.0f;
-      down = 1.0f;
+      const float r = vs == 0.0f ? 1.0f : vs / value_scale<DT>(vs);  // within 2^-8 .. 1 + 2^-11; NaN stays
+      lift = 7.0f + __builtin_amdgcn_logf(r);
+      down = 1.0f / r;
     } else {
       const float q = __builtin_amdgcn_logf(ldexpf(vs, -eR));  // log2
       lift = q < -60.0f ? -60.0f : q;                          // NaN stays
@@ -165,11 +175,10 @@ struct Rows {
     }
   }
 
-  // Scores s of 64 keys -> P as the second product's B operand p, and in fp16 what its product with the codes is
-  // to be multiplied by. cs = k_scale * sm_scale * log2(e). MASK: query c sees the tile's keys below lim[c].
+  // Scores s of 64 keys -> P as the second product's B operand p. cs = k_scale * sm_scale * log2(e). MASK: query c sees the tile's keys below lim[c].
   template <bool MASK>
   __device__ __forceinline__ void softmax(const v4f (&s)[CT][4], float cs, float vs, const int (&lim)[CT], int h4,
-                                          uint4 (&p)[CT][2], float (&pv)[CT]) {
+                                          uint4 (&p)[CT][2]) {
     int below[CT];  // the lane's keys 16 k + 4 h4 + r that are seen: 16 k + r < below
 #pragma unroll
     for (int c = 0; c < CT; ++c) below[c] = lim[c] - 4 * h4;
@@ -249,24 +258,14 @@ struct Rows {
       v4f t = {0.0f, 0.0f, 0.0f, 0.0f};
       t = mfma<DT>(ones, p[c][0], t);
       t = mfma<DT>(ones, p[c][1], t);
-      const bool none = MASK && lim[c] <= 0;  // 0 * NaN would not be 0
-      l[c] = none ? l[c] : fmaf(t[0], ps.down, l[c]);
-      pv[c] = none ? 0.0f : vs;
+      l[c] = MASK && lim[c] <= 0 ? l[c] : fmaf(t[0], ps.down, l[c]);  // 0 * NaN would not be 0
     }
   }
 
   // o of dims 16 d.. += P V, the page's values as the A operands a (32 keys each)
-  __device__ __forceinline__ void add(int d, const uint4& a0, const uint4& a1, const uint4 (&p)[CT][2], const float (&pv)[CT]) {
+  __device__ __forceinline__ void add(int d, const uint4& a0, const uint4& a1, const uint4 (&p)[CT][2]) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      if constexpr (DT == KV_BF16) {
-        o[c][d] = mfma<DT>(a1, p[c][1], mfma<DT>(a0, p[c][0], o[c][d]));
-      } else {
-        const v4f t = mfma<DT>(a1, p[c][1], mfma<DT>(a0, p[c][0], v4f{0.0f, 0.0f, 0.0f, 0.0f}));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[c][d][r] = fmaf(t[r], pv[c], o[c][d][r]);
-      }
-    }
+    for (int c = 0; c < CT; ++c) o[c][d] = mfma<DT>(a1, p[c][1], mfma<DT>(a0, p[c][0], o[c][d]));
   }
 
   // The factor that takes o to its own units
@@ -308,6 +307,17 @@ __device__ __forceinline__ void widen16(const uint4& w, uint4& a, uint4& b) {
   const uint2 x = widen4<DT, CODES>(w.x), y = widen4<DT, CODES>(w.y), z = widen4<DT, CODES>(w.z), u = widen4<DT, CODES>(w.w);
   a = make_uint4(x.x, x.y, y.x, y.y);
   b = make_uint4(z.x, z.y, u.x, u.y);
+}
+// 16 codes of values widened, times value_scale (fp16: one more packed multiplication for two)
+template <int DT, int CODES>
+__device__ __forceinline__ void widen16_v(const uint4& w, float scale, uint4& a, uint4& b) {
+  widen16<DT, CODES>(w, a, b);
+  if constexpr (DT == KV_F16) {
+    const v2h m = {(_Float16)scale, (_Float16)scale};
+    auto times = [&](uint32_t& x) { x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, x) * m); };
+    times(a.x); times(a.y); times(a.z); times(a.w);
+    times(b.x); times(b.y); times(b.z); times(b.w);
+  }
 }
 // 16-bit tail values times a power of two; places of tokens from cnt on are zero
 template <int DT>
@@ -389,12 +399,12 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     for (int u = 0; u < VU; ++u) vw[u] = at_u32(p, v0 + u * 64);
     vs = ok ? a.c.v_scale[(long long)pid * H + h] : 0.0f;
   };
-  auto weights = [&](const v4f (&s)[CT][4], float cs, float v, int pg, uint4 (&p)[CT][2], float (&pv)[CT]) {
+  auto weights = [&](const v4f (&s)[CT][4], float cs, float v, int pg, uint4 (&p)[CT][2]) {
     int lim[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
-    if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p, pv);
-    else st.template softmax<true>(s, cs, v, lim, h4, p, pv);
+    if (pg * KV_PAGE + KV_PAGE <= seen_by_all) st.template softmax<false>(s, cs, v, lim, h4, p);
+    else st.template softmax<true>(s, cs, v, lim, h4, p);
   };
 
   const int last = min(min(hi, full), cdiv(seen_by_any, KV_PAGE));
@@ -423,20 +433,20 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     const float cs = ks * a.scale, v = vs;
     if (pg + NW < last) load_k(pg + NW);
     uint4 p[CT][2];
-    float pv[CT];
-    weights(s, cs, v, pg, p, pv);
+    weights(s, cs, v, pg, p);
+    const float vscale = value_scale<DT>(v);
 #pragma unroll
     for (int d = 0; d < VU; ++d) {
       uint4 x, y;
-      widen16<DT, CODES>(vw[d], x, y);
-      st.add(d, x, y, p, pv);
+      widen16_v<DT, CODES>(vw[d], vscale, x, y);
+      st.add(d, x, y, p);
     }
     if (pg + NW < last) load_v(pg + NW);
   }
   if (bad && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
   // the unfinished page, by the wave whose turn it would be
   if (left && full >= lo && full < hi && (full - lo) % NW == w && full * KV_PAGE < seen_by_any) {
-    const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
+    const TailScale<DT> ts(a.c.tail_top[(long long)hd.slot * H + h]);
     v4f s[CT][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -450,13 +460,12 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
       }
     }
     uint4 p[CT][2];
-    float pv[CT];
-    weights(s, a.scale, ts.vs, full, p, pv);
+    weights(s, a.scale, ts.vs, full, p);
 #pragma unroll
     for (int d = 0; d < VU; ++d) {
       const uint16_t* row = hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4;
       st.add(d, tail_v8<DT>(*reinterpret_cast<const uint4*>(row), ts.down, 16 * h4, left),
-             tail_v8<DT>(*reinterpret_cast<const uint4*>(row + 8), ts.down, 16 * h4 + 8, left), p, pv);
+             tail_v8<DT>(*reinterpret_cast<const uint4*>(row + 8), ts.down, 16 * h4 + 8, left), p);
     }
   }
 
@@ -571,15 +580,16 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
     vs1 = ok ? a.c.v_scale[at] : 0.0f;
   };
   auto stage = [&](int buf) {
+    const float vscale = value_scale<DT>(vs1);
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {
       uint4 x, y;
-      widen16<DT, CODES>(cw[i], x, y);
+      widen16_v<DT, CODES>(cw[i], w * UPW + i < KU ? 1.0f : vscale, x, y);
       lds[buf][(w * UPW + i) * 128 + lane] = x;
       lds[buf][(w * UPW + i) * 128 + 64 + lane] = y;
     }
   };
-  auto stage_tail = [&](int buf, const TailScale& ts) {
+  auto stage_tail = [&](int buf, const TailScale<DT>& ts) {
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {
       const bool key = w * UPW + i < KU;
@@ -617,10 +627,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
     int lim[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) lim[c] = limit[c] - pg * KV_PAGE;
-    float pv[CT];
-    st.template softmax<MASK>(s, cs, v, lim, h4, p, pv);
+    st.template softmax<MASK>(s, cs, v, lim, h4, p);
 #pragma unroll
-    for (int d = 0; d < D / 16; ++d) st.add(d, lds[buf][(KU + d) * 128 + lane], lds[buf][(KU + d) * 128 + 64 + lane], p, pv);
+    for (int d = 0; d < D / 16; ++d) st.add(d, lds[buf][(KU + d) * 128 + lane], lds[buf][(KU + d) * 128 + 64 + lane], p);
   };
   // pages lo..open-1 are seen whole by every row of the workgroup, open..last-1 by some in part (causal)
   const int last = min(hi, full), open = max(lo, min(last, sees(row0) / KV_PAGE));
@@ -647,7 +656,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
   for (int pg = lo; pg < open; ++pg) step(std::false_type{}, pg);
   for (int pg = open; pg < last; ++pg) step(std::true_type{}, pg);
   if (full < hi) {  // the unfinished page
-    const TailScale ts(a.c.tail_top[(long long)hd.slot * H + h]);
+    const TailScale<DT> ts(a.c.tail_top[(long long)hd.slot * H + h]);
     stage_tail(0, ts);
     barrier();
     if (full * KV_PAGE < seen_by_any) compute(std::true_type{}, 0, full, a.scale, ts.vs);

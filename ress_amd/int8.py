@@ -8,6 +8,8 @@ Half the bytes of 16-bit weights, which is what a call of a few tokens costs, an
 rate for many. The reference's layers are torch's 16-bit ones; nothing here is used unless asked for.
 """
 
+import functools
+
 import torch
 import torch.nn as nn
 
@@ -27,7 +29,7 @@ def _rows(x, name):
         raise ValueError(f"{name} must have a last dim that is a multiple of 16 up to {MOST_FEATURES}, got {tuple(x.shape)}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad: the 8-bit product has no backward pass (use torch.no_grad())")
-    rows = x.reshape(-1, x.shape[-1])
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.stride(1) != 1 or (len(rows) > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()
     return rows
@@ -62,25 +64,31 @@ def int8_linear(x, w_codes, w_scale, bias=None, act=None):
     quantize_tokens; W = w_codes (N, K) int8 * w_scale (N,) float32; bias (N,) float32; act None or "gelu" (erf)."""
     rows = _rows(x, "x")
     M, K = rows.shape
-    if w_codes.dim() != 2 or w_codes.shape[1] != K or w_codes.dtype != torch.int8 or not w_codes.is_contiguous():
+    dev = x.device
+    if (w_codes.dtype is not torch.int8 or w_codes.dim() != 2 or w_codes.shape[1] != K or not w_codes.is_contiguous()):
         raise ValueError(f"w_codes must be contiguous int8 (N, {K}), got {tuple(w_codes.shape)} {w_codes.dtype}")
     N = w_codes.shape[0]
     for name, t in (("w_scale", w_scale), ("bias", bias)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (N,) or not t.is_contiguous()):
+        if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != N or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 ({N},), got {tuple(t.shape)} {t.dtype}")
-    if any(t is not None and t.device != x.device for t in (w_codes, w_scale, bias)):
-        raise ValueError(f"the weights are not on {x.device}")
+    if w_codes.device != dev or w_scale.device != dev or (bias is not None and bias.device != dev):
+        raise ValueError(f"the weights are not on {dev}")
     if act not in ACTS:
         raise ValueError(f"act must be one of {tuple(ACTS)}, got {act!r}")
-    out = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    if out.numel() == 0:
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+    if M == 0 or N == 0:
         return out
-    size = _lib.lib().ress_int8_linear_workspace_size(M, K, N)
-    work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    size = _workspace(M, K, N)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     P = _lib.ptr
-    _lib.call_on(x.device, "ress_int8_linear", P(rows), rows.stride(0), DTYPES[x.dtype], M, K, N, P(w_codes), P(w_scale),
+    _lib.call_on(dev, "ress_int8_linear", P(rows), rows.stride(0), DTYPES[x.dtype], M, K, N, P(w_codes), P(w_scale),
                  P(bias), ACTS[act], P(out), N, P(work), size)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace(M, K, N):
+    return _lib.lib().ress_int8_linear_workspace_size(M, K, N)
 
 
 class Int8Linear(nn.Module):

@@ -377,7 +377,7 @@ class PagedKVCache:
             if rope.head_dim != self.head_dim or table.device != self.device:
                 raise ValueError(f"rope is for head_dim {rope.head_dim} on {table.device}, the cache has {self.head_dim} on {self.device}")
             want = ((B, n), (B, n, 1)) if axes == 1 else ((B, n, 2),)
-            if tuple(pos.shape) not in want or pos.is_floating_point():
+            if pos.shape not in want or pos.is_floating_point():
                 raise ValueError(f"pos must be {want[0]} whole numbers, got {tuple(pos.shape)} {pos.dtype}")
             if pos.dtype is not torch.int64 or pos.device != self.device:
                 pos = pos.to(device=self.device, dtype=torch.int64)

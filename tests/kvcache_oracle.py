@@ -66,10 +66,11 @@ def attention(q, k, v, n_new, causal, scale=None):
 
 def tolerance(out, size, spread, dtype, L):
     """|error| allowed: P is rounded to 16 bits (half a step each, in the product with V: times sum p |v|, and in the
-    sum that it is divided by: times |out|) and the output once more; the scores, their exponential (2 units of 2^-23) and the sums are fp32: a score of D = 128
+    sum that it is divided by: times |out|), in fp16 the values too (a step of the type's subnormals apart at most:
+    `tiny`), and the output once more; the scores, their exponential (2 units of 2^-23) and the sums are fp32: a score of D = 128
     products and two multiplications is off by at most 130 * 2^-24 * spread, which its exponential turns into
     that relative error, and a sum of L terms by L * 2^-24 (numerator and denominator)."""
     u = half_step(dtype)
-    rel = u + 2 * (130 * 2.0 ** -24 * spread + 2.0 ** -22) + 2 * (L + 64) * 2.0 ** -24
+    rel = (2 if dtype == torch.float16 else 1) * u + 2 * (130 * 2.0 ** -24 * spread + 2.0 ** -22) + 2 * (L + 64) * 2.0 ** -24
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # half a subnormal step of the output
     return rel * size + 2 * u * out.abs() + tiny
