@@ -93,6 +93,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// The arrays that are only read, as parameters of their own: the compiler then takes page numbers and scales by
+// scalar loads (a member of the argument struct might be written through another, and goes through vector registers).
+#define RESS_READ_ONLY                                                                                           \
+  const int *__restrict__ table_all, const float *__restrict__ k_scale, const float *__restrict__ v_scale, \
+      const int *__restrict__ lens, const int *__restrict__ slots, const int *__restrict__ new_lens
+
 // One sequence and key/value head: what it holds.
 template <int D>
 struct Head {
@@ -100,10 +106,11 @@ struct Head {
   const uint8_t *kc, *vc;      // codes of page 0 of this head
   const uint16_t *tk, *tv;     // the unfinished page
   long long stride;            // bytes from page to page
-  __device__ __forceinline__ Head(const AttendArgs& a, int b, int h_) : h(h_) {
-    slot = a.slots ? a.slots[b] : b;
-    len = a.c.lens[slot];
-    nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
+  __device__ __forceinline__ Head(const AttendArgs& a, const int* __restrict__ lens, const int* __restrict__ slots,
+                                  const int* __restrict__ new_lens, int b, int h_) : h(h_) {
+    slot = slots ? slots[b] : b;
+    len = lens[slot];
+    nv = new_lens ? min(max(new_lens[b], 0), a.n) : a.n;
     const long long one = (long long)KV_PAGE * D;
     kc = reinterpret_cast<const uint8_t*>(a.c.k_codes) + h * one;
     vc = reinterpret_cast<const uint8_t*>(a.c.v_codes) + h * one;
@@ -339,7 +346,7 @@ constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D 
 // fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
 // joined in LDS.
 template <int DT, int CODES, int D, int CT>
-__global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a) {
+__global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a, RESS_READ_ONLY) {
   constexpr int NW = 4;
   constexpr int TILES = CT * D / 16;  // of the output: 16 queries, 16 dims
   __shared__ v4f so[NW][TILES][64];
@@ -347,7 +354,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h4 = lane >> 4;
   const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / a.splits / a.tiles;
   const int H = a.c.kv_heads, b = bh / H, h = bh % H;
-  const Head<D> hd(a, b, h);
+  const Head<D> hd(a, lens, slots, new_lens, b, h);
   const int rows = hd.nv * a.G, row0 = tile * 16 * CT;
   const long long all_rows = (long long)a.B * H * a.n * a.G;
   if (row0 >= rows) return;
@@ -369,7 +376,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 
   Rows<DT, D, CT> st;
   st.clear();
-  const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
+  const int* __restrict__ table = table_all + (long long)hd.slot * a.c.max_pages;
   constexpr int KU = D / 16, VU = D / 16;  // 1 KB units of a page: keys (4 tiles x D / 64 halves), values (D / 16)
   // A page's codes are loaded as soon as the registers are free: the next one's keys behind the scores, its values
   // behind P V. A bad page number reads as a page of zeros.
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     const uint4* p = reinterpret_cast<const uint4*>(hd.kc + pid * hd.stride);
 #pragma unroll
     for (int u = 0; u < KU; ++u) kw[u] = at_u32(p, k0 + u / (D / 64) * D + u % (D / 64) * 4);
-    ks = ok ? a.c.k_scale[(long long)pid * H + h] : 0.0f;
+    ks = ok ? k_scale[(long long)pid * H + h] : 0.0f;
   };
   auto load_v = [&](int pg) {
     bool ok;
@@ -397,7 +404,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     const uint4* p = reinterpret_cast<const uint4*>(hd.vc + pid * hd.stride);
 #pragma unroll
     for (int u = 0; u < VU; ++u) vw[u] = at_u32(p, v0 + u * 64);
-    vs = ok ? a.c.v_scale[(long long)pid * H + h] : 0.0f;
+    vs = ok ? v_scale[(long long)pid * H + h] : 0.0f;
   };
   auto weights = [&](const v4f (&s)[CT][4], float cs, float v, int pg, uint4 (&p)[CT][2]) {
     int lim[CT];
@@ -521,7 +528,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 // NW waves of 16 CT rows each share a page, widened into LDS in the order in which the operands are read (1 KB
 // a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page.
 template <int DT, int CODES, int D, int CT, int NW>
-__global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) void k_cache_attn_rows(AttendArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) void k_cache_attn_rows(AttendArgs a, RESS_READ_ONLY) {
   constexpr int KU = D / 16, UNITS = 2 * KU;  // 1 KB units of a page's codes: keys, then values
   constexpr int UPW = UNITS / NW;             // of each wave
   static_assert(UPW >= 1 && UPW * NW == UNITS, "every wave has whole units");
@@ -532,7 +539,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
   const int x = blockIdx.x >> 3, group = x / a.tiles * 8 + (blockIdx.x & 7), tile = a.tiles - 1 - x % a.tiles;
   if (group >= groups) return;
   const int split = group % a.splits, bh = group / a.splits, b = bh / H, h = bh % H;
-  const Head<D> hd(a, b, h);
+  const Head<D> hd(a, lens, slots, new_lens, b, h);
   const int rows = hd.nv * a.G, row0 = tile * 16 * CT * NW;
   const long long all_rows = (long long)a.B * H * a.n * a.G;
   if (row0 >= rows) return;
@@ -553,7 +560,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
 
   Rows<DT, D, CT> st;
   st.clear();
-  const int* table = a.c.table + (long long)hd.slot * a.c.max_pages;
+  const int* __restrict__ table = table_all + (long long)hd.slot * a.c.max_pages;
   // Unit u: 16 rows with four 16-code pieces each, lane l taking the piece whose two operands lie at place l of the
   // unit's blocks. Rows of the keys are tokens (D / 16 pieces), of the values dims (4 pieces).
   unsigned piece[UPW];
@@ -576,8 +583,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
     for (int i = 0; i < UPW; ++i)
       cw[i] = at_u32(reinterpret_cast<const uint4*>(w * UPW + i < KU ? kp : vp), piece[i]);
     const long long at = (long long)pid * H + h;
-    ks1 = ok ? a.c.k_scale[at] : 0.0f;
-    vs1 = ok ? a.c.v_scale[at] : 0.0f;
+    ks1 = ok ? k_scale[at] : 0.0f;
+    vs1 = ok ? v_scale[at] : 0.0f;
   };
   auto stage = [&](int buf) {
     const float vscale = value_scale<DT>(vs1);
@@ -807,6 +814,8 @@ long long part_floats(const ress_kv_cache& c, int B, int Hq, int n, const Cut& k
   return k.splits == 1 ? 0 : (long long)k.splits * B * Hq * n * (c.head_dim + 2);
 }
 
+#define RESS_READ_ONLY_ARGS a.c.table, a.c.k_scale, a.c.v_scale, a.c.lens, a.slots, a.new_lens
+
 template <int DT, int CODES, int D>
 int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
   const long long heads = (long long)a.B * a.c.kv_heads;
@@ -814,14 +823,14 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
     const long long g = heads * k.tiles * k.splits;
     RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
     if (k.ct == 1)
-      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 1>), dim3((unsigned)g), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 1>), dim3((unsigned)g), dim3(256), 0, stream, a, RESS_READ_ONLY_ARGS);
     else
-      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 2>), dim3((unsigned)g), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 2>), dim3((unsigned)g), dim3(256), 0, stream, a, RESS_READ_ONLY_ARGS);
     RESS_LAUNCHED("k_cache_attn_few");
   } else {
     const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
     RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
-    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, RESS_ROWS_CT, RESS_ROWS_NW>), dim3((unsigned)g), dim3(64 * RESS_ROWS_NW), 0, stream, a);
+    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, RESS_ROWS_CT, RESS_ROWS_NW>), dim3((unsigned)g), dim3(64 * RESS_ROWS_NW), 0, stream, a, RESS_READ_ONLY_ARGS);
     RESS_LAUNCHED("k_cache_attn_rows");
   }
   if (k.splits > 1) {
