@@ -14,42 +14,14 @@
 //
 // v_scale. In bf16 it enters as an addend of the exponent (PageScale), relative to a power of two: the codes stay whole
 // and it costs no multiplication per element. fp16 has no exponents to spare for that: there the codes are multiplied,
-// as they are widened, by v_scale rounded to fp16 (the values are in fp16's range, as the values they came from were),
-// and what that rounding took enters the exponent.
+// as they are widened, by v_scale rounded toward zero to fp16 (the products are in fp16's range, as the values they came
+// from were), and what that rounding took enters the exponent.
 // The sum of P is a product with ones on the matrix cores, of the rounded P, so numerator and denominator carry the
 // same roundings.
 //
 // Masked places (past the sequence's end, after the row's own token) are selected away after every
 // multiplication, so a NaN scale or tail element there reaches no row that does not see its page.
 #include "kvcache.h"
-
-#ifndef RESS_FEW_TARGET
-#define RESS_FEW_TARGET 2
-#endif
-#ifndef RESS_FEW_OCC64
-#define RESS_FEW_OCC64 3
-#endif
-#ifndef RESS_FEW_OCC128
-#define RESS_FEW_OCC128 2
-#endif
-#ifndef RESS_FEW_LEAST
-#define RESS_FEW_LEAST 16
-#endif
-#ifndef RESS_ROWS_NW
-#define RESS_ROWS_NW 4
-#endif
-#ifndef RESS_ROWS_LEAST
-#define RESS_ROWS_LEAST 8
-#endif
-#ifndef RESS_ROWS_OCC
-#define RESS_ROWS_OCC 4
-#endif
-#ifndef RESS_ROWS_OCC2
-#define RESS_ROWS_OCC2 2
-#endif
-#ifndef RESS_ROWS_CT
-#define RESS_ROWS_CT 2
-#endif
 
 namespace {
 
@@ -58,6 +30,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 constexpr float LOWEST = -0x1.fffffep127f;
+constexpr int CUS = 256;
 constexpr float LAZY = 8.0f;
 
 struct AttendArgs {
@@ -71,7 +44,7 @@ struct AttendArgs {
   float scale;       // sm_scale * log2(e)
   int splits, per;   // the keys are cut every `per` pages, into at most `splits` parts (the last takes the rest)
   int tiles;         // row tiles of a (sequence, kv head)
-  float *part_o, *part_ml;  // [splits][B * kv_heads * n * G][D], [..][2]
+  float *part_o, *part_ml;  // [splits][B * kv_heads * n * G][D] outputs of the parts, [..][2] their m and l
   bool qvec, ovec;
 };
 
@@ -146,15 +119,16 @@ struct TailScale {
 template <int DT>
 __device__ __forceinline__ float value_scale(float vs) {
   if constexpr (DT == KV_BF16) return 1.0f;
-  // never 0 (the smallest subnormal serves the smallest scales) and finite, so that 0 * V is 0
-  return vs > 0.0f ? fmaxf((float)(_Float16)vs, 0x1p-24f) : 1.0f;
+  // toward zero, as 127 times the nearest of 65504 / 127 is infinite; never 0 (the smallest subnormal serves the smallest
+  // scales), so that 0 * V is 0
+  return vs > 0.0f ? fmaxf((float)(_Float16)__uint_as_float(__float_as_uint(vs) & 0xffffe000u), 0x1p-24f) : 1.0f;
 }
 template <int DT>
 struct PageScale {
   float lift, down;
   __device__ __forceinline__ PageScale(float vs, int eR) {
     if constexpr (DT == KV_F16) {
-      const float r = vs == 0.0f ? 1.0f : vs / value_scale<DT>(vs);  // within 2^-8 .. 1 + 2^-11; NaN stays
+      const float r = vs == 0.0f ? 1.0f : vs / value_scale<DT>(vs);  // below 1 + 2^-10, of subnormals below 2; NaN stays
       lift = 7.0f + __builtin_amdgcn_logf(r);
       down = 1.0f / r;
     } else {
@@ -298,6 +272,20 @@ __device__ __forceinline__ void load_q(const AttendArgs& a, int b, int h, int ro
   }
 }
 
+// Twice `half`, a weighted mean of values over two. No mean passes the type's largest value, but the weights and v_scale are
+// rounded by 2^-9 (bf16) or 2^-11, so its sum may: it ends there. Infinite values in an unfinished page stay infinite.
+template <int DT>
+__device__ __forceinline__ v4f mean4(const v4f& half) {
+  constexpr float TOP = DT == KV_F16 ? 0.5f * 65504.0f : 0x0.ffp127f;
+  v4f r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = fabsf(half[i]);
+    r[i] = 2.0f * (x > TOP && x < __builtin_inff() ? copysignf(TOP, half[i]) : half[i]);
+  }
+  return r;
+}
+
 template <int DT>
 __device__ __forceinline__ void store4(uint16_t* p, const v4f& v, bool vec) {
   const uint32_t lo = pack2<DT>(v[0], v[1]), hi = pack2<DT>(v[2], v[3]);
@@ -338,13 +326,17 @@ __device__ __forceinline__ uint4 tail_v8(const uint4& w, float down, int place, 
   return pack8(e);
 }
 
-// Waves a SIMD has room for (its registers are shared out so).
-constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D == 64 ? RESS_FEW_OCC64 : RESS_FEW_OCC128; }
+// Waves that a SIMD's registers are shared out for. One more spills: 22 us for one row of 16 heads of 64 over 21,984
+// tokens instead of 20, 114 for 32 sequences of up to 8,192 tokens, 8 heads of 128, instead of 74; with 32 rows and a
+// head of 128 two spill.
+constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2; }
 
 // ---- few rows: one wave a page --------------------------------------------------------------------
 // A workgroup of four waves takes 16 CT rows of a (sequence, kv head) and a share of its pages, a wave every
 // fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
-// joined in LDS.
+// joined in LDS. Bound by the bytes of the codes where the cache is long (5 rows of 16 heads over 274,800 tokens: 98 us
+// for 563 MB, 5.7 TB/s), by one page's chain of loads, scores, exponentials and products where it is short (one row over
+// 21,984 tokens: 16 us, 2.8 TB/s).
 template <int DT, int CODES, int D, int CT>
 __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a, RESS_READ_ONLY) {
   constexpr int NW = 4;
@@ -493,7 +485,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     L[c] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NW; ++k) L[c] += sl[k][c][i] * exp2f(sm[k][c][i] - M[c]);
-    f[c] = exp2f(st.m[c] - M[c]) * st.unit();
+    f[c] = L[c] == 0.0f ? 0.0f : exp2f(st.m[c] - M[c]) * (0.5f * st.unit() / L[c]);
   }
 #pragma unroll
   for (int c = 0; c < CT; ++c)
@@ -506,13 +498,13 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     v4f t = so[0][tile][lane];
 #pragma unroll
     for (int k = 1; k < NW; ++k) t += so[k][tile][lane];
+    t = mean4<DT>(t);
     const int r = row0 + 16 * c + (lane & 15);
     if (r >= rows) continue;
     const int dim = 16 * d + 4 * h4;
     if (a.splits == 1) {
       const int tok = r / a.G, hq = h * a.G + r % a.G;
-      const float inv = L[c] == 0.0f ? 0.0f : 1.0f / L[c];
-      store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, t * inv, a.ovec);
+      store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, t, a.ovec);
     } else {
       const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
       *reinterpret_cast<v4f*>(a.part_o + at * D + dim) = t;
@@ -526,9 +518,21 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 
 // ---- many rows: pages widened once for a workgroup ---------------------------------------------------
 // NW waves of 16 CT rows each share a page, widened into LDS in the order in which the operands are read (1 KB
-// a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page.
+// a wave's read, no bank conflicts), the next page's codes loaded meanwhile; two stages, one barrier a page. Pages that
+// every row sees whole run without a mask, apart from those that a causal row ends in, so that the masks' registers
+// are not held in the loop.
+//
+// Bound by the issue of vector and matrix instructions, which hardly overlap on a SIMD: of its cycles the vector unit is
+// busy 67%, the matrix cores 37% (1,374 rows of 16 heads over 87,936 tokens; a page of 32 rows takes 36 products of
+// 16 cycles, 32 exponentials of 8 and some 150 other instructions of 4). 495 GFLOP in 625 us there: 790 TFLOP/s, 38% of
+// the 2,058 that the matrix cores reach. At that size and at 21,984 tokens: 2 tiles of 16 rows a wave 703, 189 us (3: 733,
+// 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 179. Eight waves a workgroup (half the widening a
+// row): 626, 168, but 166 for 150 at a head of 128 causal and grouped; four stay.
+constexpr int ROWS_CT = 2, ROWS_NW = 4;
+constexpr int rows_waves(int D) { return D == 64 ? 4 : 2; }  // a SIMD; 64 KB of LDS a workgroup at a head of 128
+
 template <int DT, int CODES, int D, int CT, int NW>
-__global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) void k_cache_attn_rows(AttendArgs a, RESS_READ_ONLY) {
+__global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(AttendArgs a, RESS_READ_ONLY) {
   constexpr int KU = D / 16, UNITS = 2 * KU;  // 1 KB units of a page's codes: keys, then values
   constexpr int UPW = UNITS / NW;             // of each wave
   static_assert(UPW >= 1 && UPW * NW == UNITS, "every wave has whole units");
@@ -674,17 +678,16 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
     const float L = st.l[c];
     const int r = wrow + 16 * c + (lane & 15);
     if (r >= rows) continue;
-    const float unit = st.unit();
+    const float inv = L == 0.0f ? 0.0f : 0.5f * st.unit() / L;
     if (a.splits == 1) {
       const int tok = r / a.G, hq = h * a.G + r % a.G;
-      const float inv = L == 0.0f ? 0.0f : unit / L;
       uint16_t* o = a.out + b * a.sob + hq * a.soh + tok * a.sot + 4 * h4;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) store4<DT>(o + 16 * d, st.o[c][d] * inv, a.ovec);
+      for (int d = 0; d < D / 16; ++d) store4<DT>(o + 16 * d, mean4<DT>(st.o[c][d] * inv), a.ovec);
     } else {
       const long long at = split * all_rows + (long long)bh * a.n * a.G + r;
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f*>(a.part_o + at * D + 16 * d + 4 * h4) = st.o[c][d] * unit;
+      for (int d = 0; d < D / 16; ++d) *reinterpret_cast<v4f*>(a.part_o + at * D + 16 * d + 4 * h4) = mean4<DT>(st.o[c][d] * inv);
       if (h4 == 0) {
         a.part_ml[2 * at] = st.m[c];
         a.part_ml[2 * at + 1] = L;
@@ -694,8 +697,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) 
 }
 
 // ---- joining the splits ---------------------------------------------------------------------------------
-// o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. D / 4 lanes hold a row; SG such groups share its parts
-// (SG = 1 where there are rows enough to fill the chip, so that a wave reads whole rows; else all 256 threads one row).
+// o = sum_s w_s o_s with w_s = 2^(m_s - M) l_s / sum_t 2^(m_t - M) l_t: the parts are outputs already, so that no sum
+// passes the largest value (of bf16's 3e38, say). D / 4 lanes hold a row; SG such groups share its parts
+// (SG = 1, a wave reading whole rows, from 2,048 rows on; else all 256 threads one row: 1,024 rows in 12 parts take
+// 29 us with their attention so and 32 the other way, 3,200 rows 52 and 51, 8,000 rows 89 and 76).
 template <int DT, int D, int SG>
 __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   constexpr int LPR = D / 4, RPW = 256 / (LPR * SG);
@@ -710,66 +715,65 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   const bool live = row < all_rows && tok < nv;
   const int len = a.c.lens[a.slots ? a.slots[b] : b];
   const int ns = min(a.splits, max(1, cdiv(cdiv(len, KV_PAGE), a.per)));
+  const float* ml = a.part_ml + 2 * (live ? row : 0);
+  const float* po = a.part_o + (live ? row : 0) * D + lane * 4;
   float M = LOWEST, L = 0.0f;
-  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (live) {
-    const float* ml = a.part_ml + 2 * row;
-    const float* po = a.part_o + row * D + lane * 4;
-    for (int s0 = g; s0 < ns; s0 += 4 * SG) {  // four parts at a time, their loads together
-      float m[4], l[4];
-      v4f v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = s0 + i * SG;
-        const bool in = s < ns;
-        m[i] = in ? ml[2 * s * all_rows] : LOWEST;
-        l[i] = in ? ml[2 * s * all_rows + 1] : 0.0f;
-        v[i] = in ? *reinterpret_cast<const v4f*>(po + s * all_rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-      const float t = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), M), f0 = exp2f(M - t);
-      L *= f0;
-      o *= f0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = exp2f(m[i] - t);
-        L += l[i] * f;
-        o += v[i] * f;
-      }
-      M = t;
-    }
+    for (int s = g; s < ns; s += SG) M = fmaxf(M, ml[2 * s * all_rows]);
+    for (int s = g; s < ns; s += SG) L += ml[2 * s * all_rows + 1] * exp2f(ml[2 * s * all_rows] - M);
   }
   if constexpr (SG > 1) {
     if (lane == 0) {
       sm[g][rw] = M;
       sl[g][rw] = L;
     }
+    __syncthreads();
+    M = sm[0][rw];
+#pragma unroll
+    for (int i = 1; i < SG; ++i) M = fmaxf(M, sm[i][rw]);
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SG; ++i) L += sl[i][rw] * exp2f(sm[i][rw] - M);
+  }
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (live) {
+    for (int s0 = g; s0 < ns; s0 += 4 * SG) {  // four parts at a time, their loads together
+      float f[4];
+      v4f v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * SG;
+        const bool in = s < ns;
+        f[i] = in ? ml[2 * s * all_rows + 1] * inv * exp2f(ml[2 * s * all_rows] - M) : 0.0f;
+        v[i] = in ? *reinterpret_cast<const v4f*>(po + s * all_rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o += v[i] * f[i];
+    }
+  }
+  if constexpr (SG > 1) {
     so[g][rw * LPR + lane] = o;
     __syncthreads();
     if (g) return;
-    float t = M;
 #pragma unroll
-    for (int i = 1; i < SG; ++i) t = fmaxf(t, sm[i][rw]);
-    const float f0 = exp2f(M - t);
-    L *= f0;
-    o *= f0;
-#pragma unroll
-    for (int i = 1; i < SG; ++i) {
-      const float f = exp2f(sm[i][rw] - t);
-      L += sl[i][rw] * f;
-      o += so[i][rw * LPR + lane] * f;
-    }
+    for (int i = 1; i < SG; ++i) o += so[i][rw * LPR + lane];
   }
   if (!live) return;
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  store4<DT>(a.out + b * a.sob + (h * a.G + r % a.G) * a.soh + tok * a.sot + lane * 4, o * inv, a.ovec);
+  store4<DT>(a.out + b * a.sob + (h * a.G + r % a.G) * a.soh + tok * a.sot + lane * 4, o, a.ovec);
 }
 
 // How a call is cut: which kernel, row tiles of a (sequence, kv head), and splits of the keys.
+//
+// Up to 32 rows of a (sequence, kv head) go to the few-rows kernel: 32 rows of 16 heads over 21,984 tokens take 24 us so
+// and 25 in the other, over 87,936 tokens 40 and 49; 24 to 32 grouped rows of 8 heads of 128 25 to 49 and 29 to 53.
+// It gets workgroups for half the slots (two a CU): with four a CU the five special rows over 274,800 tokens take 123 us
+// instead of 103, the ragged batch of 32 72 instead of 74.
 struct Cut {
   int ct, nw;   // nw = 0: the few-rows kernel
   int tiles, splits, per;
 };
-constexpr int CUS = 256;
+
 Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   Cut k{};
   const long long rows = (long long)n * (Hq / c.kv_heads), heads = (long long)B * c.kv_heads;
@@ -779,13 +783,13 @@ Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   if (rows <= 32) {
     k.ct = rows <= 16 ? 1 : 2;
     k.nw = 0;
-    slots = RESS_FEW_TARGET * CUS;
-    least = RESS_FEW_LEAST;
+    slots = 2 * CUS;
+    least = 16;  // four a wave; with two, one row over 344 pages takes 25 us instead of 22
   } else {
-    k.ct = RESS_ROWS_CT;
-    k.nw = RESS_ROWS_NW;
-    slots = (c.head_dim == 64 ? RESS_ROWS_OCC : RESS_ROWS_OCC2) * CUS / (RESS_ROWS_NW / 4);
-    least = RESS_ROWS_LEAST;
+    k.ct = ROWS_CT;
+    k.nw = ROWS_NW;
+    slots = (long long)rows_waves(c.head_dim) * CUS * 4 / ROWS_NW;
+    least = 8;
   }
   const int tile = 16 * k.ct * (k.nw ? k.nw : 1);
   k.tiles = (int)((rows + tile - 1) / tile);
@@ -830,12 +834,12 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
   } else {
     const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
     RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
-    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, RESS_ROWS_CT, RESS_ROWS_NW>), dim3((unsigned)g), dim3(64 * RESS_ROWS_NW), 0, stream, a, RESS_READ_ONLY_ARGS);
+    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, ROWS_CT, ROWS_NW>), dim3((unsigned)g), dim3(64 * ROWS_NW), 0, stream, a, RESS_READ_ONLY_ARGS);
     RESS_LAUNCHED("k_cache_attn_rows");
   }
   if (k.splits > 1) {
     const long long rows = heads * a.n * a.G, per = 256 / (D / 4);
-    if (rows >= 4 * CUS * per)
+    if (rows >= 2048)
       hipLaunchKernelGGL((k_cache_attn_join<DT, D, 1>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
     else
       hipLaunchKernelGGL((k_cache_attn_join<DT, D, 256 / (D / 4)>), dim3((unsigned)rows), dim3(256), 0, stream, a);

@@ -268,6 +268,21 @@ def test_attend_ranges(dev, dtype, codes, D):
 
 
 @pytest.mark.parametrize("dtype,codes,D", KINDS)
+@pytest.mark.parametrize("n,T", [(3, 100), (3, 5000), (100, 700), (100, 5000)])
+def test_attend_largest_values(dev, dtype, codes, D, n, T):
+    """Values at the type's largest under weights that are all alike: no sum of them is formed, whole or in parts."""
+    top = torch.finfo(dtype).max
+    c = _cache(dev, 1, D, 1, T, dtype, codes)
+    k = torch.zeros(1, 1, T, D, dtype=dtype, device=dev)
+    v = torch.full((1, 1, T, D), top, dtype=dtype, device=dev)
+    v[..., 1::2] *= -1
+    c.append(k, v)
+    got = c.attend(torch.ones(1, 1, n, D, dtype=dtype, device=dev)).double()
+    want = v[:, :, :n].double()
+    assert torch.isfinite(got).all() and ((got - want).abs() <= top * 3 * half_step(dtype)).all()
+
+
+@pytest.mark.parametrize("dtype,codes,D", KINDS)
 @pytest.mark.parametrize("n", [20, 100])
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("at", [100, 150])
