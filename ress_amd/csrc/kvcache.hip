@@ -164,9 +164,9 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
   uint4 kx0, ky0, vx0, vy0;
   kx0 = ky0 = vx0 = vy0 = make_uint4(0, 0, 0, 0);
   if (a.n < KV_PAGE && part == 0 && mine < fresh) token(mine, kx0, ky0, vx0, vy0);
-  const int want = len + fresh, end = min(want, cap);
+  const int end = len + min(fresh, max(cap - len, 0));
   const int p0 = len / KV_PAGE, p1 = end / KV_PAGE;  // pages p0..p1-1 get full, p1 stays open
-  if (t == 0 && part == 0 && h == 0 && want > cap) atomicOr(a.c.status, KV_ST_FULL);
+  if (t == 0 && part == 0 && h == 0 && end < len + (long long)fresh) atomicOr(a.c.status, KV_ST_FULL);
 
   auto page = [&](int pg, bool full) {
     uint4 kx[IT], ky[IT], vx[IT], vy[IT];
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
     int* arrived = a.c.arrived + (long long)slot * KV_LINE;  // a line of its own: sharing one cost 6 ns an arrival
     if (atomicAdd(arrived, 1) == all - 1) {
       *arrived = 0;
-      a.c.lens[slot] = max(end, len);
+      a.c.lens[slot] = end;
     }
   }
 }
@@ -448,7 +448,7 @@ int ress_kv_check(const ress_kv_cache* c, int B, const char* who) {
   RESS_REQUIRE(c->dtype == KV_BF16 || c->dtype == KV_F16, "%s: dtype code %d is not 1 (bf16) or 2 (fp16)", who, c->dtype);
   RESS_REQUIRE(c->codes == KV_I8 || c->codes == KV_FP8, "%s: codes %d is not 0 (int8) or 1 (e4m3)", who, c->codes);
   RESS_REQUIRE(c->n_pages > 0 && c->max_pages > 0 && c->max_seqs > 0 && c->kv_heads > 0 &&
-                   c->max_pages <= (1 << 25),
+                   c->max_pages < (1 << 25),  // tokens are counted in 32 bits
                "%s: bad cache geometry", who);
   RESS_REQUIRE(c->k_codes && c->v_codes && c->k_scale && c->v_scale && c->tail_k && c->tail_v && c->tail_top &&
                    c->table && c->held && c->lens && c->arrived && c->status,

@@ -126,8 +126,8 @@ class PagedKVCache:
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
         self.n_pages, self.kv_heads, self.head_dim, self.max_seqs = int(n_pages), int(n_kv_heads), head_dim, int(max_seqs)
         self.max_pages = self.n_pages if max_len is None else min(self.n_pages, -(-int(max_len) // PAGE))
-        if not 1 <= self.max_pages <= 1 << 25:
-            raise ValueError(f"max_len must be 1 to {PAGE << 25} tokens, got {max_len}")
+        if not 1 <= self.max_pages < 1 << 25:
+            raise ValueError(f"max_len must be 1 to {(PAGE << 25) - PAGE} tokens, got {max_len}")
         self.dtype, self.codes = dtype, codes
         P, H, D, S, dev = self.n_pages, self.kv_heads, head_dim, self.max_seqs, self.device
         code_t = torch.int8 if codes == "int8" else torch.float8_e4m3fn
@@ -168,6 +168,7 @@ class PagedKVCache:
         """The slots of a batch's rows, checked (in range, none twice) and on the device: make it once
         for calls that repeat."""
         ids = [int(i) for i in ids]
+        self._not_capturing("slots", "a SlotBatch (slots)")
         if any(not 0 <= i < self.max_seqs for i in ids):
             raise IndexError(f"slots must lie in 0..{self.max_seqs - 1}, got {ids}")
         if len(set(ids)) != len(ids):
@@ -184,6 +185,11 @@ class PagedKVCache:
         if len(slots) != B or slots.tensor.device != self.device or any(i >= self.max_seqs for i in slots.ids):
             raise ValueError(f"the batch has {B} rows and {len(slots)} slots, or they belong to another cache")
         return slots.ids, slots.tensor
+
+    @staticmethod
+    def _not_capturing(name, want):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"inside a graph capture {name} must be {want} made before it")
 
     def _settle(self):
         """Brings _bound up to date."""
@@ -339,6 +345,7 @@ class PagedKVCache:
                 raise ValueError(f"new_lens must be ({B},) int32 on {self.device}, got {tuple(new_lens.shape)} "
                                  f"{new_lens.dtype} on {new_lens.device}")
             return new_lens.contiguous(), ()
+        self._not_capturing("new_lens", "an int32 tensor")
         got = [int(x) for x in new_lens]
         if len(got) != B or any(not 0 <= x <= n for x in got):
             raise ValueError(f"new_lens must be {B} counts of 0..{n}, got {got}")
@@ -379,6 +386,8 @@ class PagedKVCache:
             want = ((B, n), (B, n, 1)) if axes == 1 else ((B, n, 2),)
             if pos.shape not in want or pos.is_floating_point():
                 raise ValueError(f"pos must be {want[0]} whole numbers, got {tuple(pos.shape)} {pos.dtype}")
+            if pos.device != self.device:
+                self._not_capturing("pos", "a tensor on the cache's device")
             if pos.dtype is not torch.int64 or pos.device != self.device:
                 pos = pos.to(device=self.device, dtype=torch.int64)
             pos = pos.contiguous()

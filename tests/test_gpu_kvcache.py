@@ -464,6 +464,12 @@ def test_captured_steps(dev, n):
     c.append(y, y)
     c.check()
     assert c.lengths() == [53 + steps * n, 64 + steps * n]
+    with pytest.raises(RuntimeError, match="made before it"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            c.append(y, y, new_lens=[3, 3])
+    with pytest.raises(RuntimeError, match="made before it"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            c.attend(y, slots=[0, 1])
     full = _cache(dev, H, D, 1, 64)
     with pytest.raises(RuntimeError, match="reserved before"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
@@ -491,6 +497,8 @@ def test_refusals(dev):
         PagedKVCache(4, 2, codes="int4", device=dev)
     with pytest.raises(ValueError, match="at least 1"):
         PagedKVCache(0, 2, device=dev)
+    with pytest.raises(ValueError, match="max_len"):
+        PagedKVCache(4, 2, max_len=0, device=dev)
     c, _, _ = _filled(dev, [70], 2)
     x = _rand((1, 2, 5, 64), BF16, dev, 0)
     rope = RotaryTable(64, 16, axes=2, device=dev)

@@ -46,7 +46,7 @@ def _args(**kw):
 
 @pytest.mark.parametrize("kw,msg", [
     (dict(head_dim=80), b"head_dim 80"), (dict(dtype=0), b"dtype code 0"), (dict(codes=2), b"codes 2"),
-    (dict(n_pages=0), b"bad cache geometry"), (dict(tail_v=None), b"null buffer"), (dict(k_codes=4104), b"aligned"),
+    (dict(n_pages=0), b"bad cache geometry"), (dict(max_pages=1 << 25), b"bad cache geometry"), (dict(tail_v=None), b"null buffer"), (dict(k_codes=4104), b"aligned"),
     (dict(max_seqs=1), b"more than the cache's 1 slots"),
 ])
 def test_the_library_refuses_a_bad_cache(kw, msg):
