@@ -1,6 +1,6 @@
 // Linear layer in 8-bit integers with a scale for each token and each output channel:
 //   a_m = max_k |x_mk|, c_mk = rne(x_mk * min(127 / a_m, FLT_MAX)), s_m = a_m * fl(1/127)
-//   y_mn = act((s_m * sum_k c_mk w_nk) * t_n + b_n)
+//   y_mn = act((sum_k c_mk w_nk * t_n) * s_m + b_n)
 // with w int8 [N][K] and t its channels' scales. The sum is exact (int32); the rest is fp32, rounded once to
 // the activations' 16-bit type. A token with an element that is not finite has scale NaN, so its row of y is NaN.
 //
@@ -44,7 +44,7 @@ __device__ __forceinline__ void finish4(const Out& o, int m, int n, const v4i& a
   uint16_t e[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    float y = (float)acc[r] * sx * ws[r];
+    float y = (float)acc[r] * ws[r] * sx;  // the weights' scale first: a token's may be near fp32's end, as bf16's is
     if (o.bias) y = y + bias[r];
     if (o.act == ACT_GELU) y = gelu(y);
     e[r] = Elem<DT>::put(y);
@@ -428,7 +428,7 @@ int linear(const void* x, long long stride, int K, const void* w, const Out& o, 
 
 int check_rows(const char* who, int dtype, int M, int K) {
   RESS_REQUIRE(dtype == KV_BF16 || dtype == KV_F16, "%s: dtype code %d is not 1 (bf16) or 2 (fp16)", who, dtype);
-  RESS_REQUIRE(M >= 0 && K >= 0 && K % 16 == 0 && K <= 131072, "%s: %d rows of %d elements (a multiple of 16, at most 131072)",
+  RESS_REQUIRE(M >= 0 && M <= (1 << 30) && K >= 0 && K % 16 == 0 && K <= 131072, "%s: %d rows of %d elements (a multiple of 16, at most 131072; at most 2^30 rows)",
                who, M, K);
   return 0;
 }

@@ -17,6 +17,7 @@ from ress_amd import _lib
 
 DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 ACTS = {None: 0, "gelu": 1}
+MOST_ROWS = 1 << 30
 MOST_FEATURES = 131072  # |sum| <= 127^2 * 131072 < 2^31
 
 
@@ -29,6 +30,8 @@ def _rows(x, name):
         raise ValueError(f"{name} must have a last dim that is a multiple of 16 up to {MOST_FEATURES}, got {tuple(x.shape)}")
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires grad: the 8-bit product has no backward pass (use torch.no_grad())")
+    if x.numel() > MOST_ROWS * x.shape[-1]:
+        raise ValueError(f"{name} must have at most {MOST_ROWS} rows, got {tuple(x.shape)}")
     rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if rows.stride(1) != 1 or (len(rows) > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()

@@ -87,6 +87,14 @@ def test_large_sums(dev):
 
 
 @pytest.mark.parametrize("M", [3, 40])
+def test_largest_activations(dev, M):
+    """Near bf16's end: the sum times a token's scale would pass it, times both scales it does not."""
+    codes, scale, bias = _weights(36, 1024, dev, 5)
+    x = _rand((M, 1024), BF16, dev, 6, 2.0 ** 120)
+    _check(x, codes, scale, bias, None, int8_linear(x, codes, scale, bias))
+
+
+@pytest.mark.parametrize("M", [3, 40])
 def test_layouts(dev, M):
     """Leading dims, rows of a wider tensor, odd offsets: as a copy does."""
     K, N = 96, 70
@@ -192,3 +200,5 @@ def test_refusals(dev):
         int8_linear(x.clone().requires_grad_(), codes, scale)
     with pytest.raises(RuntimeError, match="device tensor"):
         quantize_tokens(x.cpu())
+    with pytest.raises(ValueError, match="rows"):
+        quantize_tokens(x[:1].expand((1 << 30) + 1, 32))
