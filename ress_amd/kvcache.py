@@ -16,7 +16,9 @@ values, and half the bytes that attention reads. The tokens of a sequence's unfi
 alone and not on how they were split over calls.
 
 Every method works on torch's current stream of the cache's device and none waits for the device,
-except reserve and release (a small copy of page numbers), lengths and check. Calls that change a
+except reserve and release (a small copy of page numbers), lengths and check, and an append that needs
+pages (once the host no longer knows the lengths, as with counts on the device, it reads them first; after a
+captured append each eager one does). Calls that change a
 cache (append, restore, release) must be ordered one after the other, as on one stream, and so must
 two captured graphs that append to one cache; attend and read only read it.
 
@@ -32,6 +34,7 @@ import torch
 from ress_amd import _lib
 
 PAGE = 64
+MOST_ROWS = 1 << 30  # of an operand, over batch and heads
 CODES = {"int8": 0, "fp8": 1}
 DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 _STATUS = (
@@ -40,6 +43,10 @@ _STATUS = (
     (4, "a page number lies outside the pool (the table was changed from outside)"),
     (8, "a page holds a key or value that is not finite (queries that see it get NaN)"),
 )
+
+
+def _capturing():
+    return torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 class _CacheArgs(ctypes.Structure):
@@ -99,8 +106,8 @@ class SlotBatch:
 class Snapshot:
     """What PagedKVCache.restore needs to take appended tokens back."""
 
-    def __init__(self, state, bounds, serial):
-        self.state, self.bounds, self.serial = state, bounds, serial
+    def __init__(self, state, bounds, guessed, serial):
+        self.state, self.bounds, self.guessed, self.serial = state, bounds, guessed, serial
         self.alive = True
 
 
@@ -153,7 +160,8 @@ class PagedKVCache:
         # Appends of one batch that needed no pages, not yet in _bound: `_lag` tokens for each slot of `_key` (a
         # SlotBatch, or B for slots 0..B-1), which has room for `_slack` more and holds at most `_most`.
         self._key, self._lag, self._slack, self._most = None, 0, 0, 0
-        self._captured = False    # a captured append moves lengths that the host does not see
+        self._captured = False    # captured work moves lengths that the host does not see
+        self._guessed = False     # _bound counts padding (counts on the device)
         self._snapshots = weakref.WeakSet()
         self._serial = 0
         p = _lib.ptr
@@ -188,7 +196,7 @@ class PagedKVCache:
 
     @staticmethod
     def _not_capturing(name, want):
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             raise RuntimeError(f"inside a graph capture {name} must be {want} made before it")
 
     def _settle(self):
@@ -206,20 +214,21 @@ class PagedKVCache:
         got = self.lens.tolist()
         self._key, self._lag = None, 0
         self._bound[:] = got
+        self._guessed = False
         return got
 
     def _room(self, ids, more, exact):
         """Pages for more[i] further tokens in each slot. Bounds that the host only estimates (padded
-        batches, captured appends) are read from the device before anything is refused; where `more` is itself
-        an estimate (exact=False), a slot is given no more than max_len."""
+        batches, captured appends) are read from the device before pages are taken for them or anything is
+        refused; where `more` is itself an estimate (exact=False), a slot is given no more than max_len."""
         most = PAGE * self.max_pages
 
         def wanted():
             need = {i: self._bound[i] + m for i, m in zip(ids, more)}
             return need if exact else {i: min(n, most) for i, n in need.items()}
 
-        capturing = torch.cuda.is_current_stream_capturing()
-        if self._captured and not capturing:
+        capturing = _capturing()
+        if (self._captured or self._guessed) and not capturing:
             self.lengths()
         need = wanted()
         if all(n <= self._cap[i] for i, n in need.items()):
@@ -271,6 +280,8 @@ class PagedKVCache:
         """Empties a slot and gives its pages back. Work that reads them has to be ordered before."""
         if not 0 <= slot < self.max_seqs:
             raise IndexError(f"slot must lie in 0..{self.max_seqs - 1}, got {slot}")
+        if _capturing():
+            raise RuntimeError("release gives pages back at once: not inside a graph capture")
         self._settle()
         with torch.cuda.device(self.device):
             self.held[slot:slot + 1].fill_(0)
@@ -286,7 +297,8 @@ class PagedKVCache:
         """The state that restore goes back to (a copy of the unfinished pages and the lengths)."""
         self._settle()
         self._serial += 1
-        snap = Snapshot(self._state.clone(), list(self._bound), self._serial)
+        self._captured = self._captured or _capturing()
+        snap = Snapshot(self._state.clone(), list(self._bound), self._guessed, self._serial)
         self._snapshots.add(snap)
         return snap
 
@@ -297,9 +309,10 @@ class PagedKVCache:
             raise ValueError("the snapshot belongs to another cache")
         if not snapshot.alive:
             raise RuntimeError("the snapshot no longer holds: a slot was released, or an older snapshot restored, since")
+        self._captured = self._captured or _capturing()
         self._state.copy_(snapshot.state)
         self._key, self._lag = None, 0
-        self._bound[:] = snapshot.bounds
+        self._bound[:], self._guessed = snapshot.bounds, snapshot.guessed
         if snapshot.serial < self._serial:
             for snap in self._snapshots:
                 if snap.serial > snapshot.serial:
@@ -319,7 +332,7 @@ class PagedKVCache:
             B, H, n, D = t.shape
             st = t.stride()
             if (D == self.head_dim and st[3] == 1 and (heads is None or H == heads)
-                    and (like is None or (B == like.shape[0] and n == like.shape[2]))
+                    and (like is None or (B == like.shape[0] and n == like.shape[2])) and B * H * n <= MOST_ROWS
                     and not (t.requires_grad and torch.is_grad_enabled())):
                 return st[:3]
         if not torch.is_tensor(t) or not t.is_cuda:
@@ -332,6 +345,8 @@ class PagedKVCache:
             raise ValueError(f"{name} must be (B, {heads or 'heads'}, n, {self.head_dim}), got {tuple(t.shape)}")
         if like is not None and (t.shape[0], t.shape[2]) != (like.shape[0], like.shape[2]):
             raise ValueError(f"{name} must have the batch and tokens of k, ({like.shape[0]}, {like.shape[2]}), got {tuple(t.shape)}")
+        if t.shape[0] * t.shape[1] * t.shape[2] > MOST_ROWS:
+            raise ValueError(f"{name} must have at most {MOST_ROWS} rows, got {tuple(t.shape)}")
         if t.stride(3) != 1:
             raise ValueError(f"{name} must have a unit-stride head dim")
         raise RuntimeError(f"{name} requires grad: the cache has no backward pass (use torch.no_grad())")
@@ -396,7 +411,8 @@ class PagedKVCache:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
         if B == 0 or n == 0:
             return q_out
-        capturing = torch.cuda.is_current_stream_capturing()
+        guess = lens_t is not None and not counts
+        capturing = _capturing()
         key = B if slot_t is None else slots
         same = not counts and key == self._key and n <= self._slack and not self._captured and not capturing
         if same:
@@ -417,6 +433,7 @@ class PagedKVCache:
                 if isinstance(key, (int, SlotBatch)):
                     self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
                     self._most = max(bound[i] for i in ids)
+        self._guessed = self._guessed or guess
         P = _lib.ptr
         self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),
                    positions, axes, P(slot_t), P(lens_t), P(q_out))
@@ -450,7 +467,7 @@ class PagedKVCache:
         they see all of it, or with causal=True the tokens up to their own. scale: 1/sqrt(head_dim).
 
         Returns (B, heads, n, head_dim), zeros in padding and in rows that see nothing; a given `out` is
-        written in place, its padding left as it was."""
+        written in place, its padding left as it was; it shares no memory with q."""
         qs = self._operand(q, "q")
         B, Hq, n, D = q.shape
         if Hq == 0 or Hq % self.kv_heads:
@@ -471,7 +488,7 @@ class PagedKVCache:
                 raise ValueError("out must not be an expanded tensor")
         if q.numel() == 0:
             return out
-        if self._captured or torch.cuda.is_current_stream_capturing():
+        if self._captured or _capturing():
             most = max(self._cap[i] for i in ids)
         elif self._key is not None and self._key == (B if slot_t is None else slots):
             most = self._most

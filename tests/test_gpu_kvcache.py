@@ -371,6 +371,42 @@ def test_pages_run_out(dev):
     _check(c, q, c.attend(q))
 
 
+def test_padding_takes_no_pages(dev):
+    """Counts that the host does not see: a sequence that gets no tokens takes no further pages, calls on end."""
+    c = PagedKVCache(6, 1, 64, max_seqs=2, device=dev)
+    x = _rand((2, 1, 64, 64), BF16, dev, 0)
+    news = torch.tensor([64, 0], dtype=torch.int32, device=dev)
+    for _ in range(5):
+        c.append(x, x, new_lens=news)
+    assert c.lengths() == [320, 0] and c.free_pages() == 0
+    c.check()
+
+
+def test_captured_restore(dev):
+    """A restore recorded in a graph has not run: the host's bounds are not taken for the lengths after it."""
+    c = _cache(dev, 1, 64, 1, 64 * 6)
+    x = _rand((1, 1, 150, 64), BF16, dev, 0)
+    c.append(x[:, :, :100], x[:, :, :100])
+    snap = c.snapshot()
+    c.append(x, x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.restore(snap)
+    c.append(x[:, :, :100], x[:, :, :100])
+    assert c.lengths() == [350]
+    for m in (100, 30):
+        graph.replay()
+        torch.cuda.synchronize()
+        c.append(x[:, :, :m], x[:, :, :m])
+        assert c.lengths() == [100 + m]
+        q = x[:, :, :2].contiguous()
+        _check(c, q, c.attend(q))
+    c.check()
+    with pytest.raises(RuntimeError, match="not inside a graph capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            c.release(0)
+
+
 def test_positions_outside_the_table(dev):
     c = _cache(dev)
     rope = RotaryTable(64, 10, axes=1, device=dev)
@@ -499,6 +535,12 @@ def test_refusals(dev):
         PagedKVCache(0, 2, device=dev)
     with pytest.raises(ValueError, match="max_len"):
         PagedKVCache(4, 2, max_len=0, device=dev)
+    many = torch.zeros(1, 1, 1, 64, dtype=BF16, device=dev).expand(1, 1, (1 << 30) + 1, 64)
+    one = PagedKVCache(4, 1, device=dev)
+    with pytest.raises(ValueError, match="rows"):
+        one.append(many, many, new_lens=torch.ones(1, dtype=torch.int32, device=dev))
+    with pytest.raises(ValueError, match="rows"):
+        one.attend(many)
     c, _, _ = _filled(dev, [70], 2)
     x = _rand((1, 2, 5, 64), BF16, dev, 0)
     rope = RotaryTable(64, 16, axes=2, device=dev)
