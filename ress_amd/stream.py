@@ -19,6 +19,8 @@ from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable
 from ress_amd.qkv import _fusable, fused_qk_norm_rope, rope_base
 from ress_amd.wiring import global_blocks
 
+POSITIONS = 1024  # of the rotation tables: patches of a frame's side, and the special tokens' place
+
 
 def cached_attention(attn, x, pos, cache, tables):
     """The output of the attention module `attn` for new tokens x (B, T, dim) at positions pos (B, T, 2), which
@@ -44,7 +46,7 @@ def cached_attention(attn, x, pos, cache, tables):
         else:
             table = tables.get((hd, base))
             if table is None:
-                table = tables[(hd, base)] = RotaryTable(hd, 1024, base=base, axes=2, device=x.device)
+                table = tables[(hd, base)] = RotaryTable(hd, POSITIONS, base=base, axes=2, device=x.device)
             q = cache.append(k, v, pos=pos, rope=table, q=q)
     # written as the projection reads it
     o = torch.empty(B, T, nh, hd, dtype=x.dtype, device=x.device)
@@ -65,6 +67,7 @@ class FrameStream:
         self.frames = 0       # held now
         self.grid = None      # patch grid of the frames
         self.caches = None    # one a global layer, made with the first step
+        self._kind = None     # tokens of a frame, type and device that they were made for
         self._whole = True    # every cache holds the same frames
         self._tables = {}
 
@@ -81,6 +84,8 @@ class FrameStream:
             images = images[:, None]
         if images.dim() != 5 or images.shape[0] != self.batch or images.shape[1] < 1:
             raise ValueError(f"images must be ({self.batch}, s, 3, H, W), got {tuple(images.shape)}")
+        if images.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step counts its frames on the host: not inside a graph capture")
         if not self._whole:
             raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
         if self.frames + images.shape[1] > self.max_frames:
@@ -89,9 +94,15 @@ class FrameStream:
         x, pos, grid = agg.tokens(images, first_frame=self.frames)
         if self.grid not in (None, grid):
             raise ValueError(f"the stream's frames have a {self.grid} patch grid, got {grid}")
+        if max(grid) >= POSITIONS:
+            raise ValueError(f"a frame's side may have {POSITIONS - 1} patches, got {grid}")
         B, s, P, C = x.shape
-        if self.caches is None:
+        kind = (P, x.dtype, x.device)
+        if self.caches is None or (self._kind != kind and self.frames == 0):  # after a reset, frames of another size
             self._make(x, P)
+            self._kind = kind
+        if self._kind != kind:
+            raise ValueError(f"the stream's frames are {self._kind}, got {kind}: tokens, type and device")
         self.grid = grid
         self._whole = False
         pos_f = pos[None].expand(B * s, P, 2)
@@ -119,7 +130,7 @@ class FrameStream:
         self.frames, self._whole = frames, True
 
     def reset(self):
-        """Forgets every frame; the caches stay allocated."""
+        """Forgets every frame; the caches stay allocated, for frames of this size."""
         for c in self.caches or ():
             for slot in range(self.batch):
                 c.release(slot)

@@ -106,6 +106,15 @@ def test_stream_of_frames(dev, dtype, codes):
     s.check()
     s.reset()
     assert s.frames == 0 and torch.equal(s.step(frames[:, 0]), first)
+    s.reset()
+    larger = synthetic_frames(4, size=126, B=2, device=dev)
+    got = s.step(larger)
+    assert s.frames == 4 and torch.equal(got, FrameStream(model, 4, batch=2, codes=codes).step(larger))
+    s.check()
+    s.reset()
+    with pytest.raises(RuntimeError, match="graph capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            s.step(frames[:, 0])
 
 
 def test_all_frames_in_one_step_is_the_dense_aggregator(dev):
