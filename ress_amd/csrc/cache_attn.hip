@@ -717,11 +717,24 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   const int ns = min(a.splits, max(1, cdiv(cdiv(len, KV_PAGE), a.per)));
   const float* ml = a.part_ml + 2 * (live ? row : 0);
   const float* po = a.part_o + (live ? row : 0) * D + lane * 4;
-  float M = LOWEST, L = 0.0f;
-  if (live) {
-    for (int s = g; s < ns; s += SG) M = fmaxf(M, ml[2 * s * all_rows]);
-    for (int s = g; s < ns; s += SG) L += ml[2 * s * all_rows + 1] * exp2f(ml[2 * s * all_rows] - M);
+  // the group's parts are g + SG j; lane i weighs parts j = i, i + LPR, .. and hands the weights round (a group's lanes
+  // run alike, so those that it asks are there)
+  const int nj = live && ns > g ? cdiv(ns - g, SG) : 0;
+  const long long step = SG * all_rows;
+  auto at = [&](int j) { return g * all_rows + j * step; };
+  float M = LOWEST, L = 0.0f, m0 = LOWEST, l0 = 0.0f;
+  if (lane < nj) {
+    m0 = ml[2 * at(lane)];
+    l0 = ml[2 * at(lane) + 1];
   }
+  M = m0;
+  for (int j = lane + LPR; j < nj; j += LPR) M = fmaxf(M, ml[2 * at(j)]);
+#pragma unroll
+  for (int i = 1; i < LPR; i *= 2) M = fmaxf(M, __shfl_xor(M, i, LPR));
+  L = l0 * exp2f(m0 - M);
+  for (int j = lane + LPR; j < nj; j += LPR) L += ml[2 * at(j) + 1] * exp2f(ml[2 * at(j)] - M);
+#pragma unroll
+  for (int i = 1; i < LPR; i *= 2) L += __shfl_xor(L, i, LPR);
   if constexpr (SG > 1) {
     if (lane == 0) {
       sm[g][rw] = M;
@@ -737,19 +750,19 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   }
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (live) {
-    for (int s0 = g; s0 < ns; s0 += 4 * SG) {  // four parts at a time, their loads together
-      float f[4];
+  for (int j0 = 0; j0 < nj; j0 += LPR) {
+    if (j0 && j0 + lane < nj) {
+      m0 = ml[2 * at(j0 + lane)];
+      l0 = ml[2 * at(j0 + lane) + 1];
+    }
+    const float w = j0 + lane < nj ? l0 * inv * exp2f(m0 - M) : 0.0f;
+    for (int j = j0; j < min(j0 + LPR, nj); j += 4) {  // four parts at a time, their loads together
       v4f v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int s = s0 + i * SG;
-        const bool in = s < ns;
-        f[i] = in ? ml[2 * s * all_rows + 1] * inv * exp2f(ml[2 * s * all_rows] - M) : 0.0f;
-        v[i] = in ? *reinterpret_cast<const v4f*>(po + s * all_rows * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
-      }
+      for (int i = 0; i < 4; ++i)
+        v[i] = j + i < nj ? *reinterpret_cast<const v4f*>(po + at(j + i) * D) : v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o += v[i] * f[i];
+      for (int i = 0; i < 4; ++i) o += v[i] * __shfl(w, j - j0 + i, LPR);
     }
   }
   if constexpr (SG > 1) {
