@@ -344,8 +344,9 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   __shared__ v4f so[NW][TILES][64];
   __shared__ float sm[NW][CT][16], sl[NW][CT][16];
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h4 = lane >> 4;
-  const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / a.splits / a.tiles;
-  const int H = a.c.kv_heads, b = bh / H, h = bh % H;
+  // heads vary fastest, so every XCD gets as much of each part (the last is shorter, and short sequences have fewer)
+  const int H = a.c.kv_heads, bh = blockIdx.x % (a.B * H), split = blockIdx.x / (a.B * H) % a.splits;
+  const int tile = blockIdx.x / (a.B * H) / a.splits, b = bh / H, h = bh % H;
   const Head<D> hd(a, lens, slots, new_lens, b, h);
   const int rows = hd.nv * a.G, row0 = tile * 16 * CT;
   const long long all_rows = (long long)a.B * H * a.n * a.G;
@@ -354,6 +355,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   load_q<D, CT>(a, b, h, row0, rows, lane, qv);
 
   const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
+  const int parts = min(a.splits, cdiv(pages, a.per));
   const int lo = min(pages, split * a.per), hi = split == a.splits - 1 ? pages : min(pages, lo + a.per);
   if (split && lo >= pages) return;  // the join goes by the same count
   int limit[CT];  // tokens that the lane's query sees
@@ -502,7 +504,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     const int r = row0 + 16 * c + (lane & 15);
     if (r >= rows) continue;
     const int dim = 16 * d + 4 * h4;
-    if (a.splits == 1) {
+    if (parts <= 1) {
       const int tok = r / a.G, hq = h * a.G + r % a.G;
       store4<DT>(a.out + b * a.sob + hq * a.soh + tok * a.sot + dim, t, a.ovec);
     } else {
@@ -526,7 +528,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 // busy 67%, the matrix cores 37% (1,374 rows of 16 heads over 87,936 tokens; a page of 32 rows takes 36 products of
 // 16 cycles, 32 exponentials of 8 and some 150 other instructions of 4). 495 GFLOP in 625 us there: 790 TFLOP/s, 38% of
 // the 2,058 that the matrix cores reach. At that size and at 21,984 tokens: 2 tiles of 16 rows a wave 703, 189 us (3: 733,
-// 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 179. Eight waves a workgroup (half the widening a
+// 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 171. Eight waves a workgroup (half the widening a
 // row): 626, 168, but 166 for 150 at a head of 128 causal and grouped; four stay.
 constexpr int ROWS_CT = 2, ROWS_NW = 4;
 constexpr int rows_waves(int D) { return D == 64 ? 4 : 2; }  // a SIMD; 64 KB of LDS a workgroup at a head of 128
@@ -539,10 +541,12 @@ __global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(Atte
   __shared__ uint4 lds[2][UNITS * 128];       // a unit widened: two operand blocks of 1 KB
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, h4 = lane >> 4;
   const int H = a.c.kv_heads, groups = a.B * H * a.splits;
-  // workgroups that read the same pages go to one XCD (workgroup i runs on XCD i % 8)
+  // Workgroups that read the same pages go to one XCD (workgroup i runs on XCD i % 8), and heads vary fastest over the
+  // XCDs, as above: 1,374 rows of 16 heads over 21,984 tokens 171 us with the parts' join instead of 177, over 2 sequences of
+  // 8,000 and 2,000 tokens 102 instead of 138.
   const int x = blockIdx.x >> 3, group = x / a.tiles * 8 + (blockIdx.x & 7), tile = a.tiles - 1 - x % a.tiles;
   if (group >= groups) return;
-  const int split = group % a.splits, bh = group / a.splits, b = bh / H, h = bh % H;
+  const int split = group / (a.B * H), bh = group % (a.B * H), b = bh / H, h = bh % H;
   const Head<D> hd(a, lens, slots, new_lens, b, h);
   const int rows = hd.nv * a.G, row0 = tile * 16 * CT * NW;
   const long long all_rows = (long long)a.B * H * a.n * a.G;
@@ -554,6 +558,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(Atte
   const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
   const int before = hd.len - hd.nv;  // causal: row of token i sees before + i + 1 tokens
   auto sees = [&](int r) { return a.causal ? max(0, before + r / a.G + 1) : hd.len; };
+  const int parts = min(a.splits, cdiv(pages, a.per));
   const int lo = min(pages, split * a.per);
   if (split && lo >= pages) return;  // the join goes by the same count
   const int hi = min(split == a.splits - 1 ? pages : min(pages, lo + a.per), cdiv(sees(min(row0 + 16 * CT * NW, rows) - 1), KV_PAGE));
@@ -679,7 +684,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(Atte
     const int r = wrow + 16 * c + (lane & 15);
     if (r >= rows) continue;
     const float inv = L == 0.0f ? 0.0f : 0.5f * st.unit() / L;
-    if (a.splits == 1) {
+    if (parts <= 1) {
       const int tok = r / a.G, hq = h * a.G + r % a.G;
       uint16_t* o = a.out + b * a.sob + hq * a.soh + tok * a.sot + 4 * h4;
 #pragma unroll
@@ -712,9 +717,9 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(min(row, all_rows - 1) / per), r = (int)(row - (long long)bh * per);
   const int b = bh / H, h = bh % H, tok = r / a.G;
   const int nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
-  const bool live = row < all_rows && tok < nv;
   const int len = a.c.lens[a.slots ? a.slots[b] : b];
-  const int ns = min(a.splits, max(1, cdiv(cdiv(len, KV_PAGE), a.per)));
+  const int ns = min(a.splits, cdiv(cdiv(len, KV_PAGE), a.per));
+  const bool live = row < all_rows && tok < nv && ns > 1;  // one part is written by its workgroup
   const float* ml = a.part_ml + 2 * (live ? row : 0);
   const float* po = a.part_o + (live ? row : 0) * D + lane * 4;
   // the group's parts are g + SG j; lane i weighs parts j = i, i + LPR, .. and hands the weights round (a group's lanes
