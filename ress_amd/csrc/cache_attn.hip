@@ -528,9 +528,8 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 // busy 67%, the matrix cores 37% (1,374 rows of 16 heads over 87,936 tokens; a page of 32 rows takes 36 products of
 // 16 cycles, 32 exponentials of 8 and some 150 other instructions of 4). 495 GFLOP in 625 us there: 790 TFLOP/s, 38% of
 // the 2,058 that the matrix cores reach. At that size and at 21,984 tokens: 2 tiles of 16 rows a wave 703, 189 us (3: 733,
-// 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 171. Eight waves a workgroup (half the widening a
-// row): 626, 168, but 166 for 150 at a head of 128 causal and grouped; four stay.
-constexpr int ROWS_CT = 2, ROWS_NW = 4;
+// 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 179. Waves of a workgroup: cut().
+constexpr int ROWS_CT = 2;
 constexpr int rows_waves(int D) { return D == 64 ? 4 : 2; }  // a SIMD; 64 KB of LDS a workgroup at a head of 128
 
 template <int DT, int CODES, int D, int CT, int NW>
@@ -785,8 +784,13 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
 //
 // Up to 32 rows of a (sequence, kv head) go to the few-rows kernel: 32 rows of 16 heads over 21,984 tokens take 24 us so
 // and 25 in the other, over 87,936 tokens 40 and 49; 24 to 32 grouped rows of 8 heads of 128 25 to 49 and 29 to 53.
-// It gets workgroups for half the slots (two a CU): with four a CU the five special rows over 274,800 tokens take 123 us
+// The few-rows kernel gets workgroups for half the slots (two a CU): with four a CU the five special rows over 274,800 tokens take 123 us
 // instead of 103, the ragged batch of 32 72 instead of 74.
+//
+// Many rows: four waves a workgroup, or eight (half the widening a row) at a head of 64 where the rows fill its tiles of
+// 256 about as well and the cache is long. Eight for four, us at 8,000, 21,984 and 60,000 tokens of 16 heads: 400 rows
+// 41, 69, 159 for 43, 76, 177; 1,500 rows 78, 181, 459 for 84, 200, 513. At 3,000 tokens 28 for 27 and 45 for 46; where half of a
+// tile is empty (257 rows) 67 and 158 for 62 and 135 at the two longest; at a head of 128, causal and grouped, 166 for 150.
 struct Cut {
   int ct, nw;   // nw = 0: the few-rows kernel
   int tiles, splits, per;
@@ -805,8 +809,9 @@ Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
     least = 16;  // four a wave; with two, one row over 344 pages takes 25 us instead of 22
   } else {
     k.ct = ROWS_CT;
-    k.nw = ROWS_NW;
-    slots = (long long)rows_waves(c.head_dim) * CUS * 4 / ROWS_NW;
+    const long long tiles4 = (rows + 64 * ROWS_CT - 1) / (64 * ROWS_CT);
+    k.nw = c.head_dim == 64 && pages >= 64 && (tiles4 % 2 == 0 || tiles4 > 16) ? 8 : 4;
+    slots = (long long)rows_waves(c.head_dim) * CUS * 4 / k.nw;
     least = 8;
   }
   const int tile = 16 * k.ct * (k.nw ? k.nw : 1);
@@ -852,7 +857,14 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
   } else {
     const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
     RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
-    hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, ROWS_CT, ROWS_NW>), dim3((unsigned)g), dim3(64 * ROWS_NW), 0, stream, a, RESS_READ_ONLY_ARGS);
+    bool eight = false;
+    if constexpr (D == 64) {
+      eight = k.nw == 8;
+      if (eight)
+        hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, ROWS_CT, 8>), dim3((unsigned)g), dim3(512), 0, stream, a, RESS_READ_ONLY_ARGS);
+    }
+    if (!eight)
+      hipLaunchKernelGGL((k_cache_attn_rows<DT, CODES, D, ROWS_CT, 4>), dim3((unsigned)g), dim3(256), 0, stream, a, RESS_READ_ONLY_ARGS);
     RESS_LAUNCHED("k_cache_attn_rows");
   }
   if (k.splits > 1) {

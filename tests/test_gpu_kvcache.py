@@ -201,6 +201,41 @@ def test_attend_split(dev, dtype, codes, D, n, L):
         _check(c, q, c.attend(q, causal=causal), causal=causal)
 
 
+@pytest.mark.parametrize("dtype,codes", [(BF16, "int8"), (BF16, "fp8"), (F16, "int8"), (F16, "fp8")])
+@pytest.mark.parametrize("n,G", [(129, 1), (256, 1), (60, 4), (250, 2)])
+def test_attend_wide_tiles(dev, dtype, codes, n, G):
+    """Workgroups of eight waves, over ragged caches: the longest in parts, others in one, one shorter than its rows."""
+    lens = [5000, 4100, 700, n // 2]
+    c, _, _ = _filled(dev, lens, 1, 64, dtype, codes)
+    q = _rand((len(lens), G, n, 64), dtype, dev, 7, 1.5)
+    for causal in (False, True):
+        _check(c, q, c.attend(q, causal=causal), causal=causal)
+    news = [n, n - 100 if n > 100 else 1, 0, n // 2]
+    _check(c, q, c.attend(q, causal=True, new_lens=news), n_new=news, causal=True)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [5, 200])
+def test_attend_parts_not_finite(dev, D, n):
+    """A page that is not finite in the second part of a split cache: its rows are NaN, other sequences' as before, and
+    so are the rows of a causal chunk that end before it."""
+    T = 9000
+    c, k, v = _filled(dev, [T, T], 1, D)
+    q = _rand((2, 1, n, D), BF16, dev, 3)
+    want = c.attend(q, causal=True)
+    at = T - n // 2
+    for name in ("k", "v"):
+        d, _, _ = _filled(dev, [at, T], 1, D)
+        kk, vv = k[:, :, at:].clone(), v[:, :, at:].clone()
+        (kk if name == "k" else vv)[0, 0, 0, 3] = float("nan")
+        d.append(kk[:1], vv[:1], slots=[0])
+        got = d.attend(q, causal=True)
+        assert torch.equal(got[1], want[1])
+        hit = max(0, at // PAGE * PAGE - (T - n))
+        assert torch.isfinite(got[0, 0, :hit]).all() and got[0, 0, n - n // 2:].isnan().all()
+        assert torch.equal(got[0, 0, :hit], want[0, 0, :hit])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("n", [8, 48])
 def test_attend_rows_that_see_nothing(dev, dtype, n):
