@@ -88,8 +88,8 @@ __device__ __forceinline__ uint32_t top_bits(const uint4& v, uint32_t m) {
 //
 // A page's tokens stay in registers between its maximum and its codes, so they are read once; a head's values are
 // transposed through LDS, in rows of 17 words, and leave as whole lines. Bound by memory where there is much to append
-// (8 sequences of up to 1,000 tokens, 24 heads of 64: 33 us for 106 MB, 3.2 TB/s), else by the chain length -> tokens ->
-// maximum -> codes -> length (1,374 tokens of 16 heads, 9.5 us for 11 MB; a token each of 32 sequences, 8.4 us): with
+// (8 sequences of up to 1,000 tokens, 24 heads of 64: 32 us for 110 MB, 3.4 TB/s), else by the chain length -> tokens ->
+// maximum -> codes -> length (1,374 tokens of 16 heads, 9.6 us for 14 MB; a token each of 32 sequences, 8 us): with
 // the first tokens on their way before the length is known and each sequence's counter on a line of its own it took
 // 66 -> 50 us of the first, its reading back included.
 template <int DT, int CODES, int D>
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
 
 // Tokens start..start+n-1 of each sequence in 16 bits (zeros before its first and past its last).
 // One workgroup per page that the window can touch and head: codes transposed through LDS. Bound by memory (8 x 1,000
-// tokens of 24 heads of 64: 14 us for 74 MB, 5.1 TB/s).
+// tokens of 24 heads of 64: 14 us for 70 MB, 5 TB/s).
 template <int DT, int CODES, int D>
 __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int* __restrict__ slots,
                                                      const int* __restrict__ start, int n, int pages,
