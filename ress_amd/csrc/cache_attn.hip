@@ -354,6 +354,35 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   uint4 qv[CT][D / 32];
   load_q<D, CT>(a, b, h, row0, rows, lane, qv);
 
+  const int* __restrict__ table = table_all + (long long)hd.slot * a.c.max_pages;
+  constexpr int KU = D / 16, VU = D / 16;  // 1 KB units of a page: keys (4 tiles x D / 64 halves), values (D / 16)
+  // A page's codes are loaded as soon as the registers are free: the next one's keys behind the scores, its values
+  // behind P V; its number a page ahead of them. The first page's are on their way before the length is known (they are
+  // not used where it has none). A bad page number reads as a page of zeros.
+  uint4 kw[KU], vw[VU];
+  float ks = 0.0f, vs = 0.0f;
+  int bad = 0;
+  auto number = [&](int pg) { return pg < a.c.max_pages ? table[pg] : -1; };
+  auto there = [&](int id) { return id >= 0 && id < a.c.n_pages; };
+  const unsigned k0 = (lane & 15) * (D / 16) + h4, v0 = (lane & 15) * 4 + h4;  // in 16-byte pieces
+  auto load_k = [&](int id) {
+    const int pid = there(id) ? id : 0;
+    const uint4* p = reinterpret_cast<const uint4*>(hd.kc + pid * hd.stride);
+#pragma unroll
+    for (int u = 0; u < KU; ++u) kw[u] = at_u32(p, k0 + u / (D / 64) * D + u % (D / 64) * 4);
+    ks = there(id) ? k_scale[(long long)pid * H + h] : 0.0f;
+  };
+  auto load_v = [&](int id) {
+    const int pid = there(id) ? id : 0;
+    const uint4* p = reinterpret_cast<const uint4*>(hd.vc + pid * hd.stride);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) vw[u] = at_u32(p, v0 + u * 64);
+    vs = there(id) ? v_scale[(long long)pid * H + h] : 0.0f;
+  };
+  int id = number(split * a.per + w), next = number(split * a.per + w + NW);
+  load_k(id);
+  load_v(id);
+
   const int full = hd.len / KV_PAGE, left = hd.len % KV_PAGE, pages = full + (left ? 1 : 0);
   const int parts = min(a.splits, cdiv(pages, a.per));
   const int lo = min(pages, split * a.per), hi = split == a.splits - 1 ? pages : min(pages, lo + a.per);
@@ -370,36 +399,6 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 
   Rows<DT, D, CT> st;
   st.clear();
-  const int* __restrict__ table = table_all + (long long)hd.slot * a.c.max_pages;
-  constexpr int KU = D / 16, VU = D / 16;  // 1 KB units of a page: keys (4 tiles x D / 64 halves), values (D / 16)
-  // A page's codes are loaded as soon as the registers are free: the next one's keys behind the scores, its values
-  // behind P V. A bad page number reads as a page of zeros.
-  uint4 kw[KU], vw[VU];
-  float ks = 0.0f, vs = 0.0f;
-  int bad = 0;
-  auto page_id = [&](int pg, bool& ok) {
-    const int pid = pg < a.c.max_pages ? table[pg] : -1;
-    ok = pid >= 0 && pid < a.c.n_pages;
-    bad |= !ok;
-    return ok ? pid : 0;
-  };
-  const unsigned k0 = (lane & 15) * (D / 16) + h4, v0 = (lane & 15) * 4 + h4;  // in 16-byte pieces
-  auto load_k = [&](int pg) {
-    bool ok;
-    const int pid = page_id(pg, ok);
-    const uint4* p = reinterpret_cast<const uint4*>(hd.kc + pid * hd.stride);
-#pragma unroll
-    for (int u = 0; u < KU; ++u) kw[u] = at_u32(p, k0 + u / (D / 64) * D + u % (D / 64) * 4);
-    ks = ok ? k_scale[(long long)pid * H + h] : 0.0f;
-  };
-  auto load_v = [&](int pg) {
-    bool ok;
-    const int pid = page_id(pg, ok);
-    const uint4* p = reinterpret_cast<const uint4*>(hd.vc + pid * hd.stride);
-#pragma unroll
-    for (int u = 0; u < VU; ++u) vw[u] = at_u32(p, v0 + u * 64);
-    vs = ok ? v_scale[(long long)pid * H + h] : 0.0f;
-  };
   auto weights = [&](const v4f (&s)[CT][4], float cs, float v, int pg, uint4 (&p)[CT][2]) {
     int lim[CT];
 #pragma unroll
@@ -409,12 +408,9 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   };
 
   const int last = min(min(hi, full), cdiv(seen_by_any, KV_PAGE));
-  int pg = lo + w;
-  if (pg < last) {
-    load_k(pg);
-    load_v(pg);
-  }
-  for (; pg < last; pg += NW) {
+  for (int pg = lo + w; pg < last; pg += NW) {
+    bad |= !there(id);
+    const int after = pg + 2 * NW < last ? number(pg + 2 * NW) : -1;
     v4f s[CT][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -432,7 +428,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
       }
     }
     const float cs = ks * a.scale, v = vs;
-    if (pg + NW < last) load_k(pg + NW);
+    if (pg + NW < last) load_k(next);
     uint4 p[CT][2];
     weights(s, cs, v, pg, p);
     const float vscale = value_scale<DT>(v);
@@ -442,7 +438,9 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
       widen16_v<DT, CODES>(vw[d], vscale, x, y);
       st.add(d, x, y, p);
     }
-    if (pg + NW < last) load_v(pg + NW);
+    if (pg + NW < last) load_v(next);
+    id = next;
+    next = after;
   }
   if (bad && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
   // the unfinished page, by the wave whose turn it would be
