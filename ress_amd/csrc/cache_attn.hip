@@ -314,17 +314,32 @@ __device__ __forceinline__ void widen16_v(const uint4& w, float scale, uint4& a,
     times(b.x); times(b.y); times(b.z); times(b.w);
   }
 }
-// 16-bit tail values times a power of two; places of tokens from cnt on are zero
+// A lane's values of the unfinished page: its 16 places (16 h4 on) of a dim, two a word. keep[] clears those of tokens from
+// cnt on (all of them with down = 0); bf16: times the power of two `down` (exact but for values 2^-126 and less, which are
+// cut off). Two words' worth of instructions a word: this code runs once a call, mostly as fast as it is fetched (with
+// conversions and comparisons an element, and loads as they were needed, a call took 4 to 14 us more: 4 sequences of 1,000
+// tokens, 32 heads over 8 of 128, 25 us instead of 13).
 template <int DT>
-__device__ __forceinline__ uint4 tail_v8(const uint4& w, float down, int place, int cnt) {
-  uint16_t e[8];
+struct TailValues {
+  uint32_t keep[8];
+  float down;
+  __device__ __forceinline__ TailValues(float down_, int h4, int cnt) : down(down_) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = Elem<DT>::get(elem8(w, i));
-    e[i] = down != 0.0f && v_token(place + i) < cnt ? Elem<DT>::put(x * down) : 0;
+    for (int i = 0; i < 8; ++i) {
+      const int t = v_token(2 * i) + 4 * h4;  // v_token(16 h4 + 2 i); the next place is the next token
+      keep[i] = down == 0.0f ? 0u : t + 1 < cnt ? ~0u : t < cnt ? 0xffffu : 0u;
+    }
   }
-  return pack8(e);
-}
+  __device__ __forceinline__ uint32_t pair(uint32_t w, int i) const {
+    w &= keep[i];
+    if constexpr (DT == KV_F16) return w;
+    const float lo = __uint_as_float(w << 16) * down, hi = __uint_as_float(w & 0xffff0000u) * down;
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+  }
+  __device__ __forceinline__ uint4 half(const uint4& w, int i) const {  // places 8 i on
+    return make_uint4(pair(w.x, 4 * i), pair(w.y, 4 * i + 1), pair(w.z, 4 * i + 2), pair(w.w, 4 * i + 3));
+  }
+};
 
 // Waves that a SIMD's registers are shared out for. One more spills: 22 us for one row of 16 heads of 64 over 21,984
 // tokens instead of 20, 114 for 32 sequences of up to 8,192 tokens, 8 heads of 128, instead of 74; with 32 rows and a
@@ -445,27 +460,37 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
   if (bad && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
   // the unfinished page, by the wave whose turn it would be
   if (left && full >= lo && full < hi && (full - lo) % NW == w && full * KV_PAGE < seen_by_any) {
-    const TailScale<DT> ts(a.c.tail_top[(long long)hd.slot * H + h]);
+    // its loads together
+    const float top = a.c.tail_top[(long long)hd.slot * H + h];
+    uint4 kt[4][D / 32], vt[VU][2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e)
+        kt[k][e] = *reinterpret_cast<const uint4*>(hd.tk + (16 * k + (lane & 15)) * D + 64 * (e >> 1) + 16 * h4 + 8 * (e & 1));
+#pragma unroll
+    for (int d = 0; d < VU; ++d) {
+      const uint4* row = reinterpret_cast<const uint4*>(hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4);
+      vt[d][0] = row[0];
+      vt[d][1] = row[1];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const TailScale<DT> ts(top);
+    const TailValues<DT> tv(ts.down, h4, left);
     v4f s[CT][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) s[c][k] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) {
-        const uint4 x = *reinterpret_cast<const uint4*>(hd.tk + (16 * k + (lane & 15)) * D + 64 * (e >> 1) + 16 * h4 + 8 * (e & 1));
+      for (int e = 0; e < D / 32; ++e)
 #pragma unroll
-        for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(x, qv[c][e], s[c][k]);
-      }
+        for (int c = 0; c < CT; ++c) s[c][k] = mfma<DT>(kt[k][e], qv[c][e], s[c][k]);
     }
     uint4 p[CT][2];
     weights(s, a.scale, ts.vs, full, p);
 #pragma unroll
-    for (int d = 0; d < VU; ++d) {
-      const uint16_t* row = hd.tv + (16 * d + (lane & 15)) * KV_PAGE + 16 * h4;
-      st.add(d, tail_v8<DT>(*reinterpret_cast<const uint4*>(row), ts.down, 16 * h4, left),
-             tail_v8<DT>(*reinterpret_cast<const uint4*>(row + 8), ts.down, 16 * h4 + 8, left), p);
-    }
+    for (int d = 0; d < VU; ++d) st.add(d, tv.half(vt[d][0], 0), tv.half(vt[d][1], 1), p);
   }
 
   // join the four waves
@@ -603,14 +628,15 @@ __global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(Atte
     }
   };
   auto stage_tail = [&](int buf, const TailScale<DT>& ts) {
+    const TailValues<DT> tv(ts.down, h4, left);
 #pragma unroll
     for (int i = 0; i < UPW; ++i) {
       const bool key = w * UPW + i < KU;
       const uint4* src = reinterpret_cast<const uint4*>(key ? hd.tk : hd.tv) + 2 * piece[i];
       uint4 x = src[0], y = src[1];
       if (!key) {
-        x = tail_v8<DT>(x, ts.down, 16 * h4, left);
-        y = tail_v8<DT>(y, ts.down, 16 * h4 + 8, left);
+        x = tv.half(x, 0);
+        y = tv.half(y, 1);
       }
       lds[buf][(w * UPW + i) * 128 + lane] = x;
       lds[buf][(w * UPW + i) * 128 + 64 + lane] = y;
