@@ -351,7 +351,7 @@ constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D 
 // fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
 // joined in LDS. Bound by the bytes of the codes where the cache is long (5 rows of 16 heads over 274,800 tokens: 98 us
 // for 563 MB, 5.7 TB/s), by one page's chain of loads, scores, exponentials and products where it is short (one row over
-// 21,984 tokens: 16 us, 2.8 TB/s).
+// 21,984 tokens: 12 us, 3.8 TB/s).
 template <int DT, int CODES, int D, int CT>
 __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a, RESS_READ_ONLY) {
   constexpr int NW = 4;
@@ -809,7 +809,7 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
 // Up to 32 rows of a (sequence, kv head) go to the few-rows kernel: 32 rows of 16 heads over 21,984 tokens take 24 us so
 // and 25 in the other, over 87,936 tokens 40 and 49; 24 to 32 grouped rows of 8 heads of 128 25 to 49 and 29 to 53.
 // The few-rows kernel gets workgroups for half the slots (two a CU): with four a CU the five special rows over 274,800 tokens take 123 us
-// instead of 103, the ragged batch of 32 72 instead of 74.
+// instead of 103, the ragged batch of 32 72 instead of 74; with one 111 instead of 102 and 61 instead of 63.
 //
 // Many rows: four waves a workgroup, or eight (half the widening a row) at a head of 64 where the rows fill its tiles of
 // 256 about as well and the cache is long. Eight for four, us at 8,000, 21,984 and 60,000 tokens of 16 heads: 400 rows
@@ -830,7 +830,10 @@ Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
     k.ct = rows <= 16 ? 1 : 2;
     k.nw = 0;
     slots = 2 * CUS;
-    least = 16;  // four a wave; with two, one row over 344 pages takes 25 us instead of 22
+    // Two a wave; a second part, and with it a second launch, from 32 pages on (1,500 tokens 17 us in two parts, 13 in
+    // one). Four a wave: one row over 344 pages 18 us instead of 17, 32 rows 22 instead of 20, 4 sequences of 63 pages 20
+    // instead of 17.
+    least = pages < 32 ? 16 : 8;
   } else {
     k.ct = ROWS_CT;
     const long long tiles4 = (rows + 64 * ROWS_CT - 1) / (64 * ROWS_CT);
