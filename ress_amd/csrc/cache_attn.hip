@@ -273,7 +273,7 @@ __device__ __forceinline__ void load_q(const AttendArgs& a, int b, int h, int ro
 }
 
 // Twice `half`, a weighted mean of values over two. No mean passes the type's largest value, but the weights and v_scale are
-// rounded by 2^-9 (bf16) or 2^-11, so its sum may: it ends there. Infinite values in an unfinished page stay infinite.
+// rounded by 2^-9 (bf16) or 2^-11, so its sum may: it ends there. Infinities and NaN stay.
 template <int DT>
 __device__ __forceinline__ v4f mean4(const v4f& half) {
   constexpr float TOP = DT == KV_F16 ? 0.5f * 65504.0f : 0x0.ffp127f;
