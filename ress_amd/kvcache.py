@@ -184,15 +184,16 @@ class PagedKVCache:
         return SlotBatch(ids, self.device)
 
     def _batch(self, slots, B):
+        """(slots on the host, on the device or None, the batch's key: B where no slots are given, else a SlotBatch)."""
         if slots is None:
             if B > self.max_seqs:
                 raise ValueError(f"a batch of {B} needs {B} slots, the cache has {self.max_seqs}")
-            return range(B), None
+            return range(B), None, B
         if not isinstance(slots, SlotBatch):
             slots = self.slots(slots)
         if len(slots) != B or slots.tensor.device != self.device or any(i >= self.max_seqs for i in slots.ids):
             raise ValueError(f"the batch has {B} rows and {len(slots)} slots, or they belong to another cache")
-        return slots.ids, slots.tensor
+        return slots.ids, slots.tensor, slots
 
     @staticmethod
     def _not_capturing(name, want):
@@ -383,7 +384,7 @@ class PagedKVCache:
         ks = self._operand(k, "k", self.kv_heads)
         vs = self._operand(v, "v", self.kv_heads, like=k)
         B, n = k.shape[0], k.shape[2]
-        ids, slot_t = self._batch(slots, B)
+        ids, slot_t, key = self._batch(slots, B)
         if (pos is None) != (rope is None):
             raise ValueError("pos and rope go together")
         qs, q_out, q_heads = (0, 0, 0), None, 0
@@ -413,7 +414,6 @@ class PagedKVCache:
             return q_out
         guess = lens_t is not None and not counts
         capturing = _capturing()
-        key = B if slot_t is None else slots
         same = not counts and key == self._key and n <= self._slack and not self._captured and not capturing
         if same:
             self._lag += n
@@ -430,9 +430,8 @@ class PagedKVCache:
             else:
                 for i, c in zip(ids, counts):
                     bound[i] = min(bound[i] + c, cap[i])
-                if isinstance(key, (int, SlotBatch)):
-                    self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
-                    self._most = max(bound[i] for i in ids)
+                self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
+                self._most = max(bound[i] for i in ids)
         self._guessed = self._guessed or guess
         P = _lib.ptr
         self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),
@@ -446,7 +445,7 @@ class PagedKVCache:
         if slots is not None and not isinstance(slots, SlotBatch):
             slots = self.slots(slots)
         B = len(slots) if slots is not None else len(start) if start is not None else self.max_seqs if batch is None else batch
-        _, slot_t = self._batch(slots, B)
+        _, slot_t, _ = self._batch(slots, B)
         n = int(n)
         if n < 0:
             raise ValueError(f"n must not be negative, got {n}")
@@ -472,7 +471,7 @@ class PagedKVCache:
         B, Hq, n, D = q.shape
         if Hq == 0 or Hq % self.kv_heads:
             raise ValueError(f"q must have a multiple of {self.kv_heads} heads, got {Hq}")
-        ids, slot_t = self._batch(slots, B)
+        ids, slot_t, key = self._batch(slots, B)
         lens_t, _ = self._new_lens(new_lens, B, n)
         scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
         if not 0.0 < scale < math.inf:
@@ -490,7 +489,7 @@ class PagedKVCache:
             return out
         if self._captured or _capturing():
             most = max(self._cap[i] for i in ids)
-        elif self._key is not None and self._key == (B if slot_t is None else slots):
+        elif self._key is not None and self._key == key:
             most = self._most
         else:
             self._settle()
