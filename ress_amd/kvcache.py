@@ -261,18 +261,22 @@ class PagedKVCache:
         have, need = len(self._pages[slot]), -(-n_tokens // PAGE)
         if need <= have:
             return
-        new = [self._free.pop() for _ in range(need - have)]
-        self._pages[slot] += new
-        self._cap[slot] = PAGE * need
+        new = self._free[have - need:][::-1]
         with torch.cuda.device(self.device):
             self.table[slot, have:need] = torch.tensor(new, dtype=torch.int32, device=self.device)
             self.held[slot:slot + 1].fill_(need)
+        # the device has them: a copy that failed leaves them free
+        del self._free[have - need:]
+        self._pages[slot] += new
+        self._cap[slot] = PAGE * need
 
     def reserve(self, slot, n_tokens):
         """Pages for n_tokens tokens of a slot in all (those it holds included). append reserves by
         itself what it needs, except inside a graph capture."""
         if not 0 <= slot < self.max_seqs:
             raise IndexError(f"slot must lie in 0..{self.max_seqs - 1}, got {slot}")
+        if _capturing():
+            raise RuntimeError("reserve copies page numbers from the host: not inside a graph capture")
         self._settle()
         self._fits({slot: int(n_tokens)}, refuse=True)
         self._take(slot, int(n_tokens))

@@ -1,0 +1,53 @@
+"""Pages taken and not taken: what a refused or failed call leaves behind (no GPU)."""
+
+import pytest
+import torch
+
+from host_cache import host_cache, tokens
+from ress_amd import kvcache
+
+
+def test_reserve_refuses_a_capture(monkeypatch):
+    """Its copy of page numbers cannot be recorded: refused before anything changes."""
+    c = host_cache(monkeypatch)
+    x = tokens(1, 10)
+    c.append(x, x)
+    before = (c.free_pages(), list(c._cap), c.table.clone(), c.held.clone())
+    with monkeypatch.context() as m:
+        m.setattr(kvcache, "_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="not inside a graph capture"):
+            c.reserve(0, 200)
+    assert before[:2] == (c.free_pages(), c._cap) and torch.equal(before[2], c.table) and torch.equal(before[3], c.held)
+    c.append(tokens(1, 300), tokens(1, 300))
+    c.check()
+    assert c.lens.tolist() == [310, 0] and c.held.tolist() == [5, 0] and c.free_pages() == 3
+
+
+@pytest.mark.parametrize("where", ["table", "held"])
+def test_pages_are_taken_once_the_device_has_them(monkeypatch, where):
+    """A copy that fails (no memory, say) leaves the pages free and the slot as it was."""
+    c = host_cache(monkeypatch)
+    x = tokens(1, 10)
+    c.append(x, x)
+
+    class Fails:
+        def __init__(self, t):
+            self.t = t
+
+        def __getitem__(self, at):
+            raise torch.OutOfMemoryError("no memory")
+
+        __setitem__ = lambda self, at, value: self[at]
+
+    real = getattr(c, where)
+    setattr(c, where, Fails(real))
+    with pytest.raises(torch.OutOfMemoryError):
+        c.reserve(0, 200)
+    with pytest.raises(torch.OutOfMemoryError):
+        c.append(tokens(1, 100), tokens(1, 100))
+    setattr(c, where, real)
+    assert c.free_pages() == 7 and c._cap == [64, 0]
+    c.append(tokens(1, 300), tokens(1, 300))
+    c.check()
+    assert c.lens.tolist() == [310, 0] and c.held.tolist() == [5, 0] and c.free_pages() == 3
+    assert sorted(c.table[0, :5].tolist() + c._free) == list(range(8))
