@@ -419,27 +419,27 @@ class PagedKVCache:
         guess = lens_t is not None and not counts
         capturing = _capturing()
         same = not counts and key == self._key and n <= self._slack and not self._captured and not capturing
+        bound, cap = self._bound, self._cap
+        if not same:
+            self._settle()
+            counts = counts or [n] * B
+            if self._captured or capturing or any(bound[i] + c > cap[i] for i, c in zip(ids, counts)):
+                self._room(ids, counts, exact=not torch.is_tensor(new_lens))
+            self._captured = self._captured or capturing
+        P = _lib.ptr
+        self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),
+                   positions, axes, P(slot_t), P(lens_t), P(q_out))
+        # counted once the call is under way: one that fails appends nothing
         if same:
             self._lag += n
             self._slack -= n
             self._most += n
-        else:
-            self._settle()
-            counts = counts or [n] * B
-            bound, cap = self._bound, self._cap
-            if self._captured or capturing or any(bound[i] + c > cap[i] for i, c in zip(ids, counts)):
-                self._room(ids, counts, exact=not torch.is_tensor(new_lens))
-            if capturing:
-                self._captured = True
-            else:
-                for i, c in zip(ids, counts):
-                    bound[i] = min(bound[i] + c, cap[i])
-                self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
-                self._most = max(bound[i] for i in ids)
+        elif not capturing:
+            for i, c in zip(ids, counts):
+                bound[i] = min(bound[i] + c, cap[i])
+            self._key, self._slack = key, min(cap[i] - bound[i] for i in ids)
+            self._most = max(bound[i] for i in ids)
         self._guessed = self._guessed or guess
-        P = _lib.ptr
-        self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),
-                   positions, axes, P(slot_t), P(lens_t), P(q_out))
         return q_out
 
     def read(self, n, slots=None, start=None, batch=None):

@@ -51,3 +51,25 @@ def test_pages_are_taken_once_the_device_has_them(monkeypatch, where):
     c.check()
     assert c.lens.tolist() == [310, 0] and c.held.tolist() == [5, 0] and c.free_pages() == 3
     assert sorted(c.table[0, :5].tolist() + c._free) == list(range(8))
+
+
+@pytest.mark.parametrize("n", [10, 100])
+@pytest.mark.parametrize("again", [False, True])
+def test_a_call_that_fails_appends_nothing(monkeypatch, n, again):
+    """The library refuses or cannot launch: the host counts no token (a quick repeat of the last batch or not)."""
+    fail = {}
+    c = host_cache(monkeypatch, fail=fail)
+    x, y = tokens(1, 10), tokens(1, n)
+    c.append(x, x)
+    fail["append"] = RuntimeError("ress_kv_append failed")
+    for slots in (None, None if again else [1]):
+        with pytest.raises(RuntimeError, match="failed"):
+            c.append(y, y, slots=slots)
+    fail.clear()
+    if again:
+        c.append(x, x)
+    c._settle()
+    assert c._bound == c.lens.tolist() == [20 if again else 10, 0]
+    c.append(y, y)
+    assert c._most == int(c.lens[0])
+    c.check()
