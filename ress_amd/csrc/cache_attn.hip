@@ -872,18 +872,19 @@ long long part_floats(const ress_kv_cache& c, int B, int Hq, int n, const Cut& k
 
 template <int DT, int CODES, int D>
 int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
-  const long long heads = (long long)a.B * a.c.kv_heads;
+  const long long heads = (long long)a.B * a.c.kv_heads, rows = heads * a.n * a.G;
+  const bool wide = rows >= 2048;  // the join's workgroups take whole rows
+  const long long join = k.splits == 1 ? 0 : wide ? (rows + 1024 / D - 1) / (1024 / D) : rows;  // 256 threads, D / 4 a row
+  const long long g = k.nw == 0 ? heads * k.tiles * k.splits : (heads * k.splits + 7) / 8 * 8 * k.tiles;
+  RESS_REQUIRE(launchable(g, k.nw ? 64 * k.nw : 256) && launchable(join, 256),
+               "ress_kv_attend: the call needs 2^32 threads or more");
   if (k.nw == 0) {
-    const long long g = heads * k.tiles * k.splits;
-    RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
     if (k.ct == 1)
       hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 1>), dim3((unsigned)g), dim3(256), 0, stream, a, RESS_READ_ONLY_ARGS);
     else
       hipLaunchKernelGGL((k_cache_attn_few<DT, CODES, D, 2>), dim3((unsigned)g), dim3(256), 0, stream, a, RESS_READ_ONLY_ARGS);
     RESS_LAUNCHED("k_cache_attn_few");
   } else {
-    const long long g = (heads * k.splits + 7) / 8 * 8 * k.tiles;
-    RESS_REQUIRE(g < (1ll << 31), "ress_kv_attend: the call needs more than 2^31 workgroups");
     bool eight = false;
     if constexpr (D == 64) {
       eight = k.nw == 8;
@@ -895,11 +896,10 @@ int launch(AttendArgs& a, const Cut& k, hipStream_t stream) {
     RESS_LAUNCHED("k_cache_attn_rows");
   }
   if (k.splits > 1) {
-    const long long rows = heads * a.n * a.G, per = 256 / (D / 4);
-    if (rows >= 2048)
-      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 1>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+    if (wide)
+      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 1>), dim3((unsigned)join), dim3(256), 0, stream, a);
     else
-      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 256 / (D / 4)>), dim3((unsigned)rows), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((k_cache_attn_join<DT, D, 256 / (D / 4)>), dim3((unsigned)join), dim3(256), 0, stream, a);
     RESS_LAUNCHED("k_cache_attn_join");
   }
   return 0;

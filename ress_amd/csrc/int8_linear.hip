@@ -361,17 +361,19 @@ bool few(int M, int K) { return M <= FEW && M * padded(K) <= FEW_BYTES; }
 template <int DT>
 int quantize(const void* x, long long stride, int M, int K, void* codes, long long kp, float* scale, hipStream_t stream) {
   const bool vec = (uintptr_t)x % 16 == 0 && stride % 8 == 0;
-  hipLaunchKernelGGL(k_quantize_rows<DT>, dim3((M + 3) / 4), dim3(256), 0, stream, (const uint16_t*)x, stride, M, K,
-                     (uint8_t*)codes, kp, scale, vec);
-  RESS_LAUNCHED("k_quantize_rows");
+  constexpr int MOST = 1 << 25;  // rows of a launch, of 64 threads each
+  for (long long m = 0; m < M; m += MOST) {
+    const int rows = (int)(M - m < MOST ? M - m : MOST);
+    hipLaunchKernelGGL(k_quantize_rows<DT>, dim3((rows + 3) / 4), dim3(256), 0, stream, (const uint16_t*)x + m * stride, stride,
+                       rows, K, (uint8_t*)codes + m * kp, kp, scale + m, vec);
+    RESS_LAUNCHED("k_quantize_rows");
+  }
   return 0;
 }
 
 template <int DT, int BM, int BN, int GM, int GN>
 int gemm(const uint8_t* codes, int kp, const float* sx, const void* w, int K, const Out& o, hipStream_t stream) {
-  const long long tiles = (long long)cdiv(o.M, BM) * cdiv(o.N, BN);
-  RESS_REQUIRE(tiles < (1ll << 30), "ress_int8_linear: the call needs too many workgroups");
-  const int grid = (int)((tiles + 7) / 8 * 8);
+  const int grid = (int)(((long long)cdiv(o.M, BM) * cdiv(o.N, BN) + 7) / 8 * 8);  // launchable: linear()
   if (K == kp)
     hipLaunchKernelGGL((k_int8_gemm<DT, BM, BN, GM, GN, true>), dim3(grid), dim3(64 * GM * GN), 0, stream, codes, kp, sx,
                        (const uint8_t*)w, K, o);
@@ -388,12 +390,12 @@ int gemm(const uint8_t* codes, int kp, const float* sx, const void* w, int K, co
 //   4096 x 4096 x 4096 58, 80, 66 | 58        21984 x 1024 (N) x 4096 (K) 105, 91, 102 | 91
 //   8192 x 8192 x 8192 495, 479, 544 | 495    21984 x 4096 (N) x 1024 (K) 143, 151, 135 | 135
 // and 1374 x 1024 (N) x 4096 (K): 128 x 128 17, 64 x 128 15, 64 x 64 12 | 12.
+constexpr struct {
+  int bm, bn, threads, held;
+  double alone, full, ends;
+} tiles[] = {{256, 256, 512, 1, 1.20, 1.75, 10.0}, {192, 256, 512, 1, 0.97, 1.30, 8.5}, {128, 128, 512, 2, 0.52, 1.06, 3.7},
+             {64, 128, 256, 3, 0.47, 0.92, 2.5}, {64, 64, 256, 5, 0.37, 0.95, 2.0}};
 int pick(int M, int N, int steps) {
-  static const struct {
-    int bm, bn, held;
-    double alone, full, ends;
-  } tiles[] = {{256, 256, 1, 1.20, 1.75, 10.0}, {192, 256, 1, 0.97, 1.30, 8.5}, {128, 128, 2, 0.52, 1.06, 3.7},
-               {64, 128, 3, 0.47, 0.92, 2.5}, {64, 64, 5, 0.37, 0.95, 2.0}};
   int best = 0;
   double least = 0.0;
   for (int i = 0; i < 5; ++i) {
@@ -424,10 +426,13 @@ int linear(const void* x, long long stride, int K, const void* w, const Out& o, 
     RESS_LAUNCHED("k_int8_few");
     return 0;
   }
+  const int tile = pick(o.M, o.N, (int)(kp / 128));
+  RESS_REQUIRE(launchable((long long)cdiv(o.M, tiles[tile].bm) * cdiv(o.N, tiles[tile].bn) + 7, tiles[tile].threads),
+               "ress_int8_linear: the call needs 2^32 threads or more");
   uint8_t* codes = (uint8_t*)workspace;
   float* sx = (float*)(codes + code_bytes(o.M, K));
   if (int rc = quantize<DT>(x, stride, o.M, K, codes, kp, sx, stream)) return rc;
-  switch (pick(o.M, o.N, (int)(kp / 128))) {
+  switch (tile) {
     case 0: return gemm<DT, 256, 256, 2, 4>(codes, (int)kp, sx, w, K, o, stream);
     case 1: return gemm<DT, 192, 256, 2, 4>(codes, (int)kp, sx, w, K, o, stream);
     case 2: return gemm<DT, 128, 128, 2, 4>(codes, (int)kp, sx, w, K, o, stream);

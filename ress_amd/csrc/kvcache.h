@@ -24,6 +24,9 @@ constexpr int KV_ST_FULL = 1, KV_ST_POS = 2, KV_ST_PAGE = 4, KV_ST_NONFINITE = 8
 // Checks a cache handle on the host (kvcache.hip): 0, or -1 with the message set.
 int ress_kv_check(const ress_kv_cache* c, int B, const char* who);
 
+// A launch counts its threads in 32 bits.
+inline bool launchable(long long workgroups, long long threads) { return workgroups * threads < (1ll << 32); }
+
 // the token of place p of a value row: p = 16h + 8u + 4g + r  <->  token 32u + 16g + 4h + r
 __host__ __device__ constexpr __forceinline__ int v_token(int p) {
   return ((p >> 3) & 1) * 32 + ((p >> 2) & 1) * 16 + (p >> 4) * 4 + (p & 3);

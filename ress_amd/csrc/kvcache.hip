@@ -425,7 +425,7 @@ struct Append {
   static int go(const AppendArgs& a, hipStream_t stream) {
     const long long kv = (long long)a.B * a.c.kv_heads * a.pages;
     const long long qg = a.q_out ? (long long)a.B * cdiv(a.Hq, QH) * cdiv(a.n, THREADS / (D / 16)) : 0;
-    RESS_REQUIRE(kv + qg < (1ll << 31), "ress_kv_append: the call needs more than 2^31 workgroups");
+    RESS_REQUIRE(launchable(kv + qg, THREADS), "ress_kv_append: the call needs 2^32 threads or more");
     hipLaunchKernelGGL((k_kv_append<DT, CODES, D>), dim3((unsigned)(kv + qg)), dim3(THREADS), 0, stream, a, (int)kv);
     RESS_LAUNCHED("k_kv_append");
     return 0;
@@ -438,7 +438,7 @@ struct Read {
                 hipStream_t stream) {
     const int pages = (n + KV_PAGE - 1) / KV_PAGE + 1;
     const long long g = (long long)B * c.kv_heads * pages;
-    RESS_REQUIRE(g < (1ll << 31), "ress_kv_read: the call needs more than 2^31 workgroups");
+    RESS_REQUIRE(launchable(g, THREADS), "ress_kv_read: the call needs 2^32 threads or more");
     hipLaunchKernelGGL((k_kv_read<DT, CODES, D>), dim3((unsigned)g), dim3(THREADS), 0, stream, c, slots, start, n,
                        pages, (uint16_t*)k, (uint16_t*)v);
     RESS_LAUNCHED("k_kv_read");
