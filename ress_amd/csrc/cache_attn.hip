@@ -823,7 +823,9 @@ struct Cut {
 Cut cut(const ress_kv_cache& c, int B, int Hq, int n, int most_tokens) {
   Cut k{};
   const long long rows = (long long)n * (Hq / c.kv_heads), heads = (long long)B * c.kv_heads;
-  const int pages = cdiv(most_tokens > 0 ? most_tokens : 1, KV_PAGE);
+  // no more than the largest table holds: a larger count, rounded up to pages, would pass 32 bits
+  constexpr int MOST = ((1 << 25) - 1) * KV_PAGE;
+  const int pages = cdiv(most_tokens > MOST ? MOST : most_tokens > 0 ? most_tokens : 1, KV_PAGE);
   long long slots;  // workgroups that run at once
   int least;        // pages a split has at least
   if (rows <= 32) {
