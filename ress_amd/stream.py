@@ -17,7 +17,6 @@ import torch
 
 from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable
 from ress_amd.qkv import _fusable, fused_qk_norm_rope, rope_base
-from ress_amd.wiring import global_blocks
 
 POSITIONS = 1024  # of the rotation tables: patches of a frame's side, and the special tokens' place
 
@@ -62,7 +61,7 @@ class FrameStream:
         if int(max_frames) < 1 or int(batch) < 1:
             raise ValueError(f"max_frames and batch must be at least 1, got {max_frames} and {batch}")
         self.aggregator = model.aggregator
-        self.blocks = global_blocks(model)
+        self.blocks = self.aggregator.global_blocks  # all of them: only some may be wired for the sparse path
         self.max_frames, self.batch, self.codes = int(max_frames), int(batch), codes
         self.frames = 0       # held now
         self.grid = None      # patch grid of the frames

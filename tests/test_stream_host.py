@@ -1,0 +1,73 @@
+"""FrameStream's steps without a GPU: a 32-bit model over plain caches in the place of the 8-bit ones."""
+
+import pytest
+import torch
+
+from ress_amd import FrameStream, stream
+from ress_amd.aggregator import build_vggt_aggregator
+from ress_amd.wiring import wire_ress_attention
+
+
+class PlainCache:
+    """Keys and values as they come, rotated by the table; softmax over all of them."""
+
+    def __init__(self, n_pages, heads, head_dim, **kw):
+        self.k = self.v = None
+
+    @staticmethod
+    def _turn(x, pos, rope):
+        out = []
+        for a, part in enumerate(x.split(x.shape[-1] // rope.axes, -1)):
+            cs = rope.table[pos[..., a]][:, None]
+            x1, x2 = part.chunk(2, -1)
+            out += [x1 * cs[..., 0, :] - x2 * cs[..., 1, :], x2 * cs[..., 0, :] + x1 * cs[..., 1, :]]
+        return torch.cat(out, -1)
+
+    def append(self, k, v, pos=None, rope=None, q=None):
+        if rope is not None:
+            k, q = self._turn(k, pos, rope), self._turn(q, pos, rope)
+        self.k = k if self.k is None else torch.cat([self.k, k], 2)
+        self.v = v if self.v is None else torch.cat([self.v, v], 2)
+        return q
+
+    def attend(self, q, out):
+        out.copy_(torch.softmax(q @ self.k.transpose(2, 3) / q.shape[-1] ** 0.5, -1) @ self.v)
+
+    def snapshot(self):
+        return self.k, self.v
+
+    def restore(self, snap):
+        self.k, self.v = snap
+
+    def release(self, slot):
+        self.k = self.v = None
+
+
+@pytest.fixture
+def model(monkeypatch):
+    monkeypatch.setattr(stream, "PagedKVCache", PlainCache)
+    return build_vggt_aggregator(depth=3, dim=64, num_heads=1, device="cpu", dtype=torch.float32, wire=False)
+
+
+def _frames(n, h=28, w=42):
+    return torch.rand(1, n, 3, h, w, generator=torch.Generator().manual_seed(n))
+
+
+def _dense(model, frames):
+    with torch.no_grad():
+        return model.aggregator(frames)
+
+
+def test_all_frames_in_one_step(model):
+    """fp32 sums in another order, of a few hundred terms of a residual stream of size one."""
+    x = _frames(3)
+    assert (FrameStream(model, 3).step(x) - _dense(model, x)).abs().max() <= 1e-4
+
+
+@pytest.mark.parametrize("wired", [[1], [0, 2], [2, 1, 0], []])
+def test_layers_wired_in_part(model, wired):
+    """The stream runs every layer, in the model's order, whichever of them have been wired for the sparse path."""
+    x = _frames(2)
+    want = _dense(model, x)
+    wire_ress_attention(model, [model.aggregator.global_blocks[i] for i in wired])
+    assert (FrameStream(model, 2).step(x) - want).abs().max() <= 1e-4
