@@ -53,13 +53,40 @@ def cached_attention(attn, x, pos, cache, tables):
     return attn.proj_drop(attn.proj(o.reshape(B, T, C)))
 
 
+_PARTS = (("", ("tokens", "frame_blocks", "global_blocks")), ("block's", ("norm1", "attn", "ls1", "norm2", "mlp", "ls2")),
+          ("block's attention", ("qkv", "q_norm", "k_norm", "proj", "proj_drop", "num_heads")))
+
+
+def _check_parts(model):
+    """A step is put together from the aggregator's parts, so all have to be there."""
+    agg = getattr(model, "aggregator", None)
+    if agg is None:
+        raise TypeError(f"a FrameStream needs a model with an aggregator, {type(model).__name__} has none")
+
+    def need(obj, which):
+        whose, names = _PARTS[which]
+        missing = [n for n in names if not hasattr(obj, n)]
+        if missing:
+            raise TypeError(f"a FrameStream runs models built like ress_amd.aggregator: the {type(agg).__name__}'s {whose} "
+                            f"{', '.join(missing)} {'is' if len(missing) == 1 else 'are'} missing")
+
+    need(agg, 0)
+    for block in agg.global_blocks:
+        need(block, 1)
+        need(block.attn, 2)
+    if len(agg.frame_blocks) != len(agg.global_blocks):
+        raise TypeError(f"the aggregator has {len(agg.frame_blocks)} frame blocks and {len(agg.global_blocks)} global ones: "
+                        f"a step runs them in pairs")
+
+
 class FrameStream:
-    """Streams frames through a VGGT-style model (an `aggregator` with frame and global blocks, in bf16 or fp16
-    on the GPU). Up to max_frames frames of one size for each of `batch` scenes; codes: "int8" or "fp8" (e4m3)."""
+    """Streams frames through a VGGT-style model (built like ress_amd.aggregator's, in bf16 or fp16 on the GPU; another is
+    refused). Up to max_frames frames of one size for each of `batch` scenes; codes: "int8" or "fp8" (e4m3)."""
 
     def __init__(self, model, max_frames, batch=1, codes="int8"):
         if int(max_frames) < 1 or int(batch) < 1:
             raise ValueError(f"max_frames and batch must be at least 1, got {max_frames} and {batch}")
+        _check_parts(model)
         self.aggregator = model.aggregator
         self.blocks = self.aggregator.global_blocks  # all of them: only some may be wired for the sparse path
         self.max_frames, self.batch, self.codes = int(max_frames), int(batch), codes

@@ -71,3 +71,29 @@ def test_layers_wired_in_part(model, wired):
     want = _dense(model, x)
     wire_ress_attention(model, [model.aggregator.global_blocks[i] for i in wired])
     assert (FrameStream(model, 2).step(x) - want).abs().max() <= 1e-4
+
+
+def test_another_model_is_refused_when_the_stream_is_made(model):
+    agg = model.aggregator
+    for owner, name in ((model, "aggregator"), (agg, "frame_blocks"), (agg, "global_blocks"), (agg.global_blocks[1], "ls2"),
+                        (agg.global_blocks[2], "norm1"), (agg.global_blocks[0].attn, "q_norm")):
+        part = getattr(owner, name)
+        delattr(owner, name)
+        with pytest.raises(TypeError, match=name):
+            FrameStream(model, 2)
+        setattr(owner, name, part)
+    last = agg.frame_blocks[2]
+    del agg.frame_blocks[2]
+    with pytest.raises(TypeError, match="2 frame blocks and 3 global"):
+        FrameStream(model, 2)
+    agg.frame_blocks.append(last)
+
+    class Other(torch.nn.Module):  # an aggregator with blocks of its own and a forward over all frames at once
+        def __init__(self):
+            super().__init__()
+            self.aggregator = torch.nn.Module()
+            self.aggregator.frame_blocks, self.aggregator.global_blocks = agg.frame_blocks, agg.global_blocks
+
+    with pytest.raises(TypeError, match="tokens"):
+        FrameStream(Other(), 2)
+    FrameStream(model, 2).step(_frames(2))
