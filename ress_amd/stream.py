@@ -154,6 +154,7 @@ class FrameStream:
         for c, s in zip(self.caches, snaps):
             c.restore(s)
         self.frames, self._whole = frames, True
+        self.grid = self.grid if frames else None
 
     def reset(self):
         """Forgets every frame; the caches stay allocated, for frames of this size."""

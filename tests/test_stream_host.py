@@ -97,3 +97,21 @@ def test_another_model_is_refused_when_the_stream_is_made(model):
     with pytest.raises(TypeError, match="tokens"):
         FrameStream(Other(), 2)
     FrameStream(model, 2).step(_frames(2))
+
+
+def test_no_frames_have_no_grid(model):
+    """Taken back to no frame, a stream takes frames of another shape as a fresh one does (6 patches both)."""
+    s = FrameStream(model, 3)
+    s.step(_frames(1))
+    s.reset()
+    snap = s.snapshot()
+    s.step(_frames(1))
+    s.restore(snap)
+    assert s.frames == 0
+    x = _frames(2, 42, 28)
+    assert (s.step(x) - _dense(model, x)).abs().max() <= 1e-4
+    snap = s.snapshot()
+    s.step(x[:, :1])
+    s.restore(snap)
+    with pytest.raises(ValueError, match="patch grid"):
+        s.step(_frames(1))
