@@ -114,6 +114,10 @@ class FrameStream:
             raise RuntimeError("a step counts its frames on the host: not inside a graph capture")
         if not self._whole:
             raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
+        for block in self.blocks:
+            if any(m._forward_hooks or m._forward_pre_hooks for m in (block, block.attn)):
+                raise RuntimeError("a step calls a global block's parts, so hooks on it or on its attention module would not run: "
+                                   "put them on the parts")
         if self.frames + images.shape[1] > self.max_frames:
             raise ValueError(f"{self.frames} frames are held and {images.shape[1]} more do not fit max_frames={self.max_frames}")
         agg = self.aggregator

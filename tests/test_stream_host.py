@@ -115,3 +115,21 @@ def test_no_frames_have_no_grid(model):
     s.restore(snap)
     with pytest.raises(ValueError, match="patch grid"):
         s.step(_frames(1))
+
+
+@pytest.mark.parametrize("kind", ["register_forward_hook", "register_forward_pre_hook"])
+@pytest.mark.parametrize("where", ["block", "attn"])
+def test_hooks_that_would_not_run_are_refused(model, kind, where):
+    """A step calls a global block's parts, so hooks on it or on its attention module would be left out."""
+    s = FrameStream(model, 3)
+    block = model.aggregator.global_blocks[1]
+    handle = getattr(block if where == "block" else block.attn, kind)(lambda *a: None)
+    with pytest.raises(RuntimeError, match="hooks"):
+        s.step(_frames(1))
+    assert s.frames == 0
+    handle.remove()
+    seen = []
+    for m in (block.mlp, block.attn.proj, model.aggregator.frame_blocks[1]):  # these are called
+        m.register_forward_hook(lambda *a: seen.append(1))
+    s.step(_frames(1))
+    assert len(seen) == 3 and s.frames == 1
