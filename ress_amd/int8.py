@@ -112,11 +112,12 @@ class Int8Linear(nn.Module):
         super()._apply(fn, recurse)
         for n, t in kept.items():
             setattr(self, n, t.to(self.codes.device))
+        self.dtype = fn(torch.empty(0, dtype=self.dtype, device=self.codes.device)).dtype
         return self
 
     @property
     def weight(self):
-        """The weights that the codes stand for, in the original layer's type."""
+        """The weights that the codes stand for, in the type that the layer's own would have now."""
         return (self.codes.float() * self.scale[:, None]).to(self.dtype)
 
     def forward(self, x, act=None):

@@ -1,0 +1,24 @@
+"""Int8Linear and quantize_linears as modules of a model (no GPU)."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+from ress_amd import int8
+from ress_amd.int8 import Int8Linear, quantize_linears
+
+
+@pytest.mark.parametrize("cast", [nn.Module.half, nn.Module.bfloat16, nn.Module.float, nn.Module.double])
+def test_weight_has_the_layers_present_type(cast):
+    torch.manual_seed(0)
+    layer = nn.Linear(32, 8).to(torch.bfloat16)
+    q = Int8Linear(layer)
+    assert q.weight.dtype == torch.bfloat16
+    cast(layer)
+    codes, scale, bias = q.codes.clone(), q.scale.clone(), q.bias.clone()
+    assert cast(q) is q and q.weight.dtype == layer.weight.dtype
+    assert torch.equal(q.codes, codes) and torch.equal(q.scale, scale) and torch.equal(q.bias, bias)
+    assert q.scale.dtype == q.bias.dtype == torch.float32
+    assert cast(nn.Sequential(q))[0].weight.dtype == layer.weight.dtype
+    q.to("cpu")  # a move is no cast
+    assert q.weight.dtype == layer.weight.dtype
