@@ -129,13 +129,19 @@ class Int8Linear(nn.Module):
 
 def quantize_linears(model, keep=lambda name, linear: False):
     """Replaces every nn.Linear of the model by an Int8Linear, in place, but for those whose in_features are
-    not a multiple of 16 and those that keep(name, linear) names. Returns the names replaced."""
+    not a multiple of 16 and those that keep(name, linear) names (a layer with several names: by any of them).
+    Returns the names replaced."""
+    places = {}  # linear -> (module, child, full name) of each of its places
+    for name, module in model.named_modules():
+        for child, linear in module._modules.items():
+            if type(linear) is nn.Linear and linear.in_features % 16 == 0 and linear.in_features <= MOST_FEATURES:
+                places.setdefault(linear, []).append((module, child, f"{name}.{child}" if name else child))
     done = []
-    for name, module in list(model.named_modules()):
-        for child, linear in list(module.named_children()):
-            full = f"{name}.{child}" if name else child
-            if (type(linear) is nn.Linear and linear.in_features % 16 == 0 and linear.in_features <= MOST_FEATURES
-                    and not keep(full, linear)):
-                setattr(module, child, Int8Linear(linear))
-                done.append(full)
+    for linear, at in places.items():
+        if any(keep(full, linear) for _, _, full in at):
+            continue
+        new = Int8Linear(linear)
+        for module, child, full in at:
+            setattr(module, child, new)
+            done.append(full)
     return done

@@ -22,3 +22,22 @@ def test_weight_has_the_layers_present_type(cast):
     assert cast(nn.Sequential(q))[0].weight.dtype == layer.weight.dtype
     q.to("cpu")  # a move is no cast
     assert q.weight.dtype == layer.weight.dtype
+
+
+class Shared(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.a = nn.Linear(16, 16)
+        self.b = self.a
+        self.c = nn.Sequential(self.a, nn.Linear(16, 4))
+
+
+def test_a_layer_under_several_names():
+    """Replaced under each of them, by one layer; keep names it by any."""
+    m = Shared()
+    names = quantize_linears(m)
+    assert sorted(names) == ["a", "b", "c.0", "c.1"]
+    assert type(m.a) is Int8Linear and m.b is m.a and m.c[0] is m.a and m.c[1] is not m.a
+    m = Shared()
+    names = quantize_linears(m, keep=lambda name, linear: name == "b")
+    assert sorted(names) == ["c.1"] and type(m.a) is nn.Linear and m.b is m.a and m.c[0] is m.a
