@@ -130,16 +130,18 @@ class Int8Linear(nn.Module):
 def quantize_linears(model, keep=lambda name, linear: False):
     """Replaces every nn.Linear of the model by an Int8Linear, in place, but for those whose in_features are
     not a multiple of 16 and those that keep(name, linear) names (a layer with several names: by any of them).
-    Returns the names replaced."""
+    Returns the names replaced. A weight that is not finite is refused before any layer is replaced."""
     places = {}  # linear -> (module, child, full name) of each of its places
     for name, module in model.named_modules():
         for child, linear in module._modules.items():
             if type(linear) is nn.Linear and linear.in_features % 16 == 0 and linear.in_features <= MOST_FEATURES:
                 places.setdefault(linear, []).append((module, child, f"{name}.{child}" if name else child))
+    places = {linear: at for linear, at in places.items() if not any(keep(full, linear) for _, _, full in at)}
+    for linear, at in places.items():
+        if not torch.isfinite(linear.weight).all():
+            raise ValueError(f"{at[0][2]}: weight has values that are not finite")
     done = []
     for linear, at in places.items():
-        if any(keep(full, linear) for _, _, full in at):
-            continue
         new = Int8Linear(linear)
         for module, child, full in at:
             setattr(module, child, new)

@@ -41,3 +41,13 @@ def test_a_layer_under_several_names():
     m = Shared()
     names = quantize_linears(m, keep=lambda name, linear: name == "b")
     assert sorted(names) == ["c.1"] and type(m.a) is nn.Linear and m.b is m.a and m.c[0] is m.a
+
+
+def test_a_model_that_cannot_be_quantised_stays_whole():
+    m = nn.Sequential(nn.Linear(16, 16), nn.Linear(16, 4), nn.Linear(16, 8))
+    with torch.no_grad():
+        m[1].weight[2, 3] = float("inf")
+    with pytest.raises(ValueError, match="1: weight has values that are not finite"):
+        quantize_linears(m)
+    assert all(type(x) is nn.Linear for x in m)
+    assert quantize_linears(m, keep=lambda name, linear: name == "1") == ["0", "2"]
