@@ -105,6 +105,11 @@ class Int8Linear(nn.Module):
         self.register_buffer("codes", codes)
         self.register_buffer("scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float().contiguous())
+        # the layer's mode and forward hooks go with it; the same dicts, so that the hooks' handles still remove them
+        self.training = linear.training
+        for name in ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",
+                     "_forward_pre_hooks_with_kwargs"):
+            setattr(self, name, getattr(linear, name))
 
     def _apply(self, fn, recurse=True):
         # a cast of the model to 16 bits must not round the scales and the bias, which are fp32

@@ -51,3 +51,17 @@ def test_a_model_that_cannot_be_quantised_stays_whole():
         quantize_linears(m)
     assert all(type(x) is nn.Linear for x in m)
     assert quantize_linears(m, keep=lambda name, linear: name == "1") == ["0", "2"]
+
+
+def test_what_a_replaced_layer_keeps():
+    """Its mode and its hooks."""
+    m = nn.Sequential(nn.Linear(16, 16), nn.Linear(16, 4)).eval()
+    calls = []
+    m[0].register_forward_pre_hook(lambda mod, args: calls.append(type(mod)))
+    m[0].register_forward_hook(lambda mod, args, out, **kw: calls.append(type(mod)))
+    m[0].register_forward_pre_hook(lambda mod, args, kwargs: calls.append(kwargs), with_kwargs=True)
+    quantize_linears(m)
+    assert not m[0].training and not m[1].training
+    m[0].forward = lambda x, act=None: x
+    m[0](torch.zeros(2, 16), act="gelu")
+    assert calls == [Int8Linear, {"act": "gelu"}, Int8Linear]
