@@ -25,7 +25,7 @@ def _rows(x, name):
     if not torch.is_tensor(x) or not x.is_cuda:
         raise RuntimeError(f"{name} must be a device tensor (the 8-bit product runs only on the GPU)")
     if x.dtype not in DTYPES:
-        raise TypeError(f"{name} must be bfloat16 or float16, got {x.dtype}")
+        raise TypeError(f"{name} must be bfloat16 or float16, got {x.dtype} (cast the model, or run it under autocast)")
     if x.dim() < 1 or x.shape[-1] % 16 or not 0 < x.shape[-1] <= MOST_FEATURES:
         raise ValueError(f"{name} must have a last dim that is a multiple of 16 up to {MOST_FEATURES}, got {tuple(x.shape)}")
     if x.requires_grad and torch.is_grad_enabled():
@@ -95,7 +95,8 @@ def _workspace(M, K, N):
 
 
 class Int8Linear(nn.Module):
-    """An nn.Linear's place-holder with 8-bit weights (buffers, not parameters)."""
+    """An nn.Linear's place-holder with 8-bit weights (buffers, not parameters), for 16-bit activations; under autocast
+    they are cast to its type, as the layer's would be."""
 
     def __init__(self, linear):
         super().__init__()
@@ -126,6 +127,8 @@ class Int8Linear(nn.Module):
         return (self.codes.float() * self.scale[:, None]).to(self.dtype)
 
     def forward(self, x, act=None):
+        if torch.is_autocast_enabled(x.device.type) and x.is_floating_point() and x.dtype is not torch.float64:
+            x = x.to(torch.get_autocast_dtype(x.device.type))
         return int8_linear(x, self.codes, self.scale, self.bias, act)
 
     def extra_repr(self):
@@ -135,11 +138,12 @@ class Int8Linear(nn.Module):
 def quantize_linears(model, keep=lambda name, linear: False):
     """Replaces every nn.Linear of the model by an Int8Linear, in place, but for those whose in_features are
     not a multiple of 16 and those that keep(name, linear) names (a layer with several names: by any of them).
+    The layers then take 16-bit activations: a 32-bit model is to be cast (before or after) or run under autocast.
     Returns the names replaced. A weight that is not finite is refused before any layer is replaced."""
     places = {}  # linear -> (module, child, full name) of each of its places
     for name, module in model.named_modules():
         for child, linear in module._modules.items():
-            if type(linear) is nn.Linear and linear.in_features % 16 == 0 and linear.in_features <= MOST_FEATURES:
+            if type(linear) is nn.Linear and linear.in_features % 16 == 0 and 0 < linear.in_features <= MOST_FEATURES:
                 places.setdefault(linear, []).append((module, child, f"{name}.{child}" if name else child))
     places = {linear: at for linear, at in places.items() if not any(keep(full, linear) for _, _, full in at)}
     for linear, at in places.items():

@@ -65,3 +65,23 @@ def test_what_a_replaced_layer_keeps():
     m[0].forward = lambda x, act=None: x
     m[0](torch.zeros(2, 16), act="gelu")
     assert calls == [Int8Linear, {"act": "gelu"}, Int8Linear]
+
+
+@pytest.mark.parametrize("to", [torch.bfloat16, torch.float16])
+def test_autocast(monkeypatch, to):
+    """As torch's own linear layer does: inputs of up to 32 bits are cast to autocast's type."""
+    got = []
+    monkeypatch.setattr(int8, "int8_linear", lambda x, *a: got.append(x))
+    q = Int8Linear(nn.Linear(16, 4))
+    x = torch.rand(3, 16)
+    with torch.autocast("cpu", dtype=to):
+        for dtype in (torch.float32, torch.bfloat16, torch.float16):
+            q(x.to(dtype))
+            assert got[-1].dtype == to and torch.equal(got[-1], x.to(dtype).to(to))
+        q(x.double())
+        assert got[-1].dtype == torch.float64
+        with torch.autocast("cpu", enabled=False):
+            q(x)
+            assert got[-1] is x
+    q(x)
+    assert got[-1] is x
