@@ -74,6 +74,8 @@ def int8_linear(x, w_codes, w_scale, bias=None, act=None):
     for name, t in (("w_scale", w_scale), ("bias", bias)):
         if t is not None and (t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != N or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous float32 ({N},), got {tuple(t.shape)} {t.dtype}")
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires grad: the 8-bit product has no backward pass (use torch.no_grad())")
     if w_codes.device != dev or w_scale.device != dev or (bias is not None and bias.device != dev):
         raise ValueError(f"the weights are not on {dev}")
     if act not in ACTS:

@@ -85,3 +85,23 @@ def test_autocast(monkeypatch, to):
             assert got[-1] is x
     q(x)
     assert got[-1] is x
+
+
+@pytest.mark.parametrize("which", ["scale", "bias"])
+def test_weights_that_require_grad_are_refused(monkeypatch, which):
+    """Like x that does: there is no backward pass, and the result would be cut off from them without a word."""
+    calls = []
+    monkeypatch.setattr(int8, "_rows", lambda x, name: x)
+    monkeypatch.setattr(int8, "_workspace", lambda *a: 0)
+    monkeypatch.setattr(int8._lib, "ptr", lambda t: t)
+    monkeypatch.setattr(int8._lib, "call_on", lambda *a: calls.append(a))
+    x, codes = torch.zeros(3, 16, dtype=torch.bfloat16), torch.zeros(4, 16, dtype=torch.int8)
+    w = dict(scale=torch.ones(4), bias=torch.zeros(4))
+    w[which].requires_grad_()
+    with pytest.raises(RuntimeError, match=f"{which} requires grad"):
+        int8.int8_linear(x, codes, w["scale"], w["bias"])
+    assert not calls
+    with torch.no_grad():
+        int8.int8_linear(x, codes, w["scale"], w["bias"])
+    int8.int8_linear(x, codes, w["scale"].detach(), w["bias"].detach())
+    assert len(calls) == 2
