@@ -33,7 +33,7 @@ def bake_and_attach_M(model):
     """Attach each layer's (nh, hd, hd) M as `block.attn.M` (reference projected.py:235-244)."""
     M = bake_M(model)
     for i, block in enumerate(global_blocks(model)):
-        block.attn.M = M[i].to(next(block.attn.parameters()).device)
+        block.attn.M = M[i].to(block.attn.proj.weight.device)
     return M
 
 

@@ -105,3 +105,17 @@ def test_weights_that_require_grad_are_refused(monkeypatch, which):
         int8.int8_linear(x, codes, w["scale"], w["bias"])
     int8.int8_linear(x, codes, w["scale"].detach(), w["bias"].detach())
     assert len(calls) == 2
+
+
+def test_drift_matrices_of_8_bit_layers():
+    """An attention whose projections are all 8-bit and whose norms have no weights has no parameters."""
+    from ress_amd.aggregator import build_vggt_aggregator
+    from ress_amd.projected import bake_and_attach_M
+    model = build_vggt_aggregator(depth=2, dim=64, num_heads=1, device="cpu", dtype=torch.float32, wire=False)
+    for block in model.aggregator.global_blocks:
+        block.attn.q_norm = block.attn.k_norm = nn.Identity()
+    quantize_linears(model.aggregator.global_blocks)
+    M = bake_and_attach_M(model)
+    for m, block in zip(M, model.aggregator.global_blocks):
+        w = block.attn.proj.weight
+        assert torch.equal(block.attn.M, m) and torch.equal(m[0], w.T @ w)
