@@ -356,6 +356,8 @@ int ress_quantize_rows(const void* x, long long stride, int dtype, int M, int K,
  * ress_int8_linear_workspace_size bytes, 16-byte aligned (may be 0 bytes). No counterpart in the reference, whose
  * linear layers are torch's. */
 long long ress_int8_linear_workspace_size(int M, int K, int N);
+/* The tile that a product is cut into, tokens << 16 | channels; 0 where it needs none (a few tokens). */
+int ress_int8_linear_tile(int M, int K, int N);
 int ress_int8_linear(const void* x, long long stride, int dtype, int M, int K, int N, const void* w,
                      const float* w_scale, const float* bias, int act, void* out, long long out_stride,
                      void* workspace, long long workspace_bytes, hipStream_t stream);

@@ -74,6 +74,8 @@ def lib():
         L.ress_meansim_workspace_size.argtypes = [ctypes.c_int] * 4
         L.ress_int8_linear_workspace_size.restype = ctypes.c_longlong
         L.ress_int8_linear_workspace_size.argtypes = [ctypes.c_int] * 3
+        L.ress_int8_linear_tile.restype = ctypes.c_int
+        L.ress_int8_linear_tile.argtypes = [ctypes.c_int] * 3
         L.ress_kv_attend_workspace_size.restype = ctypes.c_longlong
         L.ress_kv_attend_workspace_size.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
         L.ress_noalloc_scratch_bytes.restype = ctypes.c_longlong
@@ -133,5 +135,5 @@ def exported_symbols():
     return list(_SIGS) + ["ress_last_error", "ress_abi_version", "ress_qattn_workspace_size",
                           "ress_attn_sched_bytes", "ress_restore_swap_workspace_size", "ress_meansim_workspace_size",
                           "ress_noalloc_scratch_bytes", "ress_kv_attend_workspace_size",
-                          "ress_int8_linear_workspace_size",
+                          "ress_int8_linear_workspace_size", "ress_int8_linear_tile",
                           "ress_noalloc_status_address"]

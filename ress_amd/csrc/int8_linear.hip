@@ -467,6 +467,12 @@ RESS_API long long ress_int8_linear_workspace_size(int M, int K, int N) {
   return few(M, K) ? 0 : code_bytes(M, K) + 4ll * M;
 }
 
+RESS_API int ress_int8_linear_tile(int M, int K, int N) {
+  if (M <= 0 || K <= 0 || N <= 0 || few(M, K)) return 0;
+  const auto& t = tiles[pick(M, N, (int)(padded(K) / 128))];
+  return t.bm << 16 | t.bn;
+}
+
 RESS_API int ress_int8_linear(const void* x, long long stride, int dtype, int M, int K, int N, const void* w,
                               const float* w_scale, const float* bias, int act, void* out, long long out_stride,
                               void* workspace, long long workspace_bytes, hipStream_t stream) {
