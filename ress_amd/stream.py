@@ -103,6 +103,10 @@ class FrameStream:
                                     max_len=self.max_frames * P, dtype=x.dtype, codes=self.codes, device=x.device)
                        for b in self.blocks]
 
+    def _check_whole(self):
+        if not self._whole:
+            raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
+
     @torch.no_grad()
     def step(self, images):
         """Tokens (B, s * P, dim) of s new frames, images (B, s, 3, H, W) or (B, 3, H, W) in [0, 1]."""
@@ -112,8 +116,7 @@ class FrameStream:
             raise ValueError(f"images must be ({self.batch}, s, 3, H, W), got {tuple(images.shape)}")
         if images.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a step counts its frames on the host: not inside a graph capture")
-        if not self._whole:
-            raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
+        self._check_whole()
         for block in self.blocks:
             if any(m._forward_hooks or m._forward_pre_hooks for m in (block, block.attn)):
                 raise RuntimeError("a step calls a global block's parts, so hooks on it or on its attention module would not run: "
@@ -149,6 +152,7 @@ class FrameStream:
         """For restore: takes back the frames of later steps (a frame that is not kept as a key frame)."""
         if self.caches is None:
             raise RuntimeError("no frame has been streamed yet")
+        self._check_whole()
         return self.frames, [c.snapshot() for c in self.caches]
 
     def restore(self, snapshot):

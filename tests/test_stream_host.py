@@ -133,3 +133,24 @@ def test_hooks_that_would_not_run_are_refused(model, kind, where):
         m.register_forward_hook(lambda *a: seen.append(1))
     s.step(_frames(1))
     assert len(seen) == 3 and s.frames == 1
+
+
+def test_a_broken_step_is_no_snapshot(model):
+    """After a step that ended in an error some layers hold its frame: nothing to come back to."""
+    s = FrameStream(model, 4)
+    s.step(_frames(1))
+    good = s.snapshot()
+    want = s.step(_frames(2))
+    s.restore(good)
+    mlp = model.aggregator.global_blocks[1].mlp
+    handle = mlp.register_forward_pre_hook(lambda *a: 1 / 0)
+    with pytest.raises(ZeroDivisionError):
+        s.step(_frames(2))
+    handle.remove()
+    with pytest.raises(RuntimeError, match="ended in an error"):
+        s.snapshot()
+    with pytest.raises(RuntimeError, match="ended in an error"):
+        s.step(_frames(2))
+    s.restore(good)
+    assert torch.equal(s.step(_frames(2)), want)
+    s.snapshot()
