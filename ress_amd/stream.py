@@ -15,7 +15,7 @@ The reference runs over all frames at once and has no counterpart.
 
 import torch
 
-from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable
+from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable, _capturing
 from ress_amd.qkv import _fusable, fused_qk_norm_rope, rope_base
 
 POSITIONS = 1024  # of the rotation tables: patches of a frame's side, and the special tokens' place
@@ -103,6 +103,11 @@ class FrameStream:
                                     max_len=self.max_frames * P, dtype=x.dtype, codes=self.codes, device=x.device)
                        for b in self.blocks]
 
+    @staticmethod
+    def _not_capturing():
+        if _capturing():
+            raise RuntimeError("a stream counts its frames on the host: not inside a graph capture")
+
     def _check_whole(self):
         if not self._whole:
             raise RuntimeError("a step ended in an error and left its frames in some layers: reset() or restore()")
@@ -114,8 +119,7 @@ class FrameStream:
             images = images[:, None]
         if images.dim() != 5 or images.shape[0] != self.batch or images.shape[1] < 1:
             raise ValueError(f"images must be ({self.batch}, s, 3, H, W), got {tuple(images.shape)}")
-        if images.is_cuda and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a step counts its frames on the host: not inside a graph capture")
+        self._not_capturing()
         self._check_whole()
         for block in self.blocks:
             if any(m._forward_hooks or m._forward_pre_hooks for m in (block, block.attn)):
@@ -150,12 +154,14 @@ class FrameStream:
 
     def snapshot(self):
         """For restore: takes back the frames of later steps (a frame that is not kept as a key frame)."""
+        self._not_capturing()
         if self.caches is None:
             raise RuntimeError("no frame has been streamed yet")
         self._check_whole()
         return self.frames, [c.snapshot() for c in self.caches]
 
     def restore(self, snapshot):
+        self._not_capturing()
         frames, snaps = snapshot
         if self.caches is None or len(snaps) != len(self.caches):
             raise ValueError("the snapshot belongs to another stream")
@@ -166,6 +172,7 @@ class FrameStream:
 
     def reset(self):
         """Forgets every frame; the caches stay allocated, for frames of this size."""
+        self._not_capturing()
         for c in self.caches or ():
             for slot in range(self.batch):
                 c.release(slot)

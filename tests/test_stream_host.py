@@ -154,3 +154,19 @@ def test_a_broken_step_is_no_snapshot(model):
     s.restore(good)
     assert torch.equal(s.step(_frames(2)), want)
     s.snapshot()
+
+
+def test_a_capture_is_refused(monkeypatch, model):
+    """Frames are counted on the host, when a call is made and not when a graph runs it."""
+    s = FrameStream(model, 4)
+    s.step(_frames(1))
+    snap = s.snapshot()
+    s.step(_frames(2))
+    with monkeypatch.context() as m:
+        m.setattr(stream, "_capturing", lambda: True, raising=False)
+        for call in (lambda: s.step(_frames(1)), s.snapshot, lambda: s.restore(snap), s.reset):
+            with pytest.raises(RuntimeError, match="not inside a graph capture"):
+                call()
+    assert s.frames == 3 and s.caches[0].k.shape[2] == 3 * 11
+    s.restore(snap)
+    assert s.frames == 1
