@@ -82,7 +82,7 @@ struct Head {
   __device__ __forceinline__ Head(const AttendArgs& a, const int* __restrict__ lens, const int* __restrict__ slots,
                                   const int* __restrict__ new_lens, int b, int h_) : h(h_) {
     slot = slots ? slots[b] : b;
-    len = lens[slot];
+    len = held_tokens(lens[slot], a.c.max_pages);
     nv = new_lens ? min(max(new_lens[b], 0), a.n) : a.n;
     const long long one = (long long)KV_PAGE * D;
     kc = reinterpret_cast<const uint8_t*>(a.c.k_codes) + h * one;
@@ -740,7 +740,7 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(min(row, all_rows - 1) / per), r = (int)(row - (long long)bh * per);
   const int b = bh / H, h = bh % H, tok = r / a.G;
   const int nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
-  const int len = a.c.lens[a.slots ? a.slots[b] : b];
+  const int len = held_tokens(a.c.lens[a.slots ? a.slots[b] : b], a.c.max_pages);
   const int ns = min(a.splits, cdiv(cdiv(len, KV_PAGE), a.per));
   const bool live = row < all_rows && tok < nv && ns > 1;  // one part is written by its workgroup
   const float* ml = a.part_ml + 2 * (live ? row : 0);

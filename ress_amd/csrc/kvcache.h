@@ -24,6 +24,10 @@ constexpr int KV_ST_FULL = 1, KV_ST_POS = 2, KV_ST_PAGE = 4, KV_ST_NONFINITE = 8
 // Checks a cache handle on the host (kvcache.hip): 0, or -1 with the message set.
 int ress_kv_check(const ress_kv_cache* c, int B, const char* who);
 
+// Tokens of a slot, as the kernels take them: between none and what its pages (or, for a reader, a table) have room for,
+// so that lengths changed from outside, as by a snapshot whose recording never ran, reach no memory but the slot's.
+__device__ __forceinline__ int held_tokens(int len, int pages) { return min(max(len, 0), pages * KV_PAGE); }
+
 // A launch counts its threads in 32 bits.
 inline bool launchable(long long workgroups, long long threads) { return workgroups * threads < (1ll << 32); }
 

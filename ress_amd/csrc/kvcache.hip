@@ -145,7 +145,8 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
   const int part = blockIdx.x % a.pages, h = blockIdx.x / a.pages % H, b = blockIdx.x / a.pages / H;
   const int slot = a.slots ? a.slots[b] : b;
 
-  const int len = a.c.lens[slot], cap = a.c.held[slot] * KV_PAGE, fresh = new_tokens(a.new_lens, b, a.n);
+  const int held = a.c.held[slot], cap = held * KV_PAGE, fresh = new_tokens(a.new_lens, b, a.n);
+  const int len = held_tokens(a.c.lens[slot], held);
   const long long tail = ((long long)slot * H + h) * KV_PAGE * D;
   uint16_t* tail_k = reinterpret_cast<uint16_t*>(a.c.tail_k) + tail;
   uint16_t* tail_v = reinterpret_cast<uint16_t*>(a.c.tail_v) + tail;
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
   const int t = threadIdx.x, H = c.kv_heads;
   const int part = blockIdx.x % pages, h = blockIdx.x / pages % H, b = blockIdx.x / pages / H;
   const int slot = slots ? slots[b] : b;
-  const int len = c.lens[slot];
+  const int len = held_tokens(c.lens[slot], c.max_pages);
   const long long s0 = start ? start[b] : (long long)len - n;
   const long long first = (s0 >= 0 ? s0 : s0 - (KV_PAGE - 1)) / KV_PAGE * KV_PAGE;  // of the window's first page
   const long long lo = first + (long long)part * KV_PAGE;
