@@ -44,7 +44,7 @@ def quantize_tokens(x):
     scale NaN and codes 0."""
     rows = _rows(x, "x")
     codes = torch.empty(rows.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(len(rows), device=x.device)
+    scale = torch.empty(len(rows), dtype=torch.float32, device=x.device)
     _lib.call_on(x.device, "ress_quantize_rows", _lib.ptr(rows), rows.stride(0), DTYPES[x.dtype], len(rows),
                  rows.shape[1], _lib.ptr(codes), rows.shape[1], _lib.ptr(scale))
     return codes.reshape(x.shape), scale.reshape(x.shape[:-1])

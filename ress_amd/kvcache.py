@@ -140,8 +140,8 @@ class PagedKVCache:
         code_t = torch.int8 if codes == "int8" else torch.float8_e4m3fn
         self.k_codes = torch.zeros(P, H, PAGE, D, dtype=torch.int8, device=dev).view(code_t)
         self.v_codes = torch.zeros(P, H, D, PAGE, dtype=torch.int8, device=dev).view(code_t)
-        self.k_scale = torch.zeros(P, H, device=dev)
-        self.v_scale = torch.zeros(P, H, device=dev)
+        self.k_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
+        self.v_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
         # what an append overwrites lies in one buffer, so that a snapshot is one copy
         tail = S * H * PAGE * D * 2
         self._state = torch.zeros(2 * tail + 4 * S * H + 4 * S, dtype=torch.uint8, device=dev)
