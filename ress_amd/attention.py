@@ -432,17 +432,17 @@ def _plain_pools(query, key):
     nq, nk = -(-Tq // KS_Q), -(-Tk // KS_K)
     BH = B * nh
     q_i8 = torch.empty(BH, nq, KS_Q, 64, dtype=torch.int8, device=dev)
-    q_scale = torch.empty(BH, nq, device=dev)
+    q_scale = torch.empty(BH, nq, dtype=torch.float32, device=dev)
     k_i8 = torch.empty(BH, nk, KS_K, 64, dtype=torch.int8, device=dev)
-    k_scale = torch.empty(BH, nk, device=dev)
-    pooled_q = torch.empty(BH, nq, 64, device=dev)
+    k_scale = torch.empty(BH, nk, dtype=torch.float32, device=dev)
+    pooled_q = torch.empty(BH, nq, 64, dtype=torch.float32, device=dev)
     P = _lib.ptr
     _lib.call("ress_per_block_int8", P(q), P(k), None, B, nh, Tq, Tk, *q.stride()[:3], *k.stride()[:3], P(q_i8),
               P(q_scale), P(k_i8), P(k_scale), P(pooled_q), _lib.stream_handle(dev))
-    ksum = torch.empty(BH, nk, 64, device=dev)
-    km = torch.empty(BH, 64, device=dev)
-    pooled_k = torch.empty(BH, nk, 64, device=dev)
-    pooled_v = torch.empty(BH, nk, 64, device=dev)
+    ksum = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
+    km = torch.empty(BH, 64, dtype=torch.float32, device=dev)
+    pooled_k = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
+    pooled_v = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
     v_pack = torch.empty(BH, nk, 4096, dtype=torch.bfloat16, device=dev)
     _lib.call("ress_prep_kv_plain", P(k), P(k), B, nh, Tk, *k.stride()[:3], *k.stride()[:3], P(ksum), P(km),
               P(pooled_k), P(pooled_v), P(v_pack), _lib.stream_handle(dev))
@@ -456,8 +456,8 @@ def predict_attention(query, key, ks_q=KS_Q, ks_k=KS_K, pool_mode="avg"):
         raise NotImplementedError("the kernels pool with 128/64 averages")
     pooled_q, pooled_k, (B, nh, nq, nk) = _plain_pools(query, key)
     dev = query.device
-    full = torch.empty(B, nh, nq, nk, device=dev)
-    cond = torch.empty(B, nh, nq, nk, device=dev)
+    full = torch.empty(B, nh, nq, nk, dtype=torch.float32, device=dev)
+    cond = torch.empty(B, nh, nq, nk, dtype=torch.float32, device=dev)
     _lib.call("ress_pooled_scores", _lib.ptr(pooled_q), _lib.ptr(pooled_k), B * nh, nq, nk, nk,
               1.0 / math.sqrt(64), _lib.ptr(full), _lib.ptr(cond), _lib.stream_handle(dev))
     return full
@@ -473,10 +473,10 @@ def block_mean_value(value, ks_k=KS_K):
     dev = v.device
     nk = -(-Tk // KS_K)
     BH = B * nh
-    ksum = torch.empty(BH, nk, 64, device=dev)
-    km = torch.empty(BH, 64, device=dev)
-    pk = torch.empty(BH, nk, 64, device=dev)
-    pv = torch.empty(BH, nk, 64, device=dev)
+    ksum = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
+    km = torch.empty(BH, 64, dtype=torch.float32, device=dev)
+    pk = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
+    pv = torch.empty(BH, nk, 64, dtype=torch.float32, device=dev)
     vp = torch.empty(BH, nk, 4096, dtype=torch.bfloat16, device=dev)
     _lib.call("ress_prep_kv_plain", _lib.ptr(v), _lib.ptr(v), B, nh, Tk, *v.stride()[:3], *v.stride()[:3],
               _lib.ptr(ksum), _lib.ptr(km), _lib.ptr(pk), _lib.ptr(pv), _lib.ptr(vp), _lib.stream_handle(dev))

@@ -32,7 +32,7 @@ def _cdiv(a, b):
 def hyperparameter_check(hyper, H, device):
     """Broadcast a scalar (or per-head tensor) hyperparameter to a (H,) fp32 tensor."""
     if isinstance(hyper, (int, float)):
-        return torch.full((H,), float(hyper), device=device)
+        return torch.full((H,), float(hyper), dtype=torch.float32, device=device)
     t = torch.as_tensor(hyper, device=device, dtype=torch.float32)
     if t.numel() != H:
         raise ValueError(f"hyperparameter has {t.numel()} values for {H} heads")
@@ -46,8 +46,8 @@ def key_mean(k):
     kb = k.to(torch.bfloat16)
     nk = _cdiv(Tk, BLKK)
     dev = k.device
-    ksum = torch.empty(B * H, nk, 64, device=dev)
-    km = torch.empty(B * H, 64, device=dev)
+    ksum = torch.empty(B * H, nk, 64, dtype=torch.float32, device=dev)
+    km = torch.empty(B * H, 64, dtype=torch.float32, device=dev)
     _lib.call("ress_key_mean", _lib.ptr(kb), B, H, Tk, *kb.stride()[:3], _lib.ptr(ksum), _lib.ptr(km),
               _lib.stream_handle(dev))
     return km
@@ -75,9 +75,9 @@ def per_block_int8(q, k, km=None, BLKQ=BLKQ, BLKK=BLKK, sm_scale=None, tensor_la
     nq, nk = _cdiv(Tq, 128), _cdiv(Tk, 64)
     q_buf = torch.empty(B, H, nq * 128, 64, dtype=torch.int8, device=dev)
     k_buf = torch.empty(B, H, nk * 64, 64, dtype=torch.int8, device=dev)
-    q_scale = torch.empty(B, H, nq, device=dev)
-    k_scale = torch.empty(B, H, nk, device=dev)
-    pooled_q = torch.empty(B * H, nq, 64, device=dev)
+    q_scale = torch.empty(B, H, nq, dtype=torch.float32, device=dev)
+    k_scale = torch.empty(B, H, nk, dtype=torch.float32, device=dev)
+    pooled_q = torch.empty(B * H, nq, 64, dtype=torch.float32, device=dev)
     _lib.call("ress_per_block_int8", _lib.ptr(qb), _lib.ptr(kb), _lib.ptr(km), B, H, Tq, Tk, *qb.stride()[:3],
               *kb.stride()[:3], _lib.ptr(q_buf), _lib.ptr(q_scale), _lib.ptr(k_buf), _lib.ptr(k_scale),
               _lib.ptr(pooled_q), _lib.stream_handle(dev))
@@ -280,10 +280,10 @@ def get_block_map_meansim_fuse_quant(q, k, km=None, is_causal=False, BLKQ=BLKQ, 
     final_map = torch.empty(B, H, nq, nk, dtype=torch.bool, device=dev)  # the kernel writes 0 / 1 bytes
     q_buf = torch.empty(B, H, nq * 128, 64, dtype=torch.int8, device=dev)
     k_buf = torch.empty(B, H, nk * 64, 64, dtype=torch.int8, device=dev)
-    q_scale = torch.empty(B, H, nq, device=dev)
-    k_scale = torch.empty(B, H, nk, device=dev)
-    pooled_q = torch.empty(B * H, nq, 64, device=dev)
-    pooled_k = torch.empty(B * H, nk, 64, device=dev)
+    q_scale = torch.empty(B, H, nq, dtype=torch.float32, device=dev)
+    k_scale = torch.empty(B, H, nk, dtype=torch.float32, device=dev)
+    pooled_q = torch.empty(B * H, nq, 64, dtype=torch.float32, device=dev)
+    pooled_k = torch.empty(B * H, nk, 64, dtype=torch.float32, device=dev)
     sim_q = torch.empty(B * H, nq, dtype=torch.uint8, device=dev)
     sim_k = torch.empty(B * H, nk, dtype=torch.uint8, device=dev)
     ws, ws_bytes = _meansim_workspace(B, H, Tq, Tk, dev)

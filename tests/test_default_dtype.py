@@ -1,6 +1,8 @@
 """What kernels write as fp32 is fp32 whatever torch's default type is: a buffer of a 16-bit default would be half the
 size that is written. Without a GPU: the buffers that reach the library calls."""
 
+import os
+
 import pytest
 import torch
 
@@ -48,3 +50,27 @@ def test_cache(monkeypatch, default):
     assert c.tail_k.dtype == c.tail_v.dtype == torch.bfloat16
     for t in (c.table, c.held, c.lens, c._arrived, c._status):
         assert t.dtype == torch.int32
+
+
+def _untyped(path):
+    import ast
+    made = ("empty", "zeros", "ones", "full", "empty_strided")
+    return [f"{os.path.basename(path)}:{node.lineno}" for node in ast.walk(ast.parse(open(path).read()))
+            if isinstance(node, ast.Call) and isinstance(node.func, ast.Attribute) and node.func.attr in made
+            and isinstance(node.func.value, ast.Name) and node.func.value.id == "torch"
+            and not any(k.arg == "dtype" for k in node.keywords)]
+
+
+def test_buffers_of_library_calls_name_their_type():
+    """In every module that calls the library."""
+    here = os.path.dirname(kvcache.__file__)
+    paths = [os.path.join(here, f) for f in sorted(os.listdir(here)) if f.endswith(".py")]
+    calling = [p for p in paths if "_lib.call" in open(p).read() or "_lib.ptr" in open(p).read()]
+    assert len(calling) >= 7
+    assert [x for p in calling for x in _untyped(p)] == []
+
+
+def test_hyperparameter_check(default):
+    from ress_amd.sparge import hyperparameter_check
+    for x in (0.5, torch.rand(4)):
+        assert hyperparameter_check(x, 4, "cpu").dtype == torch.float32
