@@ -138,21 +138,22 @@ class PagedKVCache:
         self.dtype, self.codes = dtype, codes
         P, H, D, S, dev = self.n_pages, self.kv_heads, head_dim, self.max_seqs, self.device
         code_t = torch.int8 if codes == "int8" else torch.float8_e4m3fn
-        self.k_codes = torch.zeros(P, H, PAGE, D, dtype=torch.int8, device=dev).view(code_t)
-        self.v_codes = torch.zeros(P, H, D, PAGE, dtype=torch.int8, device=dev).view(code_t)
-        self.k_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
-        self.v_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
-        # what an append overwrites lies in one buffer, so that a snapshot is one copy
-        tail = S * H * PAGE * D * 2
-        self._state = torch.zeros(2 * tail + 4 * S * H + 4 * S, dtype=torch.uint8, device=dev)
-        self.tail_k = self._state[:tail].view(dtype).view(S, H, PAGE, D)
-        self.tail_v = self._state[tail:2 * tail].view(dtype).view(S, H, D, PAGE)
-        self.tail_top = self._state[2 * tail:2 * tail + 4 * S * H].view(torch.float32).view(S, H)
-        self.lens = self._state[2 * tail + 4 * S * H:].view(torch.int32)
-        self.table = torch.full((S, self.max_pages), -1, dtype=torch.int32, device=dev)
-        self.held = torch.zeros(S, dtype=torch.int32, device=dev)
-        self._arrived = torch.zeros(S, 32, dtype=torch.int32, device=dev)
-        self._status = torch.zeros(1, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):  # buffers that calls outside of inference mode may change too
+            self.k_codes = torch.zeros(P, H, PAGE, D, dtype=torch.int8, device=dev).view(code_t)
+            self.v_codes = torch.zeros(P, H, D, PAGE, dtype=torch.int8, device=dev).view(code_t)
+            self.k_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
+            self.v_scale = torch.zeros(P, H, dtype=torch.float32, device=dev)
+            # what an append overwrites lies in one buffer, so that a snapshot is one copy
+            tail = S * H * PAGE * D * 2
+            self._state = torch.zeros(2 * tail + 4 * S * H + 4 * S, dtype=torch.uint8, device=dev)
+            self.tail_k = self._state[:tail].view(dtype).view(S, H, PAGE, D)
+            self.tail_v = self._state[tail:2 * tail].view(dtype).view(S, H, D, PAGE)
+            self.tail_top = self._state[2 * tail:2 * tail + 4 * S * H].view(torch.float32).view(S, H)
+            self.lens = self._state[2 * tail + 4 * S * H:].view(torch.int32)
+            self.table = torch.full((S, self.max_pages), -1, dtype=torch.int32, device=dev)
+            self.held = torch.zeros(S, dtype=torch.int32, device=dev)
+            self._arrived = torch.zeros(S, 32, dtype=torch.int32, device=dev)
+            self._status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._free = list(range(P - 1, -1, -1))
         self._pages = [[] for _ in range(S)]
         self._bound = [0] * S     # no slot holds more tokens than this
