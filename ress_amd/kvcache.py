@@ -130,6 +130,8 @@ class PagedKVCache:
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("a PagedKVCache lives on the GPU")
+        if _capturing():
+            raise RuntimeError("a cache is cleared when it is made: not inside a graph capture")
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
         self.n_pages, self.kv_heads, self.head_dim, self.max_seqs = int(n_pages), int(n_kv_heads), head_dim, int(max_seqs)
         self.max_pages = self.n_pages if max_len is None else min(self.n_pages, -(-int(max_len) // PAGE))

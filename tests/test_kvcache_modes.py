@@ -59,3 +59,11 @@ def test_calls_inside_and_outside(dev):
     for c, steps in ((inside, (False, True, False)), (PagedKVCache(16, 1, device=dev), (True, False, True))):
         for a, b in zip(plain, use(c, steps)):
             assert torch.equal(a, b)
+
+
+def test_a_cache_made_inside_a_capture_is_refused(monkeypatch):
+    """Its buffers would be cleared when the graph runs and not when it is made."""
+    monkeypatch.setattr(kvcache, "_capturing", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(RuntimeError, match="not inside a graph capture"):
+        PagedKVCache(4, 2)
