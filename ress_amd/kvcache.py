@@ -221,15 +221,16 @@ class PagedKVCache:
         self._guessed = False
         return got
 
-    def _room(self, ids, more, exact):
+    def _room(self, ids, more, counts=None):
         """Pages for more[i] further tokens in each slot. Bounds that the host only estimates (padded
         batches, captured appends) are read from the device before pages are taken for them or anything is
-        refused; where `more` is itself an estimate (exact=False), a slot is given no more than max_len."""
+        refused. counts: `more` is itself an estimate of these counts on the device; a slot is then given no more than
+        max_len, and they are read where the pool has too little for the estimate."""
         most = PAGE * self.max_pages
 
         def wanted():
             need = {i: self._bound[i] + m for i, m in zip(ids, more)}
-            return need if exact else {i: min(n, most) for i, n in need.items()}
+            return need if counts is None else {i: min(n, most) for i, n in need.items()}
 
         capturing = _capturing()
         if (self._captured or self._guessed) and not capturing:
@@ -241,6 +242,8 @@ class PagedKVCache:
             raise RuntimeError("an append inside a graph capture needs its pages reserved before (reserve)")
         if not self._fits(need):
             self.lengths()
+            if counts is not None and not self._fits(wanted()):
+                more = [min(max(c, 0), m) for c, m in zip(counts.tolist(), more)]
             need = wanted()
             self._fits(need, refuse=True)
         for i, n in need.items():
@@ -427,7 +430,7 @@ class PagedKVCache:
             self._settle()
             counts = counts or [n] * B
             if self._captured or capturing or any(bound[i] + c > cap[i] for i, c in zip(ids, counts)):
-                self._room(ids, counts, exact=not torch.is_tensor(new_lens))
+                self._room(ids, counts, lens_t if guess else None)
             self._captured = self._captured or capturing
         P = _lib.ptr
         self._call("ress_kv_append", self._handle, P(k), *ks, P(v), *vs, P(q), *qs, B, q_heads, n, P(pos), P(table),

@@ -36,7 +36,7 @@ def host_cache(monkeypatch, n_pages=8, max_seqs=2, max_pages=None, fail=None):
         B, n = k.shape[0], k.shape[2]
         for b in range(B):
             s = b if slots is None else int(slots[b])
-            want = int(c.lens[s]) + (n if new_lens is None else int(new_lens[b]))
+            want = int(c.lens[s]) + (n if new_lens is None else min(max(int(new_lens[b]), 0), n))
             room = PAGE * int(c.held[s])
             c.lens[s] = min(want, room)
             if want > room:

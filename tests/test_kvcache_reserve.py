@@ -73,3 +73,31 @@ def test_a_call_that_fails_appends_nothing(monkeypatch, n, again):
     c.append(y, y)
     assert c._most == int(c.lens[0])
     c.check()
+
+
+def _counts(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def test_padded_batches_that_fit_are_not_refused(monkeypatch):
+    """Counts on the device, of which the host knows that they are at most n: where the pool has no pages for n of each,
+    what counts is what they are."""
+    c = host_cache(monkeypatch, n_pages=3)
+    x = tokens(2, 100)
+    c.append(x, x, new_lens=_counts(100, 20))
+    c.check()
+    assert c.lens.tolist() == [100, 20] and c.free_pages() == 0
+    c.append(x, x, new_lens=_counts(28, 44))  # to the last place
+    c.check()
+    assert c.lens.tolist() == [128, 64]
+    with pytest.raises(RuntimeError, match="0 free pages of 3, 1 are needed"):
+        c.append(x, x, new_lens=_counts(0, 1))
+    assert c.lens.tolist() == [128, 64]
+    c.append(x, x, new_lens=_counts(0, -3))  # taken as none
+    c.check()
+    c = host_cache(monkeypatch, n_pages=8, max_pages=2)  # past max_len: dropped and reported, as documented
+    c.append(x, x, new_lens=_counts(100, 20))
+    c.append(x, x, new_lens=_counts(100, 20))
+    assert c.lens.tolist() == [128, 40]
+    with pytest.raises(RuntimeError, match="dropped"):
+        c.check()
