@@ -232,10 +232,11 @@ class PagedKVCache:
             need = {i: self._bound[i] + m for i, m in zip(ids, more)}
             return need if counts is None else {i: min(n, most) for i, n in need.items()}
 
-        capturing = _capturing()
-        if (self._captured or self._guessed) and not capturing:
+        capturing, known = _capturing(), not (self._captured or self._guessed)
+        if not known and not capturing:
             self.lengths()
-        need = wanted()
+        # lengths that cannot be read inside a capture refuse nothing that the slot's pages may hold
+        need = wanted() if known or not capturing else dict(zip(ids, more))
         if all(n <= self._cap[i] for i, n in need.items()):
             return
         if capturing:

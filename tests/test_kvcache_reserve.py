@@ -101,3 +101,32 @@ def test_padded_batches_that_fit_are_not_refused(monkeypatch):
     assert c.lens.tolist() == [128, 40]
     with pytest.raises(RuntimeError, match="dropped"):
         c.check()
+
+
+def test_a_capture_after_padded_batches(monkeypatch):
+    """The host's estimates count the padding; inside a capture, where lengths cannot be read, they refuse nothing that the
+    reserved pages may hold. What does not fit is dropped and reported when the graph runs."""
+    c = host_cache(monkeypatch)
+    x = tokens(1, 50)
+    c.reserve(0, 128)
+    for _ in range(4):
+        c.append(x, x, new_lens=_counts(5))
+    assert c.lens.tolist() == [20, 0]
+    with monkeypatch.context() as m:
+        m.setattr(kvcache, "_capturing", lambda: True)
+        c.append(x, x)
+        with pytest.raises(RuntimeError, match="reserved before"):
+            c.append(tokens(1, 129), tokens(1, 129))  # never fits
+        with pytest.raises(RuntimeError, match="reserved before"):
+            c.append(tokens(2, 1), tokens(2, 1))  # slot 1 has no pages
+    assert c.lens.tolist() == [70, 0]
+    c.append(x, x)
+    c.check()
+    assert c.lens.tolist() == [120, 0]
+    # where the lengths are known, a capture that cannot run once is refused
+    d = host_cache(monkeypatch)
+    d.append(x, x)
+    with monkeypatch.context() as m:
+        m.setattr(kvcache, "_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="reserved before"):
+            d.append(x, x)
