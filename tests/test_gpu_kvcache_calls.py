@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from ress_amd.kvcache import PAGE, PagedKVCache
+from kvcache_oracle import attention, held, tolerance
+from ress_amd.kvcache import PAGE, PagedKVCache, RotaryTable
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +79,100 @@ def test_lengths_changed_from_outside(dev, n, length):
     for a, b in zip(codes, (c.k_codes[pages], c.v_codes[pages], c.k_scale[pages], c.v_scale[pages])):
         assert torch.equal(a, b)
     assert c.held.tolist() == [4, 4, 4] and c.lens.tolist()[::2] == [200, 200]
+
+
+def _filled(dev, H, D, lens, dtype=BF16, codes="int8"):
+    c = PagedKVCache(sum(-(-(L + 200) // PAGE) for L in lens), H, D, max_seqs=len(lens), dtype=dtype, codes=codes, device=dev)
+    for b, L in enumerate(lens):
+        if L:
+            g = torch.Generator().manual_seed(b)
+            k, v = (torch.randn(1, H, L, D, generator=g).to(dev, dtype) for _ in range(2))
+            c.append(k, v, slots=[b])
+    return c
+
+
+def _check(c, q, got, causal=False, scale=None):
+    for b in range(q.shape[0]):
+        k, v = held(c, b)
+        want, size, spread = attention(q[b], k, v, q.shape[2], causal, scale)
+        err = (got[b].double().cpu() - want).abs()
+        tol = tolerance(want, size, spread, q.dtype, k.shape[1])
+        assert (err <= tol).all(), (b, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("H,G,n", [(3, 1, 7), (5, 3, 1), (1, 7, 5), (3, 5, 9), (7, 3, 40), (1, 40, 1), (2, 33, 3)])
+@pytest.mark.parametrize("dtype,codes,D", [(BF16, "int8", 64), (torch.float16, "fp8", 128)])
+def test_odd_heads(dev, dtype, codes, D, H, G, n):
+    """Heads and groups that are no powers of two: rows of a tile belong to several tokens, tiles to several heads."""
+    c = _filled(dev, H, D, [700, 65, 30], dtype, codes)
+    q = torch.randn(3, H * G, n, D, generator=torch.Generator().manual_seed(9)).to(dev, dtype)
+    for causal in (False, True):
+        for scale in (None, 0.05):
+            _check(c, q, c.attend(q, causal=causal, scale=scale), causal, scale)
+
+
+@pytest.mark.parametrize("dtype,codes,D", [(BF16, "int8", 64), (torch.float16, "int8", 128)])
+@pytest.mark.parametrize("n", [20, 90, 300])
+@pytest.mark.parametrize("L", [500, 6000])
+def test_queries_that_are_not_finite(dev, dtype, codes, D, n, L):
+    """Reach their own rows and no others, whatever rows share a tile, a wave or a register with them."""
+    c = _filled(dev, 2, D, [L], dtype, codes)
+    q = torch.randn(1, 4, n, D, generator=torch.Generator().manual_seed(9)).to(dev, dtype)
+    want = c.attend(q, causal=True)
+    for bad in (float("nan"), -float("nan"), float("inf"), -float("inf")):
+        for i in (0, 3, 17):
+            p = q.clone()
+            p[0, 1, i, 5] = bad
+            got = c.attend(p, causal=True)
+            rest = torch.ones(1, 4, n, dtype=torch.bool, device=dev)
+            rest[0, 1, i] = False
+            assert torch.equal(got[rest], want[rest])
+            assert bad == bad or got[0, 1, i].isnan().all()
+
+
+def test_expanded_operands(dev):
+    """Views that repeat rows, heads and sequences: as their copies do."""
+    x = _rand((1, 1, 1, 64), dev, 3)
+    a, b = (PagedKVCache(16, 2, max_seqs=2, device=dev) for _ in range(2))
+    rope = RotaryTable(64, 300, axes=1, device=dev)
+    pos = torch.arange(150, device=dev)[None]
+    wide = x.expand(2, 2, 150, 64)
+    qa = a.append(wide, wide, pos=pos.expand(2, 150), rope=rope, q=x.expand(2, 4, 150, 64))
+    qb = b.append(wide.contiguous(), wide.contiguous(), pos=pos.repeat(2, 1), rope=rope, q=x.repeat(2, 4, 150, 1))
+    assert torch.equal(qa, qb)
+    for t, u in zip(a.read(150), b.read(150)):
+        assert torch.equal(t, u)
+    for n in (4, 70):
+        got = a.attend(x.expand(2, 4, n, 64), causal=True)
+        assert torch.equal(got, b.attend(x.repeat(2, 4, n, 1), causal=True))
+        out = torch.full((2, n, 3, 4, 64), 9.0, dtype=BF16, device=dev)
+        assert torch.equal(a.attend(x.expand(2, 4, n, 64), causal=True, out=out[:, :, 1].transpose(1, 2)), got)
+        assert (out[:, :, 0] == 9).all() and (out[:, :, 2] == 9).all()
+
+
+def test_captured_padded_steps(dev):
+    """Counts and slots that live on the device: a graph's replays append what they say then."""
+    eager, c = (PagedKVCache(24, 2, max_seqs=4, device=dev) for _ in range(2))
+    x = _rand((2, 2, 30, 64), dev, 1)
+    counts = torch.tensor([30, 7], dtype=torch.int32, device=dev)
+    batch = c.slots([3, 1])
+    for s in (3, 1):
+        c.reserve(s, 300)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.append(x, x, slots=batch, new_lens=counts)
+        out = c.attend(x, slots=batch, new_lens=counts, causal=True)
+    for i, m in enumerate(([30, 7], [1, 0], [0, 30], [29, 30], [30, 30])):
+        x.copy_(_rand((2, 2, 30, 64), dev, 10 + i))
+        counts.copy_(torch.tensor(m, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.append(x, x, slots=[3, 1], new_lens=m)
+        want = eager.attend(x, slots=[3, 1], new_lens=m, causal=True)
+        assert eager.lengths() == c.lens.tolist()
+        for s in (3, 1):
+            for a, b in zip(held(eager, s), held(c, s)):
+                assert torch.equal(a, b)
+        assert (out.double() - want.double()).abs().max() <= 2.0 ** -8 * want.double().abs().max().clamp(min=1)
+        assert (out[0, :, m[0]:] == 0).all() and (out[1, :, m[1]:] == 0).all()
+    c.check()
