@@ -317,7 +317,7 @@ typedef struct ress_kv_cache {
 } ress_kv_cache;
 
 /* Appends n tokens a sequence: k, v (B,kv_heads,n,head_dim), element strides (sB,sH,sT), unit-stride
- * dims, to slots[b] (int32[B] in device memory, each at most once; null: slot b), the first new_lens[b] of
+ * dims, to slots[b] (int32[B] in device memory, each in the cache and at most once; null: slot b), the first new_lens[b] of
  * them (int32[B] in device memory, clamped to 0..n; null: all), and moves lens on. pos (B,n,axes) int64 or
  * null: keys, and queries q (B,Hq,n,head_dim) if given, are rotated with the rows pos of
  * rope (positions, 2, head_dim / 2 / axes) f32, cosines before sines; q_out (B,Hq,n,head_dim) receives
@@ -336,7 +336,8 @@ int ress_kv_read(const ress_kv_cache* cache, int B, int n, const int* slots, con
  * reads key/value head h / (Hq / kv_heads). Row i of sequence b sees every token, or with causal = 1 the
  * tokens up to its own, the rows being the sequence's last new_lens[b] tokens (null: n). Rows past
  * new_lens[b] are not written; rows that see nothing are zero. most_tokens: no sequence is longer (it sizes
- * the split of the keys; a longer one is still right). workspace: ress_kv_attend_workspace_size bytes,
+ * the split of the keys; a longer one is still right). P, and in fp16 the values times their scale, are rounded to the
+ * 16-bit type; sums are fp32. workspace: ress_kv_attend_workspace_size bytes,
  * 16-byte aligned, for the same arguments (may be 0 bytes). sm_scale > 0. */
 long long ress_kv_attend_workspace_size(const ress_kv_cache* cache, int B, int Hq, int n, int most_tokens);
 int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long sqB, long long sqH, long long sqT, int B,
@@ -351,10 +352,10 @@ int ress_kv_attend(const ress_kv_cache* cache, const void* q, long long sqB, lon
  * of 8) are filled with zeros from K to code_stride. No counterpart in the reference. */
 int ress_quantize_rows(const void* x, long long stride, int dtype, int M, int K, void* codes, long long code_stride,
                        float* scale, hipStream_t stream);
-/* out (M,N) = act((s_m sum_k c_mk w_nk) * w_scale_n + bias_n) in x's type, c and s being the codes and scales of x's
- * rows as above, w int8 (N,K) contiguous, 16-byte aligned. bias: f32 (N) or null. act: 0 none, 1 gelu (erf). workspace:
- * ress_int8_linear_workspace_size bytes, 16-byte aligned (may be 0 bytes). No counterpart in the reference, whose
- * linear layers are torch's. */
+/* out (M,N) = act((sum_k c_mk w_nk * w_scale_n) * s_m + bias_n) in x's type (in that order: a token's scale may be near
+ * fp32's end), c and s being the codes and scales of x's rows as above, w int8 (N,K) contiguous, 16-byte aligned. bias: f32
+ * (N) or null. act: 0 none, 1 gelu (erf). workspace: ress_int8_linear_workspace_size bytes, 16-byte aligned (may be 0
+ * bytes). No counterpart in the reference, whose linear layers are torch's. */
 long long ress_int8_linear_workspace_size(int M, int K, int N);
 /* The tile that a product is cut into, tokens << 16 | channels; 0 where it needs none (a few tokens). */
 int ress_int8_linear_tile(int M, int K, int N);

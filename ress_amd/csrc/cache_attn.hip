@@ -5,8 +5,8 @@
 // O^T += V^T P^T (A = values of 16 dims), a lane holds for ITS query four keys of each 16, which is what
 // the second product takes as its B operand once the keys of a value row are stored in that order (v_token): P
 // never leaves the registers. The codes are widened to 16 bits exactly; the scales of a page multiply
-// the scores (folded into the exponent's multiply-add) and P or P V (below), so that nothing but P and the
-// output is rounded to 16 bits. Max, sum and output accumulate in fp32.
+// the scores (folded into the exponent's multiply-add) and P or the values (below). Rounded to 16 bits are P, in fp16 each
+// value (code * v_scale) too, and the output. Max, sum and output accumulate in fp32.
 //
 // Running max. m starts at the lowest finite value and moves only when a score of the wave lies more than
 // LAZY = 8 (in log2) above its row's m: P is then at most 2^8, sums are unaffected, and most pages need
@@ -14,8 +14,9 @@
 //
 // v_scale. In bf16 it enters as an addend of the exponent (PageScale), relative to a power of two: the codes stay whole
 // and it costs no multiplication per element. fp16 has no exponents to spare for that: there the codes are multiplied,
-// as they are widened, by v_scale rounded toward zero to fp16 (the products are in fp16's range, as the values they came
-// from were), and what that rounding took enters the exponent.
+// as they are widened, by v_scale rounded toward zero to fp16 (the products are rounded to fp16, in whose range they are as the
+// values they came from were; a scale below 2^-14, which fp16 holds with fewer bits, goes to the nearest), and what the
+// scale's rounding took or added enters the exponent.
 // The sum of P is a product with ones on the matrix cores, of the rounded P, so numerator and denominator carry the
 // same roundings.
 //
@@ -119,8 +120,8 @@ struct TailScale {
 template <int DT>
 __device__ __forceinline__ float value_scale(float vs) {
   if constexpr (DT == KV_BF16) return 1.0f;
-  // toward zero, as 127 times the nearest of 65504 / 127 is infinite; never 0 (the smallest subnormal serves the smallest
-  // scales), so that 0 * V is 0
+  // toward zero, as 127 times the nearest of 65504 / 127 is infinite (what the mask leaves of a subnormal the cast rounds to
+  // nearest); never 0 (the smallest subnormal serves the smallest scales), so that 0 * V is 0
   return vs > 0.0f ? fmaxf((float)(_Float16)__uint_as_float(__float_as_uint(vs) & 0xffffe000u), 0x1p-24f) : 1.0f;
 }
 template <int DT>
@@ -341,17 +342,17 @@ struct TailValues {
   }
 };
 
-// Waves that a SIMD's registers are shared out for. One more spills: 22 us for one row of 16 heads of 64 over 21,984
-// tokens instead of 20, 114 for 32 sequences of up to 8,192 tokens, 8 heads of 128, instead of 74; with 32 rows and a
-// head of 128 two spill.
+// Waves that a SIMD's registers are shared out for. One more spills: us a call for one row of 16 heads of 64 over 21,984
+// tokens 17.3 instead of 17.1, five over 274,800 109 instead of 102, 32 sequences of up to 8,192 tokens, 8 heads of 128, 153
+// instead of 63; with 32 rows and a head of 128 two spill.
 constexpr int few_waves(int D, int CT) { return CT == 2 ? (D == 64 ? 2 : 1) : D == 64 ? 3 : 2; }
 
 // ---- few rows: one wave a page --------------------------------------------------------------------
 // A workgroup of four waves takes 16 CT rows of a (sequence, kv head) and a share of its pages, a wave every
 // fourth page, codes straight from memory into the operands (1 KB, contiguous, an access). The waves' parts are
-// joined in LDS. Bound by the bytes of the codes where the cache is long (5 rows of 16 heads over 274,800 tokens: 98 us
-// for 563 MB, 5.7 TB/s), by one page's chain of loads, scores, exponentials and products where it is short (one row over
-// 21,984 tokens: 12 us, 3.8 TB/s).
+// joined in LDS. Bound by the bytes of the codes where the cache is long (5 rows of 16 heads over 274,800 tokens: 96 us
+// for 563 MB, 5.9 TB/s), by one page's chain of loads, scores, exponentials and products where it is short (one row over
+// 21,984 tokens: 12 us, 3.8 TB/s; the call takes 16, its parts being joined in 4).
 template <int DT, int CODES, int D, int CT>
 __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(AttendArgs a, RESS_READ_ONLY) {
   constexpr int NW = 4;
@@ -547,10 +548,12 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
 // every row sees whole run without a mask, apart from those that a causal row ends in, so that the masks' registers
 // are not held in the loop.
 //
-// Bound by the issue of vector and matrix instructions, which hardly overlap on a SIMD: of its cycles the vector unit is
-// busy 67%, the matrix cores 37% (1,374 rows of 16 heads over 87,936 tokens; a page of 32 rows takes 36 products of
-// 16 cycles, 32 exponentials of 8 and some 150 other instructions of 4). 495 GFLOP in 625 us there: 790 TFLOP/s, 38% of
-// the 2,058 that the matrix cores reach. At that size and at 21,984 tokens: 2 tiles of 16 rows a wave 703, 189 us (3: 733,
+// Bound by the vector instructions beside the products: the vector unit is busy 67% of a SIMD's cycles, the matrix cores
+// 37% (1,374 rows of 16 heads over 87,936 tokens; a page of 32 rows takes 36 products of 16 cycles, 32 exponentials of 8
+// and some 150 other instructions of 4). It issues 0.39 vector instructions a busy matrix cycle where the block-sparse kernel
+// (attn.hip), whose products are 32 x 32 and whose exponentials mostly need no maximum, issues 0.15 and keeps the matrix cores
+// busy 62%, the vector unit 52%. 495 GFLOP in 630 to 665 us there (cards differ): 740 to 780 TFLOP/s, 36 to 38% of the 2,058
+// that the matrix cores reach. Calls at that size and at 21,984 tokens, when they were chosen: 2 tiles of 16 rows a wave 703, 189 us (3: 733,
 // 198; 4: 693, 187; 1: 777, 217), four waves a SIMD instead of three 619, 179. Waves of a workgroup: cut().
 constexpr int ROWS_CT = 2;
 constexpr int rows_waves(int D) { return D == 64 ? 4 : 2; }  // a SIMD; 64 KB of LDS a workgroup at a head of 128
@@ -808,7 +811,7 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
 //
 // Up to 32 rows of a (sequence, kv head) go to the few-rows kernel: 32 rows of 16 heads over 21,984 tokens take 24 us so
 // and 25 in the other, over 87,936 tokens 40 and 49; 24 to 32 grouped rows of 8 heads of 128 25 to 49 and 29 to 53.
-// The few-rows kernel gets workgroups for half the slots (two a CU): with four a CU the five special rows over 274,800 tokens take 123 us
+// The few-rows kernel gets workgroups for half the slots (two a CU; times are of calls here): with four a CU the five special rows over 274,800 tokens take 123 us
 // instead of 103, the ragged batch of 32 72 instead of 74; with one 111 instead of 102 and 61 instead of 63.
 //
 // Many rows: four waves a workgroup, or eight (half the widening a row) at a head of 64 where the rows fill its tiles of

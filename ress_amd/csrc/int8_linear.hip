@@ -155,14 +155,15 @@ __device__ __forceinline__ void dma_barrier() {
 // row of tiles, a few at a time: in one run they would hold up the products behind them. A token operand is read into
 // the registers of the one just used.
 //
-// Bound by how the products and the LDS reads that feed them share a CU: 21,984 x 1,024 x 4,096 100 us, 1.8 POP/s of the
-// 3.9 that the matrix cores reach (they are busy 36% of the launch, its rounds of 464 tiles on 256 CUs included, no LDS
-// conflicts); 4,096 cubed 60 us, 2.3 POP/s. 1,374 x 4,096 x 1,024 takes 16 us, half of it the first fill and the
-// epilogue. Measured against this form: four stages of 64 bytes with fewer tiles in flight, rows padded instead of swapped
+// Bound by waiting: the waves wait for half of their cycles (51%) while no unit is busy for more than a third of the launch
+// (21,984 tokens, 4,096 -> 1,024: matrix cores 34%, its rounds of 464 tiles on 256 CUs included, vector 15%, LDS 14%, no
+// conflicts, waits for LDS 2%). A stage's DMAs go out in one half and are waited for, all of them, after the next. 98 to 110 us
+// there on different cards, 1.7 to 1.9 POP/s of the 3.9 that the matrix cores reach; 4,096 cubed 66 us, 2.1 POP/s. 1,374
+// tokens, 1,024 -> 4,096, take 17 us, half of it the first fill and the epilogue. Measured against this form: four stages of 64 bytes with fewer tiles in flight, rows padded instead of swapped
 // and channels permuted for wider stores, all slower; the DMA as the compiler's builtin (which waits for all of them) 151
 // us for 102.
 template <int DT, int BM, int BN, int GM, int GN, bool EVEN>
-__global__ __launch_bounds__(64 * GM * GN, BM * BN / (GM * GN) > 8192 ? 1 : 2) void k_int8_gemm(const uint8_t* __restrict__ x, int kp,
+__global__ __launch_bounds__(64 * GM * GN, 2) void k_int8_gemm(const uint8_t* __restrict__ x, int kp,
                                                             const float* __restrict__ sx, const uint8_t* __restrict__ w,
                                                             int K, Out o) {
   constexpr int NW = GM * GN, WM = BM / GM, WN = BN / GN, TM = WM / 16, TN = WN / 16;
@@ -386,10 +387,10 @@ int gemm(const uint8_t* codes, int kp, const float* sx, const void* w, int K, co
 
 // The tile of a product: the one whose rounds of workgroups add up to the least time. A step (128 of K) takes `alone` us
 // where each CU has one tile and `full` where every CU holds the `held` that fit; a round's start and end (the output
-// is written then) take `ends`. Measured, us of the product (256 x 256, 192 x 256, 128 x 128 | taken):
-//   4096 x 4096 x 4096 58, 80, 66 | 58        21984 x 1024 (N) x 4096 (K) 105, 91, 102 | 91
-//   8192 x 8192 x 8192 495, 479, 544 | 495    21984 x 4096 (N) x 1024 (K) 143, 151, 135 | 135
-// and 1374 x 1024 (N) x 4096 (K): 128 x 128 17, 64 x 128 15, 64 x 64 12 | 12.
+// is written then) take `ends`. The present kernel, us of the product (256 x 256, 192 x 256, 128 x 128 | taken):
+//   4096 x 4096 x 4096 66, 87, 72 | 66        21984 x 1024 (N) x 4096 (K) 107, 98, 99 | 98
+//   8192 x 8192 x 8192 527, 511, 559 | 527    21984 x 4096 (N) x 1024 (K) 145, 149, 129 | 129
+// and 1374 x 1024 (N) x 4096 (K): 128 x 128 24, 64 x 128 22, 64 x 64 18 | 18.
 constexpr struct {
   int bm, bn, threads, held;
   double alone, full, ends;

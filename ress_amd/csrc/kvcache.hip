@@ -81,7 +81,6 @@ __device__ __forceinline__ uint32_t top_bits(const uint4& v, uint32_t m) {
   return m;
 }
 
-// One page of one head: rows t of `lo`.. that exist, as 16-bit chunk pairs in registers.
 // One workgroup handles, for a (sequence, head): workgroup 0 the page the sequence ends in and, after it,
 // the new last page; the others a page each that the call fills. The unfinished page's 16-bit tokens are
 // read and rewritten by workgroup 0 alone, in that order. The queries' workgroups follow in the same launch.

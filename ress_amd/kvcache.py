@@ -15,12 +15,13 @@ values, and half the bytes that attention reads. The tokens of a sequence's unfi
 16 bits and are quantised once, when the page is full, so the cache's contents depend on the tokens
 alone and not on how they were split over calls.
 
-Every method works on torch's current stream of the cache's device and none waits for the device,
-except reserve and release (a small copy of page numbers), lengths and check, and an append that needs
-pages (once the host no longer knows the lengths, as with counts on the device, it reads them first; after a
-captured append each eager one does). Calls that change a
-cache (append, restore, release) must be ordered one after the other, as on one stream, and so must
-two captured graphs that append to one cache; attend and read only read it.
+Every method works on torch's current stream of the cache's device. These wait for the device: lengths and
+check; reserve, and an append that needs pages (a small copy of page numbers; once the host no longer knows the
+lengths, as with counts on the device, it reads them first; after a captured append each eager one does); and
+every argument that comes from the host (slots or new_lens as a list, pos on the CPU), whose copy waits: a
+decoding loop passes a SlotBatch and tensors on the device. Calls that change a cache (append, reserve, restore,
+release) must be ordered one after the other, as on one stream, and so must two captured graphs that append to
+one cache; attend and read only read it.
 
 The reference has no counterpart: it attends over all frames at once.
 """
@@ -112,8 +113,8 @@ class Snapshot:
 
 
 class PagedKVCache:
-    """`max_seqs` sequences (slots) of at most `max_len` tokens each (default: the whole pool) in a
-    pool of `n_pages` pages of 64 tokens. dtype: bfloat16 or float16, the type of the keys, values and
+    """`max_seqs` sequences (slots) of at most `max_len` tokens each (rounded up to whole pages; default: the
+    whole pool) in a pool of `n_pages` pages of 64 tokens. dtype: bfloat16 or float16, the type of the keys, values and
     queries; codes: "int8" or "fp8" (e4m3). head_dim: 64 or 128."""
 
     def __init__(self, n_pages, n_kv_heads, head_dim=64, max_seqs=1, max_len=None, dtype=torch.bfloat16,
@@ -306,7 +307,8 @@ class PagedKVCache:
             snap.alive = False
 
     def snapshot(self):
-        """The state that restore goes back to (a copy of the unfinished pages and the lengths)."""
+        """The state that restore goes back to (a copy of the unfinished pages and the lengths). Recorded in a graph, it is
+        that of the graph's last run."""
         self._settle()
         self._serial += 1
         self._captured = self._captured or _capturing()
@@ -474,7 +476,8 @@ class PagedKVCache:
         """softmax(scale q K^T) V of the queries q (B, heads, n, head_dim; heads a multiple of kv_heads, query
         head h reading key/value head h / (heads / kv_heads)) over what the cache holds. The queries belong
         to the last n tokens of their sequence (the last new_lens[b] of them, the other rows being padding);
-        they see all of it, or with causal=True the tokens up to their own. scale: 1/sqrt(head_dim).
+        they see all of it, or with causal=True the tokens up to their own. scale: 1/sqrt(head_dim). The softmax's weights
+        (and float16 values, scaled) are rounded to the cache's type before they meet; maxima and sums are fp32.
 
         Returns (B, heads, n, head_dim), zeros in padding and in rows that see nothing; a given `out` is
         written in place, its padding left as it was; it shares no memory with q."""
