@@ -12,6 +12,9 @@ import functools
 
 import torch
 import torch.nn as nn
+from torch.nn.utils import prune
+from torch.nn.utils.spectral_norm import SpectralNorm
+from torch.nn.utils.weight_norm import WeightNorm
 
 from ress_amd import _lib
 
@@ -96,6 +99,10 @@ def _workspace(M, K, N):
     return _lib.lib().ress_int8_linear_workspace_size(M, K, N)
 
 
+# what torch's reparametrisations and pruning leave on a layer, which forms the weight anew before each forward
+_WEIGHT_HOOKS = (WeightNorm, SpectralNorm, prune.BasePruningMethod)
+
+
 class Int8Linear(nn.Module):
     """An nn.Linear's place-holder with 8-bit weights (buffers, not parameters), for 16-bit activations; under autocast
     they are cast to its type, as the layer's would be."""
@@ -108,11 +115,15 @@ class Int8Linear(nn.Module):
         self.register_buffer("codes", codes)
         self.register_buffer("scale", scale)
         self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().float().contiguous())
-        # the layer's mode and forward hooks go with it; the same dicts, so that the hooks' handles still remove them
+        # The layer's mode and forward hooks go with it (the same dicts, so that the hooks' handles still remove them), but for
+        # hooks that form its weight, for which the codes stand.
         self.training = linear.training
         for name in ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",
                      "_forward_pre_hooks_with_kwargs"):
             setattr(self, name, getattr(linear, name))
+        if any(isinstance(h, _WEIGHT_HOOKS) for h in self._forward_pre_hooks.values()):
+            self._forward_pre_hooks = type(self._forward_pre_hooks)(
+                (i, h) for i, h in self._forward_pre_hooks.items() if not isinstance(h, _WEIGHT_HOOKS))
 
     def _apply(self, fn, recurse=True):
         # a cast of the model to 16 bits must not round the scales and the bias, which are fp32

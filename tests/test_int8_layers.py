@@ -119,3 +119,27 @@ def test_drift_matrices_of_8_bit_layers():
     for m, block in zip(M, model.aggregator.global_blocks):
         w = block.attn.proj.weight
         assert torch.equal(block.attn.M, m) and torch.equal(m[0], w.T @ w)
+
+
+@pytest.mark.parametrize("way", ["weight_norm", "spectral_norm", "prune"])
+def test_layers_whose_weight_a_hook_forms(monkeypatch, way):
+    """The codes stand for the weight as it is; the hook that formed it has nothing to form any more."""
+    from torch.nn.utils import prune
+    monkeypatch.setattr(int8, "int8_linear", lambda x, codes, scale, bias, act: x @ (codes * scale[:, None]).t() + bias)
+    torch.manual_seed(0)
+    layer = nn.Linear(16, 4)
+    if way == "prune":
+        prune.l1_unstructured(layer, "weight", 0.5)
+    else:
+        getattr(nn.utils, way)(layer)
+    layer.eval()
+    x, seen = torch.rand(3, 16), []
+    layer.register_forward_pre_hook(lambda mod, args: seen.append(1))
+    m = nn.Sequential(layer)
+    with torch.no_grad():
+        want = m(x)
+        assert quantize_linears(m) == ["0"]
+        got = m(x)
+    assert len(seen) == 2
+    # half a step of 1/127 of the largest weight for each of 16 products, and fp32 sums
+    assert ((got - want).abs() <= 16 * layer.weight.abs().max() / 254 + 1e-5).all()
