@@ -92,7 +92,9 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden, dim)
 
     def forward(self, x):
-        if isinstance(self.fc1, Int8Linear) and isinstance(self.act, nn.GELU) and self.act.approximate == "none":
+        act = self.act
+        if (isinstance(self.fc1, Int8Linear) and type(act) is nn.GELU and act.approximate == "none"
+                and not (act._forward_hooks or act._forward_pre_hooks)):
             return self.fc2(self.fc1(x, act="gelu"))
         return self.fc2(self.act(self.fc1(x)))
 

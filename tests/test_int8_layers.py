@@ -143,3 +143,30 @@ def test_layers_whose_weight_a_hook_forms(monkeypatch, way):
     assert len(seen) == 2
     # half a step of 1/127 of the largest weight for each of 16 products, and fp32 sums
     assert ((got - want).abs() <= 16 * layer.weight.abs().max() / 254 + 1e-5).all()
+
+
+class CountedGelu(nn.GELU):
+    def forward(self, x):
+        self.calls = getattr(self, "calls", 0) + 1
+        return super().forward(x)
+
+
+def test_mlp_leaves_no_activation_out(monkeypatch):
+    """gelu is fused into the 8-bit layer where nothing else hangs on the activation module."""
+    from ress_amd.aggregator import Mlp
+    acts = []
+    monkeypatch.setattr(int8, "int8_linear", lambda x, codes, scale, bias, act: (acts.append(act), x.new_zeros(*x.shape[:-1], len(codes)))[1])
+    m = Mlp(16, 32)
+    quantize_linears(m)
+    x = torch.rand(3, 16)
+    m(x)
+    assert acts == ["gelu", None]
+    for kind in ("register_forward_hook", "register_forward_pre_hook"):
+        seen = []
+        handle = getattr(m.act, kind)(lambda *a: seen.append(1) and None)
+        m(x)
+        assert seen == [1] and acts[-2:] == [None, None]
+        handle.remove()
+    m.act = CountedGelu()
+    m(x)
+    assert m.act.calls == 1 and acts[-2:] == [None, None]
