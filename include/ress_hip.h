@@ -292,7 +292,8 @@ int ress_block_sparse_fwd(const void* q_i8, const void* k_i8, const void* v, int
  *   arrived [max_seqs][32] int32: zero between calls (a cache line for each slot)
  *   status int32, OR-ed: 1 tokens that found no reserved page were dropped, 2 a position outside the
  *     rotation table (clamped into it), 4 a page number outside the pool (not read or written),
- *     8 a page with a key or value that is not finite (its scale is NaN)
+ *     8 a page with a key or value that is not finite (its scale is NaN), 16 a slot outside the cache (its row
+ *     appends nothing, and reads and sees no token)
  * dtype: 1 bf16, 2 fp16 (keys, values and queries). codes: 0 int8, 1 e4m3. head_dim: 64 or 128. */
 typedef struct ress_kv_cache {
   void* k_codes;

@@ -77,13 +77,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <int D>
 struct Head {
   int len, nv, slot, h;
+  bool there;                  // the slot lies in the cache
   const uint8_t *kc, *vc;      // codes of page 0 of this head
   const uint16_t *tk, *tv;     // the unfinished page
   long long stride;            // bytes from page to page
   __device__ __forceinline__ Head(const AttendArgs& a, const int* __restrict__ lens, const int* __restrict__ slots,
                                   const int* __restrict__ new_lens, int b, int h_) : h(h_) {
-    slot = slots ? slots[b] : b;
-    len = held_tokens(lens[slot], a.c.max_pages);
+    slot = slot_of(a.c, slots, b, there);
+    len = there ? held_tokens(lens[slot], a.c.max_pages) : 0;
     nv = new_lens ? min(max(new_lens[b], 0), a.n) : a.n;
     const long long one = (long long)KV_PAGE * D;
     kc = reinterpret_cast<const uint8_t*>(a.c.k_codes) + h * one;
@@ -459,6 +460,7 @@ __global__ __launch_bounds__(256, few_waves(D, CT)) void k_cache_attn_few(Attend
     next = after;
   }
   if (bad && lane == 0) atomicOr(a.c.status, KV_ST_PAGE);
+  if (!hd.there && threadIdx.x == 0) atomicOr(a.c.status, KV_ST_SLOT);
   // the unfinished page, by the wave whose turn it would be
   if (left && full >= lo && full < hi && (full - lo) % NW == w && full * KV_PAGE < seen_by_any) {
     // its loads together
@@ -704,6 +706,7 @@ __global__ __launch_bounds__(64 * NW, rows_waves(D)) void k_cache_attn_rows(Atte
     if (full * KV_PAGE < seen_by_any) compute(std::true_type{}, 0, full, a.scale, ts.vs);
   }
   if (bad && t == 0) atomicOr(a.c.status, KV_ST_PAGE);
+  if (!hd.there && t == 0) atomicOr(a.c.status, KV_ST_SLOT);
 #pragma unroll
   for (int c = 0; c < CT; ++c) {
     const float L = st.l[c];
@@ -743,7 +746,8 @@ __global__ __launch_bounds__(256) void k_cache_attn_join(AttendArgs a) {
   const int H = a.c.kv_heads, per = a.n * a.G, bh = (int)(min(row, all_rows - 1) / per), r = (int)(row - (long long)bh * per);
   const int b = bh / H, h = bh % H, tok = r / a.G;
   const int nv = a.new_lens ? min(max(a.new_lens[b], 0), a.n) : a.n;
-  const int len = held_tokens(a.c.lens[a.slots ? a.slots[b] : b], a.c.max_pages);
+  bool there;
+  const int slot = slot_of(a.c, a.slots, b, there), len = there ? held_tokens(a.c.lens[slot], a.c.max_pages) : 0;
   const int ns = min(a.splits, cdiv(cdiv(len, KV_PAGE), a.per));
   const bool live = row < all_rows && tok < nv && ns > 1;  // one part is written by its workgroup
   const float* ml = a.part_ml + 2 * (live ? row : 0);

@@ -19,10 +19,18 @@ constexpr int KV_LINE = 32;                // ints from one slot's `arrived` to 
 constexpr int KV_I8 = 0, KV_FP8 = 1;       // ress_kv_cache.codes
 constexpr int KV_BF16 = 1, KV_F16 = 2;     // ress_kv_cache.dtype
 // ress_kv_cache.status bits
-constexpr int KV_ST_FULL = 1, KV_ST_POS = 2, KV_ST_PAGE = 4, KV_ST_NONFINITE = 8;
+constexpr int KV_ST_FULL = 1, KV_ST_POS = 2, KV_ST_PAGE = 4, KV_ST_NONFINITE = 8, KV_ST_SLOT = 16;
 
 // Checks a cache handle on the host (kvcache.hip): 0, or -1 with the message set.
 int ress_kv_check(const ress_kv_cache* c, int B, const char* who);
+
+// The slot of a batch's row, and whether it lies in the cache: one that does not (its number on the device was changed, or
+// freed under a recorded graph) is reported, and its row is one of no tokens.
+__device__ __forceinline__ int slot_of(const ress_kv_cache& c, const int* slots, int b, bool& ok) {
+  const int s = slots ? slots[b] : b;
+  ok = s >= 0 && s < c.max_seqs;
+  return ok ? s : 0;
+}
 
 // Tokens of a slot, as the kernels take them: between none and what its pages (or, for a reader, a table) have room for,
 // so that lengths changed from outside, as by a snapshot whose recording never ran, reach no memory but the slot's.

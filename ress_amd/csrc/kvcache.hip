@@ -142,7 +142,12 @@ __global__ __launch_bounds__(THREADS) void k_kv_append(AppendArgs a, int kv_grou
   }
 
   const int part = blockIdx.x % a.pages, h = blockIdx.x / a.pages % H, b = blockIdx.x / a.pages / H;
-  const int slot = a.slots ? a.slots[b] : b;
+  bool there;
+  const int slot = slot_of(a.c, a.slots, b, there);
+  if (!there) {
+    if (t == 0 && part == 0 && h == 0) atomicOr(a.c.status, KV_ST_SLOT);
+    return;
+  }
 
   const int held = a.c.held[slot], cap = held * KV_PAGE, fresh = new_tokens(a.new_lens, b, a.n);
   const int len = held_tokens(a.c.lens[slot], held);
@@ -339,8 +344,10 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
   __shared__ __align__(16) uint16_t vt[D * VROW];
   const int t = threadIdx.x, H = c.kv_heads;
   const int part = blockIdx.x % pages, h = blockIdx.x / pages % H, b = blockIdx.x / pages / H;
-  const int slot = slots ? slots[b] : b;
-  const int len = held_tokens(c.lens[slot], c.max_pages);
+  bool there;
+  const int slot = slot_of(c, slots, b, there);
+  if (!there && t == 0) atomicOr(c.status, KV_ST_SLOT);
+  const int len = there ? held_tokens(c.lens[slot], c.max_pages) : 0;
   const long long s0 = start ? start[b] : (long long)len - n;
   const long long first = (s0 >= 0 ? s0 : s0 - (KV_PAGE - 1)) / KV_PAGE * KV_PAGE;  // of the window's first page
   const long long lo = first + (long long)part * KV_PAGE;

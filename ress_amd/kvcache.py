@@ -43,6 +43,7 @@ _STATUS = (
     (2, "a position lies outside the rotation table (it was clamped into it)"),
     (4, "a page number lies outside the pool (the table was changed from outside)"),
     (8, "a page holds a key or value that is not finite (queries that see it get NaN)"),
+    (16, "a slot lies outside the cache (a SlotBatch's tensor was changed, or freed under a recorded graph)"),
 )
 
 

@@ -176,3 +176,35 @@ def test_captured_padded_steps(dev):
         assert (out.double() - want.double()).abs().max() <= 2.0 ** -8 * want.double().abs().max().clamp(min=1)
         assert (out[0, :, m[0]:] == 0).all() and (out[1, :, m[1]:] == 0).all()
     c.check()
+
+
+@pytest.mark.parametrize("n", [1, 40, 100])
+@pytest.mark.parametrize("bad", [-1, 3, 1 << 30, -(1 << 31)])
+def test_slots_outside_the_cache(dev, n, bad):
+    """A batch whose numbers on the device are changed: such a row appends nothing and sees nothing, and is reported; the
+    other rows are as ever. (Lists are checked on the host.)"""
+    a, b = (_filled(dev, 2, 64, [100, 5000, 30]) for _ in range(2))
+    x, q = _rand((2, 2, n, 64), dev, 1), _rand((2, 4, n, 64), dev, 2)
+    batch = a.slots([0, 1])
+    for c in (a, b):
+        c.reserve(1, 5200)
+    batch.tensor[0] = bad
+
+    def reported():
+        with pytest.raises(RuntimeError, match="slot lies outside"):
+            a.check()
+        a.check()
+
+    a.append(x, x, slots=batch)
+    reported()
+    b.append(x[1:], x[1:], slots=[1])
+    assert a.lens.tolist() == b.lens.tolist() == [100, 5000 + n, 30]
+    got, want = a.attend(q, slots=batch, causal=True), b.attend(q, slots=[0, 1], causal=True)
+    reported()
+    assert (got[0] == 0).all() and torch.equal(got[1], want[1])
+    k, v = a.read(n, slots=batch)
+    reported()
+    assert (k[0] == 0).all() and (v[0] == 0).all() and torch.equal(k[1], b.read(n, slots=[1])[0][0])
+    for s in range(3):
+        for t, u in zip(held(a, s), held(b, s)):
+            assert torch.equal(t, u)
