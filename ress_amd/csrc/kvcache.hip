@@ -346,8 +346,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
   const int part = blockIdx.x % pages, h = blockIdx.x / pages % H, b = blockIdx.x / pages / H;
   bool there;
   const int slot = slot_of(c, slots, b, there);
-  if (!there && t == 0) atomicOr(c.status, KV_ST_SLOT);
-  const int len = there ? held_tokens(c.lens[slot], c.max_pages) : 0;
+  const int len = held_tokens(c.lens[slot], there ? c.max_pages : 0);
   const long long s0 = start ? start[b] : (long long)len - n;
   const long long first = (s0 >= 0 ? s0 : s0 - (KV_PAGE - 1)) / KV_PAGE * KV_PAGE;  // of the window's first page
   const long long lo = first + (long long)part * KV_PAGE;
@@ -414,6 +413,7 @@ __global__ __launch_bounds__(THREADS) void k_kv_read(ress_kv_cache c, const int*
     *reinterpret_cast<uint4*>(k_out + o) = kw;
     *reinterpret_cast<uint4*>(v_out + o) = vw;
   }
+  if (!there && t == 0) atomicOr(c.status, KV_ST_SLOT);  // at the end: it would hold up the loads
 }
 
 template <template <int, int, int> class Launch, class... A>
