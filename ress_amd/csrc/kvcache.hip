@@ -87,8 +87,8 @@ __device__ __forceinline__ uint32_t top_bits(const uint4& v, uint32_t m) {
 //
 // A page's tokens stay in registers between its maximum and its codes, so they are read once; a head's values are
 // transposed through LDS, in rows of 17 words, and leave as whole lines. Bound by memory where there is much to append
-// (8 sequences of up to 1,000 tokens, 24 heads of 64: 32 us for 110 MB, 3.4 TB/s), else by the chain length -> tokens ->
-// maximum -> codes -> length (1,374 tokens of 16 heads, 9.6 us for 14 MB; a token each of 32 sequences, 8 us): with
+// (8 sequences of up to 1,000 tokens, 24 heads of 64: 30 us for 110 MB, 3.6 TB/s), else by the chain length -> tokens ->
+// maximum -> codes -> length (1,374 tokens of 16 heads, 10 us for 14 MB; a token each of 32 sequences, 8 us): with
 // the first tokens on their way before the length is known and each sequence's counter on a line of its own it took
 // 66 -> 50 us of the first, its reading back included.
 template <int DT, int CODES, int D>
