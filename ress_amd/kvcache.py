@@ -21,7 +21,7 @@ lengths, as with counts on the device, it reads them first; after a captured app
 every argument that comes from the host (slots or new_lens as a list, pos on the CPU), whose copy waits: a
 decoding loop passes a SlotBatch and tensors on the device. Calls that change a cache (append, reserve, restore,
 release) must be ordered one after the other, as on one stream, and so must two captured graphs that append to
-one cache; attend and read only read it.
+one cache; attend and read only read it, and must be ordered with the calls that change the slots they read.
 
 The reference has no counterpart: it attends over all frames at once.
 """
