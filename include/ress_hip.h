@@ -364,6 +364,43 @@ int ress_int8_linear(const void* x, long long stride, int dtype, int M, int K, i
                      const float* w_scale, const float* bias, int act, void* out, long long out_stride,
                      void* workspace, long long workspace_bytes, hipStream_t stream);
 
+/* ---- attention with a backward pass (block_attn.hip) ----------------------- */
+/* A (B, heads, tokens, head_dim) operand of 16-bit elements in device memory: element strides, unit-stride dims; 16-byte aligned,
+ * strides multiples of 8, tokens at least head_dim elements and fewer than 2^24 apart. */
+typedef struct ress_strided {
+  void* data;
+  long long sb, sh, st;
+} ress_strided;
+
+/* out = softmax(scale q K^T) V. Query head h reads key/value head h / (q_heads / kv_heads). Row i of sequence b sees the keys
+ * below k_lens[b] (int32[B] in device memory, clamped to 0..Tk; null: Tk), causal = 1: of these the ones up to
+ * i + k_lens[b] - q_lens[b]; with a map (bytes in device memory, element strides map_s*, (B, q_heads, ceil(Tq / 128),
+ * ceil(Tk / 64)), at most 2^20 tokens): of these the ones in key blocks whose byte is not 0. Rows that see nothing, and those
+ * from q_lens[b] (clamped to 0..Tq; null: Tq) on, are zero. Elements past the lengths and in blocks that the map drops reach
+ * nothing, whatever they are. dtype 1 bf16, 2 fp16; head_dim 64 or 128; scale > 0. P is rounded to the 16-bit type, sums are fp32.
+ * For the backward pass: lse (B, q_heads, Tq) f32 receives log2 of the rows' sums of exp (+inf where there is none), rest
+ * (B, q_heads, Tq, head_dim) 16-bit, contiguous, what out's rounding took (both null: no backward pass). The reference has no
+ * counterpart: its kernels run without gradients. */
+typedef struct ress_block_attn {
+  ress_strided q, k, v, out;
+  int B, q_heads, kv_heads, Tq, Tk, head_dim, dtype, causal;
+  const int* q_lens;
+  const int* k_lens;
+  const void* map;
+  long long map_sb, map_sh, map_sq, map_sk;
+  float* lse;
+  void* rest;
+  float scale;
+} ress_block_attn;
+int ress_block_attn_fwd(const ress_block_attn* args, hipStream_t stream);
+/* The gradients dq, dk, dv of the same call (zero in rows past the lengths), from its out, rest and lse and the gradient of out.
+ * P and dS are rounded to the 16-bit type (fp16: dS scaled by a power of two that uses its range), sums are fp32 and of a
+ * fixed order. workspace: ress_block_attn_bwd_workspace_size bytes, 16-byte aligned. */
+long long ress_block_attn_bwd_workspace_size(const ress_block_attn* args);
+int ress_block_attn_bwd(const ress_block_attn* args, const ress_strided* grad_out, const ress_strided* dq,
+                        const ress_strided* dk, const ress_strided* dv, void* workspace, long long workspace_bytes,
+                        hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
