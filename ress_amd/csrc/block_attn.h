@@ -10,7 +10,7 @@ constexpr float LOWEST = -0x1.fffffep127f;
 // The running maximum moves when a score lies more than this above it (in log2): P stays below 2^8, and most steps need no
 // pass over the accumulators.
 constexpr float LAZY = 8.0f;
-constexpr int VTOP_ROWS = 1024;
+constexpr int VTOP_ROWS = 1024, DELTA_ROWS = 128;  // of a workgroup
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -52,6 +52,14 @@ struct AttnArgs {
 __device__ __forceinline__ constexpr float lift(int dt) { return dt == BA_F16 ? 14.0f : 0.0f; }
 constexpr int tile_bytes(int D) { return KB * D * 2; }
 
+// f(0), .., f(N - 1) with constant indexes, whatever the unroller decides: accumulator arrays stay in registers
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
 __device__ __forceinline__ v16f zero16() {
   v16f z;
 #pragma unroll
@@ -310,22 +318,16 @@ struct WalkColumn {
 // Every step: its tile has landed, the next one's DMAs go out into the other buffer (which all waves have left), compute.
 template <class W, class F, class C>
 __device__ __forceinline__ void run_steps(const W& walk, F fetch, C compute) {
-  int cur = walk.first();
+  int cur = walk.first(), buf = 0;
   if (cur < 0) return;
   fetch(0, cur);
-  for (;;) {
-    int nxt = walk.next(cur);
+  while (cur >= 0) {
+    const int nxt = walk.next(cur);
     step_barrier();
-    if (nxt >= 0) fetch(1, nxt);
-    compute(0, cur);
-    if (nxt < 0) return;
+    if (nxt >= 0) fetch(buf ^ 1, nxt);
+    compute(buf, cur);
     cur = nxt;
-    nxt = walk.next(cur);
-    step_barrier();
-    if (nxt >= 0) fetch(0, nxt);
-    compute(1, cur);
-    if (nxt < 0) return;
-    cur = nxt;
+    buf ^= 1;
   }
 }
 

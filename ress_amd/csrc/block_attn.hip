@@ -50,20 +50,23 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
       ks.fetch(lds[buf], kb * KB, hd.klen, w);
       vs.fetch(lds[buf] + tile_bytes(D), kb * KB, hd.klen, w);
     };
-    auto compute = [&](auto mask_tag, const uint8_t* tile, int kb) {
-      constexpr bool MASK = decltype(mask_tag)::value;
-      const int below = sees - kb * KB - 4 * ln.half;
+    run_steps(walk, fetch, [&](int buf, int kb) {
+      const uint8_t* tile = lds[buf];
       v16f s[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[t] = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
+      if (kb >= nfull) {
+        const int below = sees - kb * KB - 4 * ln.half;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[t][r] = 32 * t + c_row(r) < below ? s[t][r] : -__builtin_huge_valf();
+      }
       float top = LOWEST;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if constexpr (MASK) s[t][r] = 32 * t + c_row(r) < below ? s[t][r] : -__builtin_huge_valf();
-          top = fmaxf(top, s[t][r]);
-        }
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
       top = pair_max(top);
       top = top == LOWEST ? LOWEST : top * a.scale2;
       if (__any(top > m + LAZY)) {
@@ -83,7 +86,6 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           e[r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -m));
-          if constexpr (MASK) e[r] = 32 * t + c_row(r) < below ? e[r] : 0.0f;
           l += e[r];
         }
         pack16<DT>(e, p[t]);
@@ -92,10 +94,6 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int d = 0; d < D / 32; ++d) o[d] = columns_times<DT, D>(tile + tile_bytes(D), 32 * t, d, ln, p[t], o[d]);
-    };
-    run_steps(walk, fetch, [&](int buf, int kb) {
-      if (kb < nfull) compute(std::false_type{}, lds[buf], kb);
-      else compute(std::true_type{}, lds[buf], kb);
     });
   }
   l = pair_sum(l);
@@ -110,25 +108,19 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
 // -delta_i = -dO_i.(o_i + what o's rounding took), lse less the lift of P, and fp16: the largest finite |dO| of each
 // (sequence, key/value head). Bound by its bytes.
 template <int DT, int D>
-__global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, long long rows) {
+__global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, int chunks) {
   constexpr int LR = D / 8;
-  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) / LR;
-  const int piece = threadIdx.x % LR;
+  const int bh = blockIdx.x / chunks, b = bh / a.Hq, h = bh % a.Hq, piece = threadIdx.x % LR;
+  const int from = blockIdx.x % chunks * DELTA_ROWS, end = min(a.Tq, from + DELTA_ROWS), qlen = a.q_len(b);
   float top = 0.0f;
-  int bh = 0;
-  if (r < rows) {
-    const int i = (int)(r % a.Tq);
-    bh = (int)(r / a.Tq);
-    const int b = bh / a.Hq, h = bh % a.Hq;
+  for (int i = from + threadIdx.x / LR; i < end; i += 256 / LR) {  // a row's lanes go together
     float sum = 0.0f;
-    if (i < a.q_len(b)) {
-      const uint4 g = *reinterpret_cast<const uint4*>(a.go.at(b, h, i) + 8 * piece);
-      const uint4 o = *reinterpret_cast<const uint4*>(a.o.at(b, h, i) + 8 * piece);
-      const uint4 e = *reinterpret_cast<const uint4*>(a.rest + r * D + 8 * piece);
+    const long long r = (long long)bh * a.Tq + i;
+    if (i < qlen) {
       float x[8], y[8], z[8];
-      unpack8<DT>(g, x);
-      unpack8<DT>(o, y);
-      unpack8<DT>(e, z);
+      unpack8<DT>(*reinterpret_cast<const uint4*>(a.go.at(b, h, i) + 8 * piece), x);
+      unpack8<DT>(*reinterpret_cast<const uint4*>(a.o.at(b, h, i) + 8 * piece), y);
+      unpack8<DT>(*reinterpret_cast<const uint4*>(a.rest + r * D + 8 * piece), z);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         sum = fmaf(x[u], y[u] + z[u], sum);
@@ -137,15 +129,15 @@ __global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, long long 
       }
     }
 #pragma unroll
-    for (int s = 1; s < LR; s <<= 1) {
-      sum += __shfl_xor(sum, s, 64);
-      top = fmaxf(top, __shfl_xor(top, s, 64));
-    }
+    for (int s = 1; s < LR; s <<= 1) sum += __shfl_xor(sum, s, LR);
     if (piece == 0) {
       a.ndelta[r] = -sum;
       a.lse_b[r] = a.lse[r] - lift(DT);
-      if (DT == BA_F16 && top > 0.0f) atomicMax(a.top + (long long)b * a.Hk + h / a.G, __float_as_uint(top));
     }
+  }
+  if constexpr (DT == BA_F16) {
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0 && top > 0.0f) atomicMax(a.top + (long long)b * a.Hk + h / a.G, __float_as_uint(top));
   }
 }
 __global__ void k_block_attn_clear(uint32_t* p, int n) {
@@ -225,28 +217,24 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_dq(AttnArgs a) {
       ks.fetch(lds[buf], kb * KB, hd.klen, w);
       vs.fetch(lds[buf] + tile_bytes(D), kb * KB, hd.klen, w);
     };
-    auto compute = [&](auto mask_tag, const uint8_t* tile, int kb) {
-      constexpr bool MASK = decltype(mask_tag)::value;
-      const int below = sees - kb * KB - 4 * ln.half;
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
+    run_steps(walk, fetch, [&](int buf, int kb) {
+      const uint8_t* tile = lds[buf];
+      each<2>([&](auto t_) {
+        constexpr int t = decltype(t_)::value;
         const v16f s = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
         const v16f dp = rows_times<DT, D>(tile + tile_bytes(D), 32 * t, ln, g, ndelta);
         float e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse)) * dp[r];
-          if constexpr (MASK) e[r] = 32 * t + c_row(r) < below ? e[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse)) * dp[r];
+        if (kb >= nfull) {
+          const int below = sees - kb * KB - 4 * ln.half;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) e[r] = 32 * t + c_row(r) < below ? e[r] : 0.0f;
         }
         uint4 ds[2];
         pack16<DT>(e, ds);
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]);
-      }
-    };
-    run_steps(walk, fetch, [&](int buf, int kb) {
-      if (kb < nfull) compute(std::false_type{}, lds[buf], kb);
-      else compute(std::true_type{}, lds[buf], kb);
+        each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
+      });
     });
   }
   if (row < a.Tq) store_grad<DT, D>(a.dq, it.b, it.h, row, ln.half, dq, undo, row < qlen);
@@ -289,34 +277,40 @@ __global__ __launch_bounds__(64 * NW, 2) void k_block_attn_dkv(AttnArgs a) {
         if (w == 0) fetch_row_values(a.lse_b + rows + st * QS, qlen - st * QS, lds[buf] + 2 * T);
         if (w == 1) fetch_row_values(a.ndelta + rows + st * QS, qlen - st * QS, lds[buf] + 2 * T + 256);
       };
-      auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
-        constexpr bool MASK = decltype(mask_tag)::value;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
+      run_steps(walk, fetch, [&](int buf, int st) {
+        const uint8_t* tile = lds[buf];
+        each<2>([&](auto t_) {
+          constexpr int t = decltype(t_)::value;
           const v16f s = rows_times<DT, D>(tile, 32 * t, ln, k, zero16());
           const v16f lse = row_values(tile + 2 * T, 32 * t, ln);
-          const v16f dp = rows_times<DT, D>(tile + T, 32 * t, ln, v, row_values(tile + 2 * T + 256, 32 * t, ln));
-          float e[16], d[16];
+          float e[16];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse[r]));
-            if constexpr (MASK) e[r] = st * QS + 32 * t + c_row(r) >= first ? e[r] : 0.0f;
-            d[r] = e[r] * dp[r];
-            if constexpr (DT == BA_F16) d[r] *= fp;
+          for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse[r]));
+          if (st * QS < whole) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) e[r] = st * QS + 32 * t + c_row(r) >= first ? e[r] : 0.0f;
           }
           uint4 p[2], ds[2];
           pack16<DT>(e, p);
-          pack16<DT>(d, ds);
+#ifdef SB1
+          if (D == 128) __builtin_amdgcn_sched_barrier(0);
+#endif
+          const v16f dp = rows_times<DT, D>(tile + T, 32 * t, ln, v, row_values(tile + 2 * T + 256, 32 * t, ln));
+          each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + T, 32 * t, x, ln, p, dv[x]); });
+#ifdef SB3
+          if (D == 128) __builtin_amdgcn_sched_barrier(0);
+#endif
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            dv[x] = columns_times<DT, D>(tile + T, 32 * t, x, ln, p, dv[x]);
-            dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, ds, dk[x]);
+          for (int r = 0; r < 16; ++r) {
+            e[r] *= dp[r];
+            if constexpr (DT == BA_F16) e[r] *= fp;
           }
-        }
-      };
-      run_steps(walk, fetch, [&](int buf, int st) {
-        if (st * QS >= whole) compute(std::false_type{}, lds[buf], st);
-        else compute(std::true_type{}, lds[buf], st);
+          pack16<DT>(e, ds);
+          each<D / 32>([&](auto x) { dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, ds, dk[x]); });
+#ifdef SB2
+          __builtin_amdgcn_sched_barrier(0);
+#endif
+        });
       });
     }
   }
@@ -441,7 +435,8 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   unsigned qblocks = 0, kblocks = 0, dblocks = 0, vblocks = 0;
   if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256, name, &qblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hk * cdiv(a.Tk, keys), 2 * keys, name, &kblocks)) return rc;
-  if (int rc = grid((rows * (D / 8) + 255) / 256, 256, name, &dblocks)) return rc;
+  const int dchunks = cdiv(a.Tq, DELTA_ROWS);
+  if (int rc = grid((long long)a.B * a.Hq * dchunks, 256, name, &dblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hk * chunks, 256, name, &vblocks)) return rc;
   if (dtype == BA_F16 && a.Tk) {
     hipLaunchKernelGGL(k_block_attn_clear, dim3(cdiv(2 * a.B * a.Hk, 256)), dim3(256), 0, stream, a.top, 2 * a.B * a.Hk);
@@ -451,7 +446,7 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   }
   RESS_BA_EACH({
     if (a.Tq) {
-      hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3(dblocks), dim3(256), 0, stream, a, rows);
+      hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3((unsigned)((long long)a.B * a.Hq * dchunks)), dim3(256), 0, stream, a, dchunks);
       RESS_LAUNCHED("k_block_attn_delta");
       if (a.map) hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, true>), dim3(qblocks), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
       else hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, false>), dim3(qblocks), dim3(256), 0, stream, a);
