@@ -401,6 +401,56 @@ int ress_block_attn_bwd(const ress_block_attn* args, const ress_strided* grad_ou
                         const ress_strided* dk, const ress_strided* dv, void* workspace, long long workspace_bytes,
                         hipStream_t stream);
 
+/* ---- layer norm with a backward pass (layer_norm.hip) ----------------------- */
+/* Rows (i0, i1, i2) of unit-stride elements, element strides. */
+typedef struct ress_rows {
+  void* data;
+  long long s0, s1, s2;
+} ress_rows;
+
+/* h = x + gamma * branch (no branch: data null, h = x; gamma null: 1) rounded to the type, n = (h - mean) / sqrt(var + eps) * weight + bias
+ * (null: 1 and 0) over the C elements of each of n0 x n1 x n2 rows (fewer than 2^31), C up to 8192, statistics in fp32. dtype 0
+ * fp32, 1 bf16, 2 fp16; wide = 1: gamma, weight and bias are fp32, else of that type. sum receives h (with a branch), out n, both
+ * contiguous. mean, rstd (f32, a value a row) are kept for the backward pass (both null: none). The reference's norms are torch's. */
+typedef struct ress_layer_norm {
+  ress_rows x, branch;
+  int n0, n1, n2, C, dtype, wide;
+  const void* gamma;
+  const void* weight;
+  const void* bias;
+  void* sum;
+  void* out;
+  float* mean;
+  float* rstd;
+  float eps;
+} ress_layer_norm;
+int ress_layer_norm_fwd(const ress_layer_norm* args, hipStream_t stream);
+/* The gradients of the same call from those of n (grad_out) and of h (grad_sum; null: zero), args->x being h. dx (contiguous, that of x
+ * and of h), dbranch, dgamma, dweight, dbias (the weights' type): null where not wanted. Sums over rows are fp32 and of a fixed
+ * order. workspace: ress_layer_norm_bwd_workspace_size bytes, 16-byte aligned, where a weight's gradient is wanted. */
+long long ress_layer_norm_bwd_workspace_size(const ress_layer_norm* args);
+int ress_layer_norm_bwd(const ress_layer_norm* args, const ress_rows* grad_out, const ress_rows* grad_sum, void* dx,
+                        void* dbranch, void* dgamma, void* dweight, void* dbias, void* workspace, long long workspace_bytes,
+                        hipStream_t stream);
+
+/* ---- rotary positions (rotary.hip) ------------------------------------------ */
+/* y = x with pairs of dims turned by the rows of table (positions, 2, rotary_dim / axes / 2) f32, cosines before sines, that
+ * pos (int64, element strides: batch, token, axis) names, for one or two operands (second: data null) of Hs[i] heads. x and y (B, heads, n,
+ * head_dim), 16-bit elements (dtype 1 bf16, 2 fp16), element strides, unit-stride dims. Axis a turns dims a d .. a d + d - 1,
+ * d = rotary_dim / axes (even): interleaved = 0 pairs i and i + d / 2, 1 pairs 2 i and 2 i + 1; the other dims are copied. inverse = 1: turned
+ * the other way (the backward pass). Positions outside the table are clamped and OR 1 into status. head_dim up to 256, even. */
+typedef struct ress_rotary {
+  ress_strided x[2], y[2];
+  int heads[2];
+  int B, n, head_dim, dtype, axes, rotary_dim, interleaved, inverse;
+  const long long* pos;
+  long long pos_sb, pos_st, pos_sa;
+  const float* table;
+  int positions;
+  int* status;
+} ress_rotary;
+int ress_rotate(const ress_rotary* args, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

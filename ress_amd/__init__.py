@@ -14,7 +14,7 @@ The hot path runs on hand-written HIP kernels for gfx950 (libress_hip.so, built 
 from ress_amd.api import apply_dense, apply_hess, apply_ress, apply_sparse_vggt, load_backbone
 from ress_amd.attention import check_layers
 from ress_amd.backbones import BACKBONES, get_backbone
-from ress_amd.differentiable import block_attention
+from ress_amd.differentiable import add_layer_norm, block_attention, layer_norm, rotate
 from ress_amd.int8 import Int8Linear, int8_linear, quantize_linears
 from ress_amd.kvcache import PagedKVCache, RotaryTable
 from ress_amd.qkv import declare_rope
@@ -26,6 +26,7 @@ __all__ = [
     "Int8Linear",
     "PagedKVCache",
     "RotaryTable",
+    "add_layer_norm",
     "apply_dense",
     "apply_hess",
     "apply_ress",
@@ -35,6 +36,8 @@ __all__ = [
     "declare_rope",
     "get_backbone",
     "int8_linear",
+    "layer_norm",
     "load_backbone",
     "quantize_linears",
+    "rotate",
 ]

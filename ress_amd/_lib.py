@@ -41,6 +41,9 @@ _SIGS = {
     "ress_kv_attend": "p" + "plll" + "iii" + "pp" + "ifi" + "plll" + "pl" + "s",
     "ress_block_attn_fwd": "p" + "s",
     "ress_block_attn_bwd": "ppppp" + "pl" + "s",
+    "ress_layer_norm_fwd": "p" + "s",
+    "ress_layer_norm_bwd": "ppp" + "ppppp" + "pl" + "s",
+    "ress_rotate": "p" + "s",
 }
 _CT = {
     "p": ctypes.c_void_p,
@@ -82,6 +85,8 @@ def lib():
         L.ress_kv_attend_workspace_size.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
         L.ress_block_attn_bwd_workspace_size.restype = ctypes.c_longlong
         L.ress_block_attn_bwd_workspace_size.argtypes = [ctypes.c_void_p]
+        L.ress_layer_norm_bwd_workspace_size.restype = ctypes.c_longlong
+        L.ress_layer_norm_bwd_workspace_size.argtypes = [ctypes.c_void_p]
         L.ress_noalloc_scratch_bytes.restype = ctypes.c_longlong
         L.ress_noalloc_scratch_bytes.argtypes = []
         L.ress_noalloc_status_address.restype = ctypes.c_int
@@ -140,5 +145,5 @@ def exported_symbols():
                           "ress_attn_sched_bytes", "ress_restore_swap_workspace_size", "ress_meansim_workspace_size",
                           "ress_noalloc_scratch_bytes", "ress_kv_attend_workspace_size",
                           "ress_int8_linear_workspace_size", "ress_int8_linear_tile",
-                          "ress_block_attn_bwd_workspace_size",
+                          "ress_block_attn_bwd_workspace_size", "ress_layer_norm_bwd_workspace_size",
                           "ress_noalloc_status_address"]

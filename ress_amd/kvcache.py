@@ -60,38 +60,89 @@ class _CacheArgs(ctypes.Structure):
             "n_pages", "max_pages", "max_seqs", "kv_heads", "head_dim", "dtype", "codes")]
 
 
+LAYOUTS = ("half", "interleaved")
+
+
+def _scaled(inv, d, base, scaling):
+    """(frequencies, factor of cosines and sines) of a table for contexts longer than the trained ones."""
+    if scaling is None:
+        return inv, 1.0
+    kind, factor = scaling.get("type"), float(scaling.get("factor", 0.0))
+    known = {"linear": ("type", "factor"), "ntk": ("type", "factor"),
+             "yarn": ("type", "factor", "original", "fast", "slow", "attention")}.get(kind)
+    if known is None or not factor >= 1.0 or factor == math.inf or any(k not in known for k in scaling):
+        raise ValueError(f"scaling must be a dict of type linear, ntk or yarn and a factor of at least 1 "
+                         f"({', '.join(known or ('type', 'factor'))}), got {scaling}")
+    if kind == "linear":
+        return inv / factor, 1.0
+    if kind == "ntk":
+        if d < 4:
+            raise ValueError("ntk scaling needs at least four dims")
+        return (base * factor ** (d / (d - 2.0))) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d), 1.0
+    original, fast, slow = float(scaling.get("original", 0)), float(scaling.get("fast", 32.0)), float(scaling.get("slow", 1.0))
+    if not original >= 1 or not 0.0 <= slow < fast:
+        raise ValueError(f"yarn scaling needs `original` (the trained positions) and slow < fast, got {scaling}")
+    turns = original * inv / (2.0 * math.pi)
+    keep = ((turns - slow) / (fast - slow)).clamp(0.0, 1.0)
+    attention = scaling.get("attention")
+    return inv * keep + inv / factor * (1.0 - keep), 0.1 * math.log(factor) + 1.0 if attention is None else float(attention)
+
+
 class RotaryTable:
     """Cosines and sines of positions 0..positions-1, formed in 64 bits and rounded once, for
-    PagedKVCache.append. axes=1: the rotary embedding of a token's index over the whole head dim;
+    PagedKVCache.append and ress_amd.rotate. axes=1: the rotary embedding of a token's index over the whole head dim;
     axes=2: of a row and a column over its two halves (this package's RoPE2D). Dims i and i + d/2 of
-    an axis of d dims turn together by position * base^(-2i/d)."""
+    an axis of d dims turn together by position * base^(-2i/d).
 
-    def __init__(self, head_dim, positions, base=100.0, axes=2, device="cuda"):
-        d = self._check(head_dim, axes)
+    For rotate alone: layout="interleaved" turns dims 2i and 2i + 1 together; rotary_dim: only the head's first dims turn,
+    divided among the axes; scaling, for contexts longer than a model was trained on: {"type": "linear", "factor": f} divides
+    positions by f, "ntk" multiplies the base by f^(d/(d-2)), and "yarn" (with "original", the trained positions; Peng et al.,
+    2023) divides by f the frequencies of pairs that turn less than "slow" = 1 time over the trained positions, leaves those that turn
+    more than "fast" = 32 times, goes linearly between, and multiplies cosines and sines by "attention" = 0.1 ln f + 1."""
+
+    def __init__(self, head_dim, positions, base=100.0, axes=2, device="cuda", layout="half", rotary_dim=None, scaling=None):
+        d = self._check(head_dim, axes, layout, rotary_dim)
         if int(positions) < 1 or not float(base) > 1.0:
             raise ValueError(f"a rotation table needs at least one position and a base above 1, got {positions} and {base}")
         inv = float(base) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
+        inv, gain = _scaled(inv, d, float(base), scaling)
         ang = torch.arange(int(positions), dtype=torch.float64)[:, None] * inv
-        self.table = torch.stack([ang.cos(), ang.sin()], 1).float().to(device)
-        self.head_dim, self.axes = head_dim, axes
+        self._set(torch.stack([ang.cos() * gain, ang.sin() * gain], 1).float().to(device), head_dim, axes, layout, rotary_dim)
 
     @staticmethod
-    def _check(head_dim, axes):
+    def _check(head_dim, axes, layout="half", rotary_dim=None):
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
         if axes not in (1, 2):
             raise ValueError(f"axes must be 1 or 2, got {axes}")
-        return head_dim // axes
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+        dims = head_dim if rotary_dim is None else rotary_dim
+        if not 2 * axes <= dims <= head_dim or dims % (2 * axes):
+            raise ValueError(f"rotary_dim must be a multiple of {2 * axes} up to {head_dim}, got {rotary_dim}")
+        return dims // axes
+
+    def _set(self, table, head_dim, axes, layout, rotary_dim):
+        self.table, self.head_dim, self.axes, self.layout = table, head_dim, axes, layout
+        self.rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        with torch.inference_mode(False):
+            self.status = torch.zeros(1, dtype=torch.int32, device=table.device)
 
     @classmethod
-    def from_table(cls, table, head_dim, axes):
-        """From (positions, 2, head_dim / 2 / axes) fp32 cosines and sines on the device."""
-        d = cls._check(head_dim, axes)
+    def from_table(cls, table, head_dim, axes, layout="half", rotary_dim=None):
+        """From (positions, 2, rotary_dim / 2 / axes) fp32 cosines and sines on the device."""
+        d = cls._check(head_dim, axes, layout, rotary_dim)
         if table.dtype != torch.float32 or table.dim() != 3 or tuple(table.shape[1:]) != (2, d // 2) or not len(table):
             raise ValueError(f"table must be (positions, 2, {d // 2}) float32, got {tuple(table.shape)} {table.dtype}")
         self = cls.__new__(cls)
-        self.table, self.head_dim, self.axes = table.contiguous(), head_dim, axes
+        self._set(table.contiguous(), head_dim, axes, layout, rotary_dim)
         return self
+
+    def check(self):
+        """Raises if a rotate since the last check met a position outside the table (waits for the device)."""
+        if int(self.status.item()):
+            self.status.zero_()
+            raise RuntimeError("RotaryTable: a position lies outside the rotation table (it was clamped into it)")
 
 
 class SlotBatch:
@@ -414,6 +465,8 @@ class PagedKVCache:
             if rope.head_dim != self.head_dim or table.device != self.device:
                 raise ValueError(f"rope is for head_dim {rope.head_dim} on {table.device}, the cache has {self.head_dim} on {self.device}")
             want = ((B, n), (B, n, 1)) if axes == 1 else ((B, n, 2),)
+            if rope.layout != "half" or rope.rotary_dim != self.head_dim:
+                raise ValueError("append turns whole heads by halves; turn k and q by ress_amd.rotate for other tables")
             if pos.shape not in want or pos.is_floating_point():
                 raise ValueError(f"pos must be {want[0]} whole numbers, got {tuple(pos.shape)} {pos.dtype}")
             if pos.device != self.device:
