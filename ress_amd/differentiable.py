@@ -17,8 +17,9 @@ lives. Where that is an eager one of the default stream, capturing the backward 
 a leaf is refused inside a capture (delete the eager result first, or run it on a side stream).
 """
 
-import ctypes
+import functools
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -30,62 +31,11 @@ Q_BLOCK, K_BLOCK = 128, 64
 MOST_TOKENS, MOST_MAPPED = 1 << 26, 1 << 20
 MOST_STRIDE = 1 << 24
 
-
-class _Strided(ctypes.Structure):
-    """ress_strided of include/ress_hip.h."""
-
-    _fields_ = [("data", ctypes.c_void_p), ("sb", ctypes.c_longlong), ("sh", ctypes.c_longlong), ("st", ctypes.c_longlong)]
-
-
-class _Rows(ctypes.Structure):
-    """ress_rows."""
-
-    _fields_ = [("data", ctypes.c_void_p), ("s0", ctypes.c_longlong), ("s1", ctypes.c_longlong), ("s2", ctypes.c_longlong)]
-
-
-class _NormArgs(ctypes.Structure):
-    """ress_layer_norm."""
-
-    _fields_ = ([("x", _Rows), ("branch", _Rows)] + [(n, ctypes.c_int) for n in ("n0", "n1", "n2", "C", "dtype", "wide")]
-                + [(n, ctypes.c_void_p) for n in ("gamma", "weight", "bias", "sum", "out", "mean", "rstd")] + [("eps", ctypes.c_float)])
-
-
-class _RotaryArgs(ctypes.Structure):
-    """ress_rotary."""
-
-    _fields_ = ([("x", _Strided * 2), ("y", _Strided * 2), ("heads", ctypes.c_int * 2)]
-                + [(n, ctypes.c_int) for n in ("B", "n", "head_dim", "dtype", "axes", "rotary_dim", "interleaved", "inverse")]
-                + [("pos", ctypes.c_void_p), ("pos_sb", ctypes.c_longlong), ("pos_st", ctypes.c_longlong),
-                   ("pos_sa", ctypes.c_longlong), ("table", ctypes.c_void_p), ("positions", ctypes.c_int), ("status", ctypes.c_void_p)])
-
-
-class _AttnArgs(ctypes.Structure):
-    """ress_block_attn of include/ress_hip.h."""
-
-    _fields_ = ([(n, _Strided) for n in ("q", "k", "v", "out")]
-                + [(n, ctypes.c_int) for n in ("B", "q_heads", "kv_heads", "Tq", "Tk", "head_dim", "dtype", "causal")]
-                + [("q_lens", ctypes.c_void_p), ("k_lens", ctypes.c_void_p), ("map", ctypes.c_void_p)]
-                + [(n, ctypes.c_longlong) for n in ("map_sb", "map_sh", "map_sq", "map_sk")]
-                + [("lse", ctypes.c_void_p), ("rest", ctypes.c_void_p), ("scale", ctypes.c_float)])
-
-
-def _strides(t):
-    """Strides (batch, heads, tokens) that the kernels take of t (B, H, T, D), those of single entries in their place; None
-    where they do not."""
-    B, H, T, D = t.shape
-    sb, sh, st, sd = t.stride()
-    sb, sh, st = sb if B > 1 else 0, sh if H > 1 else 0, st if T > 1 else D
-    if sd != 1 or st < D or st >= MOST_STRIDE or (sb | sh | st) & 7 or t.data_ptr() & 15:
-        return None
-    return sb, sh, st
-
-
-def _ready(t):
-    return t if t.numel() == 0 or _strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
-
-
-def _strided(t):
-    return _Strided(t.data_ptr(), *(_strides(t) if t.numel() else (0, 0, t.shape[3])))
+# The argument structs of include/ress_hip.h, packed (a call's host time is what a small one costs).
+_STRIDED = struct.Struct("@4q").pack           # ress_strided, ress_rows: data and three strides
+_ATTN = struct.Struct("@16q8i3q4q2qf4x").pack   # ress_block_attn
+_NORM = struct.Struct("@8q6i7qf4x").pack        # ress_layer_norm
+_ROTARY = struct.Struct("@16q10i5qi4xq").pack   # ress_rotary
 
 
 def _capturing():
@@ -96,21 +46,68 @@ def _differentiates(*tensors):
     """Whether a call on these tensors makes a graph; refuses leaves whose gradients cannot be captured."""
     if not torch.is_grad_enabled():
         return False
-    leaves = [t for t in tensors if t is not None and t.requires_grad]
-    if not leaves:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            break
+    else:
         return False
-    capturing = _capturing()
-    if not capturing and _lib.stream_handle(leaves[0].device):
-        return True
-    for t in leaves:
-        if t.is_leaf:
-            seen = torch.autograd.graph.get_gradient_edge(t).node.metadata  # lives as long as a graph with the leaf
-            if not capturing:
-                seen["ress_default_stream"] = True
-            elif "ress_default_stream" in seen:
-                raise RuntimeError("inside a graph capture: a result of the same leaves from outside of it, on the default "
-                                   "stream, is still alive; delete it first")
+    if torch.cuda.is_current_stream_capturing():
+        for t in tensors:
+            if t is not None and t.requires_grad and t.is_leaf:
+                if "ress_default_stream" in torch.autograd.graph.get_gradient_edge(t).node.metadata:
+                    raise RuntimeError("inside a graph capture: a result of the same leaves from outside of it, on the "
+                                       "default stream, is still alive; delete it first")
     return True
+
+
+def _mark(result, device):
+    """Notes at the leaves of a graph that was made on the default stream that it was (the note lives as long as a graph
+    with the leaf does)."""
+    if not _lib.stream_handle(device):
+        for node, _ in result.grad_fn.next_functions:
+            if node is not None and node.name() == "torch::autograd::AccumulateGrad":
+                node.metadata["ress_default_stream"] = True
+
+
+def _first_derivative(function):
+    """A backward function that makes no graph of its own; torch's guard only where one is asked for."""
+    guarded = once_differentiable(function)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else function(ctx, *grads)
+    return staticmethod(backward)
+
+
+def _empty(t):
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+# ---- attention -------------------------------------------------------------------
+def _strides(t):
+    """(address, batch, heads, tokens) of t (B, H, T, D) as the kernels take it, strides of single entries in their place;
+    None where they cannot."""
+    B, H, T, D = t.shape
+    sb, sh, st, sd = t.stride()
+    if B == 1:
+        sb = 0
+    if H == 1:
+        sh = 0
+    if T == 1:
+        st = D
+    at = t.data_ptr()
+    if sd != 1 or st < D or st >= MOST_STRIDE or (sb | sh | st) & 7 or at & 15:
+        return None if t.numel() else (at, 0, 0, D)
+    return at, sb, sh, st
+
+
+def _ready(t):
+    return t if _strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
+
+
+def _like(t):
+    """A tensor for a result laid out like t where the kernels can write that."""
+    new = torch.empty_like(t)
+    return new if _strides(new) is not None else _empty(t)
 
 
 def _lens(lens, name, B, T, device):
@@ -128,25 +125,25 @@ def _lens(lens, name, B, T, device):
     return lens.contiguous()
 
 
-def _arguments(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest):
+def _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest):
     B, Hq, Tq, D = q.shape
-    P = _lib.ptr
-    ms = block_map.stride() if block_map is not None else (0, 0, 0, 0)
-    return _AttnArgs(_strided(q), _strided(k), _strided(v), _strided(out), B, Hq, k.shape[1], Tq, k.shape[2], D, DTYPES[q.dtype],
-                     1 if causal else 0, P(q_lens), P(k_lens), P(block_map), *ms, P(lse), P(rest), scale)
+    if block_map is None:
+        m = (0, 0, 0, 0, 0)
+    else:
+        m = (block_map.data_ptr(), *block_map.stride())
+    return _ATTN(*_strides(q), *_strides(k), *_strides(v), *_strides(out), B, Hq, k.shape[1], Tq, k.shape[2], D, DTYPES[q.dtype],
+                 1 if causal else 0, 0 if q_lens is None else q_lens.data_ptr(), 0 if k_lens is None else k_lens.data_ptr(), *m,
+                 0 if lse is None else lse.data_ptr(), 0 if rest is None else rest.data_ptr(), scale)
 
 
 def _attend(q, k, v, block_map, causal, q_lens, k_lens, scale, grads):
-    out = torch.empty_like(q)
-    if out.numel() and _strides(out) is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = _like(q)
     lse = rest = None
     if grads:
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        rest = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        rest = _empty(q)
     if out.numel():
-        args = _arguments(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
-        _lib.call_on(q.device, "ress_block_attn_fwd", ctypes.addressof(args))
+        _lib.call_on(q.device, "ress_block_attn_fwd", _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest))
     return out, lse, rest
 
 
@@ -159,22 +156,23 @@ class _BlockAttention(torch.autograd.Function):
         ctx.how = causal, scale
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, grad):
         q, k, v, out, lse, rest, block_map, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.how
         grad = _ready(grad)
-        grads = [torch.empty_like(t) for t in (q, k, v)]
-        grads = [t if t.numel() == 0 or _strides(t) is not None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                 for t in grads]
-        args = _arguments(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
-        size = _lib.lib().ress_block_attn_bwd_workspace_size(ctypes.addressof(args))
+        dq, dk, dv = _like(q), _like(k), _like(v)
+        args = _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
+        size = _attn_workspace(args[128:160])
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        g = [_strided(t) for t in (grad, *grads)]
-        _lib.call_on(q.device, "ress_block_attn_bwd", ctypes.addressof(args), *(ctypes.addressof(t) for t in g), _lib.ptr(work),
-                     size)
-        return (*grads, None, None, None, None, None)
+        _lib.call_on(q.device, "ress_block_attn_bwd", args, _STRIDED(*_strides(grad)), _STRIDED(*_strides(dq)),
+                     _STRIDED(*_strides(dk)), _STRIDED(*_strides(dv)), work.data_ptr(), size)
+        return dq, dk, dv, None, None, None, None, None
+
+
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(sizes):
+    return _lib.lib().ress_block_attn_bwd_workspace_size(bytes(128) + sizes + bytes(88))
 
 
 def _check_attention(q, k, v, block_map):
@@ -227,15 +225,19 @@ def block_attention(q, k, v, block_map=None, causal=False, q_lens=None, k_lens=N
     operands and output, a tensor of the output's size (what its rounding took) and 4 bytes a row."""
     _check_attention(q, k, v, block_map)
     B, Hq, Tq, D = q.shape
-    Tk = k.shape[2]
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    q_lens, k_lens = _lens(q_lens, "q_lens", B, Tq, q.device), _lens(k_lens, "k_lens", B, Tk, q.device)
+    if q_lens is not None:
+        q_lens = _lens(q_lens, "q_lens", B, Tq, q.device)
+    if k_lens is not None:
+        k_lens = _lens(k_lens, "k_lens", B, k.shape[2], q.device)
     if block_map is not None:
         block_map = block_map.expand(B, Hq, -1, -1)
     if _differentiates(q, k, v):
-        return _BlockAttention.apply(q, k, v, block_map, causal, q_lens, k_lens, scale)
+        out = _BlockAttention.apply(q, k, v, block_map, causal, q_lens, k_lens, scale)
+        _mark(out, q.device)
+        return out
     return _attend(_ready(q), _ready(k), _ready(v), block_map, causal, q_lens, k_lens, scale, False)[0]
 
 
@@ -244,101 +246,97 @@ NORM_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MOST_WIDTH, MOST_ROWS = 8192, (1 << 31) - 1
 
 
-def _rows_of(tensors):
-    """(n0, n1, n2, {id: strides}) of rows (..., C) of several tensors of one shape; the tensors themselves, copied where
-    their rows cannot be taken in place."""
-    shape = tensors[0].shape
+def _rows(tensors):
+    """((n0, n1, n2), operands): the rows (..., C) of tensors of one shape (None stays), each as (address, three strides, tensor);
+    those whose rows the kernels cannot take are copied."""
+    first = tensors[0]
+    C = first.shape[-1]
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            break
+    else:
+        return (first.numel() // C, 1, 1), [(0, 0, 0, 0, None) if t is None else (t.data_ptr(), C, 0, 0, t) for t in tensors]
+    shape = first.shape
     lead = [i for i in range(len(shape) - 1) if shape[i] > 1]
-    if all(t.is_contiguous() for t in tensors) or len(lead) > 3 or shape[-1] == 0:
-        tensors = [t.contiguous() for t in tensors]
-        rows = 1
-        for n in shape[:-1]:
-            rows *= n
-        return (rows, 1, 1), tensors, [(shape[-1], 0, 0)] * len(tensors)
-    tensors = [t if t.stride(-1) == 1 or shape[-1] == 1 else t.contiguous() for t in tensors]
-    pad = 3 - len(lead)
-    sizes = tuple([1] * pad + [shape[i] for i in lead])
-    return sizes, tensors, [tuple([0] * pad + [t.stride(i) for i in lead]) for t in tensors]
+    if len(lead) > 3:
+        return _rows([t if t is None else t.contiguous() for t in tensors])
+    tensors = [t if t is None or t.stride(-1) == 1 or C == 1 else t.contiguous() for t in tensors]
+    pad = [None] * (3 - len(lead))
+    axes = lead + pad if len(lead) == 1 else pad + lead  # one axis goes first: its rows are found without a division
 
+    def row(t):
+        return (0, 0, 0, 0, None) if t is None else (t.data_ptr(), *(0 if i is None else t.stride(i) for i in axes), t)
 
-def _norm_args(sizes, C, x, xs, branch, bs, gamma, weight, bias, total, out, mean, rstd, eps):
-    P = _lib.ptr
-    # the axis that varies fastest last; rows of one axis go first
-    if sizes[0] == 1 and sizes[1] == 1:
-        sizes, xs, bs = (sizes[2], 1, 1), (xs[2], 0, 0), (bs[2], 0, 0)
-    wide = any(w is not None and w.dtype is torch.float32 for w in (gamma, weight, bias))
-    return _NormArgs(_Rows(P(x), *xs), _Rows(P(branch), *bs), *sizes, C, NORM_DTYPES[x.dtype], 1 if wide else 0, P(gamma), P(weight),
-                     P(bias), P(total), P(out), P(mean), P(rstd), eps)
+    return tuple(1 if i is None else shape[i] for i in axes), [row(t) for t in tensors]
 
 
 def _normalise(x, branch, gamma, weight, bias, eps, grads):
-    """(sum or None, n, mean, rstd)"""
-    operands = [x] if branch is None else [x, branch]
-    sizes, operands, strides = _rows_of(operands)
-    C = x.shape[-1]
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if branch is not None else None
-    mean = rstd = None
-    if grads:
-        mean, rstd = torch.empty((2, sizes[0] * sizes[1] * sizes[2]), dtype=torch.float32, device=x.device)
+    """(sum or None, n, mean and rstd or None)"""
+    sizes, (xr, br) = _rows((x, branch))
+    out = _empty(x)
+    total = _empty(x) if branch is not None else None
+    stats = torch.empty((2, sizes[0] * sizes[1] * sizes[2]), dtype=torch.float32, device=x.device) if grads else None
     if out.numel():
-        args = _norm_args(sizes, C, operands[0], strides[0], operands[1] if branch is not None else None,
-                          strides[-1], gamma, weight, bias, total, out, mean, rstd, eps)
-        _lib.call_on(x.device, "ress_layer_norm_fwd", ctypes.addressof(args))
-    return total, out, mean, rstd
+        at = stats.data_ptr() if grads else 0
+        w = gamma if gamma is not None else weight if weight is not None else bias
+        args = _NORM(*xr[:4], *br[:4], *sizes, x.shape[-1], NORM_DTYPES[x.dtype],
+                     1 if w is not None and w.dtype is torch.float32 else 0, 0 if gamma is None else gamma.data_ptr(),
+                     0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                     0 if total is None else total.data_ptr(), out.data_ptr(), at, at + 2 * stats.numel() if grads else 0, eps)
+        _lib.call_on(x.device, "ress_layer_norm_fwd", args)
+    return total, out, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, branch, gamma, weight, bias, eps):
         ctx.set_materialize_grads(False)
-        total, out, mean, rstd = _normalise(x, branch, gamma, weight, bias, eps, True)
-        ctx.save_for_backward(x if branch is None else total, branch, gamma, weight, bias, mean, rstd)
+        total, out, stats = _normalise(x, branch, gamma, weight, bias, eps, True)
+        ctx.save_for_backward(x if branch is None else total, branch, gamma, weight, bias, stats)
         ctx.eps = eps
         return out if branch is None else (total, out)
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, *grads):
-        h, branch, gamma, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dh, dn = grads if branch is not None else (None, grads[0])
+        h, branch, gamma, weight, bias, stats = ctx.saved_tensors
+        to_x, to_branch, to_gamma, to_weight, to_bias, _ = ctx.needs_input_grad
+        dn = grads[-1]
+        dh = grads[0] if branch is not None else None
         if dh is None and dn is None:
-            return (None,) * 6
-
-        def make(like, wanted):
-            return torch.empty(like.shape, dtype=like.dtype, device=like.device) if wanted and like is not None else None
-
-        dx = make(h, need[0] or (need[1] and gamma is None))
-        dbranch = make(h, need[1] and gamma is not None)
-        dgamma, dweight, dbias = make(gamma, need[2]), make(weight, need[3]), make(bias, need[4])
-        ends = [t for t in (dgamma, dweight, dbias) if t is not None]
+            return None, None, None, None, None, None
+        dx = _empty(h) if to_x or (to_branch and gamma is None) else None
+        dbranch = _empty(h) if to_branch and gamma is not None else None
+        dgamma = _empty(gamma) if to_gamma else None
+        dweight = _empty(weight) if to_weight else None
+        dbias = _empty(bias) if to_bias else None
         if h.numel() == 0:
-            for t in ends:
-                t.zero_()
+            for t in (dgamma, dweight, dbias):
+                if t is not None:
+                    t.zero_()
         else:
-            given = [t for t in (h, branch, dh, dn) if t is not None]
-            sizes, given, strides = _rows_of(given)
-            at = dict(zip([n for n, t in (("h", h), ("branch", branch), ("dh", dh), ("dn", dn)) if t is not None],
-                          zip(given, strides)))
-            none = (None, (0, 0, 0))
-            x_, xs = at["h"]
-            b_, bs = at.get("branch", none)
-            args = _norm_args(sizes, h.shape[-1], x_, xs, b_, bs, gamma, weight, bias, None, None, mean, rstd, ctx.eps)
-            one = sizes[0] == 1 and sizes[1] == 1
-
-            def rows(name):
-                t, s = at.get(name, none)
-                return ctypes.byref(_Rows(t.data_ptr(), *((s[2], 0, 0) if one else s))) if t is not None else None
-
-            size = _lib.lib().ress_layer_norm_bwd_workspace_size(ctypes.addressof(args)) if ends else 0
-            work = torch.empty(size, dtype=torch.uint8, device=h.device) if size else None
-            P = _lib.ptr
-            _lib.call_on(h.device, "ress_layer_norm_bwd", ctypes.addressof(args), rows("dn"), rows("dh"), P(dx), P(dbranch),
-                         P(dgamma), P(dweight), P(dbias), P(work), size)
-        if need[1] and gamma is None:
+            sizes, (hr, br, nr, sr) = _rows((h, branch, dn, dh))
+            w = gamma if gamma is not None else weight if weight is not None else bias
+            at = stats.data_ptr()
+            args = _NORM(*hr[:4], *br[:4], *sizes, h.shape[-1], NORM_DTYPES[h.dtype],
+                         1 if w is not None and w.dtype is torch.float32 else 0, 0 if gamma is None else gamma.data_ptr(),
+                         0 if weight is None else weight.data_ptr(), 0, 0, 0, at, at + 2 * stats.numel(), ctx.eps)
+            size, work = 0, None
+            if to_gamma or to_weight or to_bias:
+                size = _norm_workspace(args[64:88])
+                work = torch.empty(size, dtype=torch.uint8, device=h.device)
+            _lib.call_on(h.device, "ress_layer_norm_bwd", args, None if dn is None else _STRIDED(*nr[:4]),
+                         None if dh is None else _STRIDED(*sr[:4]), None if dx is None else dx.data_ptr(),
+                         None if dbranch is None else dbranch.data_ptr(), None if dgamma is None else dgamma.data_ptr(),
+                         None if dweight is None else dweight.data_ptr(), None if dbias is None else dbias.data_ptr(),
+                         None if work is None else work.data_ptr(), size)
+        if to_branch and gamma is None:
             dbranch = dx
-        return dx if need[0] else None, dbranch, dgamma, dweight, dbias, None
+        return dx if to_x else None, dbranch, dgamma, dweight, dbias, None
+
+
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(sizes):
+    return _lib.lib().ress_layer_norm_bwd_workspace_size(bytes(64) + sizes + bytes(64))
 
 
 def _check_norm(x, branch, gamma, weight, bias, eps):
@@ -370,9 +368,14 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     kept for the backward pass (8 bytes a row), and sums are fp32; the result is contiguous."""
     eps = float(eps)
     _check_norm(x, None, None, weight, bias, eps)
-    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
     if _differentiates(x, weight, bias):
-        return _LayerNorm.apply(x, None, None, weight, bias, eps)
+        n = _LayerNorm.apply(x, None, None, weight, bias, eps)
+        _mark(n, x.device)
+        return n
     return _normalise(x, None, None, weight, bias, eps, False)[1]
 
 
@@ -384,31 +387,32 @@ def add_layer_norm(x, branch, gamma=None, weight=None, bias=None, eps=1e-5):
     if branch is None:
         raise ValueError("branch is missing (layer_norm takes x alone)")
     _check_norm(x, branch, gamma, weight, bias, eps)
-    gamma, weight, bias = (t if t is None else t.contiguous() for t in (gamma, weight, bias))
+    gamma, weight, bias = (t if t is None or t.is_contiguous() else t.contiguous() for t in (gamma, weight, bias))
     if _differentiates(x, branch, gamma, weight, bias):
-        return _LayerNorm.apply(x, branch, gamma, weight, bias, eps)
+        both = _LayerNorm.apply(x, branch, gamma, weight, bias, eps)
+        _mark(both[0], x.device)
+        return both
     return _normalise(x, branch, gamma, weight, bias, eps, False)[:2]
 
 
 # ---- rotary positions ------------------------------------------------------------
 def _turn(xs, pos, rope, inverse):
     """The operands turned (one or two), each in a tensor laid out like it."""
-    ys = []
-    for x in xs:
-        y = torch.empty_like(x)
-        ys.append(y if y.stride(3) == 1 or y.numel() == 0 else torch.empty(x.shape, dtype=x.dtype, device=x.device))
-    B, _, n, D = xs[0].shape
-    if n and B and any(x.shape[1] for x in xs):
-        xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
-
-        def two(ts):
-            return (_Strided * 2)(*(_Strided(t.data_ptr(), *t.stride()[:3]) for t in ts))
-
-        args = _RotaryArgs(two(xs), two(ys), (ctypes.c_int * 2)(*(x.shape[1] for x in xs)), B, n, D, DTYPES[xs[0].dtype], rope.axes,
-                           rope.rotary_dim, 1 if rope.layout == "interleaved" else 0, 1 if inverse else 0, pos.data_ptr(),
-                           pos.stride(0), pos.stride(1), pos.stride(2), rope.table.data_ptr(), rope.table.shape[0],
-                           rope.status.data_ptr())
-        _lib.call_on(xs[0].device, "ress_rotate", ctypes.addressof(args))
+    xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
+    ys = [torch.empty_like(x) for x in xs]
+    ys = [y if y.stride(3) == 1 else _empty(y) for y in ys]
+    x, y = xs[0], ys[0]
+    B, H, n, D = x.shape
+    if n and B:
+        x2 = y2 = (0, 0, 0, 0)
+        H2 = 0
+        if len(xs) > 1:
+            x2, y2 = (xs[1].data_ptr(), *xs[1].stride()[:3]), (ys[1].data_ptr(), *ys[1].stride()[:3])
+            H2 = xs[1].shape[1]
+        args = _ROTARY(x.data_ptr(), *x.stride()[:3], *x2, y.data_ptr(), *y.stride()[:3], *y2, H, H2, B, n, D, DTYPES[x.dtype],
+                       rope.axes, rope.rotary_dim, 1 if rope.layout == "interleaved" else 0, 1 if inverse else 0, pos.data_ptr(),
+                       *pos.stride(), rope.table.data_ptr(), rope.table.shape[0], rope.status.data_ptr())
+        _lib.call_on(x.device, "ress_rotate", args)
     return ys
 
 
@@ -417,11 +421,10 @@ class _Rotate(torch.autograd.Function):
     def forward(ctx, pos, rope, *xs):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(pos)
-        ctx.rope, ctx.like = rope, [(x.shape, x.dtype) for x in xs]
+        ctx.rope = rope
         return tuple(_turn(xs, pos, rope, False))
 
-    @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, *grads):
         pos, = ctx.saved_tensors
         at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[2 + i]]
@@ -463,6 +466,7 @@ def rotate(x, pos, rope):
     pos = pos if pos.dim() == 3 else pos[None].expand(B, -1, -1)
     if _differentiates(*xs):
         ys = _Rotate.apply(pos, rope, *xs)
+        _mark(ys[0], first.device)
     else:
         ys = _turn(xs, pos, rope, False)
     return ys[0] if torch.is_tensor(x) else tuple(ys)
