@@ -379,8 +379,8 @@ typedef struct ress_strided {
  * from q_lens[b] (clamped to 0..Tq; null: Tq) on, are zero. Elements past the lengths and in blocks that the map drops reach
  * nothing, whatever they are. dtype 1 bf16, 2 fp16; head_dim 64 or 128; scale > 0. P is rounded to the 16-bit type, sums are fp32.
  * For the backward pass: lse (B, q_heads, Tq) f32 receives log2 of the rows' sums of exp (+inf where there is none), rest
- * (B, q_heads, Tq, head_dim) 16-bit, contiguous, what out's rounding took (both null: no backward pass). The reference has no
- * counterpart: its kernels run without gradients. */
+ * (B, q_heads, Tq, head_dim) 16-bit, contiguous, what out's rounding took (both null: no backward pass). workspace: ress_block_attn_fwd_workspace_size
+ * bytes, 16-byte aligned (may be 0 bytes; parts of calls with few rows). The reference has no counterpart: its kernels run without gradients. */
 typedef struct ress_block_attn {
   ress_strided q, k, v, out;
   int B, q_heads, kv_heads, Tq, Tk, head_dim, dtype, causal;
@@ -392,7 +392,8 @@ typedef struct ress_block_attn {
   void* rest;
   float scale;
 } ress_block_attn;
-int ress_block_attn_fwd(const ress_block_attn* args, hipStream_t stream);
+long long ress_block_attn_fwd_workspace_size(const ress_block_attn* args);
+int ress_block_attn_fwd(const ress_block_attn* args, void* workspace, long long workspace_bytes, hipStream_t stream);
 /* The gradients dq, dk, dv of the same call (zero in rows past the lengths), from its out, rest and lse and the gradient of out.
  * P and dS are rounded to the 16-bit type (fp16: dS scaled by a power of two that uses its range), sums are fp32 and of a
  * fixed order. workspace: ress_block_attn_bwd_workspace_size bytes, 16-byte aligned. */

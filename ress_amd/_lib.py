@@ -39,7 +39,7 @@ _SIGS = {
     "ress_kv_append": "p" + "plll" * 3 + "iii" + "ppii" + "ppp" + "s",
     "ress_kv_read": "pii" + "pp" + "pp" + "s",
     "ress_kv_attend": "p" + "plll" + "iii" + "pp" + "ifi" + "plll" + "pl" + "s",
-    "ress_block_attn_fwd": "p" + "s",
+    "ress_block_attn_fwd": "p" + "pl" + "s",
     "ress_block_attn_bwd": "ppppp" + "pl" + "s",
     "ress_layer_norm_fwd": "p" + "s",
     "ress_layer_norm_bwd": "ppp" + "ppppp" + "pl" + "s",
@@ -83,6 +83,8 @@ def lib():
         L.ress_int8_linear_tile.argtypes = [ctypes.c_int] * 3
         L.ress_kv_attend_workspace_size.restype = ctypes.c_longlong
         L.ress_kv_attend_workspace_size.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4
+        L.ress_block_attn_fwd_workspace_size.restype = ctypes.c_longlong
+        L.ress_block_attn_fwd_workspace_size.argtypes = [ctypes.c_void_p]
         L.ress_block_attn_bwd_workspace_size.restype = ctypes.c_longlong
         L.ress_block_attn_bwd_workspace_size.argtypes = [ctypes.c_void_p]
         L.ress_layer_norm_bwd_workspace_size.restype = ctypes.c_longlong
@@ -145,5 +147,5 @@ def exported_symbols():
                           "ress_attn_sched_bytes", "ress_restore_swap_workspace_size", "ress_meansim_workspace_size",
                           "ress_noalloc_scratch_bytes", "ress_kv_attend_workspace_size",
                           "ress_int8_linear_workspace_size", "ress_int8_linear_tile",
-                          "ress_block_attn_bwd_workspace_size", "ress_layer_norm_bwd_workspace_size",
+                          "ress_block_attn_fwd_workspace_size", "ress_block_attn_bwd_workspace_size", "ress_layer_norm_bwd_workspace_size",
                           "ress_noalloc_status_address"]

@@ -4,13 +4,16 @@
 
 namespace {
 
-constexpr int QB = 128, KB = 64, QS = 64;  // the map's query and key blocks; queries of a step of dK and dV
+constexpr int QB = 128, KB = 64;  // the map's query and key blocks
+// Rows of a streamed tile: 8 KB of an operand, in tiles of 32 for the matrix cores
+constexpr int step_rows(int D) { return 4096 / D; }
+constexpr int TILE = 8192;
 constexpr int BA_BF16 = 1, BA_F16 = 2;
 constexpr float LOWEST = -0x1.fffffep127f;
 // The running maximum moves when a score lies more than this above it (in log2): P stays below 2^8, and most steps need no
 // pass over the accumulators.
 constexpr float LAZY = 8.0f;
-constexpr int VTOP_ROWS = 1024, DELTA_ROWS = 128;  // of a workgroup
+constexpr int VTOP_ROWS = 128, DELTA_ROWS = 128;  // of a workgroup
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -39,6 +42,10 @@ struct AttnArgs {
   float scale, scale2;       // scale2 = scale log2(e)
   uint16_t* rest;            // (B, Hq, Tq, D): what o's rounding took
   float *lse, *lse_b, *ndelta;  // (B, Hq, Tq); log2
+  // A tile's steps cut into parts (where the tiles are few), a workgroup each: grid.y. Parts of rows (o or dq, and lse) or of
+  // keys (dk, dv): [part][rows][D], [part][rows]
+  int parts;
+  float *part, *part2;
   uint32_t* top;             // fp16: (B, Hk) largest |dO|, (B, Hk) largest |v|, as bits
   __device__ __forceinline__ int q_len(int b) const { return q_lens ? min(max(q_lens[b], 0), Tq) : Tq; }
   __device__ __forceinline__ int k_len(int b) const { return k_lens ? min(max(k_lens[b], 0), Tk) : Tk; }
@@ -50,7 +57,6 @@ struct AttnArgs {
 
 // P's lift in the backward pass (log2): fp16 holds 2^-28 of a row's weight with all its bits
 __device__ __forceinline__ constexpr float lift(int dt) { return dt == BA_F16 ? 14.0f : 0.0f; }
-constexpr int tile_bytes(int D) { return KB * D * 2; }
 
 // f(0), .., f(N - 1) with constant indexes, whatever the unroller decides: accumulator arrays stay in registers
 template <int N, class F>
@@ -97,31 +103,64 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = unpack1<DT>(u[i >> 1], i & 1);
 }
+__device__ __forceinline__ float sum16(const float (&e)[16]) {
+  float s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+// sum + the eight 16-bit values of w
+template <int DT>
+__device__ __forceinline__ float add8(const uint4& w, float sum) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == BA_BF16) {
+      const v2bf ones = {(__bf16)1.0f, (__bf16)1.0f};
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, u[i]), ones, sum, false);
+    } else {
+      const v2h ones = {(_Float16)1.0f, (_Float16)1.0f};
+      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, u[i]), ones, sum, false);
+    }
+  }
+  return sum;
+}
 __device__ __forceinline__ float pair_max(float x) { return fmaxf(x, xor_lane_f<32>(x)); }
 __device__ __forceinline__ float pair_sum(float x) { return x + xor_lane_f<32>(x); }
 
 // Register r of a 32x32 result: row c_row(r) + 4 half
 __device__ __forceinline__ constexpr int c_row(int r) { return (r & 3) + 8 * (r >> 2); }
 
-// LDS tiles: 64 rows of D elements, a row's 16-byte chunks at chunk ^ f(row) (of 128 bytes),
-// f(row) = 2 (row & 3) | (row >> 2 & 1): eight rows' reads of one chunk meet eight different 16-byte banks, and so do the
-// four rows of two chunks that a 16-lane transposed read takes.
+// LDS tiles: rows of D elements, a row's 16-byte chunks at chunk ^ f(row). f takes the row's bits 1, 2, 3 (D = 128: 0 to 3) from
+// the chunk's highest bit down: 16 rows' reads of one chunk meet 16 different places of the 256 bytes that the banks
+// hold, and so do the four rows of four chunks that 32 lanes of a transposed read take. (With f of three bits alone, row reads
+// met a bank twice: 40% of the LDS' cycles.)
+template <int D>
+__device__ __forceinline__ int swizzle(int row) {
+  const int f = (row & 2) << 1 | (row >> 1 & 2) | (row >> 3 & 1);
+  return D == 128 ? f | (row & 1) << 3 : f;
+}
 template <int D>
 struct Lane {
   int wave, c32, half;
-  int row_off[4];  // of chunk 2 s + half of row c32, s = 0..3 (s + 4: 128 bytes on)
-  int col_off[2];  // of the lane's 8 bytes of a transposed read, dims 32 d.., d = 0, 1 (d + 2: 128 bytes on)
+  int row_at;  // of chunk `half` of row c32: chunk 2 s + half is at row_at ^ 32 s
+  int col_at;  // of the lane's 8 bytes of a transposed read of dims 0.. of rows 0..: dims 32 d.. at col_at ^ 64 d, rows 8.. at
+               // (col_at ^ 16) + 8 rows
   __device__ __forceinline__ Lane() {
     const int l = threadIdx.x & 63, i = l & 15;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     c32 = l & 31;
     half = l >> 5;
-    const int fr = (l & 3) << 1 | (l >> 2 & 1), fc = (i >> 2) << 1 | half;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) row_off[s] = c32 * 2 * D + (((2 * s + half) ^ fr) << 4);
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-      col_off[d] = (4 * half + (i >> 2)) * 2 * D + (((4 * d + 2 * (l >> 4 & 1) + (i >> 1 & 1)) ^ fc) << 4) + 8 * (i & 1);
+    row_at = c32 * 2 * D + ((half ^ swizzle<D>(c32)) << 4);
+    const int r = 4 * half + (i >> 2);
+    col_at = r * 2 * D + (((2 * (l >> 4 & 1) + (i >> 1 & 1)) ^ swizzle<D>(r)) << 4) + 8 * (i & 1);
+  }
+  // The same, opaque to the compiler: the places derived from it are formed where they are used and not held in
+  // registers through a loop that has none to spare.
+  __device__ __forceinline__ Lane anew() const {
+    Lane x = *this;
+    asm volatile("" : "+v"(x.row_at), "+v"(x.col_at));
+    return x;
   }
 };
 
@@ -131,7 +170,7 @@ __device__ __forceinline__ v16f rows_times(const uint8_t* tile, int row0, const 
                                            v16f acc) {
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
-    const uint4 x = *reinterpret_cast<const uint4*>(tile + row0 * 2 * D + ln.row_off[s & 3] + (s >> 2) * 128);
+    const uint4 x = *reinterpret_cast<const uint4*>(tile + row0 * 2 * D + (ln.row_at ^ 32 * s));
     acc = mfma<DT>(x, b[s], acc);
   }
   return acc;
@@ -146,8 +185,8 @@ __device__ __forceinline__ v16f columns_times(const uint8_t* tile, int row0, int
                                               v16f acc) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const uint8_t* p = tile + (row0 + 16 * s) * 2 * D + ln.col_off[d & 1] + (d >> 1) * 128;
-    const uint2 lo = read_tr(p), hi = read_tr(p + 8 * 2 * D);
+    const uint8_t* p = tile + (row0 + 16 * s) * 2 * D;
+    const uint2 lo = read_tr(p + (ln.col_at ^ 64 * d)), hi = read_tr(p + 8 * 2 * D + (ln.col_at ^ 64 * d ^ 16));
     acc = mfma<DT>(make_uint4(lo.x, lo.y, hi.x, hi.y), b[s], acc);
   }
   return acc;
@@ -180,36 +219,40 @@ __device__ __forceinline__ void dma4(const v4i& rsrc, unsigned off, unsigned lds
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(rsrc)
                : "memory", "m0");
 }
-// every DMA of the wave has landed and its LDS reads are done, then the workgroup's
+// all but the wave's newest N DMAs have landed and its LDS reads are done, then the workgroup's
+template <int N>
 __device__ __forceinline__ void step_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
-// Tiles of 64 rows of a (sequence, head), filled by the workgroup's waves: 1 KB a DMA. Rows past `len` are zero.
-template <int D>
+// Tiles of ROWS rows of a (sequence, head), filled by the workgroup's NW waves: 1 KB a DMA. Rows past `len` are zero.
+template <int D, int NW, int ROWS = step_rows(D)>
 struct Stream {
-  static constexpr int RPD = 512 / D, ND = 64 / RPD;  // rows of a DMA, DMAs of a tile
+  static constexpr int RPD = 512 / D, DMAS = ROWS / RPD / NW;  // rows of a DMA, DMAs of a wave
+  static_assert(NW * RPD % 16 == 0, "a wave's DMAs go to rows of one swizzle");
   const uint16_t* base;
-  unsigned stride, lane_off;  // bytes
-  int nw;
-  __device__ __forceinline__ Stream(const View& x, const uint16_t* head, const Lane<D>& ln, int nw_) : base(head), nw(nw_) {
-    const int l = threadIdx.x & 63, r = l / (D / 8), slot = l % (D / 8);
-    const int row = D == 64 ? r : 4 * (ln.wave & 1) + r;  // & 7; a wave's DMAs are all even or all odd
+  unsigned stride, off;  // bytes
+  __device__ __forceinline__ Stream(const View& x, const uint16_t* head, const Lane<D>& ln) : base(head) {
+    const int l = threadIdx.x & 63, slot = l % (D / 8), row = ln.wave * RPD + l / (D / 8);
     stride = (unsigned)(2 * x.t);
-    lane_off = r * stride + ((slot ^ ((row & 3) << 1 | (row >> 2 & 1))) << 4);
+    off = row * stride + ((slot ^ swizzle<D>(row)) << 4);
   }
-  __device__ __forceinline__ void fetch(const uint8_t* lds, int row0, int len, int w) const {
-    const int rows = min(64, len - row0);
+  // lds: the tile's address
+  __device__ __forceinline__ void fetch(unsigned lds, int row0, int len, int w) const {
+    const int rows = min(ROWS, len - row0);
     const v4i rs = descriptor(reinterpret_cast<const char*>(base) + (long long)row0 * stride, (rows - 1) * stride + 2 * D);
-    const unsigned at = lds_address(lds);
-    for (int n = w; n < ND; n += nw) dma16(rs, lane_off + n * RPD * stride, at + n * 1024);
+    unsigned at = off;
+    asm volatile("" : "+v"(at));  // sums formed here, not held in registers through the loop
+    // the rows go into the offset that is checked, not into the scalar one
+#pragma unroll
+    for (int n = 0; n < DMAS; ++n) dma16(rs, at + n * NW * RPD * stride, lds + (n * NW + w) * 1024);
   }
 };
-// 64 values, one for each row of a tile (zero past `left`)
-__device__ __forceinline__ void fetch_row_values(const float* src, int left, const uint8_t* lds) {
-  dma4(descriptor(src, 4 * min(64, left)), 4 * (threadIdx.x & 63), lds_address(lds));
+// 64 values (zero past `left`)
+__device__ __forceinline__ void fetch_row_values(const float* src, int left, unsigned lds) {
+  dma4(descriptor(src, 4 * min(64, left)), 4 * (threadIdx.x & 63), lds);
 }
 template <int D>
 __device__ __forceinline__ v16f row_values(const uint8_t* lds, int row0, const Lane<D>& ln) {
@@ -224,27 +267,39 @@ __device__ __forceinline__ v16f row_values(const uint8_t* lds, int row0, const L
 }
 
 // ---- work -----------------------------------------------------------------------
-// A workgroup's tile. An XCD (workgroup i runs on XCD i % 8) takes consecutive tiles, so that a head's keys and values, or
-// its queries, are read through few L2s. Causal: query tiles from the last one on, which see most.
+// A workgroup's tile. Workgroup i runs on XCD i % 8: whole heads go to the XCDs in turn (their lengths differ by sequence, and
+// a head's tiles read the same keys), what eight do not divide in eight runs of tiles. Causal: the tiles that see most first.
 struct Item {
   int b, h, tile;
-  __device__ __forceinline__ bool place(const AttnArgs& a, int heads, int tiles) {
-    const long long total = (long long)a.B * heads * tiles, per = (total + 7) / 8;
-    const long long lin = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((blockIdx.x >> 3) >= per || lin >= total) return false;
-    const int bh = (int)(lin / tiles);
-    tile = (int)(lin % tiles);
-    b = bh / heads;
-    h = bh % heads;
+  __device__ __forceinline__ bool place(const AttnArgs& a, int heads, int tiles, bool by_tile) {
+    const int all = a.B * heads, x = blockIdx.x & 7, i = blockIdx.x >> 3, even = all / 8;
+    int bh;
+    if (i < even * tiles) {
+      bh = (by_tile ? i % even : i / tiles) * 8 + x;
+      tile = by_tile ? i / even : i % tiles;
+    } else {
+      const int left = (all - 8 * even) * tiles, per = (left + 7) / 8, j = i - even * tiles;
+      const int lin = x * per + j;
+      if (j >= per || lin >= left) return false;
+      bh = 8 * even + lin / tiles;
+      tile = lin % tiles;
+    }
+    // divisions go through vector registers; what follows from these must not
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    bh = __builtin_amdgcn_readfirstlane(bh);
+    b = __builtin_amdgcn_readfirstlane(bh / heads);
+    h = bh - b * heads;
     return true;
   }
   __device__ __forceinline__ bool query_tile(const AttnArgs& a) {
     const int tiles = cdiv(a.Tq, QB);
-    if (!place(a, a.Hq, tiles)) return false;
+    if (!place(a, a.Hq, tiles, a.causal)) return false;
     if (a.causal) tile = tiles - 1 - tile;
     return true;
   }
-  __device__ __forceinline__ bool key_tile(const AttnArgs& a, int keys) { return place(a, a.Hk, cdiv(a.Tk, keys)); }
+  __device__ __forceinline__ bool key_tile(const AttnArgs& a, int keys) {
+    return place(a, a.Hk, cdiv(a.Tk, keys), a.causal);
+  }
 };
 struct Head {
   int b, h, klen;
@@ -279,57 +334,68 @@ struct Bits {
     return -1;
   }
 };
-// The key blocks 0..n-1 that a query tile goes through
-template <bool MAP>
+// The steps start..n-1 that a workgroup goes through; with a map, PER of them to an entry of its line
+template <bool MAP, int PER>
 struct Walk {
   Bits bits;
-  int n;
-  __device__ __forceinline__ Walk(const AttnArgs& a, const Item& it, int n_, uint32_t* lds) : n(n_) {
-    if constexpr (MAP) bits.fill(a.map + it.b * a.mb + it.h * a.mh + it.tile * a.mq, a.mk, n, lds);
-  }
-  __device__ __forceinline__ int first() const { return next(-1); }
-  __device__ __forceinline__ int next(int i) const {
-    if constexpr (MAP) return bits.from(i + 1);
-    else return i + 1 < n ? i + 1 : -1;
-  }
-};
-// The steps of 64 queries from `start` to n-1 that key block `col` goes through
-template <bool MAP>
-struct WalkColumn {
-  Bits bits;
   int start, n;
-  __device__ __forceinline__ WalkColumn(const AttnArgs& a, int b, int h, int col, int start_, int n_, uint32_t* lds, bool again)
+  // line[i step]: the entry of steps PER i..; again: the walk before may still be in use
+  __device__ __forceinline__ Walk(const uint8_t* line, long long step, int start_, int n_, uint32_t* lds, bool again)
       : start(start_), n(n_) {
-    if (again) __syncthreads();  // the head before is done with the tiles and the bits
-    if constexpr (MAP) bits.fill(a.map + b * a.mb + h * a.mh + col * a.mk, a.mq, cdiv(n, QB / QS), lds);
+    if (again) __syncthreads();
+    if constexpr (MAP) bits.fill(line, step, cdiv(n, PER), lds);
   }
   __device__ __forceinline__ int first() const { return from(start); }
   __device__ __forceinline__ int next(int i) const { return from(i + 1); }
   __device__ __forceinline__ int from(int st) const {
     if (st >= n) return -1;
     if constexpr (MAP) {
-      const int q = bits.from(st / (QB / QS));
-      if (q < 0) return -1;
-      st = max(st, q * (QB / QS));
+      const int e = bits.from(st / PER);
+      if (e < 0) return -1;
+      st = max(st, e * PER);
     }
     return st;
   }
 };
-// Every step: its tile has landed, the next one's DMAs go out into the other buffer (which all waves have left), compute.
-template <class W, class F, class C>
-__device__ __forceinline__ void run_steps(const W& walk, F fetch, C compute) {
-  int cur = walk.first(), buf = 0;
+// Steps through NS stages of LDS, the DMAs (N a wave and stage) NS - 1 steps ahead: the step's stage has landed in every wave,
+// the DMAs of a later step go out into the stage that all waves have left, compute. The steps for which `early` holds come first
+// and are a loop of their own, with a body of their own: in one loop with two bodies the accumulators did not keep
+// their registers.
+template <int NS, int N, class W, class F, class E, class A, class B>
+__device__ __forceinline__ void run_steps(const W& walk, F fetch, E early, A compute_early, B compute_late) {
+  static_assert(NS == 2 || NS == 3, "");
+  int cur = walk.first(), stage = 0;
   if (cur < 0) return;
   fetch(0, cur);
-  while (cur >= 0) {
-    const int nxt = walk.next(cur);
-    step_barrier();
-    if (nxt >= 0) fetch(buf ^ 1, nxt);
-    compute(buf, cur);
-    cur = nxt;
-    buf ^= 1;
+  int nxt = walk.next(cur);
+  if constexpr (NS == 3) {
+    if (nxt >= 0) fetch(1, nxt);
   }
+  auto step = [&](auto compute) {
+    if constexpr (NS == 3) {
+      if (nxt >= 0) step_barrier<N>();
+      else step_barrier<0>();
+      const int after = nxt >= 0 ? walk.next(nxt) : -1;
+      if (after >= 0) fetch(stage == 0 ? 2 : stage - 1, after);
+      compute(stage, cur);
+      cur = nxt;
+      nxt = after;
+      stage = stage == 2 ? 0 : stage + 1;
+    } else {
+      step_barrier<0>();
+      if (nxt >= 0) fetch(stage ^ 1, nxt);
+      compute(stage, cur);
+      cur = nxt;
+      if (nxt >= 0) nxt = walk.next(nxt);
+      stage ^= 1;
+    }
+  };
+  while (cur >= 0 && early(cur)) step(compute_early);
+  while (cur >= 0) step(compute_late);
 }
+
+// Part p of the steps 0..n-1
+__device__ __forceinline__ int part_of(int n, int p, int parts) { return (int)((long long)n * p / parts); }
 
 // ---- results --------------------------------------------------------------------
 template <int DT, int D>
@@ -344,6 +410,19 @@ __device__ __forceinline__ void store_grad(const View& x, int b, int h, int row,
                            pack2<DT>(acc[d][4 * g + 2] * by, acc[d][4 * g + 3] * by));
       if (!live) y = make_uint2(0, 0);
       *reinterpret_cast<uint2*>(to + 32 * d + 8 * g) = y;
+    }
+}
+// a part's sums in fp32, rows of D
+template <int D>
+__device__ __forceinline__ void store_part(float* row, int half, const v16f (&acc)[D / 32], float by, bool live) {
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      v4f y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = live ? acc[d][4 * g + i] * by : 0.0f;
+      *reinterpret_cast<v4f*>(row + 32 * d + 8 * g + 4 * half) = y;
     }
 }
 template <int DT, int D>

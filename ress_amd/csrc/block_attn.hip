@@ -21,11 +21,18 @@
 
 namespace {
 
+constexpr int NS = 3;  // LDS stages
+// Below this many tiles of 128 keys (2.5 workgroups a CU) dK and dV's are tiles of 64 keys, twice as many: 16 tiles 6.7 us for 8.0, 512
+// causal ones 388 for 426, but 704 82 for 73 and 2,752 66 for 56.
+constexpr int WIDE_TILES = 640;
+
 // ---- forward ----------------------------------------------------------------
 template <int DT, int D, bool MAP>
-__global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
-  __shared__ __align__(16) uint8_t lds[2][2 * tile_bytes(D)];
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArgs a) {
+  constexpr int SR = step_rows(D), KT = SR / 32;
+  __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
+  const unsigned lds0 = lds_address(lds);
   const Lane<D> ln;
   Item it;
   if (!it.query_tile(a)) return;
@@ -41,36 +48,43 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
     const int sees = a.causal ? min(hd.klen, max(0, row + off + 1)) : hd.klen;
     const int last = min(q0 + QB, qlen) - 1;
     const int most = a.causal ? min(hd.klen, max(0, last + off + 1)) : hd.klen;
-    const int nfull = (a.causal ? min(hd.klen, max(0, q0 + off + 1)) : hd.klen) / KB;  // blocks that every row sees whole
+    const int whole = (a.causal ? min(hd.klen, max(0, q0 + off + 1)) : hd.klen) / SR;  // steps that every row sees whole
     uint4 q[D / 16];
     load_row<D>(a.q, it.b, it.h, row, row < qlen, ln.half, q);
-    Walk<MAP> walk(a, it, cdiv(most, KB), bits);
-    const Stream<D> ks(a.k, hd.kbase(a.k), ln, 4), vs(a.v, hd.kbase(a.v), ln, 4);
-    auto fetch = [&](int buf, int kb) {
-      ks.fetch(lds[buf], kb * KB, hd.klen, w);
-      vs.fetch(lds[buf] + tile_bytes(D), kb * KB, hd.klen, w);
+    const int steps = cdiv(most, SR);
+    const Walk<MAP, KB / SR> walk(a.map + it.b * a.mb + it.h * a.mh + it.tile * a.mq, a.mk, part_of(steps, blockIdx.y, a.parts),
+                                  part_of(steps, blockIdx.y + 1, a.parts), bits, false);
+    const Stream<D, 4> ks(a.k, hd.kbase(a.k), ln), vs(a.v, hd.kbase(a.v), ln);
+    auto fetch = [&](int stage, int st) {
+      ks.fetch(lds0 + stage * 2 * TILE, st * SR, hd.klen, w);
+      vs.fetch(lds0 + stage * 2 * TILE + TILE, st * SR, hd.klen, w);
     };
-    run_steps(walk, fetch, [&](int buf, int kb) {
-      const uint8_t* tile = lds[buf];
-      v16f s[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) s[t] = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
-      if (kb >= nfull) {
-        const int below = sees - kb * KB - 4 * ln.half;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
+    auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
+      v16f s[KT];
+      each<KT>([&](auto t) { s[t] = rows_times<DT, D>(tile, 32 * t, ln, q, zero16()); });
+      if constexpr (decltype(mask_tag)::value) {
+        const int below = sees - st * SR - 4 * ln.half;
+        each<KT>([&](auto t) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[t][r] = 32 * t + c_row(r) < below ? s[t][r] : -__builtin_huge_valf();
+        });
       }
-      float top = LOWEST;
+      // Whether a score lies more than LAZY above m. Where m + LAZY is not negative only positive scores can, and they
+      // order as their bits do: integer maxima of three, which need no quieting of NaNs.
+      int top = 0;
+      each<KT>([&](auto t) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int r = 0; r < 16; ++r) top = max(top, __float_as_int(s[t][r]));
+      });
+      if (__any(__int_as_float(top) * a.scale2 > m + LAZY || m + LAZY < 0.0f)) {
+        float x = LOWEST;
+        each<KT>([&](auto t) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
-      top = pair_max(top);
-      top = top == LOWEST ? LOWEST : top * a.scale2;
-      if (__any(top > m + LAZY)) {
-        const float mn = top > m + LAZY ? top : m;
+          for (int r = 0; r < 16; ++r) x = fmaxf(x, s[t][r]);
+        });
+        x = pair_max(x);
+        x = x == LOWEST ? LOWEST : x * a.scale2;
+        const float mn = x > m + LAZY ? x : m;  // a row moves by its own scores, so its bits do not hang on its neighbours
         const float f = exp2f(m - mn);
         m = mn;
         l *= f;
@@ -79,26 +93,30 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_fwd(AttnArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= f;
       }
-      uint4 p[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      each<KT>([&](auto t) {
         float e[16];
+        uint4 p[2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          e[r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -m));
-          l += e[r];
-        }
-        pack16<DT>(e, p[t]);
-      }
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d) o[d] = columns_times<DT, D>(tile + tile_bytes(D), 32 * t, d, ln, p[t], o[d]);
-    });
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale2, -m));
+        pack16<DT>(e, p);
+        // the sum before P is rounded: the backward pass forms P from it
+        l += sum16(e);
+        each<D / 32>([&](auto d) { o[d] = columns_times<DT, D>(tile + TILE, 32 * t, d, ln, p, o[d]); });
+      });
+    };
+    run_steps<NS, 2 * ks.DMAS>(
+        walk, fetch, [&](int st) { return st < whole; },
+        [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); },
+        [&](int stage, int st) { compute(std::true_type{}, lds[stage], st); });
   }
   l = pair_sum(l);
   const bool some = row < qlen && (l > 0.0f || l != l);
-  if (row < a.Tq) {
+  if (row >= a.Tq) return;
+  if (a.parts > 1) {
+    const long long r = (long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row);
+    store_part<D>(a.part + r * D, ln.half, o, 1.0f / l, some);
+    if (ln.half == 0) a.part2[r] = some ? m + log2f(l) : -__builtin_huge_valf();
+  } else {
     store_out<DT, D>(a, it, row, ln.half, o, 1.0f / l, some);
     if (a.lse && ln.half == 0) a.lse[a.row_at(it, row)] = some ? m + log2f(l) : __builtin_huge_valf();
   }
@@ -179,9 +197,11 @@ __device__ __forceinline__ float lift_ds(const AttnArgs& a, int b, int hk) {
 
 // ---- backward: dQ -----------------------------------------------------------
 template <int DT, int D, bool MAP>
-__global__ __launch_bounds__(256, 2) void k_block_attn_dq(AttnArgs a) {
-  __shared__ __align__(16) uint8_t lds[2][2 * tile_bytes(D)];
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs a) {
+  constexpr int SR = step_rows(D), KT = SR / 32;
+  __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
+  const unsigned lds0 = lds_address(lds);
   const Lane<D> ln;
   Item it;
   if (!it.query_tile(a)) return;
@@ -197,7 +217,7 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_dq(AttnArgs a) {
     const int sees = a.causal ? min(hd.klen, max(0, row + off + 1)) : hd.klen;
     const int last = min(q0 + QB, qlen) - 1;
     const int most = a.causal ? min(hd.klen, max(0, last + off + 1)) : hd.klen;
-    const int nfull = (a.causal ? min(hd.klen, max(0, q0 + off + 1)) : hd.klen) / KB;
+    const int whole = (a.causal ? min(hd.klen, max(0, q0 + off + 1)) : hd.klen) / SR;
     uint4 q[D / 16], g[D / 16];
     load_row<D>(a.q, it.b, it.h, row, row < qlen, ln.half, q);
     load_row<D>(a.go, it.b, it.h, row, row < qlen, ln.half, g);
@@ -208,50 +228,94 @@ __global__ __launch_bounds__(256, 2) void k_block_attn_dq(AttnArgs a) {
       lse = a.lse_b[a.row_at(it, row)] + lift(DT) - log2f(f);
       nd = a.ndelta[a.row_at(it, row)];
     }
+    // -delta is added by the matrix cores where 16 registers are to be had for it (2 x 16 products less a step: 144 us for 152 at a
+    // head of 128; at 64 they are not, 1,180 for 940)
     v16f ndelta;
 #pragma unroll
     for (int r = 0; r < 16; ++r) ndelta[r] = nd;
-    Walk<MAP> walk(a, it, cdiv(most, KB), bits);
-    const Stream<D> ks(a.k, hd.kbase(a.k), ln, 4), vs(a.v, hd.kbase(a.v), ln, 4);
-    auto fetch = [&](int buf, int kb) {
-      ks.fetch(lds[buf], kb * KB, hd.klen, w);
-      vs.fetch(lds[buf] + tile_bytes(D), kb * KB, hd.klen, w);
+    const int steps = cdiv(most, SR);
+    const Walk<MAP, KB / SR> walk(a.map + it.b * a.mb + it.h * a.mh + it.tile * a.mq, a.mk, part_of(steps, blockIdx.y, a.parts),
+                                  part_of(steps, blockIdx.y + 1, a.parts), bits, false);
+    const Stream<D, 4> ks(a.k, hd.kbase(a.k), ln), vs(a.v, hd.kbase(a.v), ln);
+    auto fetch = [&](int stage, int st) {
+      ks.fetch(lds0 + stage * 2 * TILE, st * SR, hd.klen, w);
+      vs.fetch(lds0 + stage * 2 * TILE + TILE, st * SR, hd.klen, w);
     };
-    run_steps(walk, fetch, [&](int buf, int kb) {
-      const uint8_t* tile = lds[buf];
-      each<2>([&](auto t_) {
-        constexpr int t = decltype(t_)::value;
+    float sum = 0.0f;
+    const uint8_t* over = nullptr;
+    int keys = 0;
+    auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
+      each<KT>([&](auto t) {
         const v16f s = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
-        const v16f dp = rows_times<DT, D>(tile + tile_bytes(D), 32 * t, ln, g, ndelta);
+        const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, g, D == 128 ? ndelta : zero16());
         float e[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse)) * dp[r];
-        if (kb >= nfull) {
-          const int below = sees - kb * KB - 4 * ln.half;
+        for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse)) * (D == 128 ? dp[r] : dp[r] + nd);
+        if constexpr (decltype(mask_tag)::value) {
+          const int below = sees - st * SR - 4 * ln.half;
 #pragma unroll
           for (int r = 0; r < 16; ++r) e[r] = 32 * t + c_row(r) < below ? e[r] : 0.0f;
         }
         uint4 ds[2];
         pack16<DT>(e, ds);
+        sum = add8<DT>(ds[1], add8<DT>(ds[0], sum));
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
       });
-    });
+      over = tile;
+      keys = min(SR, hd.klen - st * SR);
+    };
+    run_steps<NS, 2 * ks.DMAS>(
+        walk, fetch, [&](int st) { return st < whole; },
+        [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); },
+        [&](int stage, int st) { compute(std::true_type{}, lds[stage], st); });
+    // The rows of dS add up to 0. What their rounding and delta's (P's in the forward pass) made of the sum stands in dQ times the keys'
+    // weighted mean: most of it is what the keys have in common, and goes with the mean of a few of them, those of the last step,
+    // which are still in LDS, or for parts, whose sums are not 0 but add up to it, the first step's. Error of dQ, keys with an offset
+    // of half their deviation: 2.7e-3 -> 2.3e-3 of it in bf16 (1.7e-3 is the result's rounding).
+    if (keys) {
+      if (a.parts > 1) {
+        const int st = walk.from(0);
+        step_barrier<0>();
+        ks.fetch(lds0, st * SR, hd.klen, w);
+        step_barrier<0>();
+        over = lds[0];
+        keys = min(SR, hd.klen - st * SR);
+      }
+      sum = pair_sum(sum);
+      const uint32_t one = pack2<DT>(1.0f, 1.0f);
+      const uint4 ones[2] = {make_uint4(one, one, one, one), make_uint4(one, one, one, one)};
+      const float by = -sum / (float)keys;
+      each<D / 32>([&](auto d) {
+        v16f mean = zero16();
+        each<KT>([&](auto t) { mean = columns_times<DT, D>(over, 32 * t, d, ln, ones, mean); });
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[d][r] = fmaf(by, mean[r], dq[d][r]);
+      });
+    }
   }
-  if (row < a.Tq) store_grad<DT, D>(a.dq, it.b, it.h, row, ln.half, dq, undo, row < qlen);
+  if (row >= a.Tq) return;
+  if (a.parts > 1)
+    store_part<D>(a.part + ((long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row)) * D, ln.half, dq, undo, row < qlen);
+  else
+    store_grad<DT, D>(a.dq, it.b, it.h, row, ln.half, dq, undo, row < qlen);
 }
 
 // ---- backward: dK and dV ----------------------------------------------------
-template <int DT, int D, int NW, bool MAP>
-__global__ __launch_bounds__(64 * NW, 2) void k_block_attn_dkv(AttnArgs a) {
-  constexpr int T = tile_bytes(D);
-  __shared__ __align__(16) uint8_t lds[2][2 * T + 512];
+// Four waves of 32 keys, or SPLIT (under a map, where a workgroup has one key block, and where tiles are few): two waves of 32
+// keys take the first 32 queries of each step, two more with the same keys the others, and their sums are added at the end.
+template <int DT, int D, bool SPLIT, bool MAP>
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dkv(AttnArgs a) {
+  constexpr int SR = SPLIT ? 64 : step_rows(D), KT = SR / 32, TILE = SR * 2 * D, STAGE = 2 * TILE + 512;
+  constexpr int KEYS = SPLIT ? 64 : 128, STAGES = SPLIT && D == 128 ? 2 : NS;
+  __shared__ __align__(16) uint8_t lds[STAGES][STAGE];
   extern __shared__ uint32_t bits[];
-  const Lane<D> ln;
+  const unsigned lds0 = lds_address(lds);
+  const Lane<D> here;
   Item it;
-  if (!it.key_tile(a, 32 * NW)) return;
+  if (!it.key_tile(a, KEYS)) return;
   const Head hd(a, it.b, it.h);
-  const int qlen = a.q_len(it.b), k0 = it.tile * 32 * NW;
-  const int w = ln.wave, key = k0 + 32 * w + ln.c32;
+  const int qlen = a.q_len(it.b), k0 = it.tile * KEYS;
+  const int w = here.wave, key = k0 + 32 * (SPLIT ? w & 1 : w) + here.c32;
   v16f dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = zero16();
@@ -259,47 +323,48 @@ __global__ __launch_bounds__(64 * NW, 2) void k_block_attn_dkv(AttnArgs a) {
   if (k0 < hd.klen && qlen > 0) {
     const int off = hd.klen - qlen;
     uint4 k[D / 16], v[D / 16];
-    load_row<D>(a.k, it.b, it.h, key, key < hd.klen, ln.half, k);
-    load_row<D>(a.v, it.b, it.h, key, key < hd.klen, ln.half, v);
+    load_row<D>(a.k, it.b, it.h, key, key < hd.klen, here.half, k);
+    load_row<D>(a.v, it.b, it.h, key, key < hd.klen, here.half, v);
     f = lift_ds<DT, D>(a, it.b, it.h);
     const float fp = f * (DT == BA_F16 ? 0x1p-14f : 1.0f);
-    const int from = a.causal ? min(qlen, max(0, k0 - off)) : 0;          // no row before it sees a key of the tile
-    const int whole = a.causal ? max(0, k0 + 32 * NW - 1 - off) : 0;      // rows from here on see all of it
-    const int first = a.causal ? key - off - 4 * ln.half : 0;             // rows from `first` on see the lane's key
-    for (int g = 0; g < a.G; ++g) {
+    const int from = a.causal ? min(qlen, max(0, k0 - off)) : 0;      // no row before it sees a key of the tile
+    const int whole = a.causal ? max(0, k0 + KEYS - 1 - off) : 0;     // rows from here on see all of it
+    const int first = a.causal ? key - off - 4 * here.half : 0;         // rows from `first` on see the lane's key
+    // the steps of all heads that share the keys, one after the other, cut into parts
+    const int steps = cdiv(qlen, SR), lo = part_of(steps * a.G, blockIdx.y, a.parts), hi = part_of(steps * a.G, blockIdx.y + 1, a.parts);
+    for (int g = lo / steps; g * steps < hi; ++g) {
       const int h = it.h * a.G + g;
-      WalkColumn<MAP> walk(a, it.b, h, k0 / KB, from / QS, cdiv(qlen, QS), bits, g > 0);
-      const Stream<D> qs(a.q, a.q.at(it.b, h, 0), ln, NW), gs(a.go, a.go.at(it.b, h, 0), ln, NW);
-      const long long rows = ((long long)it.b * a.Hq + h) * a.Tq;
-      auto fetch = [&](int buf, int st) {
-        qs.fetch(lds[buf], st * QS, qlen, w);
-        gs.fetch(lds[buf] + T, st * QS, qlen, w);
-        if (w == 0) fetch_row_values(a.lse_b + rows + st * QS, qlen - st * QS, lds[buf] + 2 * T);
-        if (w == 1) fetch_row_values(a.ndelta + rows + st * QS, qlen - st * QS, lds[buf] + 2 * T + 256);
+      const Walk<MAP, QB / SR> walk(a.map + it.b * a.mb + h * a.mh + k0 / KB * a.mk, a.mq, max(from / SR, lo - g * steps),
+                                    min(steps, hi - g * steps), bits, g * steps > lo);
+      const Stream<D, 4, SR> qs(a.q, a.q.at(it.b, h, 0), here), gs(a.go, a.go.at(it.b, h, 0), here);
+      const float* values = ((w & 1) ? a.ndelta : a.lse_b) + ((long long)it.b * a.Hq + h) * a.Tq;
+      auto fetch = [&](int stage, int st) {
+        const unsigned to = lds0 + stage * STAGE;
+        qs.fetch(to, st * SR, qlen, w);
+        gs.fetch(to + TILE, st * SR, qlen, w);
+        // the rows' values, by every wave, so that all have as many DMAs in flight
+        fetch_row_values(values + st * SR, min(SR, qlen - st * SR), to + 2 * TILE + 256 * (w & 1));
       };
-      run_steps(walk, fetch, [&](int buf, int st) {
-        const uint8_t* tile = lds[buf];
-        each<2>([&](auto t_) {
-          constexpr int t = decltype(t_)::value;
+      auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
+        const Lane<D> ln = here.anew();
+        each<SPLIT ? 1 : KT>([&](auto t_) {
+          const int t = SPLIT ? w >> 1 : (int)t_;
           const v16f s = rows_times<DT, D>(tile, 32 * t, ln, k, zero16());
-          const v16f lse = row_values(tile + 2 * T, 32 * t, ln);
           float e[16];
+          {
+            const v16f lse = row_values(tile + 2 * TILE, 32 * t, ln);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse[r]));
-          if (st * QS < whole) {
+            for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale2, -lse[r]));
+          }
+          if constexpr (decltype(mask_tag)::value) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) e[r] = st * QS + 32 * t + c_row(r) >= first ? e[r] : 0.0f;
+            for (int r = 0; r < 16; ++r) e[r] = st * SR + 32 * t + c_row(r) >= first ? e[r] : 0.0f;
           }
           uint4 p[2], ds[2];
           pack16<DT>(e, p);
-#ifdef SB1
-          if (D == 128) __builtin_amdgcn_sched_barrier(0);
-#endif
-          const v16f dp = rows_times<DT, D>(tile + T, 32 * t, ln, v, row_values(tile + 2 * T + 256, 32 * t, ln));
-          each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + T, 32 * t, x, ln, p, dv[x]); });
-#ifdef SB3
-          if (D == 128) __builtin_amdgcn_sched_barrier(0);
-#endif
+          if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);  // reads ahead of their use would take registers that are not there
+          const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, v, row_values(tile + 2 * TILE + 256, 32 * t, ln));
+          each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + TILE, 32 * t, x, ln, p, dv[x]); });
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             e[r] *= dp[r];
@@ -307,30 +372,112 @@ __global__ __launch_bounds__(64 * NW, 2) void k_block_attn_dkv(AttnArgs a) {
           }
           pack16<DT>(e, ds);
           each<D / 32>([&](auto x) { dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, ds, dk[x]); });
-#ifdef SB2
-          __builtin_amdgcn_sched_barrier(0);
-#endif
         });
-      });
+      };
+      run_steps<STAGES, 2 * qs.DMAS + 1>(
+          walk, fetch, [&](int st) { return st * SR < whole; },
+          [&](int stage, int st) { compute(std::true_type{}, lds[stage], st); },
+          [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); });
     }
   }
-  if (key < a.Tk) {
-    store_grad<DT, D>(a.dk, it.b, it.h, key, ln.half, dk, a.scale / f, key < hd.klen);
-    store_grad<DT, D>(a.dv, it.b, it.h, key, ln.half, dv, DT == BA_F16 ? 0x1p-14f : 1.0f, key < hd.klen);
+  if constexpr (SPLIT) {
+    // waves 2 and 3 hand their sums to 0 and 1, dK's and then dV's: 16 floats of a lane and tile of 32 dims
+    static_assert(2 * (D / 32) * 16 * 64 * 4 <= (int)sizeof(lds), "the sums fit the stages");
+    float* to = reinterpret_cast<float*>(&lds[0][0]) + (w & 1) * (D / 32) * 16 * 64 + (threadIdx.x & 63);
+    auto add = [&](v16f (&acc)[D / 32]) {
+      __syncthreads();
+      if (w >= 2) each<D / 32>([&](auto x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(x * 16 + r) * 64] = acc[x][r];
+      });
+      __syncthreads();
+      if (w < 2) each<D / 32>([&](auto x) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[x][r] += to[(x * 16 + r) * 64];
+      });
+    };
+    add(dk);
+    add(dv);
+    if (w >= 2) return;
+  }
+  if (key >= a.Tk) return;
+  const float by_k = a.scale / f, by_v = DT == BA_F16 ? 0x1p-14f : 1.0f;
+  if (a.parts > 1) {
+    const long long r = (((long long)blockIdx.y * a.B + it.b) * a.Hk + it.h) * a.Tk + key;
+    store_part<D>(a.part + r * D, here.half, dk, by_k, key < hd.klen);
+    store_part<D>(a.part2 + r * D, here.half, dv, by_v, key < hd.klen);
+  } else {
+    store_grad<DT, D>(a.dk, it.b, it.h, key, here.half, dk, by_k, key < hd.klen);
+    store_grad<DT, D>(a.dv, it.b, it.h, key, here.half, dv, by_v, key < hd.klen);
+  }
+}
+
+// ---- parts joined -----------------------------------------------------------
+// A row a wave: D / 4 lanes take four dims each, and the wave's 256 / D groups of them every 256 / D-th part. OUT:
+// o = sum of 2^(lse_p - L) o_p over sum of 2^(lse_p - L), L the largest; else the sum of the parts.
+template <int DT, int D, bool OUT>
+__global__ __launch_bounds__(256) void k_block_attn_join(AttnArgs a, const float* __restrict__ part, const float* __restrict__ lse, View to,
+                                                         int heads, int T) {
+  constexpr int LR = D / 4, GROUPS = 64 / LR;
+  const long long rows = (long long)a.B * heads * T, r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 63, group = lane / LR, d = lane % LR * 4;
+  const int t = (int)(r % T), bh = (int)(r / T), b = bh / heads, h = bh % heads;
+  float top = -__builtin_huge_valf(), sum = 0.0f, mine = top;
+  if constexpr (OUT) {  // at most 64 parts
+    mine = lane < a.parts ? lse[lane * rows + r] : top;
+    top = mine;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const float x = __shfl_xor(top, s, 64);
+      top = x > top || x != x ? x : top;
+    }
+  }
+  const bool some = !OUT || top != -__builtin_huge_valf();
+  v4f x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int p0 = 0; p0 < a.parts; p0 += GROUPS) {  // every lane goes all the way: lanes ask others for their lse
+    const int p = min(p0 + group, a.parts - 1);
+    const bool there = p0 + group < a.parts;
+    v4f y = *reinterpret_cast<const v4f*>(part + (p * rows + r) * D + d);
+    if constexpr (OUT) {
+      const float l = __shfl(mine, p, 64), w = there && some && l != -__builtin_huge_valf() ? exp2f(l - top) : 0.0f;
+      sum += w;
+      y *= w;  // a part that saw nothing is zero
+      x += y;
+    } else if (there) {
+      x += y;
+    }
+  }
+#pragma unroll
+  for (int s = LR; s < 64; s <<= 1) {
+    sum += __shfl_xor(sum, s, 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += __shfl_xor(x[i], s, 64);
+  }
+  if (group) return;
+  if (OUT && some) x /= sum;
+  const uint2 y = make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+  *reinterpret_cast<uint2*>(to.at(b, h, t) + d) = y;
+  if constexpr (OUT) {
+    if (a.rest)
+      *reinterpret_cast<uint2*>(a.rest + r * D + d) =
+          make_uint2(pack2<DT>(x[0] - unpack1<DT>(y.x, 0), x[1] - unpack1<DT>(y.x, 1)),
+                     pack2<DT>(x[2] - unpack1<DT>(y.y, 0), x[3] - unpack1<DT>(y.y, 1)));
+    if (a.lse && d == 0) a.lse[r] = some ? top + log2f(sum) : __builtin_huge_valf();
   }
 }
 
 // ---- host -------------------------------------------------------------------
-bool fits(const View& x, int heads, int T, int D) {
-  const long long lo = D, most = 1ll << 24;
-  return x.p && ((uintptr_t)x.p & 15) == 0 && x.b >= 0 && x.h >= 0 && (x.b & 7) == 0 && (x.h & 7) == 0 && (x.t & 7) == 0 &&
-         x.t >= lo && x.t < most;
+bool fits(const View& x, int D) {
+  return x.p && ((uintptr_t)x.p & 15) == 0 && x.b >= 0 && x.h >= 0 && ((x.b | x.h | x.t) & 7) == 0 && x.t >= D && x.t < 1ll << 24;
 }
 int check(const AttnArgs& a, int D, int dtype, const char* name) {
   RESS_REQUIRE(D == 64 || D == 128, "%s: head_dim %d (64 or 128)", name, D);
   RESS_REQUIRE(dtype == BA_BF16 || dtype == BA_F16, "%s: dtype code %d", name, dtype);
   RESS_REQUIRE(a.B >= 0 && a.Hq >= 0 && a.Hk >= 1 && a.Tq >= 0 && a.Tk >= 0 && a.Hq % a.Hk == 0, "%s: bad geometry", name);
   RESS_REQUIRE(a.Tq <= 1 << 26 && a.Tk <= 1 << 26, "%s: more than 2^26 tokens", name);
+  RESS_REQUIRE((long long)a.Hq / a.Hk * cdiv(a.Tq, 32) < 1ll << 30, "%s: too many query heads of a key/value head", name);
   RESS_REQUIRE(!a.map || (a.Tq <= 1 << 20 && a.Tk <= 1 << 20), "%s: more than 2^20 tokens under a map", name);
   RESS_REQUIRE(a.scale > 0.0f && a.scale < __builtin_inff(), "%s: scale must be positive and finite", name);
   return 0;
@@ -385,27 +532,79 @@ AttnArgs arguments(const ress_block_attn* c) {
 
 }  // namespace
 
-RESS_API int ress_block_attn_fwd(const ress_block_attn* c, hipStream_t stream) {
-  RESS_REQUIRE(c, "ress_block_attn_fwd: null arguments");
+// Parts that a launch of `tiles` workgroups is cut into, each of at least LEAST steps: as many as fill the card's 512 places for
+// workgroups (two a CU) where a quarter of them or more would stay empty.
+constexpr int PLACES = 512, LEAST = 8, MOST_PARTS = 64;
+int parts_of(long long tiles, long long steps) {
+  if (tiles <= 0 || tiles > PLACES * 3 / 4) return 1;
+  long long n = (PLACES + tiles - 1) / tiles;
+  if (n > steps / LEAST) n = steps / LEAST;
+  return (int)(n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n);
+}
+// How a call is cut: keys a workgroup of dK and dV has, and the parts of each kernel
+struct Plan {
+  bool split;
+  int q_parts, k_parts;
+  long long q_rows, k_rows;
+  explicit Plan(const ress_block_attn* c) {
+    const int sr = step_rows(c->head_dim);
+    const long long wide = (long long)c->B * c->kv_heads * cdiv(c->Tk, 128);
+    split = c->map || wide < WIDE_TILES;
+    q_rows = (long long)c->B * c->q_heads * c->Tq;
+    k_rows = (long long)c->B * c->kv_heads * c->Tk;
+    q_parts = parts_of((long long)c->B * c->q_heads * cdiv(c->Tq, QB), cdiv(c->Tk, sr));
+    k_parts = parts_of((long long)c->B * c->kv_heads * cdiv(c->Tk, split ? 64 : 128),
+                       (long long)cdiv(c->Tq, split ? 64 : sr) * (c->q_heads / c->kv_heads));
+  }
+  long long fwd_bytes(int D) const { return q_parts > 1 ? 4 * q_parts * q_rows * (D + 1) : 0; }
+  long long bwd_part_bytes(int D) const {
+    const long long q = q_parts > 1 ? 4 * q_parts * q_rows * D : 0, k = k_parts > 1 ? 8 * k_parts * k_rows * D : 0;
+    return q > k ? q : k;
+  }
+};
+bool sizes_ok(const ress_block_attn* c) {
+  return c && c->B >= 0 && c->q_heads >= 0 && c->kv_heads >= 1 && c->q_heads % c->kv_heads == 0 && c->Tq >= 0 && c->Tk >= 0 &&
+         c->Tq <= 1 << 26 && c->Tk <= 1 << 26 && (c->head_dim == 64 || c->head_dim == 128);
+}
+
+RESS_API long long ress_block_attn_fwd_workspace_size(const ress_block_attn* c) {
+  return sizes_ok(c) ? Plan(c).fwd_bytes(c->head_dim) : -1;
+}
+
+RESS_API int ress_block_attn_fwd(const ress_block_attn* c, void* workspace, long long workspace_bytes, hipStream_t stream) {
+  const char* name = "ress_block_attn_fwd";
+  RESS_REQUIRE(c, "%s: null arguments", name);
   AttnArgs a = arguments(c);
   const int D = c->head_dim, dtype = c->dtype;
-  if (int rc = check(a, D, dtype, "ress_block_attn_fwd")) return rc;
+  if (int rc = check(a, D, dtype, name)) return rc;
   if (!a.B || !a.Hq || !a.Tq) return 0;
-  RESS_REQUIRE(fits(a.q, a.Hq, a.Tq, D) && fits(a.o, a.Hq, a.Tq, D) && (a.Tk == 0 || (fits(a.k, a.Hk, a.Tk, D) && fits(a.v, a.Hk, a.Tk, D))),
-               "ress_block_attn_fwd: operands must be 16-byte aligned, strides multiples of 8, tokens at least head_dim apart");
-  unsigned blocks;
-  if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256, "ress_block_attn_fwd", &blocks)) return rc;
+  RESS_REQUIRE(fits(a.q, D) && fits(a.o, D) && (a.Tk == 0 || (fits(a.k, D) && fits(a.v, D))),
+               "%s: operands must be 16-byte aligned, strides multiples of 8, tokens at least head_dim and fewer than 2^24 apart", name);
+  const Plan plan(c);
+  RESS_REQUIRE(workspace_bytes >= plan.fwd_bytes(D) && ((uintptr_t)workspace & 15) == 0 && (workspace || !plan.fwd_bytes(D)),
+               "%s: the workspace is too small or not aligned", name);
+  a.parts = plan.q_parts;
+  a.part = (float*)workspace;
+  a.part2 = a.part + a.parts * plan.q_rows * D;
+  unsigned blocks, jblocks;
+  if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * a.parts, name, &blocks)) return rc;
+  if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jblocks)) return rc;
   RESS_BA_EACH({
-    if (a.map) hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, true>), dim3(blocks), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
-    else hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, false>), dim3(blocks), dim3(256), 0, stream, a);
+    if (a.map) hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, true>), dim3(blocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
+    else hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, false>), dim3(blocks, a.parts), dim3(256), 0, stream, a);
+    RESS_LAUNCHED("k_block_attn_fwd");
+    if (a.parts > 1) {
+      hipLaunchKernelGGL((k_block_attn_join<DT, DIM, true>), dim3(jblocks), dim3(256), 0, stream, a, a.part, a.part2, a.o, a.Hq, a.Tq);
+      RESS_LAUNCHED("k_block_attn_join");
+    }
   })
-  RESS_LAUNCHED("k_block_attn_fwd");
   return 0;
 }
 
 RESS_API long long ress_block_attn_bwd_workspace_size(const ress_block_attn* c) {
-  if (!c || c->B < 0 || c->q_heads < 0 || c->kv_heads < 0 || c->Tq < 0) return -1;
-  return 8ll * c->B * c->q_heads * c->Tq + 8ll * c->B * c->kv_heads;
+  if (!sizes_ok(c)) return -1;
+  const Plan p(c);
+  return p.bwd_part_bytes(c->head_dim) + 8 * p.q_rows + 8ll * c->B * c->kv_heads;
 }
 
 RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* grad_out, const ress_strided* dq,
@@ -421,41 +620,57 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   const int D = c->head_dim, dtype = c->dtype;
   if (int rc = check(a, D, dtype, name)) return rc;
   if (!a.B || !a.Hq) return 0;
-  RESS_REQUIRE((a.Tq == 0 || (fits(a.q, a.Hq, a.Tq, D) && fits(a.o, a.Hq, a.Tq, D) && fits(a.go, a.Hq, a.Tq, D) && fits(a.dq, a.Hq, a.Tq, D))) &&
-                   (a.Tk == 0 || (fits(a.k, a.Hk, a.Tk, D) && fits(a.v, a.Hk, a.Tk, D) && fits(a.dk, a.Hk, a.Tk, D) && fits(a.dv, a.Hk, a.Tk, D))),
-               "%s: operands must be 16-byte aligned, strides multiples of 8, tokens at least head_dim apart", name);
+  RESS_REQUIRE((a.Tq == 0 || (fits(a.q, D) && fits(a.o, D) && fits(a.go, D) && fits(a.dq, D))) &&
+                   (a.Tk == 0 || (fits(a.k, D) && fits(a.v, D) && fits(a.dk, D) && fits(a.dv, D))),
+               "%s: operands must be 16-byte aligned, strides multiples of 8, tokens at least head_dim and fewer than 2^24 apart", name);
   RESS_REQUIRE(a.Tq == 0 || (a.rest && ((uintptr_t)a.rest & 15) == 0 && a.lse), "%s: the forward pass's rest and lse are needed", name);
-  RESS_REQUIRE(workspace_bytes >= ress_block_attn_bwd_workspace_size(c) && (workspace || !workspace_bytes), "%s: the workspace is too small", name);
-  const long long rows = (long long)a.B * a.Hq * a.Tq;
-  a.lse_b = (float*)workspace;
-  a.ndelta = a.lse_b + rows;
-  a.top = (uint32_t*)(a.ndelta + rows);
-  const bool wide = !a.map;  // 128 keys a workgroup; under a map one of its key blocks
-  const int keys = wide ? 128 : 64, chunks = cdiv(a.Tk, VTOP_ROWS);
-  unsigned qblocks = 0, kblocks = 0, dblocks = 0, vblocks = 0;
-  if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256, name, &qblocks)) return rc;
-  if (int rc = grid((long long)a.B * a.Hk * cdiv(a.Tk, keys), 2 * keys, name, &kblocks)) return rc;
-  const int dchunks = cdiv(a.Tq, DELTA_ROWS);
+  RESS_REQUIRE(workspace_bytes >= ress_block_attn_bwd_workspace_size(c) && ((uintptr_t)workspace & 15) == 0 && (workspace || !workspace_bytes),
+               "%s: the workspace is too small or not aligned", name);
+  const Plan plan(c);
+  float* const parts = (float*)workspace;  // of dQ and, once these are joined, of dK and dV
+  a.lse_b = parts + plan.bwd_part_bytes(D) / 4;
+  a.ndelta = a.lse_b + plan.q_rows;
+  a.top = (uint32_t*)(a.ndelta + plan.q_rows);
+  const int keys = plan.split ? 64 : 128, chunks = cdiv(a.Tk, VTOP_ROWS), dchunks = cdiv(a.Tq, DELTA_ROWS);
+  unsigned qblocks, kblocks, dblocks, vblocks, jq, jk;
+  if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * plan.q_parts, name, &qblocks)) return rc;
+  if (int rc = grid((long long)a.B * a.Hk * cdiv(a.Tk, keys), 256 * plan.k_parts, name, &kblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hq * dchunks, 256, name, &dblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hk * chunks, 256, name, &vblocks)) return rc;
-  if (dtype == BA_F16 && a.Tk) {
-    hipLaunchKernelGGL(k_block_attn_clear, dim3(cdiv(2 * a.B * a.Hk, 256)), dim3(256), 0, stream, a.top, 2 * a.B * a.Hk);
-    if (D == 64) hipLaunchKernelGGL((k_block_attn_vtop<64>), dim3((unsigned)((long long)a.B * a.Hk * chunks)), dim3(256), 0, stream, a, chunks);
-    else hipLaunchKernelGGL((k_block_attn_vtop<128>), dim3((unsigned)((long long)a.B * a.Hk * chunks)), dim3(256), 0, stream, a, chunks);
-    RESS_LAUNCHED("k_block_attn_vtop");
-  }
+  if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jq)) return rc;
+  if (int rc = grid((plan.k_rows + 3) / 4, 256, name, &jk)) return rc;
   RESS_BA_EACH({
+    if (dtype == BA_F16 && a.Tk) {
+      hipLaunchKernelGGL(k_block_attn_clear, dim3(cdiv(2 * a.B * a.Hk, 256)), dim3(256), 0, stream, a.top, 2 * a.B * a.Hk);
+      hipLaunchKernelGGL((k_block_attn_vtop<DIM>), dim3((unsigned)((long long)a.B * a.Hk * chunks)), dim3(256), 0, stream, a, chunks);
+      RESS_LAUNCHED("k_block_attn_vtop");
+    }
     if (a.Tq) {
       hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3((unsigned)((long long)a.B * a.Hq * dchunks)), dim3(256), 0, stream, a, dchunks);
       RESS_LAUNCHED("k_block_attn_delta");
-      if (a.map) hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, true>), dim3(qblocks), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
-      else hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, false>), dim3(qblocks), dim3(256), 0, stream, a);
+      a.parts = plan.q_parts;
+      a.part = parts;
+      if (a.map) hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, true>), dim3(qblocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
+      else hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, false>), dim3(qblocks, a.parts), dim3(256), 0, stream, a);
       RESS_LAUNCHED("k_block_attn_dq");
+      if (a.parts > 1) {
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jq), dim3(256), 0, stream, a, a.part, nullptr, a.dq, a.Hq, a.Tq);
+        RESS_LAUNCHED("k_block_attn_join");
+      }
     }
     if (a.Tk) {
-      if (a.map) hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, 2, true>), dim3(kblocks), dim3(128), bit_bytes(cdiv(a.Tq, QB)), stream, a);
-      else hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, 4, false>), dim3(kblocks), dim3(256), 0, stream, a);
+      a.parts = plan.k_parts;
+      a.part = parts;
+      a.part2 = parts + a.parts * plan.k_rows * D;
+      if (a.map) hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, true, true>), dim3(kblocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tq, QB)), stream, a);
+      else if (plan.split) hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, true, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, false, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
       RESS_LAUNCHED("k_block_attn_dkv");
+      if (a.parts > 1) {
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jk), dim3(256), 0, stream, a, a.part, nullptr, a.dk, a.Hk, a.Tk);
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jk), dim3(256), 0, stream, a, a.part2, nullptr, a.dv, a.Hk, a.Tk);
+        RESS_LAUNCHED("k_block_attn_join");
+      }
     }
   })
   return 0;

@@ -143,7 +143,11 @@ def _attend(q, k, v, block_map, causal, q_lens, k_lens, scale, grads):
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
         rest = _empty(q)
     if out.numel():
-        _lib.call_on(q.device, "ress_block_attn_fwd", _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest))
+        args = _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
+        size, work = _attn_workspace(False, args[128:160], block_map is not None), None
+        if size:
+            work = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _lib.call_on(q.device, "ress_block_attn_fwd", args, None if work is None else work.data_ptr(), size)
     return out, lse, rest
 
 
@@ -163,7 +167,7 @@ class _BlockAttention(torch.autograd.Function):
         grad = _ready(grad)
         dq, dk, dv = _like(q), _like(k), _like(v)
         args = _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
-        size = _attn_workspace(args[128:160])
+        size = _attn_workspace(True, args[128:160], block_map is not None)
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
         _lib.call_on(q.device, "ress_block_attn_bwd", args, _STRIDED(*_strides(grad)), _STRIDED(*_strides(dq)),
                      _STRIDED(*_strides(dk)), _STRIDED(*_strides(dv)), work.data_ptr(), size)
@@ -171,8 +175,9 @@ class _BlockAttention(torch.autograd.Function):
 
 
 @functools.lru_cache(maxsize=256)
-def _attn_workspace(sizes):
-    return _lib.lib().ress_block_attn_bwd_workspace_size(bytes(128) + sizes + bytes(88))
+def _attn_workspace(backward, sizes, mapped):
+    size = _lib.lib().ress_block_attn_bwd_workspace_size if backward else _lib.lib().ress_block_attn_fwd_workspace_size
+    return size(bytes(128) + sizes + struct.pack("@3q", 0, 0, 1 if mapped else 0) + bytes(64))
 
 
 def _check_attention(q, k, v, block_map):
@@ -217,8 +222,8 @@ def block_attention(q, k, v, block_map=None, causal=False, q_lens=None, k_lens=N
     bool or uint8, of these the keys of blocks that it keeps (the final_map of a block-sparse layer is one). q_lens and
     k_lens: (B,) int32 on the device (clamped into the tensors), or lists. Rows that see nothing and rows from q_lens[b] on are zero,
     in the output and the gradients. Tokens past the lengths and blocks that are dropped reach nothing, whatever they
-    hold; a key or value that is not finite makes NaN of the rows that see its block, in a causal block also of those that see
-    only a part of it.
+    hold; a key or value that is not finite makes NaN of the rows that see its block, in causal order also of the others of
+    their 128-query blocks.
 
     The probabilities, formed anew in the backward pass, and the scores' gradients are rounded to the operands' type before
     they are multiplied; sums, maxima and the softmax's statistics are fp32. A forward pass for gradients keeps, beside its

@@ -122,6 +122,24 @@ def test_what_a_map_drops_reaches_nothing(dev):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hk,Tq,Tk", [(1, 1, 3, 17000), (2, 2, 130, 3000), (3, 1, 1, 20000), (2, 1, 9000, 70), (8, 1, 2000, 1), (1, 1, 17000, 65)])
+@pytest.mark.parametrize("kind", ["dense", "causal", "map", "lengths"])
+def test_few_rows_or_few_keys(dev, dt, D, Hq, Hk, Tq, Tk, kind):
+    """Long axes that are cut into parts, some of which see nothing."""
+    q, k, v, do = make(1, Hq, Hk, Tq, Tk, D, dt)
+    kw = {}
+    if kind == "causal":
+        kw["causal"] = True
+    if kind == "lengths":
+        kw.update(q_lens=[max(1, Tq - Tq // 3)], k_lens=[max(1, Tk // 5)])
+    if kind == "map":
+        g = torch.Generator().manual_seed(2)
+        kw["block_map"] = (torch.rand(1, Hq, -(-Tq // 128), -(-Tk // 64), generator=g) < 0.05).to(dev)
+    compare(q, k, v, do, **kw)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 def test_large_scores(dev, dt):
     """Rows that one key takes whole, scores far from zero on both sides, running maxima that move many times."""
     q, k, v, do = make(1, 2, 2, 200, 700, 64, dt, size=3.0)
