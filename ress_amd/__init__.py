@@ -19,6 +19,7 @@ from ress_amd.int8 import Int8Linear, int8_linear, quantize_linears
 from ress_amd.kvcache import PagedKVCache, RotaryTable
 from ress_amd.qkv import declare_rope
 from ress_amd.stream import FrameStream
+from ress_amd.training import enable_gradients
 
 __all__ = [
     "BACKBONES",
@@ -34,6 +35,7 @@ __all__ = [
     "block_attention",
     "check_layers",
     "declare_rope",
+    "enable_gradients",
     "get_backbone",
     "int8_linear",
     "layer_norm",

@@ -68,8 +68,12 @@ class Attention(nn.Module):
         self.proj = nn.Linear(dim, dim, bias=True)
         self.proj_drop = nn.Identity()
         self.fused = True  # q/k norm + RoPE through the fused kernel when on the GPU in bf16
+        self.gradients = False  # the operators with a backward pass where gradients are asked for (ress_amd.enable_gradients)
 
     def forward(self, x, pos=None):
+        if self.gradients and torch.is_grad_enabled():
+            from ress_amd import training
+            return training.attention_forward(self, x, pos)
         from ress_amd.qkv import _fusable, fused_qk_norm_rope
         B, T, C = x.shape
         nh = self.num_heads
@@ -117,8 +121,12 @@ class Block(nn.Module):
         self.norm2 = nn.LayerNorm(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio))
         self.ls2 = LayerScale(dim)
+        self.gradients = False
 
     def forward(self, x, pos=None):
+        if self.gradients and torch.is_grad_enabled():
+            from ress_amd import training
+            return training.block_forward(self, x, pos)
         x = x + self.ls1(self.attn(self.norm1(x), pos=pos))
         return x + self.ls2(self.mlp(self.norm2(x)))
 

@@ -232,6 +232,21 @@ def sparse_global_attention(q, k, v, grid, *, num_to_select=None, budget_fn=None
     formed in that order, as if the tokens had gone through the reference's hilbert_permute
     (src/ress/models/hilbert.py:128-162), but read and written in place.
     Returns a LayerResult whose `out` is (B, H, frames*P, 64) in storage order."""
+    blocks, sel = _select(q, k, v, grid, num_to_select, budget_fn, perhead_budget_fn, joint_select_fn, block_criterion, M, qk_mode,
+                          protect_own_frame, attention_sink, patch_order)
+    with trace.stage("ress.sparse_attention"):
+        o = kernels.sparse_attention(blocks, sel.lut, sel.nvalid, out=out, out_dtype=out_dtype)
+    res = LayerResult(out=o, final_map=sel.final_map, budget_iters=sel.budget_iters, max_iters=sel.max_iters,
+                      attn_status=getattr(o, "ress_attn_status", None))
+    if keep_intermediates:
+        res.attn_full, res.attn_cond, res.v_bar_full = sel.attn_full, sel.attn_cond, sel.v_bar_full
+        res.counts, res.lut, res.nvalid, res.blocks = sel.counts, sel.lut, sel.nvalid, blocks
+    return res
+
+
+def _select(q, k, v, grid, num_to_select, budget_fn, perhead_budget_fn, joint_select_fn, block_criterion, M, qk_mode,
+            protect_own_frame, attention_sink, patch_order):
+    """(blocks, LayerResult without output): the stages of a layer up to its map."""
     sink_lead = sink_lead_blocks(attention_sink, grid)
     with trace.stage("ress.prepare_blocks"):
         blocks = kernels.prepare_blocks(q, k, v, grid, mode=qk_mode or DEFAULT_QK_MODE, patch_order=patch_order)
@@ -278,14 +293,8 @@ def sparse_global_attention(q, k, v, grid, *, num_to_select=None, budget_fn=None
     if M is not None:  # after every step that can move the map, as the reference records it
         from ress_amd import projected as _projected
         _projected.record_layer_drift(M, attn_full, v_bar_full, final_map, grid.n_cand)
-    with trace.stage("ress.sparse_attention"):
-        o = kernels.sparse_attention(blocks, lut, nvalid, out=out, out_dtype=out_dtype)
-    res = LayerResult(out=o, final_map=final_map, budget_iters=budget_iters, max_iters=max_iters,
-                      attn_status=getattr(o, "ress_attn_status", None))
-    if keep_intermediates:
-        res.attn_full, res.attn_cond, res.v_bar_full = attn_full, attn_cond, v_bar_full
-        res.counts, res.lut, res.nvalid, res.blocks = counts, lut, nvalid, blocks
-    return res
+    return blocks, LayerResult(out=None, attn_full=attn_full, attn_cond=attn_cond, v_bar_full=v_bar_full, final_map=final_map,
+                               counts=counts, lut=lut, nvalid=nvalid, budget_iters=budget_iters, max_iters=max_iters)
 
 
 def _dense_storage(q, k, v, shp):
@@ -307,7 +316,7 @@ def ress_attention_forward(self, x, pos, num_to_select=None, budget_fn=None, per
                            num_special_tokens=5, num_heads=16, shape=None, aux_store=None, aux_full=True,
                            dense=False, retain_output_grad=False, pooled_fallback=False, protect_own_frame=False,
                            attention_sink=0, patch_order=None, eager_check=False, sink_mass=False,
-                           sink_protect=True):
+                           sink_protect=True, differentiable=False):
     """Replacement forward of a global-attention block (reference attention.py:296-659),
     same arguments and return value: (B, N*P, dim) after the W_O projection.
     sink_mass / sink_protect: the reference's RESS_SINK_MASS / RESS_SINK_PROTECT process
@@ -324,17 +333,43 @@ def ress_attention_forward(self, x, pos, num_to_select=None, budget_fn=None, per
     (check_layers / LayerResult.check is the deferred check). eager_check (not a reference
     argument; the module attribute of the same name): synchronise at the end of the forward
     and raise there, as the reference raises a non-converged HeSS budget at once
-    (_proportional.py:112-113)."""
+    (_proportional.py:112-113).
+    differentiable (not a reference argument; the module attribute that ress_amd.enable_gradients sets): where gradients are
+    asked for, the layer's parts are those with a backward pass (ress_amd.training): the map is selected as ever,
+    without gradients, and the attention over it passes them to q, k and v."""
     if pool_mode != "avg":
         raise NotImplementedError("only avg pooling (the reference default) is implemented")
-    q, k, v, shp = compute_qkv(self, x, pos, num_special_tokens=num_special_tokens, num_heads=num_heads,
-                               shape=shape)
+    graded = differentiable and torch.is_grad_enabled()
+    if graded:
+        from ress_amd import training
+        q, k, v, shp = training.compute_qkv(self, x, pos, num_special_tokens, num_heads, shape)
+    else:
+        q, k, v, shp = compute_qkv(self, x, pos, num_special_tokens=num_special_tokens, num_heads=num_heads,
+                                   shape=shape)
     B, N, P, hd, nh, S = shp["B"], shp["N"], shp["P"], shp["head_dim"], shp["num_heads"], shp["S"]
     if hd != 64:
         raise ValueError(f"head_dim {hd} unsupported (the kernels are written for 64)")
     grid = LayerGrid(B=B, H=nh, frames=N, P=P, S=S, sink_protect=bool(sink_protect), sink_mass=bool(sink_mass))
     res = None
-    if dense:
+    order = None
+    if graded:
+        qb, kbf, vbf = (t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16) for t in (q, k, v))
+        if dense:
+            x_out = training.block_attention(qb, kbf, vbf)
+            sparsity = 0.0
+            self._ress_status = None
+        else:
+            order = _device_patch_order(self, patch_order, grid, q.device)
+            with torch.no_grad():
+                _, res = _select(qb, kbf, vbf, grid, num_to_select, budget_fn, perhead_budget_fn, joint_select_fn, block_criterion,
+                                 getattr(self, "M", None), None, protect_own_frame, attention_sink, order)
+            x_out = training.sparse_attention(qb, kbf, vbf, res.final_map, grid, order)
+            self._ress_status = LayerResult(out=None, unconverged=res.unconverged, budget_iters=res.budget_iters,
+                                            max_iters=res.max_iters)
+            sparsity = res.sparsity() if aux_store is not None else None
+            if eager_check and aux_store is None:
+                res.check()
+    elif dense:
         x_out = _dense_storage(q, k, v, shp).float()
         sparsity = 0.0
         self._ress_status = None   # a dense forward leaves nothing to report

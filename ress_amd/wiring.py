@@ -27,6 +27,7 @@ CALL_ATTRIBUTES = (
     ("eager_check", False),
     ("sink_mass", False),
     ("sink_protect", True),
+    ("differentiable", False),
 )
 
 
