@@ -555,6 +555,9 @@ struct Plan {
     q_parts = parts_of((long long)c->B * c->q_heads * cdiv(c->Tq, QB), cdiv(c->Tk, sr));
     k_parts = parts_of((long long)c->B * c->kv_heads * cdiv(c->Tk, split ? 64 : 128),
                        (long long)cdiv(c->Tq, split ? 64 : sr) * (c->q_heads / c->kv_heads));
+#ifdef KP
+    if (c->causal && (long long)c->B * c->kv_heads * cdiv(c->Tk, 64) <= 1024) k_parts = KP;
+#endif
   }
   long long fwd_bytes(int D) const { return q_parts > 1 ? 4 * q_parts * q_rows * (D + 1) : 0; }
   long long bwd_part_bytes(int D) const {
