@@ -7,7 +7,6 @@ namespace {
 constexpr int QB = 128, KB = 64;  // the map's query and key blocks
 // Rows of a streamed tile: 8 KB of an operand, in tiles of 32 for the matrix cores
 constexpr int step_rows(int D) { return 4096 / D; }
-constexpr int TILE = 8192;
 constexpr int BA_BF16 = 1, BA_F16 = 2;
 constexpr float LOWEST = -0x1.fffffep127f;
 // The running maximum moves when a score lies more than this above it (in log2): P stays below 2^8, and most steps need no

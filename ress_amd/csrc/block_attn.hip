@@ -23,13 +23,16 @@ namespace {
 
 constexpr int NS = 3;  // LDS stages
 // Below this many tiles of 128 keys (2.5 workgroups a CU) dK and dV's are tiles of 64 keys, twice as many: 16 tiles 6.7 us for 8.0, 512
-// causal ones 388 for 426, but 704 82 for 73 and 2,752 66 for 56.
+// causal ones 388 for 426, but 704 82 for 73 and 2,752 66 for 56 (before the head of 128 kept its registers: 281 now).
 constexpr int WIDE_TILES = 640;
 
 // ---- forward ----------------------------------------------------------------
+// A wave has 32 queries. Steps of 64 keys, at a head of 128 in two stages (three of 32 keys 153 us for 135, the causal case).
+// Bound by the vector unit where the card is full: of a step's 16 products (D = 64) and 32 exponentials a lane, the latter are
+// four times as dear as other instructions.
 template <int DT, int D, bool MAP>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArgs a) {
-  constexpr int SR = step_rows(D), KT = SR / 32;
+  constexpr int SR = 64, KT = SR / 32, TILE = SR * 2 * D, NS = D == 64 ? 3 : 2;
   __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
   const unsigned lds0 = lds_address(lds);
@@ -54,7 +57,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArg
     const int steps = cdiv(most, SR);
     const Walk<MAP, KB / SR> walk(a.map + it.b * a.mb + it.h * a.mh + it.tile * a.mq, a.mk, part_of(steps, blockIdx.y, a.parts),
                                   part_of(steps, blockIdx.y + 1, a.parts), bits, false);
-    const Stream<D, 4> ks(a.k, hd.kbase(a.k), ln), vs(a.v, hd.kbase(a.v), ln);
+    const Stream<D, 4, SR> ks(a.k, hd.kbase(a.k), ln), vs(a.v, hd.kbase(a.v), ln);
     auto fetch = [&](int stage, int st) {
       ks.fetch(lds0 + stage * 2 * TILE, st * SR, hd.klen, w);
       vs.fetch(lds0 + stage * 2 * TILE + TILE, st * SR, hd.klen, w);
@@ -196,18 +199,20 @@ __device__ __forceinline__ float lift_ds(const AttnArgs& a, int b, int hk) {
 }
 
 // ---- backward: dQ -----------------------------------------------------------
+// A wave has 32 queries and their gradients as operands. Bound by matrix and vector unit in turn (16 frames of 1,374 tokens, 30% of the
+// blocks: products 51% of the cycles, vector instructions 59%), at a clock that their power brings down to some 1.7 GHz.
 template <int DT, int D, bool MAP>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs a) {
-  constexpr int SR = step_rows(D), KT = SR / 32;
+  constexpr int SR = step_rows(D), KT = SR / 32, TILE = SR * 2 * D;
   __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
   const unsigned lds0 = lds_address(lds);
-  const Lane<D> ln;
+  const Lane<D> here;
   Item it;
   if (!it.query_tile(a)) return;
   const Head hd(a, it.b, it.h / a.G);
   const int qlen = a.q_len(it.b), q0 = it.tile * QB;
-  const int w = ln.wave, row = q0 + 32 * w + ln.c32;
+  const int w = here.wave, row = q0 + 32 * w + here.c32;
   v16f dq[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dq[d] = zero16();
@@ -219,8 +224,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
     const int most = a.causal ? min(hd.klen, max(0, last + off + 1)) : hd.klen;
     const int whole = (a.causal ? min(hd.klen, max(0, q0 + off + 1)) : hd.klen) / SR;
     uint4 q[D / 16], g[D / 16];
-    load_row<D>(a.q, it.b, it.h, row, row < qlen, ln.half, q);
-    load_row<D>(a.go, it.b, it.h, row, row < qlen, ln.half, g);
+    load_row<D>(a.q, it.b, it.h, row, row < qlen, here.half, q);
+    load_row<D>(a.go, it.b, it.h, row, row < qlen, here.half, g);
     const float f = lift_ds<DT, D>(a, it.b, it.h / a.G);
     undo = a.scale / f;
     float lse = 0.0f, nd = 0.0f;
@@ -236,15 +241,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
     const int steps = cdiv(most, SR);
     const Walk<MAP, KB / SR> walk(a.map + it.b * a.mb + it.h * a.mh + it.tile * a.mq, a.mk, part_of(steps, blockIdx.y, a.parts),
                                   part_of(steps, blockIdx.y + 1, a.parts), bits, false);
-    const Stream<D, 4> ks(a.k, hd.kbase(a.k), ln), vs(a.v, hd.kbase(a.v), ln);
+    const Stream<D, 4, SR> ks(a.k, hd.kbase(a.k), here), vs(a.v, hd.kbase(a.v), here);
     auto fetch = [&](int stage, int st) {
       ks.fetch(lds0 + stage * 2 * TILE, st * SR, hd.klen, w);
       vs.fetch(lds0 + stage * 2 * TILE + TILE, st * SR, hd.klen, w);
     };
     float sum = 0.0f;
-    const uint8_t* over = nullptr;
-    int keys = 0;
-    auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
+    int over = 0, keys = 0;
+    auto compute = [&](auto mask_tag, int stage, int st) {
+      const Lane<D> ln = here.anew();
+      const uint8_t* tile = lds[stage];
       each<KT>([&](auto t) {
         const v16f s = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
         const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, g, D == 128 ? ndelta : zero16());
@@ -261,13 +267,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
         sum = add8<DT>(ds[1], add8<DT>(ds[0], sum));
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
       });
-      over = tile;
+      over = stage;
       keys = min(SR, hd.klen - st * SR);
     };
     run_steps<NS, 2 * ks.DMAS>(
         walk, fetch, [&](int st) { return st < whole; },
-        [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); },
-        [&](int stage, int st) { compute(std::true_type{}, lds[stage], st); });
+        [&](int stage, int st) { compute(std::false_type{}, stage, st); },
+        [&](int stage, int st) { compute(std::true_type{}, stage, st); });
     // The rows of dS add up to 0. What their rounding and delta's (P's in the forward pass) made of the sum stands in dQ times the keys'
     // weighted mean: most of it is what the keys have in common, and goes with the mean of a few of them, those of the last step,
     // which are still in LDS, or for parts, whose sums are not 0 but add up to it, the first step's. Error of dQ, keys with an offset
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
         step_barrier<0>();
         ks.fetch(lds0, st * SR, hd.klen, w);
         step_barrier<0>();
-        over = lds[0];
+        over = 0;
         keys = min(SR, hd.klen - st * SR);
       }
       sum = pair_sum(sum);
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
       const float by = -sum / (float)keys;
       each<D / 32>([&](auto d) {
         v16f mean = zero16();
-        each<KT>([&](auto t) { mean = columns_times<DT, D>(over, 32 * t, d, ln, ones, mean); });
+        each<KT>([&](auto t) { mean = columns_times<DT, D>(lds[over], 32 * t, d, here, ones, mean); });
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[d][r] = fmaf(by, mean[r], dq[d][r]);
       });
@@ -295,12 +301,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
   }
   if (row >= a.Tq) return;
   if (a.parts > 1)
-    store_part<D>(a.part + ((long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row)) * D, ln.half, dq, undo, row < qlen);
+    store_part<D>(a.part + ((long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row)) * D, here.half, dq, undo, row < qlen);
   else
-    store_grad<DT, D>(a.dq, it.b, it.h, row, ln.half, dq, undo, row < qlen);
+    store_grad<DT, D>(a.dq, it.b, it.h, row, here.half, dq, undo, row < qlen);
 }
 
 // ---- backward: dK and dV ----------------------------------------------------
+// A wave has 32 keys; queries and their gradients stream past. At a head of 128 no register is left to read LDS far ahead, and the waves
+// wait for that (causal case: products 17% of the cycles). Tried there: 64 keys a wave, one wave a SIMD, every operand read meeting two
+// tiles, no wave waiting for another: 502 us for 281.
 // Four waves of 32 keys, or SPLIT (under a map, where a workgroup has one key block, and where tiles are few): two waves of 32
 // keys take the first 32 queries of each step, two more with the same keys the others, and their sums are added at the end.
 template <int DT, int D, bool SPLIT, bool MAP>
@@ -532,8 +541,9 @@ AttnArgs arguments(const ress_block_attn* c) {
 
 }  // namespace
 
-// Parts that a launch of `tiles` workgroups is cut into, each of at least LEAST steps: as many as fill the card's 512 places for
-// workgroups (two a CU) where a quarter of them or more would stay empty.
+// Parts that a launch of `tiles` workgroups is cut into, each of at least LEAST steps of 64 rows: as many as fill the card's 512 places
+// for workgroups (two a CU) where a quarter of them or more would stay empty. 16 tiles of 80 queries over 21,984 keys: forward 377 us
+// whole, 26 in 32 parts and 5 to join them; dQ 330, 27 and 5.
 constexpr int PLACES = 512, LEAST = 8, MOST_PARTS = 64;
 int parts_of(long long tiles, long long steps) {
   if (tiles <= 0 || tiles > PLACES * 3 / 4) return 1;
@@ -547,17 +557,13 @@ struct Plan {
   int q_parts, k_parts;
   long long q_rows, k_rows;
   explicit Plan(const ress_block_attn* c) {
-    const int sr = step_rows(c->head_dim);
     const long long wide = (long long)c->B * c->kv_heads * cdiv(c->Tk, 128);
     split = c->map || wide < WIDE_TILES;
     q_rows = (long long)c->B * c->q_heads * c->Tq;
     k_rows = (long long)c->B * c->kv_heads * c->Tk;
-    q_parts = parts_of((long long)c->B * c->q_heads * cdiv(c->Tq, QB), cdiv(c->Tk, sr));
+    q_parts = parts_of((long long)c->B * c->q_heads * cdiv(c->Tq, QB), cdiv(c->Tk, KB));
     k_parts = parts_of((long long)c->B * c->kv_heads * cdiv(c->Tk, split ? 64 : 128),
-                       (long long)cdiv(c->Tq, split ? 64 : sr) * (c->q_heads / c->kv_heads));
-#ifdef KP
-    if (c->causal && (long long)c->B * c->kv_heads * cdiv(c->Tk, 64) <= 1024) k_parts = KP;
-#endif
+                       (long long)cdiv(c->Tq, 64) * (c->q_heads / c->kv_heads));
   }
   long long fwd_bytes(int D) const { return q_parts > 1 ? 4 * q_parts * q_rows * (D + 1) : 0; }
   long long bwd_part_bytes(int D) const {
