@@ -106,7 +106,9 @@ class RotaryTable:
             raise ValueError(f"a rotation table needs at least one position and a base above 1, got {positions} and {base}")
         inv = float(base) ** (-torch.arange(0, d, 2, dtype=torch.float64) / d)
         inv, gain = _scaled(inv, d, float(base), scaling)
-        ang = torch.arange(int(positions), dtype=torch.float64)[:, None] * inv
+        if scaling is not None or layout != "half" or rotary_dim not in (None, head_dim):
+            inv = inv.to(device)  # formed on the device: 131,072 positions take the host 30 ms. append's tables keep the host's bits.
+        ang = torch.arange(int(positions), dtype=torch.float64, device=inv.device)[:, None] * inv
         self._set(torch.stack([ang.cos() * gain, ang.sin() * gain], 1).float().to(device), head_dim, axes, layout, rotary_dim)
 
     @staticmethod
