@@ -126,6 +126,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArg
 }
 
 // ---- backward: row sums -----------------------------------------------------
+// Raises *p to the workgroup's largest value (>= 0: bits in the values' order, so the atomics' order is the same for the result). One
+// atomic a workgroup: they meet at a few addresses.
+__device__ __forceinline__ void raise_top(uint32_t* p, float top) {
+  __shared__ float tops[4];
+  top = wave_max(top);
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    if (top > 0.0f) atomicMax(p, __float_as_uint(top));
+  }
+}
 // -delta_i = -dO_i.(o_i + what o's rounding took), lse less the lift of P, and fp16: the largest finite |dO| of each
 // (sequence, key/value head). Bound by its bytes.
 template <int DT, int D>
@@ -156,10 +168,7 @@ __global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, int chunks
       a.lse_b[r] = a.lse[r] - lift(DT);
     }
   }
-  if constexpr (DT == BA_F16) {
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0 && top > 0.0f) atomicMax(a.top + (long long)b * a.Hk + h / a.G, __float_as_uint(top));
-  }
+  if constexpr (DT == BA_F16) raise_top(a.top + (long long)b * a.Hk + h / a.G, top);
 }
 __global__ void k_block_attn_clear(uint32_t* p, int n) {
   const int i = blockIdx.x * blockDim.x + threadIdx.x;
@@ -181,8 +190,7 @@ __global__ __launch_bounds__(256) void k_block_attn_vtop(AttnArgs a, int chunks)
       if (m > top && m < __builtin_huge_valf()) top = m;
     }
   }
-  top = wave_max(top);
-  if ((threadIdx.x & 63) == 0 && top > 0.0f) atomicMax(a.top + (long long)a.B * a.Hk + bh, __float_as_uint(top));
+  raise_top(a.top + (long long)a.B * a.Hk + bh, top);
 }
 
 // fp16: dS is formed times a power of two that takes the largest possible one to 2^15 (|dP - delta| <= 2 D max|dO| max|v|,
