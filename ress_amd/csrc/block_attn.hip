@@ -547,8 +547,6 @@ AttnArgs arguments(const ress_block_attn* c) {
   return a;
 }
 
-}  // namespace
-
 // Parts that a launch of `tiles` workgroups is cut into, each of at least LEAST steps of 64 rows: as many as fill the card's 512 places
 // for workgroups (two a CU) where a quarter of them or more would stay empty. 16 tiles of 80 queries over 21,984 keys: forward 377 us
 // whole, 26 in 32 parts and 5 to join them; dQ 330, 27 and 5.
@@ -583,6 +581,8 @@ bool sizes_ok(const ress_block_attn* c) {
   return c && c->B >= 0 && c->q_heads >= 0 && c->kv_heads >= 1 && c->q_heads % c->kv_heads == 0 && c->Tq >= 0 && c->Tk >= 0 &&
          c->Tq <= 1 << 26 && c->Tk <= 1 << 26 && (c->head_dim == 64 || c->head_dim == 128);
 }
+
+}  // namespace
 
 RESS_API long long ress_block_attn_fwd_workspace_size(const ress_block_attn* c) {
   return sizes_ok(c) ? Plan(c).fwd_bytes(c->head_dim) : -1;
