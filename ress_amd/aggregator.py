@@ -56,6 +56,7 @@ class Attention(nn.Module):
     module layout the block-sparse forward reads (qkv, q_norm, k_norm, rope, proj,
     proj_drop, num_heads). On the GPU in bf16 the norms and the rotation run as one fused
     kernel (ress_qk_norm_rope); `fused = False` keeps the torch modules."""
+    gradients = False  # the operators with a backward pass where gradients are asked for (ress_amd.enable_gradients)
 
     def __init__(self, dim, num_heads, rope):
         super().__init__()
@@ -68,7 +69,6 @@ class Attention(nn.Module):
         self.proj = nn.Linear(dim, dim, bias=True)
         self.proj_drop = nn.Identity()
         self.fused = True  # q/k norm + RoPE through the fused kernel when on the GPU in bf16
-        self.gradients = False  # the operators with a backward pass where gradients are asked for (ress_amd.enable_gradients)
 
     def forward(self, x, pos=None):
         if self.gradients and torch.is_grad_enabled():
@@ -113,6 +113,8 @@ class LayerScale(nn.Module):
 
 
 class Block(nn.Module):
+    gradients = False
+
     def __init__(self, dim, num_heads, mlp_ratio, rope):
         super().__init__()
         self.norm1 = nn.LayerNorm(dim)
@@ -121,7 +123,6 @@ class Block(nn.Module):
         self.norm2 = nn.LayerNorm(dim)
         self.mlp = Mlp(dim, int(dim * mlp_ratio))
         self.ls2 = LayerScale(dim)
-        self.gradients = False
 
     def forward(self, x, pos=None):
         if self.gradients and torch.is_grad_enabled():

@@ -363,7 +363,8 @@ def ress_attention_forward(self, x, pos, num_to_select=None, budget_fn=None, per
             with torch.no_grad():
                 _, res = _select(qb, kbf, vbf, grid, num_to_select, budget_fn, perhead_budget_fn, joint_select_fn, block_criterion,
                                  getattr(self, "M", None), None, protect_own_frame, attention_sink, order)
-            x_out = training.sparse_attention(qb, kbf, vbf, res.final_map, grid, order)
+            with trace.stage("ress.sparse_attention"):
+                x_out = training.sparse_attention(qb, kbf, vbf, res.final_map, grid, order)
             self._ress_status = LayerResult(out=None, unconverged=res.unconverged, budget_iters=res.budget_iters,
                                             max_iters=res.max_iters)
             sparsity = res.sparsity() if aux_store is not None else None
@@ -415,8 +416,12 @@ def check_layers(model_or_modules):
     """Synchronise once and raise what the last forward of each block-sparse attention
     module left unreported: RuntimeError if a HeSS budget did not converge (reference
     _proportional.py:112-113), ValueError if the 16-bit attention met an operand outside
-    fp16's range. Takes a model (every submodule) or an iterable of modules."""
-    mods = model_or_modules.modules() if hasattr(model_or_modules, "modules") else model_or_modules
+    fp16's range. Takes a model (every submodule) or an iterable of modules. A model that ran with
+    gradients: also RuntimeError if a position lay outside a rotary module's table (a copy each)."""
+    mods = list(model_or_modules.modules() if hasattr(model_or_modules, "modules") else model_or_modules)
+    for m in mods:
+        for table in getattr(m, "_ress_rotary_tables", {}).values():
+            table.check()
     results = [m._ress_status for m in mods if getattr(m, "_ress_status", None) is not None]
     per = [r._status_values() for r in results]
     vals = [v for vs in per for v in vs]

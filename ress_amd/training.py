@@ -16,6 +16,7 @@ own dense attention (scripts/calibrate_fisher_scores.py).
 import torch
 import torch.nn as nn
 
+from ress_amd import _lib
 from ress_amd.differentiable import (NORM_DTYPES, Q_BLOCK, _capturing, add_layer_norm, block_attention, layer_norm,
                                       rotate)
 from ress_amd.kvcache import RotaryTable
@@ -47,7 +48,10 @@ def _table(rope, head_dim, device):
     tables = rope.__dict__.setdefault("_ress_rotary_tables", {})
     key = (head_dim, base, str(device))
     if key not in tables:
+        if _capturing():
+            raise RuntimeError("run the model once before a graph capture: its rotation tables are made then")
         tables[key] = RotaryTable(head_dim, POSITIONS, base=base, axes=2, device=device)
+        torch.cuda.current_stream(device).synchronize()  # once: other streams read it too
     return tables[key]
 
 
@@ -129,13 +133,13 @@ def _orders(grid, patch_order, device):
     return keys, k_back, queries, q_back, (len(patch), len(patch) + fill)
 
 
-_plain_orders = {}  # (frames, tokens a frame, special ones, device) -> _orders without a patch order
+_plain_orders = {}  # (frames, tokens a frame, special ones, device, stream) -> _orders without a patch order
 
 
 def _layer_orders(grid, patch_order, device):
-    key = (grid.frames, grid.P, grid.S, str(device))
     if patch_order is not None or _capturing():  # what is made inside a capture belongs to its graph
         return _orders(grid, patch_order, device)
+    key = (grid.frames, grid.P, grid.S, str(device), _lib.stream_handle(device))
     if key not in _plain_orders:
         if len(_plain_orders) >= 8:
             _plain_orders.clear()

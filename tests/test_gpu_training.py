@@ -187,3 +187,75 @@ def test_the_operators_in_a_row(dev):
     want, = torch.autograd.grad(exact(x64, pos), x64, dy.to(y.dtype).double())
     assert ((got.double() - want).norm() / want.norm()) <= MODEL_TOLERANCE / 2
     assert F.cosine_similarity(got.double().flatten(), want.flatten(), dim=0) > 0.999
+
+
+def test_a_captured_row_of_operators(dev):
+    """Residual norm, rotation and causal attention, there and back, in one graph beside eager work of the same kind: every replay as the
+    eager pass on the same inputs."""
+    g = torch.Generator().manual_seed(4)
+    rope = ress.RotaryTable(64, 300, base=10000.0, axes=1, device=dev, layout="interleaved")
+    pos = torch.arange(130, device=dev)
+
+    def inputs(seed):
+        g.manual_seed(seed)
+        shapes = ((2, 130, 128), (2, 130, 128), (128,), (128,), (128,))
+        return [torch.randn(s, generator=g).to(dev, torch.bfloat16).requires_grad_() for s in shapes]
+
+    def run(x, branch, gamma, weight, bias):
+        h, n = ress.add_layer_norm(x, branch, gamma, weight, bias)
+        q, k = (t.view(2, 130, 2, 64).transpose(1, 2) for t in (n, h))
+        q, k = ress.rotate((q, k), pos, rope)
+        out = ress.block_attention(q, k, h.view(2, 130, 2, 64).transpose(1, 2), causal=True)
+        return (out, *torch.autograd.grad(out, (x, branch, gamma, weight, bias), torch.ones_like(out)))
+
+    mine = inputs(0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run(*mine)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*mine)
+    for seed in range(4):
+        new = inputs(seed + 1)
+        with torch.no_grad():
+            for a, b in zip(mine, new):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, run(*new))), seed
+
+
+def test_positions_outside_a_models_table_are_reported(dev):
+    model = small(False, depth=1)
+    ress.enable_gradients(model)
+    block = model.aggregator.frame_blocks[0]
+    x = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=dev)
+    block(x, torch.full((1, 4, 2), 7, device=dev))
+    ress.check_layers(model)
+    block(x, torch.full((1, 4, 2), 1 << 20, device=dev))
+    with pytest.raises(RuntimeError, match="outside the rotation table"):
+        ress.check_layers(model)
+    ress.check_layers(model)
+
+
+def test_a_model_that_has_not_run_is_not_captured(dev):
+    model = small(False, depth=1)
+    ress.enable_gradients(model)
+    block = model.aggregator.frame_blocks[0]
+    x, pos = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=dev), torch.zeros(1, 4, 2, dtype=torch.int64, device=dev)
+    qkv = torch.zeros(1, 4, 384, dtype=torch.bfloat16, device=dev)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        try:
+            with pytest.raises(RuntimeError, match="once before a graph capture"):
+                training.normed_and_turned(block.attn, qkv, pos, 2)
+            x.add_(1.0)
+        finally:
+            graph.capture_end()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.isfinite(block(x, pos)).all()
