@@ -311,3 +311,19 @@ def test_a_capture_beside_an_eager_result_of_the_same_leaves_is_refused(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_tokens_far_apart(dev, D):
+    """Offsets past 2^32 bytes: operands and gradients in a buffer whose tokens lie 4 MB apart give the contiguous call's bits."""
+    T, apart = 1300, 1 << 21
+    wide = torch.empty(T, apart, dtype=torch.bfloat16, device=dev)
+    q, k, v, do = (t.detach() for t in make(1, 2, 2, T, T, D, torch.bfloat16))
+    want = run(*(t.clone().requires_grad_() for t in (q, k, v)), do, causal=True)
+    far = []
+    for i, t in enumerate((q, k, v, do)):
+        to = wide[:, apart - (i + 1) * 2 * D:][:, :2 * D].view(T, 2, D).transpose(0, 1)[None]
+        to.copy_(t)
+        far.append(to)
+    got = run(*(t.requires_grad_() for t in far[:3]), far[3], causal=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

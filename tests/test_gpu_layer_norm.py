@@ -237,3 +237,14 @@ def test_against_differences(dev):
         # fp32 gradients: 2^-18 of the terms; differences: h^2 and 2^-52 / h of the value's terms
         bound = SLACK * (got[n].double() * d).abs().sum() * 8 + 1e-6
         assert ((got[n].double() * d).sum() - diff).abs() <= bound
+
+
+def test_offsets_past_32_bits(dev):
+    """Four million rows of 1,024: the last ones as a call of their own."""
+    few = make((64, 1024), torch.bfloat16, torch.bfloat16, branch=True, gamma=True)
+    few = {n: None if t is None else t.detach() for n, t in few.items()}
+    many = {n: t.repeat(65537, 1) if t.dim() == 2 else t for n, t in few.items()}
+    a, b = ({n: t.requires_grad_() if n[0] != "d" else t for n, t in s.items()} for s in (few, many))
+    want, got = run(a), run(b)
+    for n in ("h", "n", "x", "branch"):
+        assert torch.equal(got[n][:64], want[n]) and torch.equal(got[n][-64:], want[n]), n

@@ -178,3 +178,20 @@ def test_scaled_tables(dev, scaling):
     want = torch.cat([v[:, :32] * c - v[:, 32:] * s, v[:, 32:] * c + v[:, :32] * s], -1)[None, None]
     mag = (v.abs() + v.roll(32, -1).abs())[None, None] * math.sqrt(2)
     near(ress.rotate(x, pos, rope), want, mag)
+
+
+def test_offsets_past_32_bits(dev):
+    """More than 2^32 elements, there and back: the last tokens as a call of their own."""
+    n, few = (1 << 24) + 37, 100
+    x = torch.randn(1, 2, few, 128, generator=torch.Generator().manual_seed(0)).to(dev, torch.bfloat16)
+    rope = ress.RotaryTable(128, few, base=1000.0, axes=1, device=dev, layout="interleaved")
+    pos = torch.arange(n, device=dev) % few
+    many = x.repeat(1, 1, -(-n // few), 1)[:, :, :n].contiguous().requires_grad_()
+    y = ress.rotate(many, pos, rope)
+    want = ress.rotate(x, pos[:few], rope)
+    last = n // few * few
+    assert torch.equal(y[:, :, :few], want) and torch.equal(y[:, :, last:], want[:, :, :n - last])
+    back, = torch.autograd.grad(y, many, y.detach())
+    again = ress.rotate(x.requires_grad_(), pos[:few], rope)
+    want, = torch.autograd.grad(again, x, again.detach())
+    assert torch.equal(back[:, :, :few], want) and torch.equal(back[:, :, last:], want[:, :, :n - last])
