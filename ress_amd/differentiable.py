@@ -79,7 +79,8 @@ def _first_derivative(function):
 
 
 def _empty(t):
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    """A contiguous tensor like t (empty_like takes a third of empty's host time)."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 # ---- attention -------------------------------------------------------------------
@@ -101,13 +102,22 @@ def _strides(t):
 
 
 def _ready(t):
-    return t if _strides(t) is not None else t.clone(memory_format=torch.contiguous_format)
+    """(t or a copy that the kernels can take, its _strides)"""
+    at = _strides(t)
+    if at is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        at = _strides(t)
+    return t, at
 
 
 def _like(t):
-    """A tensor for a result laid out like t where the kernels can write that."""
+    """(a tensor for a result laid out like t where the kernels can write that, its _strides)"""
     new = torch.empty_like(t)
-    return new if _strides(new) is not None else _empty(t)
+    at = _strides(new)
+    if at is None:
+        new = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        at = _strides(new)
+    return new, at
 
 
 def _lens(lens, name, B, T, device):
@@ -125,25 +135,28 @@ def _lens(lens, name, B, T, device):
     return lens.contiguous()
 
 
-def _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest):
+def _attn_args(q, k, at, block_map, causal, q_lens, k_lens, scale, lse, rest):
+    """at: the _strides of q, k, v and the output, one behind the other"""
     B, Hq, Tq, D = q.shape
     if block_map is None:
         m = (0, 0, 0, 0, 0)
     else:
         m = (block_map.data_ptr(), *block_map.stride())
-    return _ATTN(*_strides(q), *_strides(k), *_strides(v), *_strides(out), B, Hq, k.shape[1], Tq, k.shape[2], D, DTYPES[q.dtype],
+    return _ATTN(*at, B, Hq, k.shape[1], Tq, k.shape[2], D, DTYPES[q.dtype],
                  1 if causal else 0, 0 if q_lens is None else q_lens.data_ptr(), 0 if k_lens is None else k_lens.data_ptr(), *m,
                  0 if lse is None else lse.data_ptr(), 0 if rest is None else rest.data_ptr(), scale)
 
 
 def _attend(q, k, v, block_map, causal, q_lens, k_lens, scale, grads):
-    out = _like(q)
+    """q, k, v: what _ready gave for them"""
+    (q, aq), (k, ak), (v, av) = q, k, v
+    out, ao = _like(q)
     lse = rest = None
     if grads:
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
         rest = _empty(q)
     if out.numel():
-        args = _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
+        args = _attn_args(q, k, aq + ak + av + ao, block_map, causal, q_lens, k_lens, scale, lse, rest)
         size, work = _attn_workspace(False, args[128:160], block_map is not None), None
         if size:
             work = torch.empty(size, dtype=torch.uint8, device=q.device)
@@ -156,7 +169,7 @@ class _BlockAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, block_map, causal, q_lens, k_lens, scale):
         q, k, v = _ready(q), _ready(k), _ready(v)
         out, lse, rest = _attend(q, k, v, block_map, causal, q_lens, k_lens, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, rest, block_map, q_lens, k_lens)
+        ctx.save_for_backward(q[0], k[0], v[0], out, lse, rest, block_map, q_lens, k_lens)
         ctx.how = causal, scale
         return out
 
@@ -164,13 +177,14 @@ class _BlockAttention(torch.autograd.Function):
     def backward(ctx, grad):
         q, k, v, out, lse, rest, block_map, q_lens, k_lens = ctx.saved_tensors
         causal, scale = ctx.how
-        grad = _ready(grad)
-        dq, dk, dv = _like(q), _like(k), _like(v)
-        args = _attn_args(q, k, v, out, block_map, causal, q_lens, k_lens, scale, lse, rest)
+        grad, ag = _ready(grad)
+        (dq, aq), (dk, ak), (dv, av) = _like(q), _like(k), _like(v)
+        args = _attn_args(q, k, _strides(q) + _strides(k) + _strides(v) + _strides(out), block_map, causal, q_lens, k_lens, scale,
+                          lse, rest)
         size = _attn_workspace(True, args[128:160], block_map is not None)
         work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _lib.call_on(q.device, "ress_block_attn_bwd", args, _STRIDED(*_strides(grad)), _STRIDED(*_strides(dq)),
-                     _STRIDED(*_strides(dk)), _STRIDED(*_strides(dv)), work.data_ptr(), size)
+        _lib.call_on(q.device, "ress_block_attn_bwd", args, _STRIDED(*ag), _STRIDED(*aq), _STRIDED(*ak), _STRIDED(*av),
+                     work.data_ptr(), size)
         return dq, dk, dv, None, None, None, None, None
 
 
