@@ -5,7 +5,8 @@
     out = model(images)
 
 Frames that arrive one after the other go through FrameStream, over 8-bit key/value caches; with
-quantize_linears the model's linear layers run in 8-bit integers.
+quantize_linears the model's linear layers run in 8-bit integers. enable_gradients has a model's blocks, sparse layers
+included, run on operators with a backward pass.
 
 The hot path runs on hand-written HIP kernels for gfx950 (libress_hip.so, built by
 `python -m ress_amd.build`); see ress_amd.attention for the per-layer pipeline.
