@@ -9,7 +9,9 @@
 // many rows, so that the weights are read and the sums are written a few hundred times and not once a row, and a row's loads are in
 // flight while the row before is computed. 21,984 rows of 1,024 in bf16, residual sum and LayerScale included: forward 33 us
 // (180 MB, 5.5 TB/s; without the loads ahead 45), backward 47 (270 MB, 5.8 TB/s; 80) and 4 for the parts' sums. Four waves a
-// workgroup and 512 workgroups; eight waves 35 + 48, half the workgroups 34 + 47, twice as many 35 + 49.
+// workgroup and 512 workgroups; eight waves 35 + 48, half the workgroups 34 + 47, twice as many 35 + 49. Rows that cannot be read
+// 16 bytes at a time go element by element, without a branch between the loads: 9,470 rows of 1,637 in fp32, residual sum
+// included, forward 44 us and backward 54 (with one 138 and 259), in bf16 30 and 48.
 #include "../../include/ress_hip.h"
 #include "common.h"
 
@@ -67,7 +69,8 @@ __device__ __forceinline__ int place(int t, int k, int u) {
 // Piece k of a row as it is loaded, and its values (zeros past the row's end)
 template <int DT, int TPR, bool VEC>
 struct Piece {
-  static constexpr int N = DT == LN_F32 ? 2 : 1;
+  // 16-bit elements that come by themselves stay in a register each (packing would wait for them) where there are enough
+  static constexpr int N = DT == LN_F32 || (!VEC && TPR < 1024) ? 2 : 1;
   uint4 v[N];
   __device__ __forceinline__ void load(const char* row, int t, int k, int C) {
     if constexpr (VEC) {
@@ -79,27 +82,30 @@ struct Piece {
       uint32_t x[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const int at = place<TPR, false>(t, k, u);
-        x[u] = 0;
-        if (at < C) x[u] = DT == LN_F32 ? reinterpret_cast<const uint32_t*>(row)[at] : reinterpret_cast<const uint16_t*>(row)[at];
+        const int at = min(place<TPR, false>(t, k, u), C - 1);  // no branch between the loads
+        x[u] = DT == LN_F32 ? reinterpret_cast<const uint32_t*>(row)[at] : reinterpret_cast<const uint16_t*>(row)[at];
       }
-      if constexpr (DT == LN_F32) {
+      if constexpr (N == 2) {
         v[0] = make_uint4(x[0], x[1], x[2], x[3]);
-        v[N - 1] = make_uint4(x[4], x[5], x[6], x[7]);
+        v[1] = make_uint4(x[4], x[5], x[6], x[7]);
       } else {
         v[0] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
       }
     }
   }
-  __device__ __forceinline__ void values(float (&x)[8]) const {
-    if constexpr (DT == LN_F32) {
+  __device__ __forceinline__ void values(int t, int k, int C, float (&x)[8]) const {
+    if constexpr (N == 2) {
       const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[N - 1].x, v[N - 1].y, v[N - 1].z, v[N - 1].w};
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = __uint_as_float(w[u]);
+      for (int u = 0; u < 8; ++u) x[u] = DT == LN_F32 ? __uint_as_float(w[u]) : to_f32<DT>(w[u]);
     } else {
       const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
       for (int u = 0; u < 8; ++u) x[u] = to_f32<DT>(u & 1 ? w[u >> 1] >> 16 : w[u >> 1] & 0xffffu);
+    }
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = place<TPR, false>(t, k, u) < C ? x[u] : 0.0f;
     }
   }
 };
@@ -107,7 +113,7 @@ template <int DT, int TPR, bool VEC>
 __device__ __forceinline__ void load8(const char* row, int t, int k, int C, float (&x)[8]) {
   Piece<DT, TPR, VEC> p;
   p.load(row, t, k, C);
-  p.values(x);
+  p.values(t, k, C, x);
 }
 template <int DT, int TPR, bool VEC>
 __device__ __forceinline__ void store8(char* row, int t, int k, int C, const float (&x)[8]) {
@@ -172,6 +178,13 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* lds) {
   }
 }
 constexpr int ln_threads(int TPR) { return TPR > 256 ? TPR : 256; }
+// A thread's row of its workgroup's; where a wave has one row alone the compiler shall know it, and keep addresses in scalar registers
+template <int TPR>
+__device__ __forceinline__ int row_in_group() {
+  if constexpr (TPR >= 256) return 0;
+  else if constexpr (TPR >= 64) return __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+  else return threadIdx.x / TPR;
+}
 
 template <int DT, int TPR, int K, bool VEC>
 __global__ __launch_bounds__(ln_threads(TPR)) void k_layer_norm_fwd(NormArgs a) {
@@ -199,17 +212,17 @@ __global__ __launch_bounds__(ln_threads(TPR)) void k_layer_norm_fwd(NormArgs a) 
     }
   };
   const long long step = (long long)gridDim.x * RPG;
-  long long r = (long long)blockIdx.x * RPG + threadIdx.x / TPR;
+  long long r = (long long)blockIdx.x * RPG + row_in_group<TPR>();
   if (r < a.rows) load(r);
   for (; r < a.rows; r += step) {  // a row's threads go together, and only they wait for each other
     float x[K][8];
 #pragma unroll
-    for (int k = 0; k < K; ++k) px[k].values(x[k]);
+    for (int k = 0; k < K; ++k) px[k].values(t, k, a.C, x[k]);
     if (a.branch.p) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float y[8];
-        pb[k].values(y);
+        pb[k].values(t, k, a.C, y);
         // the norm is that of the sum as it is returned, and the backward pass reads that
 #pragma unroll
         for (int u = 0; u < 8; ++u) x[k][u] = rounded<DT>(fmaf(gm[k][u], y[u], x[k][u]));
@@ -251,6 +264,7 @@ __global__ __launch_bounds__(ln_threads(TPR)) void k_layer_norm_fwd(NormArgs a) 
 template <int DT, int TPR, int K, bool VEC>
 __global__ __launch_bounds__(ln_threads(TPR)) void k_layer_norm_bwd(NormArgs a) {
   constexpr int NT = ln_threads(TPR), RPG = NT / TPR, SZ = bytes_of<DT>(), COLS = TPR * K * 8;
+  constexpr bool AHEAD = TPR < 1024;  // 128 registers a lane are too few for a row's loads beside the row before (692 us for 896)
   constexpr int PER = TPR <= 64 ? NT / 64 : 1;  // parts of a column in the workgroup: one a wave
   __shared__ float lds[TPR > 64 ? 2 * (TPR / 64) : PER * COLS];
   const int t = threadIdx.x % TPR;
@@ -280,19 +294,20 @@ __global__ __launch_bounds__(ln_threads(TPR)) void k_layer_norm_bwd(NormArgs a) 
     row(pb, a.branch);
   };
   const long long step = (long long)gridDim.x * RPG;
-  long long r = (long long)blockIdx.x * RPG + threadIdx.x / TPR;
-  if (r < a.rows) load(r);
+  long long r = (long long)blockIdx.x * RPG + row_in_group<TPR>();
+  if (AHEAD && r < a.rows) load(r);
   for (; r < a.rows; r += step) {
+    if (!AHEAD) load(r);
     float xh[K][8], g[K][8], more[K][8], y[K][8];
     const float m = mean, rs = rstd;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      px[k].values(xh[k]);
-      if (a.dn.p) pn[k].values(g[k]);
-      if (a.dh.p) ph[k].values(more[k]);
-      if (a.branch.p) pb[k].values(y[k]);
+      px[k].values(t, k, a.C, xh[k]);
+      if (a.dn.p) pn[k].values(t, k, a.C, g[k]);
+      if (a.dh.p) ph[k].values(t, k, a.C, more[k]);
+      if (a.branch.p) pb[k].values(t, k, a.C, y[k]);
     }
-    if (r + step < a.rows) load(r + step);
+    if (AHEAD && r + step < a.rows) load(r + step);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -381,7 +396,9 @@ __global__ __launch_bounds__(1024) void k_layer_norm_ends(const float* __restric
   }
 }
 
-// The shape that takes rows of C elements: as few threads a row as leave a thread 16 elements at most
+// The shape that takes rows of C elements: as few threads a row as leave a thread 16 elements at most, 8 where they are loaded one by
+// one (16: 1,637 in fp32 184 and 531 us). 9,470 rows of 8,000 in 512 threads for 1,024: bf16 109 + 191 us for 141 + 190, fp32 222 +
+// 328 for 225 + 505.
 template <class F>
 void with_shape(int C, bool vec, F f) {
 #define RESS_LN_SHAPE(T, K, V) f(std::integral_constant<int, T>{}, std::integral_constant<int, K>{}, std::integral_constant<bool, V>{})
@@ -392,10 +409,11 @@ void with_shape(int C, bool vec, F f) {
     else if (C <= 1024) RESS_LN_SHAPE(64, 2, true);
     else if (C <= 2048) RESS_LN_SHAPE(256, 1, true);
     else if (C <= 4096) RESS_LN_SHAPE(256, 2, true);
-    else RESS_LN_SHAPE(1024, 1, true);
+    else RESS_LN_SHAPE(512, 2, true);
   } else {
     if (C <= 512) RESS_LN_SHAPE(64, 1, false);
-    else if (C <= 4096) RESS_LN_SHAPE(256, 2, false);
+    else if (C <= 2048) RESS_LN_SHAPE(256, 1, false);
+    else if (C <= 4096) RESS_LN_SHAPE(512, 1, false);
     else RESS_LN_SHAPE(1024, 1, false);
   }
 }
