@@ -102,6 +102,19 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = unpack1<DT>(u[i >> 1], i & 1);
 }
+// What rounding took of e, rounded in its turn
+template <int DT>
+__device__ __forceinline__ void pack_rest(const float (&e)[16], const uint4 (&p)[2], uint4 (&rest)[2]) {
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float y[8];
+    unpack8<DT>(p[i], y);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x[8 * i + u] = e[8 * i + u] - y[u];
+  }
+  pack16<DT>(x, rest);
+}
 __device__ __forceinline__ float sum16(const float (&e)[16]) {
   float s[4];
 #pragma unroll

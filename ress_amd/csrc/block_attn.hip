@@ -12,6 +12,7 @@
 // once its A operand holds the 16 places in the same order, so P and dS go from one product's registers into the next:
 //   forward, dQ:  S^T = K Q^T (column: the lane's query), O^T += V^T P^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   dK and dV:    S = Q K^T (column: the lane's key), dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
+// P and dS are rounded to the operands' type for that; FINE: what the rounding took is multiplied too.
 // Transposed A operands (V^T, K^T, dO^T, Q^T) come out of the row-major LDS tiles by ds_read_tr16_b64, which gives lane i of 16 the
 // i-th column of a 4 x 16 block. dQ and dK/dV are kernels of their own, each the owner of its rows: S and dP are computed
 // twice (18 products' worth of operations for the 14 that a step needs), and nothing is added by atomics, so results
@@ -30,8 +31,8 @@ constexpr int WIDE_TILES = 640;
 // A wave has 32 queries. Steps of 64 keys, at a head of 128 in two stages (three of 32 keys 153 us for 135, the causal case).
 // Bound by the vector unit where the card is full: of a step's 16 products (D = 64) and 32 exponentials a lane, the latter are
 // four times as dear as other instructions.
-template <int DT, int D, bool MAP>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArgs a) {
+template <int DT, int D, bool MAP, bool FINE>
+__global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArgs a) {
   constexpr int SR = 64, KT = SR / 32, TILE = SR * 2 * D, NS = D == 64 ? 3 : 2;
   __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
@@ -105,6 +106,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_fwd(AttnArg
         // the sum before P is rounded: the backward pass forms P from it
         l += sum16(e);
         each<D / 32>([&](auto d) { o[d] = columns_times<DT, D>(tile + TILE, 32 * t, d, ln, p, o[d]); });
+        if constexpr (FINE) {
+          uint4 rest[2];
+          pack_rest<DT>(e, p, rest);
+          each<D / 32>([&](auto d) { o[d] = columns_times<DT, D>(tile + TILE, 32 * t, d, ln, rest, o[d]); });
+        }
       });
     };
     run_steps<NS, 2 * ks.DMAS>(
@@ -209,8 +215,8 @@ __device__ __forceinline__ float lift_ds(const AttnArgs& a, int b, int hk) {
 // ---- backward: dQ -----------------------------------------------------------
 // A wave has 32 queries and their gradients as operands. Bound by matrix and vector unit in turn (16 frames of 1,374 tokens, 30% of the
 // blocks: products 51% of the cycles, vector instructions 59%), at a clock that their power brings down to some 1.7 GHz.
-template <int DT, int D, bool MAP>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs a) {
+template <int DT, int D, bool MAP, bool FINE>
+__global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs a) {
   constexpr int SR = step_rows(D), KT = SR / 32, TILE = SR * 2 * D;
   __shared__ __align__(16) uint8_t lds[NS][2 * TILE];
   extern __shared__ uint32_t bits[];
@@ -274,6 +280,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
         pack16<DT>(e, ds);
         sum = add8<DT>(ds[1], add8<DT>(ds[0], sum));
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
+        if constexpr (FINE) {
+          uint4 rest[2];
+          pack_rest<DT>(e, ds, rest);
+          sum = add8<DT>(rest[1], add8<DT>(rest[0], sum));
+          each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, rest, dq[d]); });
+        }
       });
       over = stage;
       keys = min(SR, hd.klen - st * SR);
@@ -322,8 +334,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs
 // for another: 502 us for 281. The tiles of a causal launch cut in two by their steps: 250 us and 40 to join them for 244.
 // Four waves of 32 keys, or SPLIT (under a map, where a workgroup has one key block, and where tiles are few): two waves of 32
 // keys take the first 32 queries of each step, two more with the same keys the others, and their sums are added at the end.
-template <int DT, int D, bool SPLIT, bool MAP>
-__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dkv(AttnArgs a) {
+template <int DT, int D, bool SPLIT, bool MAP, bool FINE>
+__global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_dkv(AttnArgs a) {
   constexpr int SR = SPLIT ? 64 : step_rows(D), KT = SR / 32, TILE = SR * 2 * D, STAGE = 2 * TILE + 512;
   constexpr int KEYS = SPLIT ? 64 : 128, STAGES = SPLIT && D == 128 ? 2 : NS;
   __shared__ __align__(16) uint8_t lds[STAGES][STAGE];
@@ -379,11 +391,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dkv(AttnArg
 #pragma unroll
             for (int r = 0; r < 16; ++r) e[r] = st * SR + 32 * t + c_row(r) >= first ? e[r] : 0.0f;
           }
-          uint4 p[2], ds[2];
+          uint4 p[2], ds[2], rest[2];
           pack16<DT>(e, p);
+          if constexpr (FINE) pack_rest<DT>(e, p, rest);
           if constexpr (D == 128) __builtin_amdgcn_sched_barrier(0);  // reads ahead of their use would take registers that are not there
           const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, v, row_values(tile + 2 * TILE + 256, 32 * t, ln));
           each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + TILE, 32 * t, x, ln, p, dv[x]); });
+          if constexpr (FINE) each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + TILE, 32 * t, x, ln, rest, dv[x]); });
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             e[r] *= dp[r];
@@ -391,6 +405,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void k_block_attn_dkv(AttnArg
           }
           pack16<DT>(e, ds);
           each<D / 32>([&](auto x) { dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, ds, dk[x]); });
+          if constexpr (FINE) {
+            pack_rest<DT>(e, ds, rest);
+            each<D / 32>([&](auto x) { dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, rest, dk[x]); });
+          }
         });
       };
       run_steps<STAGES, 2 * qs.DMAS + 1>(
@@ -559,15 +577,20 @@ int parts_of(long long tiles, long long steps) {
   if (n > steps / LEAST) n = steps / LEAST;
   return (int)(n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n);
 }
+// Up to so many probabilities P and dS are not rounded, but multiplied in two terms: where a few of them make a result, their rounding
+// does not average out (one row of two heads over five keys in bf16: dV off by 2.9e-3 of it, the result's own rounding 1.7e-3), and
+// what the second products take is small beside the launch.
+constexpr int FEW = 1 << 14;
 // How a call is cut: keys a workgroup of dK and dV has, and the parts of each kernel
 struct Plan {
-  bool split;
+  bool split, fine;
   int q_parts, k_parts;
   long long q_rows, k_rows;
   explicit Plan(const ress_block_attn* c) {
     const long long wide = (long long)c->B * c->kv_heads * cdiv(c->Tk, 128);
-    split = c->map || wide < WIDE_TILES;
     q_rows = (long long)c->B * c->q_heads * c->Tq;
+    fine = q_rows <= FEW && q_rows * c->Tk <= FEW;
+    split = c->map || fine || wide < WIDE_TILES;
     k_rows = (long long)c->B * c->kv_heads * c->Tk;
     q_parts = parts_of((long long)c->B * c->q_heads * cdiv(c->Tq, QB), cdiv(c->Tk, KB));
     k_parts = parts_of((long long)c->B * c->kv_heads * cdiv(c->Tk, split ? 64 : 128),
@@ -579,6 +602,13 @@ struct Plan {
     return q > k ? q : k;
   }
 };
+template <class F>
+void with_plan(bool map, bool fine, F f) {
+  if (map && fine) f(std::true_type{}, std::true_type{});
+  else if (map) f(std::true_type{}, std::false_type{});
+  else if (fine) f(std::false_type{}, std::true_type{});
+  else f(std::false_type{}, std::false_type{});
+}
 bool sizes_ok(const ress_block_attn* c) {
   return c && c->B >= 0 && c->q_heads >= 0 && c->kv_heads >= 1 && c->q_heads % c->kv_heads == 0 && c->Tq >= 0 && c->Tk >= 0 &&
          c->Tq <= 1 << 26 && c->Tk <= 1 << 26 && (c->head_dim == 64 || c->head_dim == 128);
@@ -609,8 +639,10 @@ RESS_API int ress_block_attn_fwd(const ress_block_attn* c, void* workspace, long
   if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * a.parts, name, &blocks)) return rc;
   if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jblocks)) return rc;
   RESS_BA_EACH({
-    if (a.map) hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, true>), dim3(blocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
-    else hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, false>), dim3(blocks, a.parts), dim3(256), 0, stream, a);
+    with_plan(a.map, plan.fine, [&](auto map, auto fine) {
+      hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, decltype(map)::value, decltype(fine)::value>), dim3(blocks, a.parts), dim3(256),
+                         map ? bit_bytes(cdiv(a.Tk, KB)) : 0, stream, a);
+    });
     RESS_LAUNCHED("k_block_attn_fwd");
     if (a.parts > 1) {
       hipLaunchKernelGGL((k_block_attn_join<DT, DIM, true>), dim3(jblocks), dim3(256), 0, stream, a, a.part, a.part2, a.o, a.Hq, a.Tq);
@@ -669,8 +701,10 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
       RESS_LAUNCHED("k_block_attn_delta");
       a.parts = plan.q_parts;
       a.part = parts;
-      if (a.map) hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, true>), dim3(qblocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tk, KB)), stream, a);
-      else hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, false>), dim3(qblocks, a.parts), dim3(256), 0, stream, a);
+      with_plan(a.map, plan.fine, [&](auto map, auto fine) {
+        hipLaunchKernelGGL((k_block_attn_dq<DT, DIM, decltype(map)::value, decltype(fine)::value>), dim3(qblocks, a.parts), dim3(256),
+                           map ? bit_bytes(cdiv(a.Tk, KB)) : 0, stream, a);
+      });
       RESS_LAUNCHED("k_block_attn_dq");
       if (a.parts > 1) {
         hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jq), dim3(256), 0, stream, a, a.part, nullptr, a.dq, a.Hq, a.Tq);
@@ -681,9 +715,12 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
       a.parts = plan.k_parts;
       a.part = parts;
       a.part2 = parts + a.parts * plan.k_rows * D;
-      if (a.map) hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, true, true>), dim3(kblocks, a.parts), dim3(256), bit_bytes(cdiv(a.Tq, QB)), stream, a);
-      else if (plan.split) hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, true, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
-      else hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, false, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
+      if (plan.split)
+        with_plan(a.map, plan.fine, [&](auto map, auto fine) {
+          hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, true, decltype(map)::value, decltype(fine)::value>), dim3(kblocks, a.parts),
+                             dim3(256), map ? bit_bytes(cdiv(a.Tq, QB)) : 0, stream, a);
+        });
+      else hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, false, false, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
       RESS_LAUNCHED("k_block_attn_dkv");
       if (a.parts > 1) {
         hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jk), dim3(256), 0, stream, a, a.part, nullptr, a.dk, a.Hk, a.Tk);

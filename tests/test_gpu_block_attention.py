@@ -327,3 +327,31 @@ def test_tokens_far_apart(dev, D):
         far.append(to)
     got = run(*(t.requires_grad_() for t in far[:3]), far[3], causal=True)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dt,u", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Tq,Tk", [(1, 5), (4, 14), (40, 70)])
+def test_few_probabilities_are_not_rounded(dev, dt, u, D, Tq, Tk):
+    """P and dS in two terms: each element is off by its own rounding and by 2^-14 of what its sums add up (two terms of 8 bits and a sign
+    leave 2^-17 of a factor, exponentials, sums and delta 2^-18 each and less; P alone rounded to bf16 would leave 2^-8)."""
+    q, k, v, do = make(1, 2, 2, Tq, Tk, D, dt)
+    out, dq, dk, dv = run(q, k, v, do)
+    q, k, v, g = (t.detach().double() for t in (q, k, v, do))
+    scale = 1.0 / math.sqrt(D)
+    p = (torch.matmul(q, k.transpose(2, 3)) * scale).softmax(-1)
+    o = torch.matmul(p, v)
+    dp = torch.matmul(g, v.transpose(2, 3))
+    delta = (g * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    size = p * (torch.matmul(g.abs(), v.abs().transpose(2, 3)) + (g.abs() * torch.matmul(p, v.abs())).sum(-1, keepdim=True))
+    # a score is a sum, too: 2^-18 of its terms moves p by as much of itself, times the terms' sum
+    size = size * (1 + scale * torch.matmul(q.abs(), k.abs().transpose(2, 3)))
+    wide = p * (1 + scale * torch.matmul(q.abs(), k.abs().transpose(2, 3)))
+    far = k.abs().amax(2, keepdim=True)
+    for got, want, mag in ((out, o, torch.matmul(wide, v.abs())),
+                           (dq, scale * torch.matmul(ds, k), scale * (size.sum(-1, keepdim=True) * far)),
+                           (dk, scale * torch.matmul(ds.transpose(2, 3), q), scale * torch.matmul(size.transpose(2, 3), q.abs())),
+                           (dv, torch.matmul(p.transpose(2, 3), g), torch.matmul(wide.transpose(2, 3), g.abs()))):
+        bound = u * want.abs() + 2.0 ** -14 * mag + (2.0 ** -25 if dt is torch.float16 else 0.0)
+        assert ((got.double() - want).abs() <= bound).all()
