@@ -355,3 +355,12 @@ def test_few_probabilities_are_not_rounded(dev, dt, u, D, Tq, Tk):
                            (dv, torch.matmul(p.transpose(2, 3), g), torch.matmul(wide.transpose(2, 3), g.abs()))):
         bound = u * want.abs() + 2.0 ** -14 * mag + (2.0 ** -25 if dt is torch.float16 else 0.0)
         assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Tq,Tk,causal", [(1, 64, False), (2, 65, True), (31, 33, False), (64, 64, True), (127, 129, True), (129, 200, False)])
+def test_small_sizes_of_many_heads(dev, dt, D, Tq, Tk, causal):
+    """More than 2^18 probabilities: rounded ones."""
+    H = 2 * ((1 << 17) // (Tq * Tk) + 1)
+    compare(*make(1, H, H // 2, Tq, Tk, D, dt), causal=causal)
