@@ -121,22 +121,6 @@ __device__ __forceinline__ float sum16(const float (&e)[16]) {
   for (int i = 0; i < 4; ++i) s[i] = (e[i] + e[4 + i]) + (e[8 + i] + e[12 + i]);
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
-// sum + the eight 16-bit values of w
-template <int DT>
-__device__ __forceinline__ float add8(const uint4& w, float sum) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (DT == BA_BF16) {
-      const v2bf ones = {(__bf16)1.0f, (__bf16)1.0f};
-      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, u[i]), ones, sum, false);
-    } else {
-      const v2h ones = {(_Float16)1.0f, (_Float16)1.0f};
-      sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, u[i]), ones, sum, false);
-    }
-  }
-  return sum;
-}
 __device__ __forceinline__ float pair_max(float x) { return fmaxf(x, xor_lane_f<32>(x)); }
 __device__ __forceinline__ float pair_sum(float x) { return x + xor_lane_f<32>(x); }
 

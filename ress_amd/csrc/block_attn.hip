@@ -12,7 +12,7 @@
 // once its A operand holds the 16 places in the same order, so P and dS go from one product's registers into the next:
 //   forward, dQ:  S^T = K Q^T (column: the lane's query), O^T += V^T P^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   dK and dV:    S = Q K^T (column: the lane's key), dP = dO V^T, dV^T += dO^T P, dK^T += Q^T dS
-// P and dS are rounded to the operands' type for that; FINE: what the rounding took is multiplied too.
+// P and dS are rounded to the operands' type for that; FINE: what the rounding took is multiplied too (of dQ's half in any case).
 // Transposed A operands (V^T, K^T, dO^T, Q^T) come out of the row-major LDS tiles by ds_read_tr16_b64, which gives lane i of 16 the
 // i-th column of a 4 x 16 block. dQ and dK/dV are kernels of their own, each the owner of its rows: S and dP are computed
 // twice (18 products' worth of operations for the 14 that a step needs), and nothing is added by atomics, so results
@@ -260,11 +260,8 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
       ks.fetch(lds0 + stage * 2 * TILE, st * SR, hd.klen, w);
       vs.fetch(lds0 + stage * 2 * TILE + TILE, st * SR, hd.klen, w);
     };
-    float sum = 0.0f;
-    int over = 0, keys = 0;
-    auto compute = [&](auto mask_tag, int stage, int st) {
+    auto compute = [&](auto mask_tag, const uint8_t* tile, int st) {
       const Lane<D> ln = here.anew();
-      const uint8_t* tile = lds[stage];
       each<KT>([&](auto t) {
         const v16f s = rows_times<DT, D>(tile, 32 * t, ln, q, zero16());
         const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, g, D == 128 ? ndelta : zero16());
@@ -278,46 +275,26 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
         }
         uint4 ds[2];
         pack16<DT>(e, ds);
-        sum = add8<DT>(ds[1], add8<DT>(ds[0], sum));
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
-        if constexpr (FINE) {
+        // Half of dS, or all (FINE), in two terms: its rows add up to 0, and what its rounding and delta's (P's in the forward pass) make of
+        // that sum goes into dQ times what the keys have in common. Keys with an offset of half their deviation, bf16: dQ off by 2.7e-3 in
+        // one term, 2.4e-3 so (1.7e-3 is the result's rounding); four frames 60 us for 68. Taking the sum out times some mean of the keys
+        // is cheaper, but lets keys in that the row does not see or that weigh nothing for it.
+        auto fine = [&] {
           uint4 rest[2];
           pack_rest<DT>(e, ds, rest);
-          sum = add8<DT>(rest[1], add8<DT>(rest[0], sum));
           each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, rest, dq[d]); });
+        };
+        if constexpr (FINE || (KT == 2 && decltype(t)::value == 0)) fine();
+        else if constexpr (KT == 1) {
+          if (!(st & 1)) fine();
         }
       });
-      over = stage;
-      keys = min(SR, hd.klen - st * SR);
     };
     run_steps<NS, 2 * ks.DMAS>(
         walk, fetch, [&](int st) { return st < whole; },
-        [&](int stage, int st) { compute(std::false_type{}, stage, st); },
-        [&](int stage, int st) { compute(std::true_type{}, stage, st); });
-    // The rows of dS add up to 0. What their rounding and delta's (P's in the forward pass) made of the sum stands in dQ times the keys'
-    // weighted mean: most of it is what the keys have in common, and goes with the mean of a few of them, those of the last step,
-    // which are still in LDS, or for parts, whose sums are not 0 but add up to it, the first step's. Error of dQ, keys with an offset
-    // of half their deviation: 2.7e-3 -> 2.3e-3 of it in bf16 (1.7e-3 is the result's rounding).
-    if (keys) {
-      if (a.parts > 1) {
-        const int st = walk.from(0);
-        step_barrier<0>();
-        ks.fetch(lds0, st * SR, hd.klen, w);
-        step_barrier<0>();
-        over = 0;
-        keys = min(SR, hd.klen - st * SR);
-      }
-      sum = pair_sum(sum);
-      const uint32_t one = pack2<DT>(1.0f, 1.0f);
-      const uint4 ones[2] = {make_uint4(one, one, one, one), make_uint4(one, one, one, one)};
-      const float by = -sum / (float)keys;
-      each<D / 32>([&](auto d) {
-        v16f mean = zero16();
-        each<KT>([&](auto t) { mean = columns_times<DT, D>(lds[over], 32 * t, d, here, ones, mean); });
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dq[d][r] = fmaf(by, mean[r], dq[d][r]);
-      });
-    }
+        [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); },
+        [&](int stage, int st) { compute(std::true_type{}, lds[stage], st); });
   }
   if (row >= a.Tq) return;
   if (a.parts > 1)
