@@ -395,7 +395,7 @@ typedef struct ress_block_attn {
 long long ress_block_attn_fwd_workspace_size(const ress_block_attn* args);
 int ress_block_attn_fwd(const ress_block_attn* args, void* workspace, long long workspace_bytes, hipStream_t stream);
 /* The gradients dq, dk, dv of the same call (zero in rows past the lengths), from its out, rest and lse and the gradient of out.
- * P and dS are rounded to the 16-bit type (fp16: dS scaled by a power of two that uses its range), sums are fp32 and of a
+ * P and dS are rounded to the 16-bit type (fp16: dS scaled by a power of two of each row of dQ and key of dK that uses its range), sums are fp32 and of a
  * fixed order. workspace: ress_block_attn_bwd_workspace_size bytes, 16-byte aligned. */
 long long ress_block_attn_bwd_workspace_size(const ress_block_attn* args);
 int ress_block_attn_bwd(const ress_block_attn* args, const ress_strided* grad_out, const ress_strided* dq,

@@ -12,7 +12,7 @@ constexpr float LOWEST = -0x1.fffffep127f;
 // The running maximum moves when a score lies more than this above it (in log2): P stays below 2^8, and most steps need no
 // pass over the accumulators.
 constexpr float LAZY = 8.0f;
-constexpr int VTOP_ROWS = 128, DELTA_ROWS = 128;  // of a workgroup
+constexpr int DELTA_ROWS = 128;  // of a workgroup
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -45,7 +45,6 @@ struct AttnArgs {
   // keys (dk, dv): [part][rows][D], [part][rows]
   int parts;
   float *part, *part2;
-  uint32_t* top;             // fp16: (B, Hk) largest |dO|, (B, Hk) largest |v|, as bits
   __device__ __forceinline__ int q_len(int b) const { return q_lens ? min(max(q_lens[b], 0), Tq) : Tq; }
   __device__ __forceinline__ int k_len(int b) const { return k_lens ? min(max(k_lens[b], 0), Tk) : Tk; }
   template <class I>

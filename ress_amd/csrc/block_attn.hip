@@ -132,26 +132,13 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
 }
 
 // ---- backward: row sums -----------------------------------------------------
-// Raises *p to the workgroup's largest value (>= 0: bits in the values' order, so the atomics' order is the same for the result). One
-// atomic a workgroup: they meet at a few addresses.
-__device__ __forceinline__ void raise_top(uint32_t* p, float top) {
-  __shared__ float tops[4];
-  top = wave_max(top);
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    if (top > 0.0f) atomicMax(p, __float_as_uint(top));
-  }
-}
-// -delta_i = -dO_i.(o_i + what o's rounding took), lse less the lift of P, and fp16: the largest finite |dO| of each
-// (sequence, key/value head). Bound by its bytes: 21,904 rows of 16 heads 24 us, 5.7 TB/s.
+// -delta_i = -dO_i.(o_i + what o's rounding took), and lse less the lift of P. Bound by its bytes: 21,904 rows of 16 heads 24 us,
+// 5.7 TB/s.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, int chunks) {
   constexpr int LR = D / 8;
   const int bh = blockIdx.x / chunks, b = bh / a.Hq, h = bh % a.Hq, piece = threadIdx.x % LR;
   const int from = blockIdx.x % chunks * DELTA_ROWS, end = min(a.Tq, from + DELTA_ROWS), qlen = a.q_len(b);
-  float top = 0.0f;
   for (int i = from + threadIdx.x / LR; i < end; i += 256 / LR) {  // a row's lanes go together
     float sum = 0.0f;
     const long long r = (long long)bh * a.Tq + i;
@@ -161,11 +148,7 @@ __global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, int chunks
       unpack8<DT>(*reinterpret_cast<const uint4*>(a.o.at(b, h, i) + 8 * piece), y);
       unpack8<DT>(*reinterpret_cast<const uint4*>(a.rest + r * D + 8 * piece), z);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        sum = fmaf(x[u], y[u] + z[u], sum);
-        const float m = fabsf(x[u]);
-        if (m > top && m < __builtin_huge_valf()) top = m;
-      }
+      for (int u = 0; u < 8; ++u) sum = fmaf(x[u], y[u] + z[u], sum);
     }
 #pragma unroll
     for (int s = 1; s < LR; s <<= 1) sum += __shfl_xor(sum, s, LR);
@@ -174,42 +157,30 @@ __global__ __launch_bounds__(256) void k_block_attn_delta(AttnArgs a, int chunks
       a.lse_b[r] = a.lse[r] - lift(DT);
     }
   }
-  if constexpr (DT == BA_F16) raise_top(a.top + (long long)b * a.Hk + h / a.G, top);
-}
-__global__ void k_block_attn_clear(uint32_t* p, int n) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) p[i] = 0;
-}
-// the largest finite |v| of each (sequence, key/value head), fp16
-template <int D>
-__global__ __launch_bounds__(256) void k_block_attn_vtop(AttnArgs a, int chunks) {
-  constexpr int LR = D / 8;
-  const int bh = blockIdx.x / chunks, chunk = blockIdx.x % chunks, b = bh / a.Hk, h = bh % a.Hk;
-  const int end = min(a.k_len(b), (chunk + 1) * VTOP_ROWS);
-  float top = 0.0f;
-  for (int i = chunk * VTOP_ROWS + threadIdx.x / LR; i < end; i += 256 / LR) {
-    float x[8];
-    unpack8<BA_F16>(*reinterpret_cast<const uint4*>(a.v.at(b, h, i) + 8 * (threadIdx.x % LR)), x);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const float m = fabsf(x[u]);
-      if (m > top && m < __builtin_huge_valf()) top = m;
-    }
-  }
-  raise_top(a.top + (long long)a.B * a.Hk + bh, top);
 }
 
-// fp16: dS is formed times a power of two that takes the largest possible one to 2^15 (|dP - delta| <= 2 D max|dO| max|v|,
-// P <= 1): a gradient far below fp16's smallest number keeps its bits. bf16 has fp32's range.
-template <int DT, int D>
-__device__ __forceinline__ float lift_ds(const AttnArgs& a, int b, int hk) {
-  if constexpr (DT == BA_BF16) return 1.0f;
-  const int at = b * a.Hk + hk;
-  const float most = __uint_as_float(a.top[at]) * __uint_as_float(a.top[(long long)a.B * a.Hk + at]);
-  if (!(most > 0.0f)) return 1.0f;
-  int e;
-  frexpf(most, &e);  // most < 2^e
-  return ldexpf(1.0f, min(max(15 - (D == 64 ? 7 : 8) - e, -100), 100));
+// fp16: dS is formed times a power of two, one for each row of dQ and each key of dK, so that a gradient far below fp16's smallest
+// number keeps its bits and nothing takes them but what the row or the key itself meets: 2^60 to begin with (fp32 holds that
+// times the largest dP - delta there is, 2^41), and where a |dS| passes 2^15, less by what takes that below 2^12, with the sum so far.
+constexpr float DS_LIFT = 60.0f;
+// Whether a row (key) of the wave has such a one; high: the lane's largest
+__device__ __forceinline__ bool over(const float (&e)[16], float lift, float& high) {
+  high = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) high = fmaxf(high, fabsf(e[r]));
+  high *= lift;
+  return __any(high > 0x1p15f);
+}
+__device__ __forceinline__ int shift_of(float high) {
+  high = pair_max(high);  // the row's (key's) other half decides alike; what is not finite makes the row so whatever the shift is
+  return high > 0x1p15f && high < __builtin_huge_valf() ? 12 - __builtin_amdgcn_frexp_expf(high) : 0;
+}
+template <int N>
+__device__ __forceinline__ void scale_all(v16f (&acc)[N], float by) {
+#pragma unroll
+  for (int d = 0; d < N; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] *= by;
 }
 
 // ---- backward: dQ -----------------------------------------------------------
@@ -230,7 +201,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
   v16f dq[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dq[d] = zero16();
-  float undo = 0.0f;
+  float up = DT == BA_F16 ? exp2f(DS_LIFT) : 1.0f;  // dS's lift
   if (q0 < qlen) {
     const int off = hd.klen - qlen;
     const int sees = a.causal ? min(hd.klen, max(0, row + off + 1)) : hd.klen;
@@ -240,11 +211,9 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
     uint4 q[D / 16], g[D / 16];
     load_row<D>(a.q, it.b, it.h, row, row < qlen, here.half, q);
     load_row<D>(a.go, it.b, it.h, row, row < qlen, here.half, g);
-    const float f = lift_ds<DT, D>(a, it.b, it.h / a.G);
-    undo = a.scale / f;
     float lse = 0.0f, nd = 0.0f;
     if (row < qlen) {
-      lse = a.lse_b[a.row_at(it, row)] + lift(DT) - log2f(f);
+      lse = a.lse_b[a.row_at(it, row)] + lift(DT) - (DT == BA_F16 ? DS_LIFT : 0.0f);
       nd = a.ndelta[a.row_at(it, row)];
     }
     // -delta is added by the matrix cores where 16 registers are to be had for it (2 x 16 products less a step: 144 us for 152 at a
@@ -273,6 +242,18 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
 #pragma unroll
           for (int r = 0; r < 16; ++r) e[r] = 32 * t + c_row(r) < below ? e[r] : 0.0f;
         }
+        if constexpr (DT == BA_F16) {
+          float high;
+          if (over(e, 1.0f, high)) {
+            const int shift = shift_of(high);
+            const float by = ldexpf(1.0f, shift);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) e[r] *= by;
+            scale_all(dq, by);
+            lse -= shift;
+            up *= by;
+          }
+        }
         uint4 ds[2];
         pack16<DT>(e, ds);
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
@@ -298,9 +279,9 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
   }
   if (row >= a.Tq) return;
   if (a.parts > 1)
-    store_part<D>(a.part + ((long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row)) * D, here.half, dq, undo, row < qlen);
+    store_part<D>(a.part + ((long long)blockIdx.y * a.B * a.Hq * a.Tq + a.row_at(it, row)) * D, here.half, dq, a.scale / up, row < qlen);
   else
-    store_grad<DT, D>(a.dq, it.b, it.h, row, here.half, dq, undo, row < qlen);
+    store_grad<DT, D>(a.dq, it.b, it.h, row, here.half, dq, a.scale / up, row < qlen);
 }
 
 // ---- backward: dK and dV ----------------------------------------------------
@@ -327,14 +308,12 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
   v16f dk[D / 32], dv[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) dk[d] = dv[d] = zero16();
-  float f = 1.0f;
+  float fp = DT == BA_F16 ? exp2f(DS_LIFT - lift(DT)) : 1.0f;  // P's lift to dS's
   if (k0 < hd.klen && qlen > 0) {
     const int off = hd.klen - qlen;
     uint4 k[D / 16], v[D / 16];
     load_row<D>(a.k, it.b, it.h, key, key < hd.klen, here.half, k);
     load_row<D>(a.v, it.b, it.h, key, key < hd.klen, here.half, v);
-    f = lift_ds<DT, D>(a, it.b, it.h);
-    const float fp = f * (DT == BA_F16 ? 0x1p-14f : 1.0f);
     const int from = a.causal ? min(qlen, max(0, k0 - off)) : 0;      // no row before it sees a key of the tile
     const int whole = a.causal ? max(0, k0 + KEYS - 1 - off) : 0;     // rows from here on see all of it
     const int first = a.causal ? key - off - 4 * here.half : 0;         // rows from `first` on see the lane's key
@@ -375,10 +354,21 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
           const v16f dp = rows_times<DT, D>(tile + TILE, 32 * t, ln, v, row_values(tile + 2 * TILE + 256, 32 * t, ln));
           each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + TILE, 32 * t, x, ln, p, dv[x]); });
           if constexpr (FINE) each<D / 32>([&](auto x) { dv[x] = columns_times<DT, D>(tile + TILE, 32 * t, x, ln, rest, dv[x]); });
+          if constexpr (DT == BA_F16) {
+            // products of their own: with dS itself formed in front of the branch its registers are not to be had (dK and dV 290 us for 246)
+            float ds[16], high;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = e[r] * dp[r];
+            if (over(ds, fp, high)) {
+              const float by = ldexpf(1.0f, shift_of(high));
+              scale_all(dk, by);
+              fp *= by;
+            }
+          }
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            e[r] *= dp[r];
             if constexpr (DT == BA_F16) e[r] *= fp;
+            e[r] *= dp[r];
           }
           pack16<DT>(e, ds);
           each<D / 32>([&](auto x) { dk[x] = columns_times<DT, D>(tile, 32 * t, x, ln, ds, dk[x]); });
@@ -394,7 +384,14 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
           [&](int stage, int st) { compute(std::false_type{}, lds[stage], st); });
     }
   }
+  float by_k = a.scale;
+  const float by_v = DT == BA_F16 ? 0x1p-14f : 1.0f;
+  if constexpr (DT == BA_F16) by_k = a.scale * 0x1p-14f / fp;
   if constexpr (SPLIT) {
+    if constexpr (DT == BA_F16) {  // the two waves' lifts differ
+      scale_all(dk, by_k);
+      by_k = 1.0f;
+    }
     // waves 2 and 3 hand their sums to 0 and 1, dK's and then dV's: 16 floats of a lane and tile of 32 dims
     static_assert(2 * (D / 32) * 16 * 64 * 4 <= (int)sizeof(lds), "the sums fit the stages");
     float* to = reinterpret_cast<float*>(&lds[0][0]) + (w & 1) * (D / 32) * 16 * 64 + (threadIdx.x & 63);
@@ -415,7 +412,6 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
     if (w >= 2) return;
   }
   if (key >= a.Tk) return;
-  const float by_k = a.scale / f, by_v = DT == BA_F16 ? 0x1p-14f : 1.0f;
   if (a.parts > 1) {
     const long long r = (((long long)blockIdx.y * a.B + it.b) * a.Hk + it.h) * a.Tk + key;
     store_part<D>(a.part + r * D, here.half, dk, by_k, key < hd.klen);
@@ -632,6 +628,7 @@ RESS_API int ress_block_attn_fwd(const ress_block_attn* c, void* workspace, long
 RESS_API long long ress_block_attn_bwd_workspace_size(const ress_block_attn* c) {
   if (!sizes_ok(c)) return -1;
   const Plan p(c);
+  // 8 bytes a key/value head more than is used: the size stays what it was for callers that have set it aside
   return p.bwd_part_bytes(c->head_dim) + 8 * p.q_rows + 8ll * c->B * c->kv_heads;
 }
 
@@ -658,21 +655,14 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   float* const parts = (float*)workspace;  // of dQ and, once these are joined, of dK and dV
   a.lse_b = parts + plan.bwd_part_bytes(D) / 4;
   a.ndelta = a.lse_b + plan.q_rows;
-  a.top = (uint32_t*)(a.ndelta + plan.q_rows);
-  const int keys = plan.split ? 64 : 128, chunks = cdiv(a.Tk, VTOP_ROWS), dchunks = cdiv(a.Tq, DELTA_ROWS);
-  unsigned qblocks, kblocks, dblocks, vblocks, jq, jk;
+  const int keys = plan.split ? 64 : 128, dchunks = cdiv(a.Tq, DELTA_ROWS);
+  unsigned qblocks, kblocks, dblocks, jq, jk;
   if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * plan.q_parts, name, &qblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hk * cdiv(a.Tk, keys), 256 * plan.k_parts, name, &kblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hq * dchunks, 256, name, &dblocks)) return rc;
-  if (int rc = grid((long long)a.B * a.Hk * chunks, 256, name, &vblocks)) return rc;
   if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jq)) return rc;
   if (int rc = grid((plan.k_rows + 3) / 4, 256, name, &jk)) return rc;
   RESS_BA_EACH({
-    if (dtype == BA_F16 && a.Tk) {
-      hipLaunchKernelGGL(k_block_attn_clear, dim3(cdiv(2 * a.B * a.Hk, 256)), dim3(256), 0, stream, a.top, 2 * a.B * a.Hk);
-      hipLaunchKernelGGL((k_block_attn_vtop<DIM>), dim3((unsigned)((long long)a.B * a.Hk * chunks)), dim3(256), 0, stream, a, chunks);
-      RESS_LAUNCHED("k_block_attn_vtop");
-    }
     if (a.Tq) {
       hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3((unsigned)((long long)a.B * a.Hq * dchunks)), dim3(256), 0, stream, a, dchunks);
       RESS_LAUNCHED("k_block_attn_delta");
