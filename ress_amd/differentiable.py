@@ -8,7 +8,8 @@ The block-sparse layers run without gradients. Calibration tables (a head's Fish
 map need them; ress_amd.training puts these operators into a model's blocks.
 
 Every operator works on torch's current stream of its operands' device, waits for nothing and repeats bit for bit: no sum
-is made by atomics. Gradients are formed once (no second derivatives), in the operands' types with 32-bit sums.
+is made by atomics. Gradients are formed once (no second derivatives, none in forward mode: dual tensors are refused), in the
+operands' types with 32-bit sums.
 Operands with strides that a kernel cannot take are copied first. The reference has no counterpart: its kernels have no
 backward pass.
 
@@ -22,6 +23,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ress_amd import _lib
@@ -43,7 +45,11 @@ def _capturing():
 
 
 def _differentiates(*tensors):
-    """Whether a call on these tensors makes a graph; refuses leaves whose gradients cannot be captured."""
+    """Whether a call on these tensors makes a graph; refuses tangents, and leaves whose gradients cannot be captured."""
+    if forward_ad._current_level >= 0:  # inside a dual level, with gradients or without
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the operators have a backward pass but no forward-mode derivatives (a dual tensor was given)")
     if not torch.is_grad_enabled():
         return False
     for t in tensors:
