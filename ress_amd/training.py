@@ -140,11 +140,13 @@ def _layer_orders(grid, patch_order, device):
     if patch_order is not None or _capturing():  # what is made inside a capture belongs to its graph
         return _orders(grid, patch_order, device)
     key = (grid.frames, grid.P, grid.S, str(device), _lib.stream_handle(device))
-    if key not in _plain_orders:
+    orders = _plain_orders.get(key)  # by itself: other threads put tables in and clear them
+    if orders is None:
+        orders = _orders(grid, None, device)
         if len(_plain_orders) >= 8:
             _plain_orders.clear()
-        _plain_orders[key] = _orders(grid, None, device)
-    return _plain_orders[key]
+        _plain_orders[key] = orders
+    return orders
 
 
 def sparse_attention(q, k, v, final_map, grid, patch_order=None):
