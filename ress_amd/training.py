@@ -17,23 +17,35 @@ import torch
 import torch.nn as nn
 
 from ress_amd import _lib
-from ress_amd.differentiable import (NORM_DTYPES, Q_BLOCK, _capturing, add_layer_norm, block_attention, layer_norm,
-                                      rotate)
+from ress_amd.differentiable import (MOST_ROWS, MOST_WIDTH, NORM_DTYPES, Q_BLOCK, _capturing, add_layer_norm,
+                                      block_attention, layer_norm, rotate)
 from ress_amd.kvcache import RotaryTable
 from ress_amd.qkv import grid_shape, rope_base
 from ress_amd.stream import POSITIONS
 
 _HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+_GLOBAL_HOOKS = tuple("_global" + h for h in _HOOKS)
+
+
+def _untouched(module):
+    """Whether a call of the module runs its class' forward and nothing else: no hooks, its own or those on every module, and no
+    forward put on the instance."""
+    return ("forward" not in getattr(module, "__dict__", ()) and not any(getattr(module, h, None) for h in _HOOKS)
+            and not any(getattr(nn.modules.module, h, None) for h in _GLOBAL_HOOKS))
 
 
 def _bare(module, kind):
     """Whether a module is one of `kind` itself and nothing hangs on it, so that its arithmetic can be done in its place."""
-    return type(module) is kind and not any(getattr(module, h, None) for h in _HOOKS)
+    return type(module) is kind and _untouched(module)
 
 
 def _norm_takes(norm, x):
-    return (_bare(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.dtype in NORM_DTYPES
-            and all(w is None or w.dtype in (x.dtype, torch.float32) for w in (norm.weight, norm.bias)))
+    if not (_bare(norm, nn.LayerNorm) and len(norm.normalized_shape) == 1 and x.is_cuda and x.dtype in NORM_DTYPES):
+        return False
+    width = norm.normalized_shape[0]
+    kinds = {w.dtype for w in (norm.weight, norm.bias) if w is not None}
+    return (x.shape[-1] == width <= MOST_WIDTH and x.numel() <= MOST_ROWS * width and len(kinds) <= 1
+            and kinds <= {x.dtype, torch.float32})
 
 
 def _norm(norm, x):
