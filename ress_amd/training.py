@@ -53,8 +53,11 @@ def _norm(norm, x):
 
 
 def _table(rope, head_dim, device):
-    """The rotation table of a rotary module of known base, made once and kept on it (not in its state)."""
-    base = rope_base(rope)
+    """The rotation table of a rotary module of known base (RoPE2D itself or a declared module, with nothing on it), made once and
+    kept on it (not in its state)."""
+    from ress_amd.aggregator import RoPE2D
+    known = type(rope) is RoPE2D or not isinstance(rope, RoPE2D) or getattr(rope, "ress_rope", None) is not None
+    base = rope_base(rope) if known and _untouched(rope) else None
     if base is None:
         return None
     tables = rope.__dict__.setdefault("_ress_rotary_tables", {})
