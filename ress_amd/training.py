@@ -52,34 +52,40 @@ def _norm(norm, x):
     return layer_norm(x, norm.weight, norm.bias, norm.eps) if _norm_takes(norm, x) else norm(x)
 
 
-def _table(rope, head_dim, device):
-    """The rotation table of a rotary module of known base (RoPE2D itself or a declared module, with nothing on it), made once and
-    kept on it (not in its state)."""
+def _table(rope, head_dim, device, last):
+    """The rotation table of a rotary module of known base (RoPE2D itself or a declared module, with nothing on it) for positions up to
+    `last`, made once for each power of two of them and kept on the module (not in its state)."""
     from ress_amd.aggregator import RoPE2D
     known = type(rope) is RoPE2D or not isinstance(rope, RoPE2D) or getattr(rope, "ress_rope", None) is not None
     base = rope_base(rope) if known and _untouched(rope) else None
     if base is None:
         return None
     tables = rope.__dict__.setdefault("_ress_rotary_tables", {})
-    key = (head_dim, base, str(device))
-    if key not in tables:
+    positions = max(POSITIONS, 1 << int(last).bit_length())
+    key = (head_dim, base, str(device), positions)
+    table = tables.get(key)
+    if table is None:
         if _capturing():
             raise RuntimeError("run the model once before a graph capture: its rotation tables are made then")
-        tables[key] = RotaryTable(head_dim, POSITIONS, base=base, axes=2, device=device)
-        torch.cuda.current_stream(device).synchronize()  # once: other streams read it too
-    return tables[key]
+        table = RotaryTable(head_dim, positions, base=base, axes=2, device=device)
+        torch.cuda.current_stream(device).synchronize()  # once: other streams, and threads that find it, read it too
+        tables[key] = table
+    return table
 
 
 def normed_and_turned(attn, qkv, pos, nh):
     """q, k, v (B, heads, T, head_dim) of a projection's output (B, T, 3 heads head_dim), after the module's q and k norms and its
-    rotation, with gradients. Norms and rotary modules that the kernels do not stand for run as they are."""
+    rotation, with gradients. Norms and rotary modules that the kernels do not stand for run as they are. Positions that no grid of the
+    call's tokens has, and none of a table, are clamped and reported by check_layers."""
     B, T, C = qkv.shape
     hd = C // (3 * nh)
     q, k, v = qkv.reshape(B, T, 3, nh, hd).permute(2, 0, 3, 1, 4).unbind(0)
     q, k = _norm(attn.q_norm, q), _norm(attn.k_norm, k)
     rope = getattr(attn, "rope", None)
     if rope is not None and pos is not None:
-        table = _table(rope, hd, q.device) if hd in (64, 128) and q.dtype in (torch.bfloat16, torch.float16) and q.is_cuda else None
+        # a grid its maker has put on the positions, else no side is longer than all tokens
+        last = max(getattr(pos, "ress_patch_grid", None) or (T,))
+        table = _table(rope, hd, q.device, last) if hd in (64, 128) and q.dtype in (torch.bfloat16, torch.float16) and q.is_cuda else None
         if table is None:
             q, k = rope(q, pos), rope(k, pos)
         else:
