@@ -141,7 +141,9 @@ class RotaryTable:
         return self
 
     def check(self):
-        """Raises if a rotate since the last check met a position outside the table (waits for the device)."""
+        """Raises if a rotate since the last check, on any stream, met a position outside the table (waits for the device)."""
+        if self.status.is_cuda:
+            torch.cuda.synchronize(self.status.device)
         if int(self.status.item()):
             self.status.zero_()
             raise RuntimeError("RotaryTable: a position lies outside the rotation table (it was clamped into it)")

@@ -1,0 +1,37 @@
+"""What RotaryTable.check and check_layers report, from any stream and for any list of modules; tables that are views."""
+
+import pytest
+import torch
+
+import ress_amd as ress
+
+
+@pytest.mark.gpu
+def test_a_position_turned_on_another_stream(dev):
+    """check waits for the device, not for the current stream alone, and a second one finds nothing."""
+    rope = ress.RotaryTable(64, 8, axes=1, device=dev)
+    x, a = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16, device=dev), torch.randn(4096, 4096, device=dev)
+    pos = torch.arange(6, 10, device=dev)
+    ress.rotate(x, pos - 6, rope)
+    rope.check()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(40):  # some 40 ms in front of it
+            b = torch.matmul(a, a)
+        ress.rotate(x, pos, rope)
+    with pytest.raises(RuntimeError, match="outside the rotation table"):
+        rope.check()
+    rope.check()
+    torch.cuda.synchronize()
+    rope.check()
+    assert b.shape == a.shape
+
+
+def test_check_on_the_host():
+    rope = ress.RotaryTable(64, 8, axes=1, device="cpu")
+    rope.check()
+    rope.status.fill_(1)
+    with pytest.raises(RuntimeError, match="outside the rotation table"):
+        rope.check()
+    rope.check()
