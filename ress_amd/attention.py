@@ -417,9 +417,10 @@ def check_layers(model_or_modules):
     module left unreported: RuntimeError if a HeSS budget did not converge (reference
     _proportional.py:112-113), ValueError if the 16-bit attention met an operand outside
     fp16's range. Takes a model (every submodule) or an iterable of modules. A model that ran with
-    gradients: also RuntimeError if a position lay outside a rotary module's table (a copy each)."""
+    gradients: also RuntimeError if a position lay outside the table of a rotary module in them (a copy each)."""
     mods = list(model_or_modules.modules() if hasattr(model_or_modules, "modules") else model_or_modules)
-    for m in mods:
+    below = {id(s): s for m in mods for s in (m.modules() if hasattr(m, "modules") else (m,))}  # rotary modules lie in attentions
+    for m in below.values():
         for table in getattr(m, "_ress_rotary_tables", {}).values():
             table.check()
     results = [m._ress_status for m in mods if getattr(m, "_ress_status", None) is not None]

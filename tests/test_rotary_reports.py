@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import ress_amd as ress
+from ress_amd.aggregator import Block, RoPE2D
 
 
 @pytest.mark.gpu
@@ -26,6 +27,22 @@ def test_a_position_turned_on_another_stream(dev):
     torch.cuda.synchronize()
     rope.check()
     assert b.shape == a.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", ["model", "blocks", "attentions"])
+def test_a_list_of_modules(dev, given):
+    """The rotary modules below the given ones are looked at, too."""
+    block = ress.enable_gradients(Block(128, 2, 2.0, RoPE2D()).to(dev, torch.bfloat16))
+    model = torch.nn.Sequential(block)
+    modules = {"model": model, "blocks": [block], "attentions": [block.attn]}[given]
+    x = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=dev)
+    block(x, torch.full((1, 4, 2), 7, device=dev))
+    ress.check_layers(modules)
+    block(x, torch.full((1, 4, 2), 1 << 20, device=dev))
+    with pytest.raises(RuntimeError, match="outside the rotation table"):
+        ress.check_layers(modules)
+    ress.check_layers(modules)
 
 
 def test_check_on_the_host():
