@@ -137,7 +137,10 @@ class RotaryTable:
         if table.dtype != torch.float32 or table.dim() != 3 or tuple(table.shape[1:]) != (2, d // 2) or not len(table):
             raise ValueError(f"table must be (positions, 2, {d // 2}) float32, got {tuple(table.shape)} {table.dtype}")
         self = cls.__new__(cls)
-        self._set(table.contiguous(), head_dim, axes, layout, rotary_dim)
+        table = table.contiguous()
+        if table.data_ptr() & 15:  # the kernels read four values at a time
+            table = table.clone()
+        self._set(table, head_dim, axes, layout, rotary_dim)
         return self
 
     def check(self):

@@ -52,3 +52,17 @@ def test_check_on_the_host():
     with pytest.raises(RuntimeError, match="outside the rotation table"):
         rope.check()
     rope.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", [0, 1, 2, 3])
+def test_a_table_anywhere_in_memory(dev, at):
+    """from_table takes a contiguous view that starts at any element."""
+    angles = torch.arange(16, dtype=torch.float64)[:, None] * 100.0 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)
+    values = torch.stack([angles.cos(), angles.sin()], 1).float()
+    memory = torch.empty(values.numel() + 4, device=dev)
+    view = memory[at:at + values.numel()].view(values.shape)
+    view.copy_(values)
+    x, pos = torch.randn(1, 2, 16, 64, generator=torch.Generator().manual_seed(0)).to(dev, torch.bfloat16), torch.arange(16, device=dev)
+    got = ress.rotate(x, pos, ress.RotaryTable.from_table(view, 64, 1))
+    assert torch.equal(got, ress.rotate(x, pos, ress.RotaryTable.from_table(values.to(dev), 64, 1)))
