@@ -353,23 +353,26 @@ def ress_attention_forward(self, x, pos, num_to_select=None, budget_fn=None, per
     res = None
     order = None
     if graded:
-        qb, kbf, vbf = (t if t.dtype == torch.bfloat16 else t.to(torch.bfloat16) for t in (q, k, v))
+        # 16-bit activations in their own type; 32-bit ones by torch where the layer is dense, else in bfloat16
+        kind = q.dtype if q.dtype in training.DTYPES else torch.bfloat16
         if dense:
-            x_out = training.block_attention(qb, kbf, vbf)
+            x_out = training.block_attention(q, k, v) if q.dtype == kind else _dense_storage(q, k, v, shp)
             sparsity = 0.0
             self._ress_status = None
         else:
             order = _device_patch_order(self, patch_order, grid, q.device)
             with torch.no_grad():
-                _, res = _select(qb, kbf, vbf, grid, num_to_select, budget_fn, perhead_budget_fn, joint_select_fn, block_criterion,
-                                 getattr(self, "M", None), None, protect_own_frame, attention_sink, order)
+                _, res = _select(*(t.to(torch.bfloat16) for t in (q, k, v)), grid, num_to_select, budget_fn, perhead_budget_fn,
+                                 joint_select_fn, block_criterion, getattr(self, "M", None), None, protect_own_frame, attention_sink, order)
             with trace.stage("ress.sparse_attention"):
-                x_out = training.sparse_attention(qb, kbf, vbf, res.final_map, grid, order)
+                x_out = training.sparse_attention(*(t.to(kind) for t in (q, k, v)), res.final_map, grid, order)
             self._ress_status = LayerResult(out=None, unconverged=res.unconverged, budget_iters=res.budget_iters,
                                             max_iters=res.max_iters)
             sparsity = res.sparsity() if aux_store is not None else None
             if eager_check and aux_store is None:
                 res.check()
+        if aux_store is not None and aux_full:
+            x_out = x_out.float()  # as the other paths record it; its gradient has 32 bits, too
     elif dense:
         x_out = _dense_storage(q, k, v, shp).float()
         sparsity = 0.0

@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 
 from ress_amd import _lib
-from ress_amd.differentiable import (MOST_ROWS, MOST_WIDTH, NORM_DTYPES, Q_BLOCK, _capturing, add_layer_norm,
+from ress_amd.differentiable import (DTYPES, MOST_ROWS, MOST_WIDTH, NORM_DTYPES, Q_BLOCK, _capturing, add_layer_norm,
                                       block_attention, layer_norm, rotate)
 from ress_amd.kvcache import RotaryTable
 from ress_amd.qkv import grid_shape, rope_base
@@ -211,8 +211,8 @@ def block_forward(block, x, pos=None):
 
 def enable_gradients(model, on=True):
     """Has the model's blocks (those of ress_amd.aggregator) and its wired attentions run on operators with a backward pass wherever
-    gradients are asked for, on the GPU in 16 bits (a 32-bit model under autocast, or wired: the sparse layers run in bfloat16).
-    Heads of 64 or 128. on=False takes it back. Returns the model."""
+    gradients are asked for, on the GPU in 16 bits (a 32-bit model under autocast, or wired: its sparse layers run in bfloat16, its dense
+    ones by torch in 32 bits). Heads of 64 or 128. on=False takes it back. Returns the model."""
     from ress_amd.aggregator import Attention, Block
     from ress_amd.wiring import SparseAttentionForward
     found = []
