@@ -52,6 +52,14 @@ def _norm(norm, x):
     return layer_norm(x, norm.weight, norm.bias, norm.eps) if _norm_takes(norm, x) else norm(x)
 
 
+def _head_norm(norm, x):
+    """_norm of queries or keys. Autocast has a norm hand on 32 bits, which the rotation behind it then takes (by the module): nothing is
+    rounded between the two."""
+    if x.is_cuda and torch.is_autocast_enabled("cuda") and x.dtype is not torch.float32 and _norm_takes(norm, x):
+        x = x.float()
+    return _norm(norm, x)
+
+
 def _table(rope, head_dim, device, last):
     """The rotation table of a rotary module of known base (RoPE2D itself or a declared module, with nothing on it) for positions up to
     `last`, made once for each power of two of them and kept on the module (not in its state)."""
@@ -80,7 +88,7 @@ def normed_and_turned(attn, qkv, pos, nh):
     B, T, C = qkv.shape
     hd = C // (3 * nh)
     q, k, v = qkv.reshape(B, T, 3, nh, hd).permute(2, 0, 3, 1, 4).unbind(0)
-    q, k = _norm(attn.q_norm, q), _norm(attn.k_norm, k)
+    q, k = _head_norm(attn.q_norm, q), _head_norm(attn.k_norm, k)
     rope = getattr(attn, "rope", None)
     if rope is not None and pos is not None:
         # a grid its maker has put on the positions, else no side is longer than all tokens

@@ -80,3 +80,40 @@ def test_recorded_outputs_and_their_gradients_have_32_bits(dev, mode, dtype):
         attn(x, pos)
     off = (stores[0]["value"].output - o).abs().max() / o.abs().max()
     assert off <= math.ldexp(1.0, -5)  # the inference path's 8-bit scores
+
+
+def test_queries_and_keys_under_autocast(dev):
+    """As torch's modules under autocast: from the projection's rounding to the attention's operands one more, where a rounding between
+    norm and rotation would make two (2^-8 of an element each, and its partner's share in it)."""
+    block = build_vggt_aggregator(depth=1, dim=128, num_heads=2, seed=0, dtype=torch.float32, wire=False).aggregator.frame_blocks[0]
+    attn = block.attn
+    g = torch.Generator().manual_seed(5)
+    with torch.no_grad():
+        for norm in (attn.q_norm, attn.k_norm):
+            norm.weight.copy_(1 + 0.3 * torch.randn(64, generator=g))
+            norm.bias.copy_(0.3 * torch.randn(64, generator=g))
+    qkv = torch.randn(2, 150, 384, generator=g).to(dev, torch.bfloat16).requires_grad_()
+    pos = torch.randint(0, 37, (2, 150, 2), generator=g).to(dev)
+    dy = torch.randn(2, 2, 2, 150, 64, generator=g).to(dev, torch.bfloat16)
+    with torch.autocast("cuda", torch.bfloat16):
+        got = training.normed_and_turned(attn, qkv, pos, 2)
+    assert all(t.dtype == torch.bfloat16 for t in got)
+    grad, = torch.autograd.grad(got[:2], qkv, list(dy))
+    exact = qkv.detach().double().requires_grad_()
+    heads = exact.view(2, 150, 3, 2, 64).permute(2, 0, 3, 1, 4)
+    want = []
+    for t, norm in zip(heads, (attn.q_norm, attn.k_norm)):
+        t = torch.nn.functional.layer_norm(t, (64,), norm.weight.double(), norm.bias.double(), norm.eps)
+        turned = []
+        for axis in (0, 1):
+            inv = 100.0 ** (-torch.arange(0, 32, 2, dtype=torch.float64, device=dev) / 32)
+            z = torch.complex(t[..., 32 * axis:32 * axis + 16], t[..., 32 * axis + 16:32 * axis + 32])
+            z = z * torch.polar(torch.ones_like(inv), pos[:, None, :, axis, None].double() * inv)
+            turned += [z.real, z.imag]
+        want.append(torch.cat(turned, -1))
+    for x, y in zip(got, want):
+        # half a step, and 2^-17 of the elements' size: angles of up to 37 in 32 bits (the module's), products and sums
+        assert ((x.double() - y).abs() <= 2.0 ** -8 * y.abs() + 2.0 ** -17 * y.abs().amax()).all()
+    wanted, = torch.autograd.grad(want, exact, list(dy.double()))
+    # the projection's gradient is rounded once, and so is dy turned back where the module hands on 16 bits
+    assert ((grad.double() - wanted).norm() / wanted.norm()) <= 2.0 ** -8
