@@ -550,9 +550,10 @@ int parts_of(long long tiles, long long steps) {
   if (n > steps / LEAST) n = steps / LEAST;
   return (int)(n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n);
 }
-// Up to so many probabilities P and dS are not rounded, but multiplied in two terms: where a few of them make a result, their rounding
-// does not average out (one row of two heads over five keys in bf16: dV off by 2.9e-3 of it, the result's own rounding 1.7e-3), and
-// what the second products take is small beside the launch (16 heads of 126 tokens: 29.6 us of kernels for 27.4).
+// Calls of up to so many probabilities multiply P and dS in two terms: 1.7e-3 off in bf16 (the result's own rounding) for up to 2.4e-3,
+// however many terms stand behind a result. A trade of time for accuracy where a call is small, and the rule goes by the whole call because
+// that bounds the time: 16 heads of 126 tokens 29.4 us of kernels, of 128 x 129 in one term 29.4; four of 256 35.3 for 39.4; 64 of 64 22.4
+// for 21.5; one of 512 50.5 for 45.4; 1,024 heads of a row over 256 keys 107 for 93; one row over 2^18 keys 351 for 266.
 constexpr int FEW = 1 << 18;
 // How a call is cut: keys a workgroup of dK and dV has, and the parts of each kernel
 struct Plan {
