@@ -503,7 +503,8 @@ RESS_API int ress_layer_norm_bwd(const ress_layer_norm* c, const ress_rows* grad
   a.dx = (char*)dx;
   a.dbranch = (char*)dbranch;
   const bool ends = dgamma || dweight || dbias;
-  RESS_REQUIRE(!ends || workspace_bytes >= ress_layer_norm_bwd_workspace_size(c), "%s: the workspace is too small", name);
+  RESS_REQUIRE(!ends || (workspace_bytes >= ress_layer_norm_bwd_workspace_size(c) && ((uintptr_t)workspace & 15) == 0 && (workspace || !a.rows)),
+               "%s: the workspace is too small or not aligned", name);
   RESS_REQUIRE(!a.rows || (a.x.p && a.mean && a.rstd), "%s: null buffer", name);
   RESS_REQUIRE(a.branch.p || (!dbranch && !dgamma) || !a.rows, "%s: no branch", name);
   a.part = ends ? (float*)workspace : nullptr;
