@@ -645,11 +645,12 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   a.dv = view(*dv);
   const int D = c->head_dim, dtype = c->dtype;
   if (int rc = check(a, D, dtype, name)) return rc;
-  if (!a.B || !a.Hq) return 0;
-  RESS_REQUIRE((a.Tq == 0 || (fits(a.q, D) && fits(a.o, D) && fits(a.go, D) && fits(a.dq, D))) &&
+  if (!a.B) return 0;
+  const bool rows = a.Hq && a.Tq;  // without any, dk and dv are zero
+  RESS_REQUIRE((!rows || (fits(a.q, D) && fits(a.o, D) && fits(a.go, D) && fits(a.dq, D))) &&
                    (a.Tk == 0 || (fits(a.k, D) && fits(a.v, D) && fits(a.dk, D) && fits(a.dv, D))),
                "%s: operands must be 16-byte aligned, strides multiples of 8, tokens at least head_dim and fewer than 2^24 apart", name);
-  RESS_REQUIRE(a.Tq == 0 || (a.rest && ((uintptr_t)a.rest & 15) == 0 && a.lse), "%s: the forward pass's rest and lse are needed", name);
+  RESS_REQUIRE(!rows || (a.rest && ((uintptr_t)a.rest & 15) == 0 && a.lse), "%s: the forward pass's rest and lse are needed", name);
   RESS_REQUIRE(workspace_bytes >= ress_block_attn_bwd_workspace_size(c) && ((uintptr_t)workspace & 15) == 0 && (workspace || !workspace_bytes),
                "%s: the workspace is too small or not aligned", name);
   const Plan plan(c);
@@ -664,7 +665,7 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jq)) return rc;
   if (int rc = grid((plan.k_rows + 3) / 4, 256, name, &jk)) return rc;
   RESS_BA_EACH({
-    if (a.Tq) {
+    if (rows) {
       hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3((unsigned)((long long)a.B * a.Hq * dchunks)), dim3(256), 0, stream, a, dchunks);
       RESS_LAUNCHED("k_block_attn_delta");
       a.parts = plan.q_parts;
