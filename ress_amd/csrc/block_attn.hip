@@ -498,6 +498,8 @@ int grid(long long items, int threads, const char* name, unsigned* blocks) {
   *blocks = (unsigned)n;
   return 0;
 }
+// of joined rows: tiles that are cut are few, 384 of 128 rows
+unsigned join_blocks(long long rows) { return (unsigned)((rows + 3) / 4); }
 size_t bit_bytes(int n) { return 8 * (size_t)cdiv(n, 64); }
 
 #define RESS_BA_CASE(DT_, D_, ...)        \
@@ -609,9 +611,8 @@ RESS_API int ress_block_attn_fwd(const ress_block_attn* c, void* workspace, long
   a.parts = plan.q_parts;
   a.part = (float*)workspace;
   a.part2 = a.part + a.parts * plan.q_rows * D;
-  unsigned blocks, jblocks;
+  unsigned blocks;
   if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * a.parts, name, &blocks)) return rc;
-  if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jblocks)) return rc;
   RESS_BA_EACH({
     with_plan(a.map, plan.fine, [&](auto map, auto fine) {
       hipLaunchKernelGGL((k_block_attn_fwd<DT, DIM, decltype(map)::value, decltype(fine)::value>), dim3(blocks, a.parts), dim3(256),
@@ -619,7 +620,8 @@ RESS_API int ress_block_attn_fwd(const ress_block_attn* c, void* workspace, long
     });
     RESS_LAUNCHED("k_block_attn_fwd");
     if (a.parts > 1) {
-      hipLaunchKernelGGL((k_block_attn_join<DT, DIM, true>), dim3(jblocks), dim3(256), 0, stream, a, a.part, a.part2, a.o, a.Hq, a.Tq);
+      hipLaunchKernelGGL((k_block_attn_join<DT, DIM, true>), dim3(join_blocks(plan.q_rows)), dim3(256), 0, stream, a, a.part, a.part2,
+                         a.o, a.Hq, a.Tq);
       RESS_LAUNCHED("k_block_attn_join");
     }
   })
@@ -658,12 +660,10 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
   a.lse_b = parts + plan.bwd_part_bytes(D) / 4;
   a.ndelta = a.lse_b + plan.q_rows;
   const int keys = plan.split ? 64 : 128, dchunks = cdiv(a.Tq, DELTA_ROWS);
-  unsigned qblocks, kblocks, dblocks, jq, jk;
+  unsigned qblocks, kblocks, dblocks;
   if (int rc = grid((long long)a.B * a.Hq * cdiv(a.Tq, QB), 256 * plan.q_parts, name, &qblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hk * cdiv(a.Tk, keys), 256 * plan.k_parts, name, &kblocks)) return rc;
   if (int rc = grid((long long)a.B * a.Hq * dchunks, 256, name, &dblocks)) return rc;
-  if (int rc = grid((plan.q_rows + 3) / 4, 256, name, &jq)) return rc;
-  if (int rc = grid((plan.k_rows + 3) / 4, 256, name, &jk)) return rc;
   RESS_BA_EACH({
     if (rows) {
       hipLaunchKernelGGL((k_block_attn_delta<DT, DIM>), dim3((unsigned)((long long)a.B * a.Hq * dchunks)), dim3(256), 0, stream, a, dchunks);
@@ -676,7 +676,8 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
       });
       RESS_LAUNCHED("k_block_attn_dq");
       if (a.parts > 1) {
-        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jq), dim3(256), 0, stream, a, a.part, nullptr, a.dq, a.Hq, a.Tq);
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(join_blocks(plan.q_rows)), dim3(256), 0, stream, a, a.part,
+                           nullptr, a.dq, a.Hq, a.Tq);
         RESS_LAUNCHED("k_block_attn_join");
       }
     }
@@ -692,8 +693,10 @@ RESS_API int ress_block_attn_bwd(const ress_block_attn* c, const ress_strided* g
       else hipLaunchKernelGGL((k_block_attn_dkv<DT, DIM, false, false, false>), dim3(kblocks, a.parts), dim3(256), 0, stream, a);
       RESS_LAUNCHED("k_block_attn_dkv");
       if (a.parts > 1) {
-        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jk), dim3(256), 0, stream, a, a.part, nullptr, a.dk, a.Hk, a.Tk);
-        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(jk), dim3(256), 0, stream, a, a.part2, nullptr, a.dv, a.Hk, a.Tk);
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(join_blocks(plan.k_rows)), dim3(256), 0, stream, a, a.part,
+                           nullptr, a.dk, a.Hk, a.Tk);
+        hipLaunchKernelGGL((k_block_attn_join<DT, DIM, false>), dim3(join_blocks(plan.k_rows)), dim3(256), 0, stream, a, a.part2,
+                           nullptr, a.dv, a.Hk, a.Tk);
         RESS_LAUNCHED("k_block_attn_join");
       }
     }
