@@ -23,8 +23,9 @@
 namespace {
 
 constexpr int NS = 3;  // LDS stages
-// Below this many tiles of 128 keys (2.5 workgroups a CU) dK and dV's are tiles of 64 keys, twice as many: 16 tiles 6.7 us for 8.0, 512
-// causal ones 388 for 426, but 704 82 for 73 and 2,752 66 for 56 (before the head of 128 kept its registers: 281 now).
+// Below this many tiles of 128 keys (2.5 workgroups a CU) dK and dV's are tiles of 64 keys, twice as many. In us, 128 keys / 64: 16 heads of
+// 1,374 in bf16, 176 tiles 31 / 29, 352 43 / 43, 528 65 / 66, 704 72 / 80, 2,816 268 / 300; a head of 128, causal, 2,048 tokens, four query
+// heads a key head in fp16, 256 tiles 232 / 217, 512 417 / 332, 640 444 / 415, 768 495 / 485, 1,024 620 / 643.
 constexpr int WIDE_TILES = 640;
 
 // ---- forward ----------------------------------------------------------------

@@ -98,7 +98,8 @@ class RotaryTable:
     divided among the axes; scaling, for contexts longer than a model was trained on: {"type": "linear", "factor": f} divides
     positions by f, "ntk" multiplies the base by f^(d/(d-2)), and "yarn" (with "original", the trained positions; Peng et al.,
     2023) divides by f the frequencies of pairs that turn less than "slow" = 1 time over the trained positions, leaves those that turn
-    more than "fast" = 32 times, goes linearly between, and multiplies cosines and sines by "attention" = 0.1 ln f + 1."""
+    more than "fast" = 32 times, goes linearly between in the number of turns, as the paper has it, and multiplies cosines and sines by
+    "attention" = 0.1 ln f + 1. Models whose tables go linearly in the pairs' index instead are served by from_table."""
 
     def __init__(self, head_dim, positions, base=100.0, axes=2, device="cuda", layout="half", rotary_dim=None, scaling=None):
         d = self._check(head_dim, axes, layout, rotary_dim)
