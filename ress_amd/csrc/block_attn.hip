@@ -15,8 +15,8 @@
 // P and dS are rounded to the operands' type for that; FINE: what the rounding took is multiplied too (of dQ's half in any case).
 // Transposed A operands (V^T, K^T, dO^T, Q^T) come out of the row-major LDS tiles by ds_read_tr16_b64, which gives lane i of 16 the
 // i-th column of a 4 x 16 block. dQ and dK/dV are kernels of their own, each the owner of its rows: S and dP are computed
-// twice (18 products' worth of operations for the 14 that a step needs), and nothing is added by atomics, so results
-// repeat bit for bit.
+// twice (with dQ's half in two terms 19 products' worth of operations for the 14 that a step needs), and nothing is added by
+// atomics, so results repeat bit for bit.
 #include "../../include/ress_hip.h"
 #include "block_attn.h"
 
@@ -186,7 +186,7 @@ __device__ __forceinline__ void scale_all(v16f (&acc)[N], float by) {
 
 // ---- backward: dQ -----------------------------------------------------------
 // A wave has 32 queries and their gradients as operands. Bound by matrix and vector unit in turn (16 frames of 1,374 tokens, 30% of the
-// blocks: products 51% of the cycles, vector instructions 59%), at a clock that their power brings down to some 1.7 GHz.
+// blocks: products 53% of the cycles, vector instructions 62%), at a clock that their power brings down to some 1.7 GHz.
 template <int DT, int D, bool MAP, bool FINE>
 __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_dq(AttnArgs a) {
   constexpr int SR = step_rows(D), KT = SR / 32, TILE = SR * 2 * D;
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
         each<D / 32>([&](auto d) { dq[d] = columns_times<DT, D>(tile, 32 * t, d, ln, ds, dq[d]); });
         // Half of dS, or all (FINE), in two terms: its rows add up to 0, and what its rounding and delta's (P's in the forward pass) make of
         // that sum goes into dQ times what the keys have in common. Keys with an offset of half their deviation, bf16: dQ off by 2.7e-3 in
-        // one term, 2.4e-3 so (1.7e-3 is the result's rounding); four frames 60 us for 68. Taking the sum out times some mean of the keys
+        // one term, 2.4e-3 so (1.7e-3 is the result's rounding); four frames 72 us for 60. Taking the sum out times some mean of the keys
         // is cheaper, but lets keys in that the row does not see or that weigh nothing for it.
         auto fine = [&] {
           uint4 rest[2];
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) void k_block_attn_
 
 // ---- backward: dK and dV ----------------------------------------------------
 // A wave has 32 keys; queries and their gradients stream past. At a head of 64 bound by the products and what stands between them (16
-// sparse frames: matrix cores 46% of the cycles, vector unit 42%, waves waiting 44%). At a head of 128 no register is left to read
+// sparse frames: matrix cores 47% of the cycles, vector unit 43%, waves waiting 44%). At a head of 128 no register is left to read
 // LDS far ahead, and a wave alone on its SIMD takes 1.5 us a step of 32 queries of which the products are 0.6; two share it at 2.1
 // (full card: matrix cores 47%). Tried there: 64 keys a wave, one wave a SIMD, every operand read meeting two tiles, no wave waiting
 // for another: 502 us for 281. The tiles of a causal launch cut in two by their steps: 250 us and 40 to join them for 244.
@@ -545,7 +545,7 @@ AttnArgs arguments(const ress_block_attn* c) {
 
 // Parts that a launch of `tiles` workgroups is cut into, each of at least LEAST steps of 64 rows: as many as fill the card's 512 places
 // for workgroups (two a CU) where a quarter of them or more would stay empty. 16 tiles of 80 queries over 21,984 keys: forward 377 us
-// whole, 26 in 32 parts and 5 to join them; dQ 330, 27 and 5.
+// whole, 26 in 32 parts and 5 to join them; dQ 330, 27 and 5 (in one term; now 32).
 constexpr int PLACES = 512, LEAST = 8, MOST_PARTS = 64;
 int parts_of(long long tiles, long long steps) {
   if (tiles <= 0 || tiles > PLACES * 3 / 4) return 1;

@@ -14,8 +14,9 @@ Operands with strides that a kernel cannot take are copied first. The reference 
 backward pass.
 
 In a captured graph: torch accumulates a leaf's gradient on the stream on which the leaf entered the oldest graph that still
-lives. Where that is an eager one of the default stream, capturing the backward pass would end the process: a call with such
-a leaf is refused inside a capture (delete the eager result first, or run it on a side stream).
+lives. Where that is an eager one of the default stream, capturing the backward pass would end the process: a call with a leaf
+of which these operators have made such a graph is refused inside a capture (delete the eager result first, or run it on a side stream;
+graphs that torch's operators alone have made of a leaf cannot be told).
 """
 
 import functools
