@@ -252,6 +252,8 @@ def block_attention(q, k, v, block_map=None, causal=False, q_lens=None, k_lens=N
     operands and output, a tensor of the output's size (what its rounding took) and 4 bytes a row."""
     _check_attention(q, k, v, block_map)
     B, Hq, Tq, D = q.shape
+    if torch.is_tensor(scale) and scale.requires_grad and torch.is_grad_enabled():
+        raise ValueError("scale gets no gradient: give a number, and multiply q by what is learnt")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
@@ -484,6 +486,8 @@ def rotate(x, pos, rope):
     B, _, n, _ = first.shape
     if rope.table.device != first.device:
         raise ValueError(f"rope is on {rope.table.device}, x on {first.device}")
+    if rope.table.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the rotation table gets no gradient: give one that does not require it")
     axes = rope.axes
     want = [(B, n), (n,)] if axes == 1 else [(B, n, 2), (n, 2)]
     if not torch.is_tensor(pos) or pos.is_floating_point() or tuple(pos.shape) not in want or pos.device != first.device:
