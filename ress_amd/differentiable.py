@@ -247,9 +247,10 @@ def block_attention(q, k, v, block_map=None, causal=False, q_lens=None, k_lens=N
     their 128-query blocks.
 
     The probabilities, formed anew in the backward pass, and the scores' gradients are rounded to the operands' type before
-    they are multiplied; half of the latter, for dq, and both in calls of up to 2^18 probabilities (all sequences and heads, whatever a
-    map or the causal order leaves), are multiplied in two terms. Sums, maxima and the softmax's statistics are fp32. A forward pass for gradients keeps, beside its
-    operands and output, a tensor of the output's size (what its rounding took) and 4 bytes a row."""
+    they are multiplied; half of the latter, for dq, and both in calls of up to 2^18 probabilities (all sequences and heads,
+    whatever a map or the causal order leaves), are multiplied in two terms. Sums, maxima and the softmax's statistics are
+    fp32. A forward pass for gradients keeps, beside its operands and output, a tensor of the output's size (what its
+    rounding took) and 4 bytes a row."""
     _check_attention(q, k, v, block_map)
     B, Hq, Tq, D = q.shape
     if torch.is_tensor(scale) and scale.requires_grad and torch.is_grad_enabled():
